@@ -44,7 +44,8 @@
 extern "C" {
 #endif
 
-enum b2q_type { B2Q_TYPE_F32 = 0, B2Q_TYPE_F16 = 1, B2Q_TYPE_Q4_0 = 2, B2Q_TYPE_Q8_0 = 8, B2Q_TYPE_Q4_K = 12 };
+enum b2q_type { B2Q_TYPE_F32 = 0, B2Q_TYPE_F16 = 1, B2Q_TYPE_Q4_0 = 2, B2Q_TYPE_Q8_0 = 8, B2Q_TYPE_Q4_K = 12,
+                B2Q_TYPE_BF16 = 30 };  /* BF16: the cached-decoding entries only */
 
 /* Activation-quantizer variant (fp32 -> Q8_0 rounding).
  *   B2Q_ACT_X86: the from_float of ggml's CPU backend on x86 (the host the
@@ -531,6 +532,99 @@ B2Q_API int b2q_sparse_scatter_plan(const int32_t* row_indices, int64_t fine_row
 B2Q_API int b2q_sparse_scatter_mean_f16_planned(const void* features16, int64_t fine_rows, int64_t channels,
                                                 const void* plan, const float* counts, int64_t coarse_rows,
                                                 void* out16, void* stream);
+
+/* --------------------------------------------------------- cached decoding
+ * A transformer step over new tokens whose earlier keys and values are kept in
+ * a paged cache: plan the pages, append k and v while the q / k / v rows get
+ * their positions, attend, and run the few-token linears on 4-bit weights.  No
+ * counterpart in the reference, whose graphs keep no cache between runs; in
+ * ggml terms these take the place of ROPE (multi-section), SET_ROWS into a KV
+ * cache, FLASH_ATTN_EXT with a mask, and MUL_MAT of a few columns.
+ *
+ * The cache: k and v pools [n_pages][Hkv][page_size][D] of 16-bit values
+ * (B2Q_TYPE_F16 or B2Q_TYPE_BF16; 16-byte aligned), page_size a power of two from 16 to 256.  A slot
+ * number is page * page_size + token in page.  A block table has one int32 row
+ * per request (table_row_stride_bytes apart): entry j is the page of tokens
+ * j * page_size .. , -1 (or any number outside the pool) for none.
+ * Page sizes, D and types outside these return B2Q_ERR_UNSUPPORTED.
+ *
+ * b2q_kv_cache_plan: from each request's cached and new token counts (device
+ * int32 [B]; negative counts as 0), in one launch:
+ *   block_table[b][j]  for the new pages ceil(cached/ps) <= j < ceil((cached+new)/ps)
+ *                      the next entries of free_pages, requests in order; -1 in
+ *                      every later column; the columns before are read only
+ *   cu_new [B+1]       first new token of each request, and their number
+ *   kv_len [B]         cached + new
+ *   slots, positions   [max_tokens] of every new token, requests in order: its
+ *                      slot (int64; -1 where the free pages or the table's
+ *                      columns ran out) and its position (cached + index); -1
+ *                      past the last token
+ *   counts [2]         pages that the new tokens need (they took the first
+ *                      min(counts[0], n_free) entries of free_pages), and
+ *                      tokens left without a slot
+ * Tokens past max_tokens are not planned (cu_new and kv_len count the planned
+ * ones).  free_pages holds page numbers (>= 0).  The call does not depend on
+ * its own outputs: repeating it with the same lengths gives the same plan.  B
+ * at most 16384; slots and positions 16-byte aligned. */
+B2Q_API int b2q_kv_cache_plan(const int32_t* cached_len, const int32_t* new_len, int64_t B, int64_t page_size,
+                              const int32_t* free_pages, int64_t n_free, int32_t* block_table, int64_t table_width,
+                              int64_t table_row_stride_bytes, int64_t max_tokens, int64_t* slots, int32_t* positions,
+                              int32_t* cu_new, int32_t* kv_len, int32_t* counts, void* stream);
+/* b2q_qkv_rope_cache: fused qkv projection rows, fp32 [T][(Hq + 2 Hkv) * D]
+ * (q heads, k heads, v heads; qkv_row_stride_bytes apart, 16-byte aligned) ->
+ * q rows of out_type [T][Hq * D] (q_row_stride_bytes apart, 8-byte aligned),
+ * and k, v of token t written into slot slots[t] of the cache (a slot outside
+ * 0 .. n_pages * page_size - 1 is skipped; equal slots race).  norm = 1: the
+ * per-head RMS norm of b2q_qkv_heads on q and k first (gamma_q [Hq * D],
+ * gamma_k [Hkv * D], 16-byte aligned, either may be NULL).
+ * Rotary positions with `axes` axes (0 to 3; time, height, width or x, y, z):
+ * sections (HOST array) gives each axis its number of consecutive pairs, R in
+ * all (R <= D / 2); pair i turns by positions[axis * pos_stride + t] *
+ * inv_freq[i] (int32; fp32 [R], device).  Pair i is dims (i, i + R), or
+ * (2 i, 2 i + 1) when interleaved; dims from 2 R on are left as they are.
+ * Angles are reduced in double, everything else is fp32, rounded once. */
+B2Q_API int b2q_qkv_rope_cache(const float* qkv, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                               int64_t qkv_row_stride_bytes, int norm, const float* gamma_q, const float* gamma_k,
+                               float eps, const int32_t* positions, int64_t pos_stride, int axes,
+                               const int32_t* sections, const float* inv_freq, int interleaved, int out_type, void* q,
+                               int64_t q_row_stride_bytes, void* k_cache, void* v_cache, const int64_t* slots,
+                               int64_t n_pages, int64_t page_size, void* stream);
+/* b2q_attention_paged: each request's new tokens (rows cu_new[b] ..
+ * cu_new[b+1] - 1 of q [T][Hq * D] of `type`, which is the cache's type too)
+ * over its kv_len[b] keys, the new tokens' own included: new token i of n sits
+ * at position p = kv_len - n + i and sees key j when j < kv_len, the table has
+ * its page, j <= p (causal = 1) and, when window > 0 (causal only), j > p -
+ * window or j < sinks.  Query head h reads kv head h / (Hq / Hkv).
+ *   o[t][h*D + d] = sum_j softmax_j(scale * q . k_j) v_j
+ * Scores, maxima and sums in fp32; a row that sees no key is 0; what keys that
+ * a row does not see hold (infinities, NaN) does not reach it.  Rows of o past
+ * cu_new[B] are not written.  max_new and max_kv bound the requests' new tokens
+ * and lengths on the host (tokens past max_new are not computed; longer lengths
+ * are, only slower); nothing is read back.  q, o 16-byte aligned with strides
+ * multiples of 16 bytes; workspace 256-byte aligned, at least
+ * b2q_attention_paged_workspace_bytes of the same sizes (0: may be NULL).
+ * D is 64 or 128.  Results do not depend on timing. */
+B2Q_API size_t b2q_attention_paged_workspace_bytes(int64_t B, int64_t T, int64_t max_new, int64_t max_kv, int64_t Hq,
+                                                   int64_t Hkv, int64_t D, int causal, int64_t window, int64_t sinks);
+B2Q_API int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_bytes, const int32_t* cu_new, int64_t B,
+                                int64_t T, int64_t max_new, const void* k_cache, const void* v_cache, int64_t n_pages,
+                                int64_t page_size, const int32_t* block_table, int64_t table_width,
+                                int64_t table_row_stride_bytes, const int32_t* kv_len, int64_t max_kv, int64_t Hq,
+                                int64_t Hkv, int64_t D, float scale, int causal, int64_t window, int64_t sinks,
+                                void* o, int64_t o_row_stride_bytes, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* b2q_mul_vec: y[m][n] = sum_k w[n][k] x[m][k] (+ bias), or resid + gate *
+ * (that), for m <= 8 tokens and a 4-bit weight whose dequantized values meet
+ * the activations unrounded -- the arithmetic of b2q_dequantize +
+ * b2q_mul_mat_f32 (matmul_weight's cast, cpp_ggml/src/ss_flow_graph.cpp:13-34)
+ * without the fp32 weight, where b2q_mul_mat_prepared_q4_0 / _q4_k round x to
+ * 8 bits first.  wtype B2Q_TYPE_Q4_0: packed by b2q_weight_pack_q4_0;
+ * B2Q_TYPE_Q4_K: packed by b2q_weight_pack.  x of xtype F32, F16 or BF16, rows
+ * x_row_stride_bytes apart (aligned to its element).  Sums in fp32.  gate needs
+ * resid; resid and y the same buffer with the same stride, or disjoint. */
+B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, const void* x, int64_t m,
+                        int64_t x_row_stride_bytes, const float* bias, const float* gate, const float* resid,
+                        int64_t resid_row_stride_bytes, float* y, int64_t y_row_stride_bytes, void* stream);
 
 /* Fault-free test of the failure path: launches the GEMM of
  * b2q_mul_mat_prepared with its TMA producer withholding every stage, so the

@@ -21,7 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libb2q.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "b2q.h")
 
-TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K = 0, 1, 2, 8, 12
+TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K, TYPE_BF16 = 0, 1, 2, 8, 12, 30
 ACT_X86, ACT_REF, ACT_Q8_K = 0, 1, 2
 QK, QK_K = 32, 256
 BLOCK_BYTES = {TYPE_Q8_0: 34, TYPE_Q4_0: 18}
@@ -113,6 +113,13 @@ def _lib_obj():
             "b2q_sparse_conv_f16_planned_workspace_bytes": (SZ, [I64, I64, I64]),
             "b2q_sparse_conv_f16_planned": (I, [P, I64, I64, P, I64, P, P, P, P, SZ, P]),
             "b2q_sparse_scatter_mean_f16_planned": (I, [P, I64, I64, P, P, I64, P, P]),
+            "b2q_kv_cache_plan": (I, [P, P, I64, I64, P, I64, P, I64, I64, I64, P, P, P, P, P, P]),
+            "b2q_qkv_rope_cache": (I, [P, I64, I64, I64, I64, I64, I, P, P, ctypes.c_float, P, I64, I, P, P, I, I, P,
+                                       I64, P, P, P, I64, I64, P]),
+            "b2q_attention_paged_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64, I64, I, I64, I64]),
+            "b2q_attention_paged": (I, [I, P, I64, P, I64, I64, I64, P, P, I64, I64, P, I64, I64, P, I64, I64, I64,
+                                        I64, ctypes.c_float, I, I64, I64, P, I64, P, SZ, P]),
+            "b2q_mul_vec": (I, [I, P, I64, I64, I, P, I64, I64, P, P, P, I64, P, I64, P]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -721,6 +728,129 @@ def mul_mat_q_simt(wtype: int, w, a, k: int, stream=None):
                                   _ptr(y), y.stride(0) * 4, _stream(stream))
     _check("b2q_mul_mat_q_simt", rc)
     return y
+
+
+def _type16(dtype) -> int:
+    torch = _torch()
+    assert dtype in (torch.float16, torch.bfloat16)
+    return TYPE_F16 if dtype == torch.float16 else TYPE_BF16
+
+
+def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_tokens: int, out=None, stream=None):
+    """Pages, slots and positions of each request's new tokens in a paged cache:
+    cached, new int32 [B], free_pages int32 [F], block_table int32 [B, W] (its
+    columns past the cached pages are written) -> (slots int64 [max_tokens],
+    positions int32 [max_tokens], cu_new int32 [B+1], kv_len int32 [B],
+    counts int32 [2]: pages needed, tokens without a slot).  out: those five
+    tensors, to be written again."""
+    torch = _torch()
+    B, W = block_table.shape
+    for t in (cached, new, free_pages, block_table):
+        assert t.dtype == torch.int32
+    assert cached.shape == (B,) and new.shape == (B,) and (B == 0 or W <= 1 or block_table.stride(1) == 1)
+    assert cached.is_contiguous() and new.is_contiguous() and free_pages.is_contiguous()
+    if out is None:
+        e = lambda n, dt: torch.empty(n, dtype=dt, device=block_table.device)  # noqa: E731
+        out = (e(max_tokens, torch.int64), e(max_tokens, torch.int32), e(B + 1, torch.int32), e(B, torch.int32),
+               e(2, torch.int32))
+    slots, positions, cu, kv_len, counts = out
+    rc = lib().b2q_kv_cache_plan(_ptr(cached), _ptr(new), B, page_size, _ptr(free_pages), free_pages.numel(),
+                                 _ptr(block_table), W, max(block_table.stride(0), W) * 4, max_tokens, _ptr(slots),
+                                 _ptr(positions), _ptr(cu), _ptr(kv_len), _ptr(counts), _stream(stream))
+    _check("b2q_kv_cache_plan", rc)
+    return out
+
+
+def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq, slots, k_cache, v_cache,
+                   norm: bool = False, gamma_q=None, gamma_k=None, eps: float = 1e-6, interleaved: bool = False,
+                   out=None, stream=None):
+    """fused qkv rows fp32 [T, (Hq + 2 Hkv) * D] -> q rows [T, Hq * D] of the
+    cache's type, with rotary positions (int32 [axes, T]; sections: pairs per
+    axis; inv_freq fp32 [sum(sections)]) on q and k after an optional per-head
+    RMS norm; k and v go to slots (int64 [T]) of k_cache, v_cache
+    [pages, Hkv, page size, D], in place."""
+    torch = _torch()
+    T = qkv.shape[0]
+    axes = len(sections)
+    assert qkv.dtype == torch.float32 and qkv.shape[1] == (Hq + 2 * Hkv) * D and qkv.stride(1) == 1
+    assert k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype
+    assert k_cache.shape[1] == Hkv and k_cache.shape[3] == D and k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert slots.dtype == torch.int64 and slots.shape == (T,) and slots.is_contiguous()
+    if axes:
+        assert positions.dtype == torch.int32 and positions.shape == (axes, T) and (T <= 1 or positions.stride(1) == 1)
+        assert inv_freq.dtype == torch.float32 and inv_freq.numel() == sum(sections) and inv_freq.is_contiguous()
+    if out is None:
+        out = torch.empty((T, Hq * D), dtype=k_cache.dtype, device=qkv.device)
+    assert out.dtype == k_cache.dtype
+    sec = (ctypes.c_int32 * max(axes, 1))(*sections)
+    rc = lib().b2q_qkv_rope_cache(_ptr(qkv), T, Hq, Hkv, D, qkv.stride(0) * 4, 1 if norm else 0, _ptr(gamma_q),
+                                  _ptr(gamma_k), eps, _ptr(positions) if axes else None,
+                                  positions.stride(0) if axes > 1 else T, axes, sec,
+                                  _ptr(inv_freq) if axes else None, 1 if interleaved else 0, _type16(k_cache.dtype),
+                                  _ptr(out), out.stride(0) * 2, _ptr(k_cache), _ptr(v_cache), _ptr(slots),
+                                  k_cache.shape[0], k_cache.shape[2], _stream(stream))
+    _check("b2q_qkv_rope_cache", rc)
+    return out
+
+
+def attention_paged_workspace_bytes(B: int, T: int, max_new: int, max_kv: int, Hq: int, Hkv: int, D: int,
+                                    causal: bool = True, window: int = 0, sinks: int = 0) -> int:
+    return lib().b2q_attention_paged_workspace_bytes(B, T, max_new, max_kv, Hq, Hkv, D, 1 if causal else 0, window,
+                                                     sinks)
+
+
+def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: int, max_kv: int, Hq: int,
+                    scale: float | None = None, causal: bool = True, window: int = 0, sinks: int = 0, out=None,
+                    ws=None, stream=None):
+    """New tokens' rows q [T, Hq * D] (request b's at cu_new[b] .. cu_new[b+1])
+    over the kv_len[b] cached keys of [pages, Hkv, page size, D] pools through
+    block_table int32 [B, W] -> [T, Hq * D].  window > 0 keeps the last `window`
+    keys and the first `sinks`; max_new / max_kv bound the requests."""
+    import math
+    torch = _torch()
+    T = q.shape[0]
+    n_pages, Hkv, page_size, D = k_cache.shape
+    B, W = block_table.shape
+    assert q.dtype == k_cache.dtype == v_cache.dtype and k_cache.shape == v_cache.shape
+    assert q.shape[1] == Hq * D and q.stride(1) == 1
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and (W <= 1 or block_table.stride(1) == 1)
+    assert block_table.dtype == kv_len.dtype == cu_new.dtype == torch.int32
+    assert kv_len.shape == (B,) and cu_new.shape == (B + 1,) and kv_len.is_contiguous() and cu_new.is_contiguous()
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if out is None:
+        out = torch.empty((T, Hq * D), dtype=q.dtype, device=q.device)
+    if ws is None:
+        need = attention_paged_workspace_bytes(B, T, max_new, max_kv, Hq, Hkv, D, causal, window, sinks)
+        ws = _empty_aligned(need, q.device) if need else None
+    rc = lib().b2q_attention_paged(_type16(q.dtype), _ptr(q), q.stride(0) * 2, _ptr(cu_new), B, T, max_new,
+                                   _ptr(k_cache), _ptr(v_cache), n_pages, page_size, _ptr(block_table), W,
+                                   max(block_table.stride(0), W) * 4, _ptr(kv_len), max_kv, Hq, Hkv, D, scale,
+                                   1 if causal else 0, window, sinks, _ptr(out), out.stride(0) * 2, _ptr(ws),
+                                   ws.numel() if ws is not None else 0, _stream(stream))
+    _check("b2q_attention_paged", rc)
+    return out
+
+
+MUL_VEC_MAX_M = 8
+
+
+def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=None, out=None, stream=None):
+    """At most 8 rows x [m, k] (fp32, fp16 or bf16) times a 4-bit weight
+    (TYPE_Q4_0 from weight_pack_q4_0, TYPE_Q4_K from weight_pack) taken at its
+    dequantized values -> fp32 [m, n]; with resid: resid + gate * (w.x + bias)
+    (out=resid updates in place)."""
+    torch = _torch()
+    m = x.shape[0]
+    assert x.shape[1] == k and (k <= 1 or x.stride(1) == 1)
+    xtype = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}[x.dtype]
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.float32, device=x.device)
+    rc = lib().b2q_mul_vec(wtype, _ptr(packed), n, k, xtype, _ptr(x), m, x.stride(0) * x.element_size(), _ptr(bias),
+                           _ptr(gate), _ptr(resid), resid.stride(0) * 4 if resid is not None else 0, _ptr(out),
+                           out.stride(0) * 4, _stream(stream))
+    _check("b2q_mul_vec", rc)
+    return out
 
 
 def device_status(clear: bool = True) -> int:

@@ -1159,4 +1159,225 @@ int b2q_device_status(unsigned int* code, int clear) {
   return *code ? B2Q_ERR_DEVICE : B2Q_OK;
 }
 
+// ------------------------------------------------------------ cached decoding
+
+// Page sizes of the cache: powers of two from 16 to 256 tokens.
+static int page_shift_of(int64_t page_size) {
+  for (int sh = 4; sh <= 8; ++sh)
+    if (page_size == (int64_t{1} << sh)) return sh;
+  return -1;
+}
+
+int b2q_kv_cache_plan(const int32_t* cached_len, const int32_t* new_len, int64_t B, int64_t page_size,
+                      const int32_t* free_pages, int64_t n_free, int32_t* block_table, int64_t table_width,
+                      int64_t table_row_stride_bytes, int64_t max_tokens, int64_t* slots, int32_t* positions,
+                      int32_t* cu_new, int32_t* kv_len, int32_t* counts, void* stream) {
+  if (B < 0 || n_free < 0 || table_width < 0 || max_tokens < 0) return B2Q_ERR_INVALID_ARG;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return B2Q_ERR_UNSUPPORTED;
+  if (B > kPlanMaxB || n_free > INT_MAX || table_width > INT_MAX || max_tokens > INT_MAX) return B2Q_ERR_TOO_LARGE;
+  if (table_row_stride_bytes < table_width * 4) return B2Q_ERR_INVALID_ARG;
+  if (!cu_new || !counts || (B > 0 && (!cached_len || !new_len || !kv_len)) || (n_free > 0 && !free_pages) ||
+      (B > 0 && table_width > 0 && !block_table) || (max_tokens > 0 && (!slots || !positions)))
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(cached_len, 4) || !aligned(new_len, 4) || !aligned(free_pages, 4) || !aligned(block_table, 4) ||
+      table_row_stride_bytes % 4 != 0 || !aligned(slots, 16) || !aligned(positions, 16) || !aligned(cu_new, 4) ||
+      !aligned(kv_len, 4) || !aligned(counts, 4))
+    return B2Q_ERR_MISALIGNED;
+  int sms = 0;
+  if (int rc = check_device(&sms)) return rc;
+  return from_cuda(launch_kv_plan(cached_len, new_len, B, shift, free_pages, n_free, block_table, table_width,
+                                  table_row_stride_bytes / 4, max_tokens, slots, positions, cu_new, kv_len, counts,
+                                  sms, static_cast<cudaStream_t>(stream)));
+}
+
+int b2q_qkv_rope_cache(const float* qkv, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t qkv_row_stride_bytes,
+                       int norm, const float* gamma_q, const float* gamma_k, float eps, const int32_t* positions,
+                       int64_t pos_stride, int axes, const int32_t* sections, const float* inv_freq, int interleaved,
+                       int out_type, void* q, int64_t q_row_stride_bytes, void* k_cache, void* v_cache,
+                       const int64_t* slots, int64_t n_pages, int64_t page_size, void* stream) {
+  if (T < 0 || Hq < 0 || Hkv < 0 || Hq + Hkv <= 0 || n_pages < 0 || (norm != 0 && norm != 1) ||
+      (interleaved != 0 && interleaved != 1) || (norm && !(eps >= 0.0f)))
+    return B2Q_ERR_INVALID_ARG;
+  if (D != 64 && D != 128) return B2Q_ERR_UNSUPPORTED;
+  if (out_type != B2Q_TYPE_F16 && out_type != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return B2Q_ERR_UNSUPPORTED;
+  if (axes < 0 || axes > 3 || (axes > 0 && !sections)) return B2Q_ERR_INVALID_ARG;
+  int64_t rot = 0, start[4] = {0, 0, 0, 0};
+  for (int i = 0; i < axes; ++i) {
+    if (sections[i] < 0) return B2Q_ERR_INVALID_ARG;
+    start[i] = rot;
+    rot += sections[i];
+  }
+  if (rot > D / 2) return B2Q_ERR_INVALID_ARG;
+  if (T > INT_MAX || Hq > 4096 || Hkv > 4096 || n_pages > INT_MAX) return B2Q_ERR_TOO_LARGE;
+  if (T > 0 && (!qkv || (Hq > 0 && !q) || (Hkv > 0 && (!k_cache || !v_cache || !slots)) ||
+                (rot > 0 && (!positions || !inv_freq))))
+    return B2Q_ERR_INVALID_ARG;
+  if (qkv_row_stride_bytes < (Hq + 2 * Hkv) * D * 4 || (Hq > 0 && q_row_stride_bytes < Hq * D * 2) ||
+      (axes > 1 && pos_stride < T))
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(qkv, 16) || qkv_row_stride_bytes % 16 != 0 || (Hq > 0 && (!aligned(q, 8) || q_row_stride_bytes % 8 != 0)) ||
+      !aligned(k_cache, 8) || !aligned(v_cache, 8) || !aligned(gamma_q, 16) || !aligned(gamma_k, 16) ||
+      !aligned(positions, 4) || !aligned(inv_freq, 4) || !aligned(slots, 8))
+    return B2Q_ERR_MISALIGNED;
+  if (T == 0) return B2Q_OK;
+  int sms = 0;
+  if (int rc = check_device(&sms)) return rc;
+  RopeArgs a{};
+  a.qkv = qkv;
+  a.T = T;
+  a.ldqkv = qkv_row_stride_bytes / 4;
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.norm = norm;
+  a.eps = eps;
+  a.gamma_q = norm ? gamma_q : nullptr;
+  a.gamma_k = norm ? gamma_k : nullptr;
+  a.pos = positions;
+  a.ldpos = pos_stride;
+  a.sec1 = static_cast<int>(axes > 1 ? start[1] : rot);
+  a.sec2 = static_cast<int>(axes > 2 ? start[2] : rot);
+  a.rot = static_cast<int>(rot);
+  a.inv_freq = inv_freq;
+  a.interleaved = interleaved;
+  a.q = static_cast<uint16_t*>(q);
+  a.ldq = q_row_stride_bytes / 2;
+  a.k_cache = static_cast<uint16_t*>(k_cache);
+  a.v_cache = static_cast<uint16_t*>(v_cache);
+  a.slots = slots;
+  a.n_slots = n_pages << shift;
+  a.page_shift = shift;
+  return from_cuda(launch_rope_cache(a, static_cast<int>(D), out_type == B2Q_TYPE_BF16, sms,
+                                     static_cast<cudaStream_t>(stream)));
+}
+
+// The arguments that size an attention over the paged cache.
+static int paged_sizes(int64_t B, int64_t T, int64_t max_new, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,
+                       int causal, int64_t window, int64_t sinks) {
+  if (B < 0 || T < 0 || max_new < 0 || max_kv < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || window < 0 || sinks < 0 ||
+      (causal != 0 && causal != 1) || (!causal && window > 0))
+    return B2Q_ERR_INVALID_ARG;
+  if (D != 64 && D != 128) return B2Q_ERR_UNSUPPORTED;
+  if (B > 65535 || Hkv > 65535 || Hq > 65535 || T > INT_MAX || max_new > INT_MAX || max_kv > INT_MAX ||
+      window > INT_MAX || sinks > INT_MAX || max_new * Hq > INT_MAX)
+    return B2Q_ERR_TOO_LARGE;
+  return B2Q_OK;
+}
+
+size_t b2q_attention_paged_workspace_bytes(int64_t B, int64_t T, int64_t max_new, int64_t max_kv, int64_t Hq,
+                                           int64_t Hkv, int64_t D, int causal, int64_t window, int64_t sinks) {
+  if (paged_sizes(B, T, max_new, max_kv, Hq, Hkv, D, causal, window, sinks) != B2Q_OK) return 0;
+  const PagedPlan p = paged_plan(B, T, max_new, max_kv, Hq, Hkv, D, causal != 0, window, sinks);
+  return static_cast<size_t>(p.part_o_bytes + p.part_ml_bytes);
+}
+
+int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_bytes, const int32_t* cu_new, int64_t B,
+                        int64_t T, int64_t max_new, const void* k_cache, const void* v_cache, int64_t n_pages,
+                        int64_t page_size, const int32_t* block_table, int64_t table_width,
+                        int64_t table_row_stride_bytes, const int32_t* kv_len, int64_t max_kv, int64_t Hq, int64_t Hkv,
+                        int64_t D, float scale, int causal, int64_t window, int64_t sinks, void* o,
+                        int64_t o_row_stride_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  if (type != B2Q_TYPE_F16 && type != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
+  if (int rc = paged_sizes(B, T, max_new, max_kv, Hq, Hkv, D, causal, window, sinks)) return rc;
+  if (!std::isfinite(scale) || n_pages < 0 || table_width < 0) return B2Q_ERR_INVALID_ARG;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return B2Q_ERR_UNSUPPORTED;
+  if (n_pages > INT_MAX || table_width > (INT_MAX >> shift)) return B2Q_ERR_TOO_LARGE;
+  const bool any = B > 0 && T > 0 && max_new > 0;
+  if (any && (!q || !o || !cu_new || !kv_len || (table_width > 0 && !block_table) ||
+              (n_pages > 0 && table_width > 0 && (!k_cache || !v_cache))))
+    return B2Q_ERR_INVALID_ARG;
+  if (q_row_stride_bytes < Hq * D * 2 || o_row_stride_bytes < Hq * D * 2 || table_row_stride_bytes < table_width * 4)
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(q, 16) || q_row_stride_bytes % 16 != 0 || !aligned(o, 16) || o_row_stride_bytes % 16 != 0 ||
+      !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(cu_new, 4) || !aligned(kv_len, 4) ||
+      !aligned(block_table, 4) || table_row_stride_bytes % 4 != 0 || !aligned(workspace, 256))
+    return B2Q_ERR_MISALIGNED;
+  if (!any) return B2Q_OK;
+  const PagedPlan p = paged_plan(B, T, max_new, max_kv, Hq, Hkv, D, causal != 0, window, sinks);
+  if (p.part_o_bytes > 0 &&
+      (!workspace || workspace_bytes < static_cast<size_t>(p.part_o_bytes + p.part_ml_bytes)))
+    return B2Q_ERR_WORKSPACE;
+  if (int rc = check_device(nullptr)) return rc;
+  PagedArgs a{};
+  a.q = q;
+  a.ldq = q_row_stride_bytes / 2;
+  a.T = T;
+  a.max_q = max_new;
+  a.B = B;
+  a.cu_q = cu_new;
+  a.kv_len = kv_len;
+  a.table = block_table;
+  a.width = table_width;
+  a.ldt = table_row_stride_bytes / 4;
+  a.k = static_cast<const uint16_t*>(k_cache);
+  a.v = static_cast<const uint16_t*>(v_cache);
+  a.n_pages = n_pages;
+  a.page_shift = shift;
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.G = static_cast<int>(Hq / Hkv);
+  a.c2 = scale * 1.4426950408889634f;  // log2(e)
+  a.causal = causal;
+  a.window = window;
+  a.sinks = sinks;
+  a.o = o;
+  a.ldo = o_row_stride_bytes / 2;
+  a.splits = static_cast<int>(p.splits);
+  a.split_units = p.split_units;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.part_o_bytes);
+  return from_cuda(
+      launch_attention_paged(a, static_cast<int>(D), type == B2Q_TYPE_BF16, static_cast<cudaStream_t>(stream)));
+}
+
+int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, const void* x, int64_t m,
+                int64_t x_row_stride_bytes, const float* bias, const float* gate, const float* resid,
+                int64_t resid_row_stride_bytes, float* y, int64_t y_row_stride_bytes, void* stream) {
+  if (wtype != B2Q_TYPE_Q4_0 && wtype != B2Q_TYPE_Q4_K) return B2Q_ERR_UNSUPPORTED;
+  if (xtype != B2Q_TYPE_F32 && xtype != B2Q_TYPE_F16 && xtype != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
+  const bool q4k = wtype == B2Q_TYPE_Q4_K;
+  const int xs = xtype == B2Q_TYPE_F32 ? 4 : 2;
+  if (n < 0 || m < 0 || k <= 0 || k % (q4k ? kQKK : kQK) != 0 || (gate && !resid)) return B2Q_ERR_INVALID_ARG;
+  if (n > INT_MAX || k > INT_MAX || m > kMulVecMaxM) return B2Q_ERR_TOO_LARGE;
+  if (m > 0 && n > 0 && (!packed || !x || !y)) return B2Q_ERR_INVALID_ARG;
+  if (x_row_stride_bytes < k * xs || y_row_stride_bytes < n * 4 || (resid && resid_row_stride_bytes < n * 4))
+    return B2Q_ERR_INVALID_ARG;
+  if (resid && resid == y && resid_row_stride_bytes != y_row_stride_bytes) return B2Q_ERR_INVALID_ARG;
+  if (!aligned(packed, 256) || !aligned(x, xs) || x_row_stride_bytes % xs != 0 || !aligned(y, 4) ||
+      y_row_stride_bytes % 4 != 0 || (resid && (!aligned(resid, 4) || resid_row_stride_bytes % 4 != 0)) ||
+      (bias && !aligned(bias, 4)) || (gate && !aligned(gate, 4)))
+    return B2Q_ERR_MISALIGNED;
+  if (m == 0 || n == 0) return B2Q_OK;
+  int sms = 0;
+  if (int rc = check_device(&sms)) return rc;
+  MulVecArgs a{};
+  if (q4k) {
+    const Q4kWeight w = q4k_at(static_cast<uint8_t*>(const_cast<void*>(packed)), n, k);
+    a.w = w.raw;
+    a.row_bytes = w.row_bytes;
+  } else {
+    const Q4cWeight w = q4c_at(static_cast<uint8_t*>(const_cast<void*>(packed)), n, k);
+    a.w = w.nibbles;
+    a.row_bytes = k / 2;
+    a.scales = w.scales;
+    a.lds = w.ld;
+  }
+  a.x = x;
+  a.ldx = x_row_stride_bytes / xs;
+  a.N = n;
+  a.K = k;
+  a.M = static_cast<int>(m);
+  a.bias = bias;
+  a.gate = gate;
+  a.resid = resid;
+  a.ldr = resid ? resid_row_stride_bytes / 4 : 0;
+  a.y = y;
+  a.ldy = y_row_stride_bytes / 4;
+  const int xt = xtype == B2Q_TYPE_F32 ? kXF32 : xtype == B2Q_TYPE_F16 ? kXF16 : kXBF16;
+  return from_cuda(launch_mul_vec(a, q4k, xt, sms, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -291,4 +291,79 @@ constexpr int64_t kGemvMaxM = 8;
 cudaError_t launch_gemv(const GemmArgs& args, cudaStream_t s);
 cudaError_t read_device_status(unsigned int* value, bool clear);
 
+// ---- cached decoding: page plan, rope + cache append, paged attention, 4-bit few-token product ----
+constexpr int64_t kPlanMaxB = 16384;  // requests of one plan (two ints each in shared memory)
+cudaError_t launch_kv_plan(const int32_t* cached, const int32_t* fresh, int64_t B, int page_shift,
+                           const int32_t* free_pages, int64_t n_free, int32_t* table, int64_t width, int64_t ldt,
+                           int64_t max_tokens, int64_t* slots, int32_t* pos, int32_t* cu, int32_t* kv_len,
+                           int32_t* counts, int num_sms, cudaStream_t s);
+
+struct RopeArgs {
+  const float* qkv;  // [T] rows of (Hq + 2 Hkv) * D, ldqkv floats apart
+  int64_t T, ldqkv;
+  int Hq, Hkv;
+  int norm;          // RMS norm of every q and k head before the rotation
+  float eps;
+  const float *gamma_q, *gamma_k;  // [H * D] or nullptr
+  const int32_t* pos;              // [axes][ldpos]
+  int64_t ldpos;
+  int sec1, sec2, rot;             // first pair of axis 1 and of axis 2 (rot where absent); pairs rotated
+  const float* inv_freq;           // [rot]
+  int interleaved;
+  uint16_t* q;                     // [T] rows, ldq elements apart
+  int64_t ldq;
+  uint16_t *k_cache, *v_cache;     // [pages][Hkv][page][D]
+  const int64_t* slots;
+  int64_t n_slots;                 // pages * page size
+  int page_shift;
+};
+cudaError_t launch_rope_cache(const RopeArgs& a, int D, bool bf16, int num_sms, cudaStream_t s);
+
+struct PagedArgs {
+  const void* q;  // [T] rows of Hq * D 16-bit values, ldq elements apart
+  int64_t ldq, T, max_q;
+  int64_t B;
+  const int32_t* cu_q;    // [B + 1]
+  const int32_t* kv_len;  // [B]
+  const int32_t* table;   // [B] rows of width entries, ldt apart
+  int64_t width, ldt;
+  const uint16_t *k, *v;  // [n_pages][Hkv][page][D]
+  int64_t n_pages;
+  int page_shift;
+  int Hq, Hkv, G;         // G = Hq / Hkv
+  float c2;               // scale * log2(e)
+  int causal;
+  int64_t window, sinks;  // window 0: no limit
+  void* o;
+  int64_t ldo;
+  // Keys split into stretches of split_units units (a padding of 1 stretch: no join).
+  int splits;
+  int64_t split_units;
+  float* part_o;          // [T][Hq][splits][D]
+  float2* part_ml;        // [T][Hq][splits] (max, sum)
+};
+struct PagedPlan {
+  int64_t splits = 1, split_units = 0, part_o_bytes = 0, part_ml_bytes = 0;
+};
+PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,
+                     bool causal, int64_t window, int64_t sinks);
+cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, cudaStream_t s);
+
+constexpr int kMulVecMaxM = 8;
+enum { kXF32 = 0, kXF16 = 1, kXBF16 = 2 };
+struct MulVecArgs {
+  const uint8_t* w;        // Q4_0: nibbles [N][K/2]; Q4_K: GGUF rows
+  const uint16_t* scales;  // Q4_0: fp16 [K/32][lds]
+  int64_t lds, row_bytes;
+  const void* x;           // [M] rows, ldx elements apart
+  int64_t ldx;
+  int64_t N, K;
+  int M;
+  const float *bias, *gate, *resid;
+  int64_t ldr;
+  float* y;
+  int64_t ldy;
+};
+cudaError_t launch_mul_vec(const MulVecArgs& a, bool q4k, int xt, int num_sms, cudaStream_t s);
+
 }  // namespace b2q

@@ -620,7 +620,10 @@ B2Q_API int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_by
  * without the fp32 weight, where b2q_mul_mat_prepared_q4_0 / _q4_k round x to
  * 8 bits first.  wtype B2Q_TYPE_Q4_0: packed by b2q_weight_pack_q4_0;
  * B2Q_TYPE_Q4_K: packed by b2q_weight_pack.  x of xtype F32, F16 or BF16, rows
- * x_row_stride_bytes apart (aligned to its element).  Sums in fp32.  gate needs
+ * x_row_stride_bytes apart (aligned to its element).  x is held to 2^-23 of the
+ * largest magnitude of its 32-value block or better, sums are fp32; |x| < 2^112
+ * (beyond that, sums overflow early; a token with an infinity or a NaN gives
+ * NaN).  gate needs
  * resid; resid and y the same buffer with the same stride, or disjoint. */
 B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, const void* x, int64_t m,
                         int64_t x_row_stride_bytes, const float* bias, const float* gate, const float* resid,

@@ -1341,7 +1341,7 @@ int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, 
   const bool q4k = wtype == B2Q_TYPE_Q4_K;
   const int xs = xtype == B2Q_TYPE_F32 ? 4 : 2;
   if (n < 0 || m < 0 || k <= 0 || k % (q4k ? kQKK : kQK) != 0 || (gate && !resid)) return B2Q_ERR_INVALID_ARG;
-  if (n > INT_MAX || k > INT_MAX || m > kMulVecMaxM) return B2Q_ERR_TOO_LARGE;
+  if (n > INT_MAX || k > (1 << 28) || m > kMulVecMaxM) return B2Q_ERR_TOO_LARGE;
   if (m > 0 && n > 0 && (!packed || !x || !y)) return B2Q_ERR_INVALID_ARG;
   if (x_row_stride_bytes < k * xs || y_row_stride_bytes < n * 4 || (resid && resid_row_stride_bytes < n * 4))
     return B2Q_ERR_INVALID_ARG;

@@ -18,13 +18,14 @@
 // exact in int32; they are read as fp32 through an accumulator that starts at
 // the bits of 1.5 * 2^23 (|sum| < 2^22), scaled and added in fp32.
 //
-// One CTA per SM, 16 warps.  The activations of a run of K ("chunk") are split
+// One CTA per SM, 16 or 24 warps.  The activations of a run of K ("chunk") are split
 // into digits once per CTA and stay in shared memory; then the CTA walks its
 // row tiles.  A warp's unit is 16 rows x 256 values, fetched with cp.async into
 // the warp's own ring: no barrier inside a tile.  The warps of a tile share out
-// its units (WK of them; the other factor of 16, WR, is row tiles side by
+// its units (WK of them; the other factor, WR, is row tiles side by
 // side) and are summed at its end in a fixed order.
-//   up to 2 tokens (WIDE false): the 8 columns of one product are token x digit
+//   up to 2 tokens (WIDE false): a token's columns are (p0, p1, -, p2), so a
+//     lane's pair of sums is 256 p0 + p1, or p2: one number to scale
 //   3 to 8 tokens (WIDE true): one product per digit, columns are tokens
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
@@ -36,15 +37,25 @@ namespace b2q {
 
 namespace {
 
-constexpr int kMvWarps = 16, kMvThreads = kMvWarps * 32;
-constexpr int kMvStages = 3;
 constexpr int kMvUnitK = 256;
-constexpr int kMvUnitBytes = 16 * 144;   // Q4_K: 16 rows of a super-block; Q4_0: 2048 of nibbles + 256 of scales
-constexpr int kMvTiles = 32;             // row tiles whose sums a CTA keeps while it walks the chunks
-constexpr int kMvXBytes = 76 * 1024;     // shared memory for a chunk's activations
-constexpr int kMvRing = kMvWarps * kMvStages * kMvUnitBytes;
-constexpr int kMvRed = 2 * kMvWarps * 16 * 8 * 4;
-constexpr int kMvAcc = kMvTiles * 16 * kMulVecMaxM * 4;
+// A stage: Q4_K 16 super-blocks of 144 bytes; Q4_0 16 rows of 128 bytes of
+// nibbles, 16-byte chunks swizzled, and 8 x 16 fp16 scales.  A lane's rows of a
+// tile are neighbours: the 8-byte reads of rows 0, 2, 4, 6 (288 bytes apart)
+// then meet all banks, and two rows' Q4_0 scales are one word.
+constexpr int kMvUnitBytes = 16 * kQ4KBytes;
+constexpr int kMvSmem = 227 * 1024;
+// The sums of 3 to 8 tokens take more registers a warp, so 16 warps and one more stage each.
+template <bool WIDE>
+struct MvShape {
+  static constexpr int WARPS = WIDE ? 16 : 24, THREADS = WARPS * 32;
+  static constexpr int STAGES = WIDE ? 3 : 2;
+  static constexpr int TILES = 32;                           // row tiles whose sums a CTA keeps over the chunks
+  static constexpr int RING = WARPS * STAGES * kMvUnitBytes;
+  static constexpr int SCALES = WARPS * 8 * 16 * 4;          // Q4_K: a unit's d * sc per warp
+  static constexpr int RED = 2 * WARPS * 16 * (WIDE ? 8 : 4) * 4;
+  static constexpr int ACC = TILES * 16 * (WIDE ? 8 : 2) * 4;
+  static constexpr int X = kMvSmem - RING - SCALES - RED - ACC;  // a chunk's activations
+};
 constexpr int kMvMagic = 0x4B400000;     // bits of 1.5 * 2^23
 
 struct MvPlan {
@@ -91,18 +102,19 @@ __device__ __forceinline__ float pow2(int e) {
   return e >= -126 ? __int_as_float((e + 127) << 23) : __int_as_float(1 << (e + 149));
 }
 
+// All four sums start at `init`.
 template <bool UNSIGNED_A>
-__device__ __forceinline__ void mma_i8_16832(int (&d)[4], const uint32_t (&a)[4], uint2 b) {
+__device__ __forceinline__ void mma_i8_16832(int (&d)[4], const uint32_t (&a)[4], uint2 b, int init) {
   if constexpr (UNSIGNED_A)
     asm volatile(
         "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kMvMagic));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(init));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kMvMagic));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(init));
 }
 
 __device__ __forceinline__ void mv_cp16(uint32_t dst, const void* src, bool real) {
@@ -110,99 +122,104 @@ __device__ __forceinline__ void mv_cp16(uint32_t dst, const void* src, bool real
 }
 
 template <bool Q4K, bool WIDE, int XT>
-__global__ void __launch_bounds__(kMvThreads, 1) mul_vec_kernel(const MulVecArgs a, const MvPlan p) {
+__global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(const MulVecArgs a, const MvPlan p) {
+  using S = MvShape<WIDE>;
   extern __shared__ __align__(128) uint8_t mv_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int WK = 1 << p.wk_shift, WR = kMvWarps >> p.wk_shift;
+  const int WK = 1 << p.wk_shift, WR = S::WARPS >> p.wk_shift;
   const int wk = warp & (WK - 1), wr = warp >> p.wk_shift;
-  const int cols = 3 * a.M;
-  uint8_t* ring = mv_smem + warp * kMvStages * kMvUnitBytes;
+  const int row0 = 2 * g, row1 = 2 * g + 1;  // of a tile
+  uint8_t* ring = mv_smem + warp * S::STAGES * kMvUnitBytes;
   const uint32_t ring_a = smem_u32(ring);
-  float* red = reinterpret_cast<float*>(mv_smem + kMvRing);          // [2][warp][16][8]
-  float* acc_s = reinterpret_cast<float*>(mv_smem + kMvRing + kMvRed);  // [tile][16][M]
-  uint8_t* xs = mv_smem + kMvRing + kMvRed + kMvAcc;
-  uint8_t* digits = xs;                                              // [col][pitch], digit-major columns when WIDE
-  const int nb_chunk = p.chunk_units * (kMvUnitK / 32);
-  // per block: WIDE: s of each token; else s times the digit's weight of each column
-  float* tab = reinterpret_cast<float*>(xs + static_cast<int64_t>(cols) * p.pitch);
-  float* sums = tab + nb_chunk * 8;                    // Q4_K: sum of x per token (WIDE) or column
+  float* scales = reinterpret_cast<float*>(mv_smem + S::RING) + warp * 128;  // [block % 4][block / 4][row]
+  float* red = reinterpret_cast<float*>(mv_smem + S::RING + S::SCALES);        // [2][warp][16][8 or 4]
+  float* acc_s = reinterpret_cast<float*>(mv_smem + S::RING + S::SCALES + S::RED);  // [tile][16][M]
+  uint8_t* digits = mv_smem + S::RING + S::SCALES + S::RED + S::ACC;  // [digit][token] (WIDE), [token][digit]; pitch
+  // per token, the chunk's blocks: s; then (Q4_K) the sum of the block's x
+  const int nb_pitch = p.chunk_units * (kMvUnitK / 32) + 4;  // floats; tokens meet different banks
+  float* tab = reinterpret_cast<float*>(digits + 3 * a.M * p.pitch);
+  float* sums = tab + a.M * nb_pitch;
+  constexpr int TC = WIDE ? 8 : 4;
 
-  const int64_t own = blockIdx.x < p.supers ? (p.supers - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
-  const int group = kMvTiles / WR;  // super-tiles whose sums are kept at once (all, when there is one chunk)
-  const int64_t group_n = p.chunks == 1 ? own : group;
+  const int own = blockIdx.x < p.supers ? static_cast<int>((p.supers - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
+  const int group_n = p.chunks == 1 ? own : S::TILES / WR;  // super-tiles whose sums are kept at once
 
   // The warp's sequence of units: for each group, each chunk, each super-tile, its units of the chunk.
-  struct Seq {
-    int64_t g0, i;
-    int chunk, u;
-  };
-  auto settle = [&](Seq& s) {  // to the next unit that exists, from (g0, i, chunk, u) on
-    while (s.g0 < own) {
-      const int end = min(p.units, (s.chunk + 1) * p.chunk_units);
-      if (s.u < end) return;
-      s.u = s.chunk * p.chunk_units + wk;
-      if (++s.i >= min(own, s.g0 + group_n)) {
-        if (++s.chunk == p.chunks) {
-          s.chunk = 0;
-          s.g0 += group_n;
-        }
-        s.i = s.g0;
-        s.u = s.chunk * p.chunk_units + wk;
-      }
+  int q_g0 = 0, q_i = 0, q_chunk = 0, q_u = wk, q_end = min(p.units, p.chunk_units);
+  const uint8_t* q_src = nullptr;  // the warp's tile
+  int64_t q_n0 = 0;
+  uint32_t src_off[5];             // this lane's 16-byte pieces of a unit
+  auto enter_tile = [&] {
+    q_n0 = ((blockIdx.x + static_cast<int64_t>(q_i) * gridDim.x) * WR + wr) * 16;
+    q_n0 = min(q_n0, (a.N - 1) / 16 * 16);  // (a tile past the end repeats the last one, unused)
+    q_src = a.w + q_n0 * a.row_bytes;
+    const int last = static_cast<int>(min(a.N - 1 - q_n0, int64_t{15}));
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const int x = lane + 32 * j;
+      if constexpr (Q4K)
+        src_off[j] = static_cast<uint32_t>(min(x / 9, last)) * static_cast<uint32_t>(a.row_bytes) + (x % 9) * 16;
+      else
+        src_off[j] = static_cast<uint32_t>(min(x / 8, last)) * static_cast<uint32_t>(a.row_bytes) + (x % 8) * 16;
     }
   };
-  auto load = [&](const Seq& s, int stage) {
-    if (s.g0 < own) {
-      const int64_t n0 = ((blockIdx.x + s.i * gridDim.x) * WR + wr) * 16;
+  auto settle = [&] {  // to the next unit that exists
+    while (q_u >= q_end && q_g0 < own) {
+      if (++q_i >= min(own, q_g0 + group_n)) {
+        if (++q_chunk == p.chunks) {
+          q_chunk = 0;
+          q_g0 += group_n;
+        }
+        q_i = q_g0;
+        q_end = min(p.units, (q_chunk + 1) * p.chunk_units);
+      }
+      q_u = q_chunk * p.chunk_units + wk;
+      enter_tile();
+    }
+  };
+  auto load = [&](int stage) {
+    if (q_g0 < own) {
       const uint32_t dst = ring_a + stage * kMvUnitBytes;
       if constexpr (Q4K) {
-        const uint8_t* src = a.w + n0 * a.row_bytes + static_cast<int64_t>(s.u) * kQ4KBytes;
+        const uint8_t* src = q_src + static_cast<int64_t>(q_u) * kQ4KBytes;
 #pragma unroll
-        for (int j = 0; j < 5; ++j) {
-          const int x = lane + 32 * j;
-          const int r = x / 9, ch = x - 9 * r;
-          const bool real = n0 + r < a.N;
-          if (x < 144) mv_cp16(dst + x * 16, real ? src + r * a.row_bytes + ch * 16 : a.w, real);
-        }
+        for (int j = 0; j < 4; ++j) mv_cp16(dst + (lane + 32 * j) * 16, src + src_off[j], true);
+        if (lane < 16) mv_cp16(dst + (lane + 128) * 16, src + src_off[4], true);
       } else {
-        const int64_t k2 = a.K / 2;
         const int ch = lane & 7;
-        const bool in_k = s.u * (kMvUnitK / 2) + ch * 16 < k2;
-        const uint8_t* src = a.w + static_cast<int64_t>(s.u) * (kMvUnitK / 2) + ch * 16;
+        const bool in_k = q_u * (kMvUnitK / 2) + ch * 16 < a.row_bytes;
+        const uint8_t* src = q_src + q_u * (kMvUnitK / 2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = (lane >> 3) + 4 * j;
-          const bool real = in_k && n0 + r < a.N;
-          mv_cp16(dst + r * 128 + ((ch ^ r) & 7) * 16, real ? src + (n0 + r) * k2 : a.w, real);
+          mv_cp16(dst + r * 128 + ((ch ^ (r >> 1)) & 7) * 16, in_k ? src + src_off[j] : a.w, in_k);
         }
         if (lane < 16) {
-          const int64_t blk = static_cast<int64_t>(s.u) * 8 + (lane >> 1), n8 = n0 + (lane & 1) * 8;
+          const int64_t blk = static_cast<int64_t>(q_u) * 8 + (lane >> 1), n8 = q_n0 + (lane & 1) * 8;
           const bool real = blk < a.K / 32 && n8 < a.lds;
           mv_cp16(dst + 2048 + lane * 16, real ? a.scales + blk * a.lds + n8 : a.scales, real);
         }
       }
+      q_u += WK;
+      settle();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  Seq pre{0, 0, 0, wk};
-  settle(pre);
+  enter_tile();
+  settle();
 #pragma unroll
-  for (int s = 0; s < kMvStages - 1; ++s) {
-    load(pre, s);
-    pre.u += WK;
-    settle(pre);
-  }
-  int stage = 0, fill = kMvStages - 1, buf = 0;
+  for (int s = 0; s < S::STAGES - 1; ++s) load(s);
+  int stage = 0, fill = S::STAGES - 1, buf = 0;
 
-  for (int64_t g0 = 0; g0 < own; g0 += group_n) {
+  for (int g0 = 0; g0 < own; g0 += group_n) {
     for (int chunk = 0; chunk < p.chunks; ++chunk) {
       const int cu0 = chunk * p.chunk_units, cu1 = min(p.units, cu0 + p.chunk_units);
       if (p.chunks > 1 || g0 == 0) {
         // ---- the chunk's activations: eight lanes per (token, block), four values each
         const int nb = (cu1 - cu0) * (kMvUnitK / 32);
-        for (int j = threadIdx.x >> 3; j < nb * a.M; j += kMvThreads / 8) {
+        for (int j = threadIdx.x >> 3; j < nb * a.M; j += S::THREADS / 8) {
           const int m = j / nb, b = j - m * nb, i = threadIdx.x & 7;
           const int64_t k0 = (static_cast<int64_t>(cu0) * (kMvUnitK / 32) + b) * 32 + i * 4;
           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -238,12 +255,14 @@ __global__ void __launch_bounds__(kMvThreads, 1) mul_vec_kernel(const MulVecArgs
             d1 |= (mid & 255u) << (8 * x);
             d0 |= (((hi - mid) >> 8) & 255u) << (8 * x);
           }
-          // lane c of the product reads words (4c ..) and (16 + 4c ..) together
-          const int at = b * 32 + (i & 3) * 8 + (i >> 2) * 4;
+          // Lane c of the product has values 4c .. and 16 + 4c .. (Q4_0) or 8c .. 8c + 7 (Q4_K) of
+          // a block; its pieces of two neighbouring blocks are one 16-byte word.
+          const int lc = Q4K ? i >> 1 : i & 3, half = Q4K ? i & 1 : i >> 2;
+          const int at = (b >> 1) * 64 + lc * 16 + (b & 1) * 8 + half * 4;
           const int c0 = WIDE ? m : 3 * m, cs = WIDE ? a.M : 1;
-          *reinterpret_cast<uint32_t*>(digits + static_cast<int64_t>(c0) * p.pitch + at) = d0;
-          *reinterpret_cast<uint32_t*>(digits + static_cast<int64_t>(c0 + cs) * p.pitch + at) = d1;
-          *reinterpret_cast<uint32_t*>(digits + static_cast<int64_t>(c0 + 2 * cs) * p.pitch + at) = d2;
+          *reinterpret_cast<uint32_t*>(digits + c0 * p.pitch + at) = d0;
+          *reinterpret_cast<uint32_t*>(digits + (c0 + cs) * p.pitch + at) = d1;
+          *reinterpret_cast<uint32_t*>(digits + (c0 + 2 * cs) * p.pitch + at) = d2;
           int xsum = 0;
           if constexpr (Q4K) {  // |sum| <= 32 * 2^23
             xsum = (q[0] + q[1]) + (q[2] + q[3]);
@@ -253,160 +272,168 @@ __global__ void __launch_bounds__(kMvThreads, 1) mul_vec_kernel(const MulVecArgs
           if (i == 0) {
             // Q4_0 codes go in as 16 (q - 8)
             const float s = fin ? pow2(Q4K ? e : e - 4) : __int_as_float(0x7fc00000);
-            if constexpr (WIDE) {
-              tab[b * 8 + m] = s;
-              if constexpr (Q4K) sums[b * 8 + m] = s * static_cast<float>(xsum);
-            } else {
-              tab[b * 8 + 3 * m] = s * 65536.0f;
-              tab[b * 8 + 3 * m + 1] = s * 256.0f;
-              tab[b * 8 + 3 * m + 2] = s;
-              if constexpr (Q4K) {
-                sums[b * 8 + 3 * m] = s * static_cast<float>(xsum);
-                sums[b * 8 + 3 * m + 1] = 0.0f;
-                sums[b * 8 + 3 * m + 2] = 0.0f;
-              }
-            }
+            tab[m * nb_pitch + b] = s;
+            if constexpr (Q4K) sums[m * nb_pitch + b] = s * static_cast<float>(xsum);
           }
-        }
-        // columns past the tokens: their products are scaled by 0
-        const int used = WIDE ? a.M : cols;
-        for (int j = threadIdx.x; j < nb * (8 - used); j += kMvThreads) {
-          const int b = j / (8 - used), x = used + j - b * (8 - used);
-          tab[b * 8 + x] = 0.0f;
-          if constexpr (Q4K) sums[b * 8 + x] = 0.0f;
         }
         __syncthreads();
       }
 
-      for (int64_t i = g0; i < min(own, g0 + group_n); ++i) {
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (row g, columns 2c, 2c+1), (row g + 8, ...)
-        // B operand: this lane's column is g (of the digit's eight when WIDE)
-        const uint8_t* bcol = digits + static_cast<int64_t>(WIDE ? min(g, a.M - 1) : min(g, cols - 1)) * p.pitch + c * 8;
+      // B operand: this lane's column is g
+      const int d_of_g = (g & 3) == 3 ? 2 : (g & 1);  // (p0, p1, p0 unused, p2)
+      const uint8_t* bcol =
+          digits + (WIDE ? min(g, a.M - 1) : 3 * min(g >> 2, a.M - 1) + d_of_g) * p.pitch + c * 16;
+      const int dstep = a.M * p.pitch;          // WIDE: to the next digit
+      const int mul = (c & 1) ? 0 : 256;        // narrow: weight of the first of the lane's two columns
+      // s of this lane's token (WIDE: tokens 2c and 2c + 1); columns past the tokens repeat the last one, unused
+      const float* tab0 = tab + min(WIDE ? 2 * c : c >> 1, a.M - 1) * nb_pitch;
+      const float* tab1 = tab + min(2 * c + 1, a.M - 1) * nb_pitch;
+      for (int i = g0; i < min(own, g0 + group_n); ++i) {
+        // (the first row that this warp will finish: its bias is on its way while the units run)
+        const int64_t n_first = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * WR * 16 + warp;
+        const float bias_first = a.bias && n_first < a.N ? __ldg(a.bias + n_first) : 0.0f;
+        float macc[Q4K ? (WIDE ? kMulVecMaxM : 2) : 1] = {};  // Q4_K: minima, of row lane % 16, half of the blocks
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // WIDE: (row0, tokens 2c, 2c + 1), (row1, ..); else row0, row1
         for (int u = cu0 + wk; u < cu1; u += WK) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kMvStages - 2) : "memory");
+          asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
           __syncwarp();
-          load(pre, fill);
-          pre.u += WK;
-          settle(pre);
+          load(fill);
           const uint8_t* st = ring + stage * kMvUnitBytes;
+          const uint8_t* bu = bcol + (u - cu0) * kMvUnitK;
           const int kb0 = (u - cu0) * 8;
-          // one block: A operand, scales, table row -> acc
-          auto fold = [&](const uint32_t (&af)[4], int kb, float ds0, float ds1, float dm0, float dm1) {
+          // two blocks: A operands, scales of (row0, row1), s of the token(s) -> acc
+          auto fold = [&](const uint32_t (&af)[2][4], int pair, const float2 (&sr)[2], const float (&t0)[2],
+                          const float (&t1)[2]) {
+            const uint4 b0 = *reinterpret_cast<const uint4*>(bu + pair * 64);
+            uint4 b1, b2;
             if constexpr (WIDE) {
-              int s0[4], s1[4], s2[4];
-              const int64_t ps = static_cast<int64_t>(a.M) * p.pitch;
-              mma_i8_16832<Q4K>(s0, af, *reinterpret_cast<const uint2*>(bcol + kb * 32));
-              mma_i8_16832<Q4K>(s1, af, *reinterpret_cast<const uint2*>(bcol + ps + kb * 32));
-              mma_i8_16832<Q4K>(s2, af, *reinterpret_cast<const uint2*>(bcol + 2 * ps + kb * 32));
-              const float2 s = *reinterpret_cast<const float2*>(tab + kb * 8 + 2 * c);
-              float2 sx = make_float2(0.0f, 0.0f);
-              if constexpr (Q4K) sx = *reinterpret_cast<const float2*>(sums + kb * 8 + 2 * c);
+              b1 = *reinterpret_cast<const uint4*>(bu + dstep + pair * 64);
+              b2 = *reinterpret_cast<const uint4*>(bu + 2 * dstep + pair * 64);
+            }
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float v = fmaf(__int_as_float(s0[x]) - 12582912.0f, 65536.0f,
-                                     fmaf(__int_as_float(s1[x]) - 12582912.0f, 256.0f,
-                                          __int_as_float(s2[x]) - 12582912.0f));
-                const float d = x < 2 ? ds0 : ds1;
-                acc[x] = fmaf(v * ((x & 1) ? s.y : s.x), d, acc[x]);
-                if constexpr (Q4K) acc[x] = fmaf(x < 2 ? dm0 : dm1, (x & 1) ? sx.y : sx.x, acc[x]);
-              }
-            } else {
-              int s[4];
-              mma_i8_16832<Q4K>(s, af, *reinterpret_cast<const uint2*>(bcol + kb * 32));
-              const float2 f = *reinterpret_cast<const float2*>(tab + kb * 8 + 2 * c);
+            for (int h = 0; h < 2; ++h) {
+              int x0[4];
+              mma_i8_16832<Q4K>(x0, af[h], h ? make_uint2(b0.z, b0.w) : make_uint2(b0.x, b0.y), WIDE ? kMvMagic : 0);
+              if constexpr (WIDE) {
+                int x1[4], x2[4];
+                mma_i8_16832<Q4K>(x1, af[h], h ? make_uint2(b1.z, b1.w) : make_uint2(b1.x, b1.y), 0);
+                mma_i8_16832<Q4K>(x2, af[h], h ? make_uint2(b2.z, b2.w) : make_uint2(b2.x, b2.y), 0);
 #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                acc[x] = fmaf((__int_as_float(s[x]) - 12582912.0f) * ((x & 1) ? f.y : f.x), x < 2 ? ds0 : ds1, acc[x]);
-              if constexpr (Q4K) {
-                const float2 sx = *reinterpret_cast<const float2*>(sums + kb * 8 + 2 * c);
-                acc[0] = fmaf(dm0, sx.x, acc[0]);
-                acc[1] = fmaf(dm0, sx.y, acc[1]);
-                acc[2] = fmaf(dm1, sx.x, acc[2]);
-                acc[3] = fmaf(dm1, sx.y, acc[3]);
+                for (int x = 0; x < 4; ++x) {
+                  const float v = fmaf(__int_as_float(x0[x]) - 12582912.0f, 65536.0f,
+                                       static_cast<float>(x1[x] * 256 + x2[x]));
+                  acc[x] = fmaf(v * ((x & 1) ? t1[h] : t0[h]), x < 2 ? sr[h].x : sr[h].y, acc[x]);
+                }
+              } else {
+                acc[0] = fmaf(static_cast<float>(x0[0] * mul + x0[1]) * t0[h], sr[h].x, acc[0]);
+                acc[1] = fmaf(static_cast<float>(x0[2] * mul + x0[3]) * t0[h], sr[h].y, acc[1]);
               }
             }
           };
-          if constexpr (Q4K) {
-            // headers of rows g and g + 8: (d, dmin), then the 6-bit scales and minima of the eight blocks
-            float d[2], dm[2];
-            uint32_t sc[2][2], mn[2][2];
+          if constexpr (Q4K) {  // the unit's scales and minima: lane -> row lane % 16, four blocks
+            const int half = lane >> 4, row = lane & 15;
+            const uint4 h = *reinterpret_cast<const uint4*>(st + row * kQ4KBytes);
+            const float2 dd = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
+            const uint32_t sc = half ? (h.w & 0x0f0f0f0fu) | ((h.y >> 2) & 0x30303030u) : h.y & 0x3f3f3f3fu;
+            const uint32_t mn = half ? ((h.w >> 4) & 0x0f0f0f0fu) | ((h.z >> 2) & 0x30303030u) : h.z & 0x3f3f3f3fu;
+            const float d1 = dd.x * 0.0625f;  // odd blocks' codes are read as 16 q
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              scales[j * 32 + lane] = ((j & 1) ? d1 : dd.x) * static_cast<float>((sc >> (8 * j)) & 255u);
+            const float m0 = static_cast<float>(mn & 255u), m1 = static_cast<float>((mn >> 8) & 255u),
+                        m2 = static_cast<float>((mn >> 16) & 255u), m3 = static_cast<float>(mn >> 24);
+#pragma unroll
+            for (int m = 0; m < (WIDE ? kMulVecMaxM : 2); ++m) {
+              if (m >= a.M) break;
+              const float4 sx = *reinterpret_cast<const float4*>(sums + m * nb_pitch + kb0 + half * 4);
+              macc[m] = fmaf(-dd.y, fmaf(m0, sx.x, fmaf(m1, sx.y, fmaf(m2, sx.z, m3 * sx.w))), macc[m]);
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {  // four blocks
+            const float4 ta = *reinterpret_cast<const float4*>(tab0 + kb0 + 4 * q);
+            float4 tb = ta;
+            if constexpr (WIDE) tb = *reinterpret_cast<const float4*>(tab1 + kb0 + 4 * q);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const uint4 h = *reinterpret_cast<const uint4*>(st + (g + 8 * r) * 144);
-              const float2 dd = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
-              d[r] = dd.x;
-              dm[r] = -dd.y;
-              sc[r][0] = h.y & 0x3f3f3f3fu;
-              mn[r][0] = h.z & 0x3f3f3f3fu;
-              sc[r][1] = (h.w & 0x0f0f0f0fu) | ((h.y >> 2) & 0x30303030u);
-              mn[r][1] = ((h.w >> 4) & 0x0f0f0f0fu) | ((h.z >> 2) & 0x30303030u);
-            }
+              const int j = 2 * q + r;  // blocks 2j, 2j + 1
+              uint32_t af[2][4];
+              float2 sr[2];
+              if constexpr (Q4K) {  // low nibbles: block 2j; high ones (16 q): block 2j + 1
+                const uint2 w0 = *reinterpret_cast<const uint2*>(st + row0 * kQ4KBytes + 16 + 32 * j + 8 * c);
+                const uint2 w1 = *reinterpret_cast<const uint2*>(st + row1 * kQ4KBytes + 16 + 32 * j + 8 * c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[2][2];
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                  w[r][x] = *reinterpret_cast<const uint32_t*>(st + (g + 8 * r) * 144 + 16 + 32 * j + 16 * x + 4 * c);
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {  // low nibbles: block 2j; high ones (16 q): block 2j + 1
-                const uint32_t mask = x ? 0xf0f0f0f0u : 0x0f0f0f0fu;
-                const uint32_t af[4] = {w[0][0] & mask, w[1][0] & mask, w[0][1] & mask, w[1][1] & mask};
-                const int bi = 2 * j + x;
-                float ds[2], ms[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  ds[r] = d[r] * static_cast<float>((sc[r][bi >> 2] >> (8 * (bi & 3))) & 255u) * (x ? 0.0625f : 1.0f);
-                  ms[r] = dm[r] * static_cast<float>((mn[r][bi >> 2] >> (8 * (bi & 3))) & 255u);
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t mask = h ? 0xf0f0f0f0u : 0x0f0f0f0fu;
+                  af[h][0] = w0.x & mask;
+                  af[h][1] = w1.x & mask;
+                  af[h][2] = w0.y & mask;
+                  af[h][3] = w1.y & mask;
+                  sr[h] = *reinterpret_cast<const float2*>(scales + ((2 * j + h) & 3) * 32 + q * 16 + row0);
                 }
-                fold(af, kb0 + bi, ds[0], ds[1], ms[0], ms[1]);
-              }
-            }
-          } else {
-            const uint16_t* sc = reinterpret_cast<const uint16_t*>(st + 2048);
+              } else {
 #pragma unroll
-            for (int bi = 0; bi < 8; ++bi) {
-              const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + g * 128 + ((bi ^ g) & 7) * 16 + c * 4);
-              const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (g + 8) * 128 + ((bi ^ g) & 7) * 16 + c * 4);
-              const uint32_t af[4] = {((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u, ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u,
-                                      (w0 & 0xf0f0f0f0u) ^ 0x80808080u, (w1 & 0xf0f0f0f0u) ^ 0x80808080u};
-              fold(af, kb0 + bi, __half2float(__ushort_as_half(sc[bi * 16 + g])),
-                   __half2float(__ushort_as_half(sc[bi * 16 + g + 8])), 0.0f, 0.0f);
+                for (int h = 0; h < 2; ++h) {
+                  const int bi = 2 * j + h, at = ((bi ^ g) & 7) * 16 + c * 4;
+                  const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + row0 * 128 + at);
+                  const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + row1 * 128 + at);
+                  af[h][0] = ((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                  af[h][1] = ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                  af[h][2] = (w0 & 0xf0f0f0f0u) ^ 0x80808080u;
+                  af[h][3] = (w1 & 0xf0f0f0f0u) ^ 0x80808080u;
+                  sr[h] = __half22float2(reinterpret_cast<const __half2*>(st + 2048)[bi * 8 + g]);
+                }
+              }
+              const float t0[2] = {r ? ta.z : ta.x, r ? ta.w : ta.y}, t1[2] = {r ? tb.z : tb.x, r ? tb.w : tb.y};
+              fold(af, j, sr, t0, t1);
             }
           }
           __syncwarp();  // every lane has read the stage before it is refilled
-          stage = stage + 1 == kMvStages ? 0 : stage + 1;
-          fill = fill + 1 == kMvStages ? 0 : fill + 1;
+          stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+          fill = fill + 1 == S::STAGES ? 0 : fill + 1;
         }
-        float* mine = red + (buf * kMvWarps + warp) * 128;
-        *reinterpret_cast<float2*>(mine + g * 8 + 2 * c) = make_float2(acc[0], acc[1]);
-        *reinterpret_cast<float2*>(mine + (g + 8) * 8 + 2 * c) = make_float2(acc[2], acc[3]);
+        float* mine = red + (buf * S::WARPS + warp) * 16 * TC;
+        if constexpr (WIDE) {
+          *reinterpret_cast<float2*>(mine + row0 * TC + 2 * c) = make_float2(acc[0], acc[1]);
+          *reinterpret_cast<float2*>(mine + row1 * TC + 2 * c) = make_float2(acc[2], acc[3]);
+        } else {
+          const float f = (c & 1) ? 1.0f : 256.0f;
+          mine[row0 * TC + c] = acc[0] * f;
+          mine[row1 * TC + c] = acc[1] * f;
+        }
+        if constexpr (Q4K) {
+          __syncwarp();
+#pragma unroll
+          for (int m = 0; m < (WIDE ? kMulVecMaxM : 2); ++m) {
+            const float v = macc[m] + __shfl_xor_sync(0xffffffffu, macc[m], 16);
+            if (lane < 16 && m < a.M) mine[lane * TC + (WIDE ? m : 2 * m + 1)] += v;
+          }
+        }
         __syncthreads();  // and the other buffer's readers are done before it is written again
         // Warp w sums rows w, w + 16, .. of the super-tile: lanes over (warp of the tile, column).
-        for (int r = warp; r < 16 * WR; r += kMvWarps) {
-          const float* part = red + (buf * kMvWarps + ((r >> 4) << p.wk_shift)) * 128 + (r & 15) * 8;
+        for (int r = warp; r < 16 * WR; r += S::WARPS) {
+          const float* part = red + ((buf * S::WARPS + ((r >> 4) << p.wk_shift)) * 16 + (r & 15)) * TC;
           float v = 0.0f;
-          for (int x = lane >> 3; x < WK; x += 4) v += part[x * 128 + (lane & 7)];
-          v += __shfl_xor_sync(0xffffffffu, v, 8);
-          v += __shfl_xor_sync(0xffffffffu, v, 16);
+          for (int x = lane / TC; x < WK; x += 32 / TC) v += part[x * 16 * TC + lane % TC];
+#pragma unroll
+          for (int o = TC; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          int m = lane;  // lane's token
           if constexpr (!WIDE) {
-            const int t3 = 3 * min(lane, a.M - 1);
-            const float v0 = __shfl_sync(0xffffffffu, v, t3), v1 = __shfl_sync(0xffffffffu, v, t3 + 1),
-                        v2 = __shfl_sync(0xffffffffu, v, t3 + 2);
-            v = v0 + (v1 + v2);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            m = (lane & 1) ? kMulVecMaxM : lane >> 1;
           }
-          const int64_t n = (blockIdx.x + i * gridDim.x) * WR * 16 + r;
-          if (lane < a.M && n < a.N) {
+          const int64_t n = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * WR * 16 + r;
+          if (m < a.M && n < a.N) {
             if (p.chunks > 1) {
-              float* slot = acc_s + (static_cast<int>(i - g0) * 16 * WR + r) * a.M + lane;
+              float* slot = acc_s + ((i - g0) * 16 * WR + r) * a.M + m;
               if (chunk > 0) v += *slot;
               *slot = v;
             }
             if (chunk == p.chunks - 1) {
-              if (a.bias) v = __fadd_rn(v, a.bias[n]);
-              if (a.resid) v = __fadd_rn(a.resid[lane * a.ldr + n], a.gate ? __fmul_rn(v, a.gate[n]) : v);
-              a.y[lane * a.ldy + n] = v;
+              if (a.bias) v = __fadd_rn(v, r == warp ? bias_first : __ldg(a.bias + n));
+              if (a.resid) v = __fadd_rn(a.resid[m * a.ldr + n], a.gate ? __fmul_rn(v, a.gate[n]) : v);
+              a.y[m * a.ldy + n] = v;
             }
           }
         }
@@ -419,29 +446,35 @@ __global__ void __launch_bounds__(kMvThreads, 1) mul_vec_kernel(const MulVecArgs
 
 template <bool Q4K, bool WIDE, int XT>
 cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
+  using S = MvShape<WIDE>;
   auto kern = mul_vec_kernel<Q4K, WIDE, XT>;
   MvPlan p{};
   p.units = static_cast<int>((a.K + kMvUnitK - 1) / kMvUnitK);
-  // Shared memory per value of K: the digits, and per 32 values the table and the sums.
-  const int per_k = 3 * a.M + 1 + (Q4K ? 1 : 0);
-  const int most = kMvXBytes / (per_k * kMvUnitK) - 1;  // (the digit rows' padding fits one unit)
+  // Shared memory per unit: the digits, and per block s and the sum.
+  const int per_unit = a.M * (3 * kMvUnitK + (Q4K ? 64 : 32));
+  const int most = (S::X - a.M * (3 * 64 + 32)) / per_unit;
   p.chunks = (p.units + most - 1) / most;
   p.chunk_units = (p.units + p.chunks - 1) / p.chunks;
   p.chunks = (p.units + p.chunk_units - 1) / p.chunk_units;
-  p.pitch = p.chunk_units * kMvUnitK + 32;
+  p.pitch = p.chunk_units * kMvUnitK + 64;
   const int64_t tiles = (a.N + 15) / 16;
-  // WK, the warps that share a tile's units: all 16 while that gives each two
-  // units of a chunk (long runs per warp keep the sums at a tile's end cheap);
-  // fewer rows than SMs: as many as there are units.
-  int sh = 4;
-  while (sh > 0 && (1 << sh) * 2 > p.chunk_units && tiles > static_cast<int64_t>(num_sms) * (kMvWarps >> sh)) --sh;
-  while (sh > 0 && (1 << sh) > p.chunk_units) --sh;
+  // WK, the warps that share a tile's units: what finishes first when a tile's
+  // end costs as much as 0.75 units and the super-tiles go round the SMs.
+  // Measured at 49152 x 8192, Q4_K, one token: WK 1 67 us, 2 68, 4 69.5, 8 68.5.
+  int sh = 0;
+  double best = 0.0;
+  for (int x = 0; x <= 3 && (1 << x) <= p.chunk_units; ++x) {
+    const int64_t super = (tiles + (S::WARPS >> x) - 1) / (S::WARPS >> x);
+    const double cost = static_cast<double>((super + num_sms - 1) / num_sms) *
+                        ((p.units + (1 << x) - 1) / (1 << x) + 0.75 * p.chunks);
+    if (x == 0 || cost < best) best = cost, sh = x;
+  }
   p.wk_shift = sh;
-  const int wr = kMvWarps >> sh;
+  const int wr = S::WARPS >> sh;
   p.supers = (tiles + wr - 1) / wr;
   const uintptr_t xa = reinterpret_cast<uintptr_t>(a.x);
   p.vec = XT == kXF32 ? (xa % 16 == 0 && a.ldx % 4 == 0) : (xa % 8 == 0 && a.ldx % 4 == 0);
-  const int smem = kMvRing + kMvRed + kMvAcc + kMvXBytes;
+  const int smem = kMvSmem;
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
@@ -451,7 +484,7 @@ cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
     attr_set[dev] = true;
   }
   const int64_t grid = p.supers < num_sms ? p.supers : num_sms;
-  kern<<<static_cast<unsigned>(grid), kMvThreads, smem, s>>>(a, p);
+  kern<<<static_cast<unsigned>(grid), S::THREADS, smem, s>>>(a, p);
   return cudaGetLastError();
 }
 

@@ -1156,6 +1156,8 @@ int b2q_device_status(unsigned int* code, int clear) {
   unsigned int attn = 0;
   if (read_attention_status(&attn, clear != 0) != cudaSuccess) return B2Q_ERR_CUDA;
   if (!*code) *code = attn;
+  if (read_paged_status(&attn, clear != 0) != cudaSuccess) return B2Q_ERR_CUDA;
+  if (!*code) *code = attn;
   return *code ? B2Q_ERR_DEVICE : B2Q_OK;
 }
 
@@ -1284,7 +1286,7 @@ int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_bytes, con
   if (!std::isfinite(scale) || n_pages < 0 || table_width < 0) return B2Q_ERR_INVALID_ARG;
   const int shift = page_shift_of(page_size);
   if (shift < 0) return B2Q_ERR_UNSUPPORTED;
-  if (n_pages > INT_MAX || table_width > (INT_MAX >> shift)) return B2Q_ERR_TOO_LARGE;
+  if (n_pages > INT_MAX || n_pages * Hkv > INT_MAX || table_width > (INT_MAX >> shift)) return B2Q_ERR_TOO_LARGE;
   const bool any = B > 0 && T > 0 && max_new > 0;
   if (any && (!q || !o || !cu_new || !kv_len || (table_width > 0 && !block_table) ||
               (n_pages > 0 && table_width > 0 && (!k_cache || !v_cache))))
@@ -1330,7 +1332,8 @@ int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_bytes, con
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.part_o_bytes);
   return from_cuda(
-      launch_attention_paged(a, static_cast<int>(D), type == B2Q_TYPE_BF16, static_cast<cudaStream_t>(stream)));
+      launch_attention_paged(a, static_cast<int>(D), type == B2Q_TYPE_BF16, p.tiles,
+                             static_cast<cudaStream_t>(stream)));
 }
 
 int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, const void* x, int64_t m,

@@ -23,6 +23,7 @@
 // Stretches are split over CTAs when the rows alone do not fill the GPU; a
 // second kernel then joins their outputs by their maxima and sums.
 #include "b2q_internal.h"
+#include "b2q_paged.cuh"
 #include "b2q_ptx.cuh"
 
 #include <cuda_bf16.h>
@@ -37,32 +38,6 @@ namespace {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kUnit = 16;  // keys
-constexpr int64_t kNowhere = -(int64_t{1} << 60);  // position of a padding row: before every key
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t u) {
-  if constexpr (BF16) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
-  }
-}
-// Either half of the pair is an infinity or a NaN.
-template <bool BF16>
-__device__ __forceinline__ bool nonfinite2(uint32_t u) {
-  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  return (u & e) == e || (u & (e << 16)) == (e << 16);
-}
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -99,52 +74,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// The new tokens of one request and the keys that a run of them can see.
-struct Request {
-  int64_t t0;     // first row of q
-  int64_t n;      // new tokens
-  int64_t len;    // keys the table can hold and the request has
-  int64_t first;  // position of the first new token
-};
-__device__ __forceinline__ Request request_of(const PagedArgs& a, int b) {
-  Request r;
-  const int64_t lo = min(max(static_cast<int64_t>(a.cu_q[b]), int64_t{0}), a.T);
-  const int64_t hi = min(max(static_cast<int64_t>(a.cu_q[b + 1]), lo), a.T);
-  r.t0 = lo;
-  r.n = min(hi - lo, a.max_q);
-  const int64_t len = max(a.kv_len[b], 0);
-  r.first = len - (hi - lo);
-  r.len = min(len, a.width << a.page_shift);
-  return r;
-}
-// Units of `unit` keys seen by some token at positions p_lo .. p_hi: the sinks'
-// units 0 .. su - 1, then wu .. hu - 1.
-struct Units {
-  int64_t su, wu, hu;
-  int64_t win_lo;  // first key of the window of p_lo
-  __device__ __forceinline__ int64_t count() const { return su + (hu - wu); }
-  __device__ __forceinline__ int64_t at(int64_t i) const { return i < su ? i : wu + (i - su); }
-};
-__device__ __forceinline__ Units units_of(const PagedArgs& a, int64_t len, int64_t p_lo, int64_t p_hi, int unit) {
-  Units u;
-  const int64_t hi = a.causal ? min(len, p_hi + 1) : len;
-  u.hu = hi > 0 ? (hi + unit - 1) / unit : 0;
-  u.win_lo = a.window > 0 ? max(int64_t{0}, p_lo - a.window + 1) : 0;
-  u.wu = min(u.win_lo / unit, u.hu);
-  const int64_t sk = a.window > 0 ? min(a.sinks, u.win_lo) : 0;
-  u.su = min((sk + unit - 1) / unit, u.wu);
-  return u;
-}
-__device__ __forceinline__ bool sees(const PagedArgs& a, int64_t p, int64_t j, int64_t len) {
-  return j < len && (!a.causal || j <= p) && (a.window <= 0 || j > p - a.window || j < a.sinks);
-}
-
 template <int D>
 struct RowsShape {
   static constexpr int STAGES = D == 64 ? 4 : 3;
@@ -438,19 +367,20 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
 #pragma unroll
       for (int w = 0; w < kRowsWarps; ++w) {
         const float2 x = ml[w * 16 + row];
-        f[w] = x.x == -INFINITY ? 0.0f : ex2(x.x - M);
+        f[w] = x.x == -INFINITY ? x.y * 0.0f : ex2(x.x - M);  // (no finite score: 0, or NaN where one was NaN)
         sum += f[w] * x.y;
       }
       const int64_t t = rq.t0 + r / a.G;
       const int64_t h = static_cast<int64_t>(hk) * a.G + r % a.G;
       const bool whole = a.splits == 1;
-      const float inv = whole ? (M == -INFINITY ? 0.0f : 1.0f / sum) : 1.0f;
+      const bool empty = M == -INFINITY && sum == 0.0f;
+      const float inv = whole ? (empty ? 0.0f : 1.0f / sum) : 1.0f;
       const int64_t pi = (t * a.Hq + h) * a.splits + split;
       if (!whole && part == 0) a.part_ml[pi] = make_float2(M, sum);
 #pragma unroll
       for (int d = part * 2; d < D; d += TPR * 2) {
         float x = 0.0f, y = 0.0f;
-        if (M != -INFINITY) {
+        if (!empty) {
 #pragma unroll
           for (int w = 0; w < kRowsWarps; ++w) {
             const float2 v = *reinterpret_cast<const float2*>(ow + (w * 16 + row) * D + d);
@@ -473,7 +403,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
 // One warp per (token, query head): o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s
 // over the splits that hold keys, in their order.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int tile_rows) {
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int tile_rows, int unit) {
   const int lane = threadIdx.x & 31;
   const int b = blockIdx.y;
   const Request rq = request_of(a, b);
@@ -483,7 +413,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int 
   // the split count of the row's tile
   const int64_t r0 = (i * a.G + h % a.G) / tile_rows * tile_rows;
   const int64_t p_lo = rq.first + r0 / a.G, p_hi = rq.first + min(rq.n * a.G - 1, r0 + tile_rows - 1) / a.G;
-  const int64_t units = units_of(a, rq.len, p_lo, p_hi, kUnit).count();
+  const int64_t units = units_of(a, rq.len, p_lo, p_hi, unit).count();
   const int ns = static_cast<int>(
       min(static_cast<int64_t>(a.splits), max(int64_t{1}, (units + a.split_units - 1) / a.split_units)));
   const int64_t pi = ((rq.t0 + i) * a.Hq + h) * a.splits;
@@ -493,11 +423,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int 
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   constexpr int E = D / 32;
   float acc[E] = {}, sum = 0.0f;
-  if (M != -INFINITY) {
+  {
     for (int s = 0; s < ns; ++s) {
       const float2 ml = a.part_ml[pi + s];
-      if (ml.x == -INFINITY) continue;
-      const float f = ex2(ml.x - M);
+      if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key
+      const float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - M);  // (only NaN scores: NaN)
       sum = fmaf(f, ml.y, sum);
       const float* src = a.part_o + (pi + s) * D + lane * E;
 #pragma unroll
@@ -508,10 +438,17 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int 
       }
     }
   }
-  const float inv = M == -INFINITY ? 0.0f : 1.0f / sum;
+  const float inv = M == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
   uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo + h * D + lane * E);
 #pragma unroll
   for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
+}
+
+template <int D, bool BF16>
+cudaError_t launch_join(const PagedArgs& a, int tile_rows, int unit, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((a.max_q * a.Hq + 3) / 4), static_cast<unsigned>(a.B));
+  paged_join_kernel<D, BF16><<<grid, 128, 0, s>>>(a, tile_rows, unit);
+  return cudaGetLastError();
 }
 
 template <int D, bool BF16, int MT>
@@ -530,11 +467,8 @@ cudaError_t launch_rows(const PagedArgs& a, cudaStream_t s) {
   if (tiles * a.splits > INT32_MAX) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(tiles * a.splits), static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.B));
   kern<<<grid, kRowsThreads, RowsShape<D>::BYTES, s>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
-  const dim3 jgrid(static_cast<unsigned>((a.max_q * a.Hq + 3) / 4), static_cast<unsigned>(a.B));
-  paged_join_kernel<D, BF16><<<jgrid, 128, 0, s>>>(a, 16 * MT);
-  return cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess || a.splits == 1 ? e : launch_join<D, BF16>(a, 16 * MT, kUnit, s);
 }
 
 template <int D, bool BF16>
@@ -545,21 +479,29 @@ cudaError_t launch_paged_t(const PagedArgs& a, cudaStream_t s) {
 
 }  // namespace
 
+// Which kernel, and how the keys are split.  Up to 32 rows a (request, kv head)
+// the rows kernel; above, its 32-row tiles would read the keys once more for
+// every 32 rows, and the tile kernel takes 256 rows at a time.
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,
                      bool causal, int64_t window, int64_t sinks) {
   PagedPlan p;
-  const int64_t G = Hq / Hkv;
-  const int64_t tile_rows = max_q * G <= 16 ? 16 : 32;
-  // Keys that the newest rows of a request can see, in units.
+  const int64_t G = Hq / Hkv, rows = max_q * G;
+  p.tiles = rows > 32 && G <= kTileRows;
+  const int unit = p.tiles ? kTileKeys : kUnit;
+  const int64_t tile_rows = p.tiles ? 2 * (kTileRows / G) * G : rows <= 16 ? 16 : 32;
+  // Keys that the rows of one CTA can see, in units.
   int64_t span = max_kv;
   if (causal && window > 0 && window + tile_rows + sinks < span) span = window + tile_rows + sinks;
-  const int64_t units = span / kUnit + 3;
-  const int64_t ctas = B * Hkv * ((max_q * G + tile_rows - 1) / tile_rows);
-  // Stretches short enough that the GPU's 148 SMs x 2 CTAs each get eight of
-  // them where the requests are alike, and none shorter than 256 keys.
-  const int64_t want = ctas >= 148 * 16 ? 1 : (148 * 16 + ctas - 1) / (ctas > 0 ? ctas : 1);
+  const int64_t units = span / unit + 3;
+  const int64_t ctas = B * Hkv * ((rows + tile_rows - 1) / tile_rows);
+  // Rows kernel: stretches short enough that the GPU's 148 SMs x 2 CTAs each get
+  // eight of them where the requests are alike, and none shorter than 256 keys.
+  // Tile kernel (one CTA per SM): split only while CTAs are fewer than SMs, into
+  // stretches of 512 keys or more.
+  const int64_t goal = p.tiles ? 148 : 148 * 16, least = p.tiles ? 4 : 16;
+  const int64_t want = ctas >= goal ? 1 : p.tiles ? goal / (ctas > 0 ? ctas : 1) : (goal + ctas - 1) / (ctas > 0 ? ctas : 1);
   int64_t per = (units + want - 1) / want;
-  if (per < 16) per = 16;
+  if (per < least) per = least;
   if (units <= per) per = units;
   p.split_units = per;
   p.splits = (units + per - 1) / per;
@@ -570,9 +512,17 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
   return p;
 }
 
-cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, cudaStream_t s) {
-  if (D == 64) return bf16 ? launch_paged_t<64, true>(a, s) : launch_paged_t<64, false>(a, s);
-  return bf16 ? launch_paged_t<128, true>(a, s) : launch_paged_t<128, false>(a, s);
+cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, int tile_rows, int unit, cudaStream_t s) {
+  if (D == 64) return bf16 ? launch_join<64, true>(a, tile_rows, unit, s) : launch_join<64, false>(a, tile_rows, unit, s);
+  return bf16 ? launch_join<128, true>(a, tile_rows, unit, s) : launch_join<128, false>(a, tile_rows, unit, s);
+}
+
+cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, bool tiles, cudaStream_t s) {
+  if (tiles && a.n_pages > 0) return launch_paged_tiles(a, D, bf16, s);
+  PagedArgs r = a;
+  if (a.n_pages == 0) r.splits = 1;  // no keys at all
+  if (D == 64) return bf16 ? launch_paged_t<64, true>(r, s) : launch_paged_t<64, false>(r, s);
+  return bf16 ? launch_paged_t<128, true>(r, s) : launch_paged_t<128, false>(r, s);
 }
 
 }  // namespace b2q

@@ -219,6 +219,10 @@ bool make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* ba
                         uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                         CUtensorMapSwizzle swz);
 
+// The same for three dimensions (strides of the outer two in bytes).
+bool make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t (&dims)[3],
+                        const uint64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swz);
+
 // Q4_K x Q8_K GEMM (b2q_gemm_q4k.cuh):
 //   weight: block_q4_K rows, ldw_bytes apart (16-byte aligned base and stride);
 //   activations: int8 Q8_K codes [M][K], fp32 d [K/256][lda].
@@ -336,18 +340,24 @@ struct PagedArgs {
   int64_t window, sinks;  // window 0: no limit
   void* o;
   int64_t ldo;
-  // Keys split into stretches of split_units units (a padding of 1 stretch: no join).
+  // Keys split into stretches of split_units units, joined afterwards (splits 1: not split).
   int splits;
   int64_t split_units;
   float* part_o;          // [T][Hq][splits][D]
   float2* part_ml;        // [T][Hq][splits] (max, sum)
 };
+constexpr int kTileRows = 128, kTileKeys = 128;  // of the tensor-memory kernel
 struct PagedPlan {
+  bool tiles = false;  // the tile kernel (b2q_attention_paged_tile.cu), else the rows kernel
   int64_t splits = 1, split_units = 0, part_o_bytes = 0, part_ml_bytes = 0;
 };
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,
                      bool causal, int64_t window, int64_t sinks);
-cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, cudaStream_t s);
+cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, bool tiles, cudaStream_t s);
+cudaError_t launch_paged_tiles(const PagedArgs& a, int D, bool bf16, cudaStream_t s);
+cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, int tile_rows, int unit, cudaStream_t s);
+// Status word of the tile kernel's bounded waits (its own translation unit).
+cudaError_t read_paged_status(unsigned int* value, bool clear);
 
 constexpr int kMulVecMaxM = 8;
 enum { kXF32 = 0, kXF16 = 1, kXBF16 = 2 };

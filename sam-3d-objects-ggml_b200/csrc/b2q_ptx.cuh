@@ -125,6 +125,17 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+// The same for a 3-D tensor.  A box that lies outside the tensor in y or z
+// arrives as zeros (and counts its full bytes on the barrier).
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x,
+                                            int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 // 2-D tiled TMA store of a box from shared memory to global memory, tracked by
 // this thread's bulk async-groups.  The writers of the box make their
 // generic-proxy stores visible first (fence_proxy_async_smem + a sync); boxes

@@ -498,7 +498,7 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
   // eight of them where the requests are alike, and none shorter than 256 keys.
   // Tile kernel (one CTA per SM): split only while CTAs are fewer than SMs, into
   // stretches of 512 keys or more.
-  const int64_t goal = p.tiles ? 148 : 148 * 16, least = p.tiles ? 4 : 16;
+  const int64_t goal = p.tiles ? 148 : 148 * 16, least = p.tiles ? 512 / kTileKeys : 16;
   const int64_t want = ctas >= goal ? 1 : p.tiles ? goal / (ctas > 0 ? ctas : 1) : (goal + ctas - 1) / (ctas > 0 ? ctas : 1);
   int64_t per = (units + want - 1) / want;
   if (per < least) per = least;

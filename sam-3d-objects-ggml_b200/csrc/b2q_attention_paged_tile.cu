@@ -3,13 +3,14 @@
 // pay for, so bound by the tensor cores and the exponentials.
 //
 // One CTA per SM takes 2 x 128 rows of one (request, kv head): two query tiles
-// of floor(128 / G) tokens x G heads each, and walks the keys in tiles of 128:
+// of floor(128 / G) tokens x G heads each, and walks the keys in tiles of 64:
 //   warp 0       producer: Q once; K and V tiles into two rings, one TMA box per
 //                page and 64 columns, issued by as many lanes.  Pages that are
 //                absent, or past the length, are boxes outside the tensor: zeros
-//   warp 1       TMEM and the MMAs: S_i = Q_i K^T (M 128, N 128, K D) and
-//                O_i += P_i V (M 128, N D, K 128; P from tensor memory)
-//   warps 2, 3   V of the edge tiles (below)
+//   warps 1, 2   the MMAs of query tile 0 and 1, one thread each: S_i = Q_i K^T (M 128,
+//                N 64, K D) and O_i += P_i V (M 128, N D, K 64; P from tensor memory).
+//                One thread polling for both was the limit: 1177 us where two take 993
+//   warp 3       V of the edge tiles (below)
 //   warpgroups 1, 2: softmax of query tile 0 and 1, one row per thread: mask,
 //                maximum, exp2, P rounded to the cache's type into tensor memory,
 //                row sum of the unrounded P; the maximum in use is raised, and O
@@ -17,14 +18,20 @@
 // P rounded to 16 bits once, as the dense F16 attention has it: on random values
 // that costs as much accuracy as rounding the output does, and a second P V for
 // what it leaves would cost half the tensor time.
-// D = 128: P takes the place of S in tensor memory (S, O and P of two tiles
-// would need 640 columns of 512), so the next S of a tile is issued behind its
-// P V; the other tile's work covers the wait.  D = 64: P has its own columns.
+// Tensor memory: O_i (D columns each), and two 64-column buffers of S per query
+// tile; P takes the place of its S.  So the next S of a query tile is computed
+// while its softmax works on this one, and a softmax warp never waits for a round
+// trip through the tensor pipe.  With tiles of 128 keys there is room for one S a
+// query tile only: S, softmax and P V then follow one another (1027 us).
+// Measured on two chunks of 3.9k tokens over 4k and 7.5k cached, 32 / 8 heads of
+// 128: 993 us, 1010 TFLOP/s, the tensor pipe active half of the time; the
+// softmax warps' own chain (loads from tensor memory, maximum, exps, stores) is
+// what a tile waits for.
 //
 // Edge tiles -- not every row sees every key -- are masked in the scores.  Their V
 // may hold an infinity or a NaN in keys that some rows do not see, and P = 0
-// does not cover those.  Warps 2 and 3 zero V rows that no row of the CTA sees,
-// look the rest of an edge tile's rows through, and take non-finite ones out of
+// does not cover those.  Warp 3 zeroes V rows that no row of the CTA sees,
+// looks the rest of an edge tile's rows through, and takes non-finite ones out of
 // the product; the rows that do see such a key add its share themselves, at the
 // end, from global memory.
 #include "b2q_paged.cuh"
@@ -41,21 +48,21 @@ __device__ unsigned int g_paged_status = 0;
 constexpr int kPtThreads = 384;
 constexpr int kPtLaunchRegs = 168, kPtRegsControl = 56, kPtRegsSoftmax = 224;
 static_assert(128 * kPtRegsControl + 256 * kPtRegsSoftmax <= kPtThreads * kPtLaunchRegs, "register split");
-constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 columns
-constexpr int kMaxEdges = 16;     // edge tiles of a CTA that can hold non-finite keys
+constexpr int kQHalf = 128 * 128, kHalf = kTileKeys * 128;  // bytes of 64 columns of Q, and of K or V
+constexpr int kPolyPairs = 1;     // of every 4 pairs of exps, on the FMA pipe (0: 1076 us on the listed chunk, 1: 993, 2: 1005)
+constexpr int kMaxEdges = 24;     // edge tiles of a CTA that can hold non-finite keys
 
 template <int D>
 struct PtShape {
   static constexpr int HALVES = D / 64;
-  static constexpr int TILE = HALVES * kHalf;
-  static constexpr int STAGES = D == 64 ? 4 : 2;           // of the K ring and of the V ring
-  static constexpr bool ALIAS = D == 128;                  // P in S's columns
-  // TMEM columns
-  static constexpr uint32_t S = 0, O = 256, P = ALIAS ? 0 : 384, PSTEP = ALIAS ? 128 : 64;
+  static constexpr int QTILE = HALVES * kQHalf, TILE = HALVES * kHalf;
+  static constexpr int STAGES = D == 64 ? 8 : 4;           // of the K ring and of the V ring
+  // TMEM columns: S (and P) of query tile i, buffer x at S + 128 i + 64 x; O_i at O + D i
+  static constexpr uint32_t S = 0, O = 256;
   static constexpr int Q_OFF = 0;
-  static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
+  static constexpr int K_OFF = 2 * QTILE, V_OFF = K_OFF + STAGES * TILE;
   static constexpr int BAR_OFF = V_OFF + STAGES * TILE;
-  static constexpr int NBAR = 1 + 5 * STAGES + 10 + 1;
+  static constexpr int NBAR = 1 + 5 * STAGES + 12 + 4;
   static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
   // tmem holder, abort flag, number of bad tiles; bad tile numbers, bad key masks
   static constexpr int BYTES = MISC_OFF + 16 + kMaxEdges * (4 + 16) + 1024;
@@ -84,8 +91,8 @@ __device__ __forceinline__ uint64_t pt_desc_v(uint32_t addr, uint32_t lbo) {
 }
 
 // exp2 of a pair on the FMA pipe (the dense F16 attention has the derivation:
-// Cody-Waite, cubic of least maximum relative error 7.5e-5), half of them here
-// and half on the MUFU.
+// Cody-Waite, cubic of least maximum relative error 7.5e-5); the others go to
+// the MUFU.
 __device__ __forceinline__ float2 pt_ex2_poly(float2 x) {
   constexpr float kRound = 12582912.0f;
   const float2 one = make_float2(1.0f, 1.0f), neg = make_float2(-1.0f, -1.0f);
@@ -143,8 +150,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const int u1 = split == a.splits - 1 ? u_all
                                        : static_cast<int>(min(static_cast<int64_t>(u_all), u0 + a.split_units));
   if (split > 0 && u0 >= u_all) return;  // the joining kernel knows
-  TileList own[2];
-  int j0[2], j1[2];
+  TileList own[2];  // of the whole range of keys
+  int j0[2], j1[2];  // and those of the stretch
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (i < nq) {
@@ -158,8 +165,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
   }
   const int nu = u1 - u0;
-  // a query tile's tile j: its number within the stretch
-  auto place = [&](int i, int j) { return j < j1[i] ? all.before(own[i].at(j)) - u0 : nu; };
   const int64_t key_end = a.causal ? min(rq.len, p_hi + 1) : rq.len;
   // every row of the CTA sees every key of tile kt (absent pages aside)
   auto plain = [&](int kt) {
@@ -175,12 +180,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* v_full = k_empty + ST;
   uint64_t* v_ok = v_full + ST;      // V landed and looked through
   uint64_t* v_empty = v_ok + ST;
-  uint64_t* s_full = v_empty + ST;   // [2] per query tile
-  uint64_t* s_empty = s_full + 2;
-  uint64_t* p_full = s_empty + 2;
-  uint64_t* p_empty = p_full + 2;
-  uint64_t* pv_full = p_empty + 2;
-  uint64_t* done = pv_full + 2;
+  uint64_t* s_full = v_empty + ST;   // [query tile][buffer]
+  uint64_t* p_full = s_full + 4;     // [query tile][buffer]
+  uint64_t* pv_full = p_full + 4;    // [query tile][buffer]
+  uint64_t* o_full = pv_full + 4;    // [query tile] all of P V, once
+  uint64_t* done = o_full + 2;
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + S::MISC_OFF);
   uint32_t* tmem_holder = misc;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
@@ -190,26 +194,27 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   unsigned int* status = &g_paged_status;
   const int32_t* table = a.table + static_cast<int64_t>(b) * a.ldt;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int box = 1 << min(a.page_shift, 7);  // keys of one TMA box
+  const int box = min(1 << a.page_shift, kTileKeys);  // keys of one TMA box
   const int boxes = kTileKeys / box;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < ST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], nq);   // one per query tile
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_ok[s], 2);     // warps 2 and 3
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_ok[s], 1);
+      mbar_init(&v_empty[s], nq);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 4);  // one arrival per softmax warp
-      mbar_init(&p_full[i], 4);
-      mbar_init(&p_empty[i], 1);
-      mbar_init(&pv_full[i], 1);
+    for (int x = 0; x < 4; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);   // one arrival per softmax warp
+      mbar_init(&pv_full[x], 1);
     }
-    mbar_init(done, 1);
+    mbar_init(&o_full[0], 1);
+    mbar_init(&o_full[1], 1);
+    mbar_init(&done[0], 1);
+    mbar_init(&done[1], 1);
     *abort_flag = 0;
     *n_edges = 0;
     fence_mbarrier_init();
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       __syncwarp();
       if (lane < nq * HV) {
         const int i = lane / HV, h = lane % HV;
-        tma_load_3d(smem + S::Q_OFF + i * S::TILE + h * kHalf, &maps.q, q_full, h * 64, hk * a.G,
+        tma_load_3d(smem + S::Q_OFF + i * S::QTILE + h * kQHalf, &maps.q, q_full, h * 64, hk * a.G,
                     static_cast<int32_t>(rq.t0 + i0 + i * tok));
       }
       const int32_t none = static_cast<int32_t>(a.n_pages * a.Hkv);  // a box outside the pool
@@ -278,88 +283,66 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         mbar_wait(&k_full[u % ST], (u / ST) & 1u, status, kDevWaitDrain, nullptr);
       for (int u = max(0, v_laps - ST); u < v_laps; ++u)
         mbar_wait(&v_full[u % ST], (u / ST) & 1u, status, kDevWaitDrain, nullptr);
-    } else if (warp == 1) {
-      // -------------------------------------------------------- MMA issuer
-      if (elect_one()) {
-        constexpr uint32_t idesc_qk = idesc_16<BF16>(128, 128);
+    } else if (warp <= 2) {
+      // ------------------------------------------- MMAs of query tile warp - 1
+      const int i = warp - 1;
+      if (i < nq && elect_one()) {
+        constexpr uint32_t idesc_qk = idesc_16<BF16>(128, kTileKeys);
         constexpr uint32_t idesc_pv = idesc_16<BF16>(128, D) | (1u << 16);  // B (V) MN-major
+        const TileList mine = i == 0 ? own[0] : own[1];
+        const uint64_t q_desc = smem_desc_k_sw128(smem_u32(smem + S::Q_OFF + i * S::QTILE));
+        const uint64_t k_desc = smem_desc_k_sw128(smem_u32(smem + S::K_OFF));
+        const uint64_t v_desc = pt_desc_v(smem_u32(smem + S::V_OFF), HV > 1 ? kHalf : 0);
+        const uint32_t s_tmem = tmem + S::S + i * 128, o_tmem = tmem + S::O + i * D;
         bool ok = mbar_wait(q_full, 0, status, kDevWaitMma, abort_flag);
-        auto issue_s = [&](int i, int st) {
-          const uint32_t k_addr = smem_u32(smem + S::K_OFF + st * S::TILE);
-          const uint32_t q_addr = smem_u32(smem + S::Q_OFF + i * S::TILE);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * kHalf + (kk % 4) * 32;
-            mma_f16(tmem + S::S + i * 128, smem_desc_k_sw128(q_addr + off), smem_desc_k_sw128(k_addr + off), idesc_qk,
-                    kk > 0 ? 1u : 0u);
-          }
-          mma_commit(&s_full[i]);
-        };
-        auto issue_pv = [&](int i, int st, bool first) {
-          const uint32_t v_addr = smem_u32(smem + S::V_OFF + st * S::TILE);
-#pragma unroll
-          for (int kk = 0; kk < kTileKeys / 16; ++kk)
-            mma_f16_ts(tmem + S::O + i * D, tmem + S::P + i * S::PSTEP + kk * 8,
-                       pt_desc_v(v_addr + kk * 2048, HV > 1 ? kHalf : 0), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
-        };
-        int ns[2] = {j0[0], j0[1]}, npv[2] = {j0[0], j0[1]};
-        int s_at[2] = {place(0, j0[0]), place(1, j0[1])}, pv_at[2] = {s_at[0], s_at[1]};
-        int k_rel = 0, v_rel = 0;
-        unsigned long long t_last = globaltimer_ns();
-        uint32_t idle = 0;
-        while (ok && v_rel < nu) {
-          bool progress = false;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i >= nq) continue;
-            const int j = npv[i], u = pv_at[i];
-            if (j < ns[i] && mbar_test(&p_full[i], (j - j0[i]) & 1u) && mbar_test(&v_ok[u % ST], (u / ST) & 1u)) {
+        // Tiles in the order of the rings; of the tile's own ones, S of the next is
+        // issued ahead of P V of this one.  A stage that this query tile does not
+        // need is released once it has landed.
+        int n = 0, prev = -1;  // own tiles so far; number of the previous tile if it is an own one
+        bool first = true;
+        for (int u = 0; u <= nu && ok; ++u) {
+          int x = -1;
+          if (u < nu) {
+            const int st = u % ST, kt = all.at(u0 + u);
+            ok = mbar_wait(&k_full[st], (u / ST) & 1u, status, kDevWaitMma, abort_flag);
+            if (!ok) break;
+            if (kt < mine.su || (kt >= mine.wu && kt < mine.hu)) {
+              x = n++;
               tc_fence_after();
-              issue_pv(i, u % ST, j == j0[i]);
-              if (!S::ALIAS) mma_commit(&p_empty[i]);
-              npv[i] = j + 1;
-              pv_at[i] = place(i, j + 1);
-              if (j + 1 == j1[i]) mma_commit(&pv_full[i]);
-              progress = true;
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)  // descriptor addresses are in 16-byte units
+                mma_f16(s_tmem + (x & 1) * 64, q_desc + ((kk / 4) * kQHalf + (kk % 4) * 32) / 16,
+                        k_desc + st * (S::TILE / 16) + ((kk / 4) * kHalf + (kk % 4) * 32) / 16, idesc_qk, kk > 0 ? 1u : 0u);
+              mma_commit(&s_full[2 * i + (x & 1)]);
+              mma_commit(&k_empty[st]);
+            } else {
+              mbar_arrive(&k_empty[st]);
             }
-            const int js = ns[i], us = s_at[i];
-            // S may be overwritten: P read (ALIAS; the MMAs run in order), or the scores read
-            if (js < j1[i] && (S::ALIAS ? npv[i] == js : mbar_test(&s_empty[i], ((js - j0[i]) & 1u) ^ 1u)) &&
-                mbar_test(&k_full[us % ST], (us / ST) & 1u)) {
+          }
+          if (u > 0) {
+            const int st = (u - 1) % ST;
+            ok = mbar_wait(&v_ok[st], ((u - 1) / ST) & 1u, status, kDevWaitMma, abort_flag);
+            if (!ok) break;
+            if (prev >= 0) {
+              ok = mbar_wait(&p_full[2 * i + (prev & 1)], (prev >> 1) & 1u, status, kDevWaitMma, abort_flag);
+              if (!ok) break;
               tc_fence_after();
-              issue_s(i, us % ST);
-              ns[i] = js + 1;
-              s_at[i] = place(i, js + 1);
-              progress = true;
+#pragma unroll
+              for (int kk = 0; kk < kTileKeys / 16; ++kk)
+                mma_f16_ts(o_tmem, s_tmem + (prev & 1) * 64 + kk * 8, v_desc + st * (S::TILE / 16) + kk * (2048 / 16),
+                           idesc_pv, (kk > 0 || !first) ? 1u : 0u);
+              first = false;
+              mma_commit(&pv_full[2 * i + (prev & 1)]);
+              mma_commit(&v_empty[st]);
+            } else {
+              mbar_arrive(&v_empty[st]);
             }
           }
-          const int ks = nq > 1 ? min(s_at[0], s_at[1]) : s_at[0], vs = nq > 1 ? min(pv_at[0], pv_at[1]) : pv_at[0];
-          // a stage that no query tile needed is released once it has landed
-          while (k_rel < ks && mbar_test(&k_full[k_rel % ST], (k_rel / ST) & 1u)) {
-            mma_commit(&k_empty[k_rel % ST]);
-            ++k_rel;
-            progress = true;
-          }
-          while (v_rel < vs && mbar_test(&v_ok[v_rel % ST], (v_rel / ST) & 1u)) {
-            mma_commit(&v_empty[v_rel % ST]);
-            ++v_rel;
-            progress = true;
-          }
-          if (progress) {
-            t_last = globaltimer_ns();
-            idle = 0;
-          } else if ((++idle & 63u) == 0) {
-            if (*abort_flag) {
-              ok = false;
-            } else if (globaltimer_ns() - t_last > kWaitBudgetNs) {
-              record_device_error(status, kDevWaitMma);
-              *abort_flag = 1;
-              ok = false;
-            }
-          }
+          prev = x;
         }
-        mma_commit(done);
-        mbar_wait(done, 0, status, kDevWaitDrain, nullptr);
+        if (ok) mma_commit(&o_full[i]);
+        mma_commit(&done[i]);
+        mbar_wait(&done[i], 0, status, kDevWaitDrain, nullptr);
       }
       __syncwarp();
     } else {
@@ -374,7 +357,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           uint8_t* v = smem + S::V_OFF + st * S::TILE;
           const int e = min(edges, kMaxEdges - 1);
           ++edges;
-          for (int r = (warp - 2) * 32 + lane; r < kTileKeys; r += 64) {
+          for (int r = lane; r < kTileKeys; r += 32) {
             const int64_t key = k0 + r;
             const bool some = key < key_end && (a.window <= 0 || key > p_lo - a.window || key < a.sinks);
             bool zero = !some;
@@ -400,7 +383,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_ok[st]);
       }
-      asm volatile("bar.sync 1, 320;" ::: "memory");  // the list of bad keys is complete
+      asm volatile("bar.sync 1, 288;" ::: "memory");  // the list of bad keys is complete
     }
   } else {
     // ---------------------------------------------------------------- softmax
@@ -413,33 +396,59 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const bool real = i < nq && row < tok * a.G && t < rq.n;
     const int64_t pos = real ? rq.first + t : kNowhere;
     const uint32_t lane_addr = static_cast<uint32_t>(qw * 32) << 16;
-    const uint32_t ts = tmem + lane_addr + S::S + i * 128;
+    const uint32_t ts0 = tmem + lane_addr + S::S + i * 128;
     const uint32_t to = tmem + lane_addr + S::O + i * D;
-    const uint32_t tp = tmem + lane_addr + S::P + i * S::PSTEP;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const int jb = i == 0 ? j0[0] : j0[1], je = i == 0 ? j1[0] : j1[1];
     const TileList mine = i == 0 ? own[0] : own[1];
+    // Which pages of a tile exist is asked tile by tile only if one of the stretch's is
+    // absent (a table read and a vote in every tile cost a tenth of it).
+    auto entry = [&](int kt) -> int32_t {  // lane's page of tile kt (present where there is none to ask for)
+      const int64_t key = static_cast<int64_t>(kt) * kTileKeys + lane * box;
+      return lane < boxes && key < rq.len ? __ldg(table + (key >> a.page_shift)) : 0;
+    };
+    bool holes = false;
+    if (jb < je) {
+      const int last = mine.at(je - 1);
+      auto scan = [&](int from, int to) {  // tiles from .. to
+        const int64_t e0 = (static_cast<int64_t>(from) * kTileKeys) >> a.page_shift;
+        const int64_t e1 = min(static_cast<int64_t>(to) * kTileKeys + kTileKeys - 1, rq.len - 1) >> a.page_shift;
+        for (int64_t e = e0 + lane; e <= e1; e += 32) {
+          const int32_t pg = __ldg(table + e);
+          holes |= pg < 0 || pg >= a.n_pages;
+        }
+      };
+      if (jb < mine.su) scan(mine.at(jb), min(last, mine.su - 1));
+      if (je > mine.su) scan(mine.at(max(jb, mine.su)), last);
+      holes = __any_sync(0xffffffffu, holes);
+    }
+    // tiles below plain_hi, at or past plain_lo or below plain_sk, are seen whole by every row
+    const int plain_hi = static_cast<int>(max(int64_t{0}, (a.causal ? min(rq.len, p_lo + 1) : rq.len)) / kTileKeys);
+    const int plain_lo =
+        a.window > 0 ? static_cast<int>((max(int64_t{0}, p_hi - a.window + 1) + kTileKeys - 1) / kTileKeys) : 0;
+    const int plain_sk = static_cast<int>(a.window > 0 ? min(a.sinks, rq.len) / kTileKeys : 0);
+    const int row_bit = min(a.page_shift, 6);
+    const bool positive = a.c2 > 0.0f;
+    const float cc = positive ? a.c2 : 1.0f;  // scores times this are in powers of two
     for (int j = jb; j < je; ++j) {
-      const uint32_t par = (j - jb) & 1u;
-      const int kt = mine.at(j);
-      // which of the tile's pages exist (read while the scores are on their way)
-      const int64_t box_key = static_cast<int64_t>(kt) * kTileKeys + lane * box;
-      int32_t pg = -1;
-      if (lane < boxes && box_key < rq.len) pg = __ldg(table + (box_key >> a.page_shift));
-      const uint32_t pages = __ballot_sync(0xffffffffu, pg >= 0 && pg < a.n_pages);
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], par, status, kDevWaitEpilogue, abort_flag));
+      const int x01 = (j - jb) & 1;
+      const uint32_t par = ((j - jb) >> 1) & 1u, ts = ts0 + x01 * 64;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&s_full[2 * i + x01], par)))
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * i + x01], par, status, kDevWaitEpilogue, abort_flag));
       if (!ok) break;
       tc_fence_after();
       uint32_t sr[kTileKeys];
 #pragma unroll
       for (int x = 0; x < kTileKeys; x += 32) tmem_ld_32x32b_x32(ts + x, *reinterpret_cast<uint32_t(*)[32]>(&sr[x]));
       tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (!S::ALIAS && lane == 0) mbar_arrive(&s_empty[i]);
-      const uint32_t whole = (1u << boxes) - 1u;
-      if (!plain(kt) || pages != whole) {
+      const int kt = mine.at(j);
+      if (holes || kt >= plain_hi || (kt < plain_lo && kt >= plain_sk)) {
+        uint32_t pages = 0xffffffffu;
+        if (holes) {
+          const int32_t pg = entry(kt);
+          pages = __ballot_sync(0xffffffffu, pg >= 0 && pg < a.n_pages);
+        }
         const int64_t k0 = static_cast<int64_t>(kt) * kTileKeys;
         // visible: x < hi and (x >= lo or x < sk), page present
         const int64_t hi64 = (a.causal ? min(rq.len, pos + 1) : (real ? rq.len : 0)) - k0;
@@ -448,26 +457,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int hi = static_cast<int>(max(int64_t{-1}, min(hi64, int64_t{kTileKeys})));
         const int lo = static_cast<int>(max(int64_t{-1}, min(lo64, int64_t{kTileKeys})));
         const int sk = static_cast<int>(max(int64_t{-1}, min(sk64, int64_t{kTileKeys})));
-        const int bs = min(a.page_shift, 7);
 #pragma unroll
         for (int x = 0; x < kTileKeys; ++x)
-          if (!(x < hi && (x >= lo || x < sk) && ((pages >> (x >> bs)) & 1u))) sr[x] = __float_as_uint(-INFINITY);
+          if (!(x < hi && (x >= lo || x < sk) && ((pages >> (x >> row_bit)) & 1u))) sr[x] = __float_as_uint(-INFINITY);
       }
-      // Row max of the scaled scores (the scale may be negative: scale first)
-      float mx8[8];
-      const float2 c2 = make_float2(a.c2, a.c2), zero2 = make_float2(-0.0f, -0.0f);
-      if (a.c2 < 0.0f || a.c2 == 0.0f) {  // keep masked scores at -inf: max over the visible ones only
+      if (!positive) {  // rare: the order of the scaled scores is another one
 #pragma unroll
         for (int x = 0; x < kTileKeys; ++x)
           if (sr[x] != __float_as_uint(-INFINITY)) sr[x] = __float_as_uint(__uint_as_float(sr[x]) * a.c2);
-      } else {
-#pragma unroll
-        for (int x = 0; x < kTileKeys; x += 2) {
-          const float2 v = ffma2(make_float2(__uint_as_float(sr[x]), __uint_as_float(sr[x + 1])), c2, zero2);
-          sr[x] = __float_as_uint(v.x);
-          sr[x + 1] = __float_as_uint(v.y);
-        }
       }
+      float mx8[8];  // row max: three-input max, eight chains
 #pragma unroll
       for (int x = 0; x < 8; ++x) mx8[x] = __uint_as_float(sr[x]);
 #pragma unroll
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
         for (int y = 0; y < 8; ++y)
           mx8[y] = pt_max3(mx8[y], __uint_as_float(sr[x + y]), x + 8 + y < kTileKeys ? __uint_as_float(sr[x + 8 + y]) : mx8[y]);
-      const float mx = pt_max3(pt_max3(mx8[0], mx8[1], mx8[2]), pt_max3(mx8[3], mx8[4], mx8[5]), pt_max3(mx8[6], mx8[7], mx8[7]));
+      const float mx = cc * pt_max3(pt_max3(mx8[0], mx8[1], mx8[2]), pt_max3(mx8[3], mx8[4], mx8[5]), pt_max3(mx8[6], mx8[7], mx8[7]));
       if (!(mx < INFINITY)) l = NAN;  // a NaN or an infinite score: the row is NaN, whatever its exps give
       float m_new = fmaxf(m, mx);
       const bool grow = m_new > m + 8.0f || (m == -INFINITY && m_new != -INFINITY);
@@ -484,23 +483,24 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const float alpha = !grow || m == -INFINITY ? (grow ? 0.0f : 1.0f) : ex2(m - m_new);
       uint32_t pk[kTileKeys / 2];
       {
-        const float2 nm = make_float2(-base, -base), one = make_float2(1.0f, 1.0f);
+        const float2 nm = make_float2(-base, -base), one = make_float2(1.0f, 1.0f), c2 = make_float2(cc, cc);
         float2 ls[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int x = 0; x < kTileKeys; x += 2) {
-          const float2 z = ffma2(make_float2(__uint_as_float(sr[x]), __uint_as_float(sr[x + 1])), one, nm);
-          const float2 y = ((x >> 1) & 3) < 2 ? pt_ex2_poly(z) : make_float2(ex2(z.x), ex2(z.y));
+          const float2 z = ffma2(make_float2(__uint_as_float(sr[x]), __uint_as_float(sr[x + 1])), c2, nm);
+          const float2 y = ((x >> 1) & 3) < kPolyPairs ? pt_ex2_poly(z) : make_float2(ex2(z.x), ex2(z.y));
           pk[x >> 1] = pack2<BF16>(y.x, y.y);
           ls[(x >> 1) & 3] = ffma2(y, one, ls[(x >> 1) & 3]);
         }
         l = fmaf(l, alpha, ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y)) + ((ls[2].x + ls[2].y) + (ls[3].x + ls[3].y)));
       }
-      if (!S::ALIAS) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&p_empty[i], par ^ 1u, status, kDevWaitEpilogue, abort_flag));
-        if (!ok) break;
-      }
       if (j > jb && __any_sync(0xffffffffu, grow)) {
-        // The previous P V is complete (p_empty; ALIAS: S was issued behind it): rescale O.
+        // Rescale O, once the previous P V is in it.  Its barrier can be in that phase or
+        // just past it: the P V two before that came ahead of a score tile already read,
+        // the next one waits for this warp.
+        const int prev = j - jb - 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&pv_full[2 * i + (prev & 1)], (prev >> 1) & 1u, status, kDevWaitEpilogue, abort_flag));
+        if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int d = 0; d < D; d += 32) {
@@ -512,17 +512,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           tmem_st_32x32b_x32(to + d, r);
         }
       }
-      tmem_st_32x32b_x32(tp, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
-      tmem_st_32x32b_x32(tp + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+      tmem_st_32x32b_x32(ts, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[i]);
+      if (lane == 0) mbar_arrive(&p_full[2 * i + x01]);
       m = m_new;
     }
     if (ok && je > jb)
-      ok = __all_sync(0xffffffffu, mbar_wait(&pv_full[i], 0, status, kDevWaitEpilogue, abort_flag));
-    asm volatile("bar.sync 1, 320;" ::: "memory");  // the list of bad keys is complete
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[i], 0, status, kDevWaitEpilogue, abort_flag));
+    asm volatile("bar.sync 1, 288;" ::: "memory");  // the list of bad keys is complete
     tc_fence_after();
     if (ok && i < nq) {
       const int64_t tr = rq.t0 + t;
@@ -614,7 +613,7 @@ cudaError_t launch_tiles(const PagedArgs& a, cudaStream_t s) {
   const uint32_t qb[3] = {64, static_cast<uint32_t>(a.G), static_cast<uint32_t>(tok)};
   const uint64_t kd[3] = {D, page, static_cast<uint64_t>(a.n_pages) * a.Hkv};
   const uint64_t ks[2] = {D * 2, page * D * 2};
-  const uint32_t kb[3] = {64, static_cast<uint32_t>(page < 128 ? page : 128), 1};
+  const uint32_t kb[3] = {64, static_cast<uint32_t>(page < kTileKeys ? page : kTileKeys), 1};
   if (!make_tensor_map_3d(&maps.q, dt, a.q, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_3d(&maps.k, dt, a.k, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_3d(&maps.v, dt, a.v, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B))

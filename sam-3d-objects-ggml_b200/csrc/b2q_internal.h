@@ -346,7 +346,7 @@ struct PagedArgs {
   float* part_o;          // [T][Hq][splits][D]
   float2* part_ml;        // [T][Hq][splits] (max, sum)
 };
-constexpr int kTileRows = 128, kTileKeys = 128;  // of the tensor-memory kernel
+constexpr int kTileRows = 128, kTileKeys = 64;  // of the tensor-memory kernel
 struct PagedPlan {
   bool tiles = false;  // the tile kernel (b2q_attention_paged_tile.cu), else the rows kernel
   int64_t splits = 1, split_units = 0, part_o_bytes = 0, part_ml_bytes = 0;

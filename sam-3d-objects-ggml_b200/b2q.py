@@ -730,10 +730,21 @@ def mul_mat_q_simt(wtype: int, w, a, k: int, stream=None):
     return y
 
 
+# The cached-decoding calls below are a few microseconds of device work at small
+# sizes, so their wrappers read each tensor property once and take the current
+# stream's handle without building a Stream object.
+def _raw_stream(stream, t) -> int:
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _type16(dtype) -> int:
     torch = _torch()
-    assert dtype in (torch.float16, torch.bfloat16)
-    return TYPE_F16 if dtype == torch.float16 else TYPE_BF16
+    if dtype is torch.float16:
+        return TYPE_F16
+    assert dtype is torch.bfloat16
+    return TYPE_BF16
 
 
 def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_tokens: int, out=None, stream=None):
@@ -744,20 +755,25 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
     counts int32 [2]: pages needed, tokens without a slot).  out: those five
     tensors, to be written again."""
     torch = _torch()
+    i32 = torch.int32
     B, W = block_table.shape
-    for t in (cached, new, free_pages, block_table):
-        assert t.dtype == torch.int32
-    assert cached.shape == (B,) and new.shape == (B,) and (B == 0 or W <= 1 or block_table.stride(1) == 1)
+    assert cached.dtype is i32 and new.dtype is i32 and free_pages.dtype is i32 and block_table.dtype is i32
+    assert cached.numel() == B and new.numel() == B
     assert cached.is_contiguous() and new.is_contiguous() and free_pages.is_contiguous()
+    ldt, ldc = block_table.stride()
+    assert ldc == 1 or W <= 1 or B == 0
     if out is None:
-        e = lambda n, dt: torch.empty(n, dtype=dt, device=block_table.device)  # noqa: E731
-        out = (e(max_tokens, torch.int64), e(max_tokens, torch.int32), e(B + 1, torch.int32), e(B, torch.int32),
-               e(2, torch.int32))
+        dev = block_table.device
+        out = (torch.empty(max_tokens, dtype=torch.int64, device=dev), torch.empty(max_tokens, dtype=i32, device=dev),
+               torch.empty(B + 1, dtype=i32, device=dev), torch.empty(B, dtype=i32, device=dev),
+               torch.empty(2, dtype=i32, device=dev))
     slots, positions, cu, kv_len, counts = out
-    rc = lib().b2q_kv_cache_plan(_ptr(cached), _ptr(new), B, page_size, _ptr(free_pages), free_pages.numel(),
-                                 _ptr(block_table), W, max(block_table.stride(0), W) * 4, max_tokens, _ptr(slots),
-                                 _ptr(positions), _ptr(cu), _ptr(kv_len), _ptr(counts), _stream(stream))
-    _check("b2q_kv_cache_plan", rc)
+    rc = (_lib or _lib_obj()).b2q_kv_cache_plan(
+        cached.data_ptr(), new.data_ptr(), B, page_size, free_pages.data_ptr(), free_pages.numel(),
+        block_table.data_ptr(), W, 4 * (ldt if ldt > W else W), max_tokens, slots.data_ptr(), positions.data_ptr(),
+        cu.data_ptr(), kv_len.data_ptr(), counts.data_ptr(), _raw_stream(stream, block_table))
+    if rc:
+        _check("b2q_kv_cache_plan", rc)
     return out
 
 
@@ -770,26 +786,35 @@ def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq
     RMS norm; k and v go to slots (int64 [T]) of k_cache, v_cache
     [pages, Hkv, page size, D], in place."""
     torch = _torch()
-    T = qkv.shape[0]
+    T, width = qkv.shape
+    n_pages, kv_heads, page_size, dim = k_cache.shape
+    dt = k_cache.dtype
     axes = len(sections)
-    assert qkv.dtype == torch.float32 and qkv.shape[1] == (Hq + 2 * Hkv) * D and qkv.stride(1) == 1
-    assert k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype
-    assert k_cache.shape[1] == Hkv and k_cache.shape[3] == D and k_cache.is_contiguous() and v_cache.is_contiguous()
-    assert slots.dtype == torch.int64 and slots.shape == (T,) and slots.is_contiguous()
+    ld, ldc = qkv.stride()
+    assert qkv.dtype is torch.float32 and width == (Hq + 2 * Hkv) * D and (ldc == 1 or T == 0)
+    assert v_cache.shape == k_cache.shape and v_cache.dtype is dt and kv_heads == Hkv and dim == D
+    assert k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert slots.dtype is torch.int64 and slots.numel() == T and slots.is_contiguous()
+    pos_ptr = freq_ptr = None
+    pos_stride = T
     if axes:
-        assert positions.dtype == torch.int32 and positions.shape == (axes, T) and (T <= 1 or positions.stride(1) == 1)
-        assert inv_freq.dtype == torch.float32 and inv_freq.numel() == sum(sections) and inv_freq.is_contiguous()
+        assert positions.dtype is torch.int32 and positions.shape == (axes, T)
+        assert inv_freq.dtype is torch.float32 and inv_freq.numel() == sum(sections) and inv_freq.is_contiguous()
+        pos_ptr, freq_ptr = positions.data_ptr(), inv_freq.data_ptr()
+        pos_stride, step = positions.stride()
+        assert step == 1 or T <= 1
+        if axes == 1:
+            pos_stride = T
     if out is None:
-        out = torch.empty((T, Hq * D), dtype=k_cache.dtype, device=qkv.device)
-    assert out.dtype == k_cache.dtype
-    sec = (ctypes.c_int32 * max(axes, 1))(*sections)
-    rc = lib().b2q_qkv_rope_cache(_ptr(qkv), T, Hq, Hkv, D, qkv.stride(0) * 4, 1 if norm else 0, _ptr(gamma_q),
-                                  _ptr(gamma_k), eps, _ptr(positions) if axes else None,
-                                  positions.stride(0) if axes > 1 else T, axes, sec,
-                                  _ptr(inv_freq) if axes else None, 1 if interleaved else 0, _type16(k_cache.dtype),
-                                  _ptr(out), out.stride(0) * 2, _ptr(k_cache), _ptr(v_cache), _ptr(slots),
-                                  k_cache.shape[0], k_cache.shape[2], _stream(stream))
-    _check("b2q_qkv_rope_cache", rc)
+        out = torch.empty((T, Hq * D), dtype=dt, device=qkv.device)
+    assert out.dtype is dt
+    sec = (ctypes.c_int32 * 3)(*sections)
+    rc = (_lib or _lib_obj()).b2q_qkv_rope_cache(
+        qkv.data_ptr(), T, Hq, Hkv, D, ld * 4, 1 if norm else 0, _ptr(gamma_q), _ptr(gamma_k), eps, pos_ptr, pos_stride,
+        axes, sec, freq_ptr, 1 if interleaved else 0, _type16(dt), out.data_ptr(), out.stride(0) * 2, k_cache.data_ptr(),
+        v_cache.data_ptr(), slots.data_ptr(), n_pages, page_size, _raw_stream(stream, qkv))
+    if rc:
+        _check("b2q_qkv_rope_cache", rc)
     return out
 
 
@@ -806,29 +831,38 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
     over the kv_len[b] cached keys of [pages, Hkv, page size, D] pools through
     block_table int32 [B, W] -> [T, Hq * D].  window > 0 keeps the last `window`
     keys and the first `sinks`; max_new / max_kv bound the requests."""
-    import math
     torch = _torch()
-    T = q.shape[0]
+    T, width = q.shape
     n_pages, Hkv, page_size, D = k_cache.shape
     B, W = block_table.shape
-    assert q.dtype == k_cache.dtype == v_cache.dtype and k_cache.shape == v_cache.shape
-    assert q.shape[1] == Hq * D and q.stride(1) == 1
-    assert k_cache.is_contiguous() and v_cache.is_contiguous() and (W <= 1 or block_table.stride(1) == 1)
-    assert block_table.dtype == kv_len.dtype == cu_new.dtype == torch.int32
-    assert kv_len.shape == (B,) and cu_new.shape == (B + 1,) and kv_len.is_contiguous() and cu_new.is_contiguous()
+    dt, i32 = q.dtype, torch.int32
+    ldq, ldc = q.stride()
+    ldt, ldtc = block_table.stride()
+    assert k_cache.dtype is dt and v_cache.dtype is dt and v_cache.shape == k_cache.shape
+    assert width == Hq * D and (ldc == 1 or T == 0) and (ldtc == 1 or W <= 1 or B == 0)
+    assert k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert block_table.dtype is i32 and kv_len.dtype is i32 and cu_new.dtype is i32
+    assert kv_len.numel() == B and cu_new.numel() == B + 1 and kv_len.is_contiguous() and cu_new.is_contiguous()
+    L = _lib or _lib_obj()
     if scale is None:
-        scale = 1.0 / math.sqrt(D)
+        scale = D ** -0.5
     if out is None:
-        out = torch.empty((T, Hq * D), dtype=q.dtype, device=q.device)
-    if ws is None:
-        need = attention_paged_workspace_bytes(B, T, max_new, max_kv, Hq, Hkv, D, causal, window, sinks)
-        ws = _empty_aligned(need, q.device) if need else None
-    rc = lib().b2q_attention_paged(_type16(q.dtype), _ptr(q), q.stride(0) * 2, _ptr(cu_new), B, T, max_new,
-                                   _ptr(k_cache), _ptr(v_cache), n_pages, page_size, _ptr(block_table), W,
-                                   max(block_table.stride(0), W) * 4, _ptr(kv_len), max_kv, Hq, Hkv, D, scale,
-                                   1 if causal else 0, window, sinks, _ptr(out), out.stride(0) * 2, _ptr(ws),
-                                   ws.numel() if ws is not None else 0, _stream(stream))
-    _check("b2q_attention_paged", rc)
+        out = torch.empty((T, width), dtype=dt, device=q.device)
+    ws_ptr, ws_bytes = None, 0
+    if ws is not None:
+        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
+    else:
+        ws_bytes = L.b2q_attention_paged_workspace_bytes(B, T, max_new, max_kv, Hq, Hkv, D, 1 if causal else 0, window, sinks)
+        if ws_bytes:  # the allocator's blocks are 512-byte aligned
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            ws_ptr = ws.data_ptr()
+    rc = L.b2q_attention_paged(
+        _type16(dt), q.data_ptr(), ldq * 2, cu_new.data_ptr(), B, T, max_new, k_cache.data_ptr(), v_cache.data_ptr(),
+        n_pages, page_size, block_table.data_ptr(), W, 4 * (ldt if ldt > W else W), kv_len.data_ptr(), max_kv, Hq, Hkv, D,
+        scale, 1 if causal else 0, window, sinks, out.data_ptr(), out.stride(0) * 2, ws_ptr, ws_bytes,
+        _raw_stream(stream, q))
+    if rc:
+        _check("b2q_attention_paged", rc)
     return out
 
 
@@ -841,15 +875,24 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
     dequantized values -> fp32 [m, n]; with resid: resid + gate * (w.x + bias)
     (out=resid updates in place)."""
     torch = _torch()
-    m = x.shape[0]
-    assert x.shape[1] == k and (k <= 1 or x.stride(1) == 1)
-    xtype = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}[x.dtype]
+    m, width = x.shape
+    ld, ldc = x.stride()
+    assert width == k and (ldc == 1 or k <= 1 or m == 0)
+    dt = x.dtype
+    if dt is torch.float32:
+        xtype, size = TYPE_F32, 4
+    elif dt is torch.float16:
+        xtype, size = TYPE_F16, 2
+    else:
+        assert dt is torch.bfloat16
+        xtype, size = TYPE_BF16, 2
     if out is None:
         out = torch.empty((m, n), dtype=torch.float32, device=x.device)
-    rc = lib().b2q_mul_vec(wtype, _ptr(packed), n, k, xtype, _ptr(x), m, x.stride(0) * x.element_size(), _ptr(bias),
-                           _ptr(gate), _ptr(resid), resid.stride(0) * 4 if resid is not None else 0, _ptr(out),
-                           out.stride(0) * 4, _stream(stream))
-    _check("b2q_mul_vec", rc)
+    rc = (_lib or _lib_obj()).b2q_mul_vec(
+        wtype, packed.data_ptr(), n, k, xtype, x.data_ptr(), m, ld * size, _ptr(bias), _ptr(gate), _ptr(resid),
+        0 if resid is None else resid.stride(0) * 4, out.data_ptr(), out.stride(0) * 4, _raw_stream(stream, x))
+    if rc:
+        _check("b2q_mul_vec", rc)
     return out
 
 

@@ -8,11 +8,14 @@
 //   k, v of token t to slot[t] of [page][kv head][token in page][D]
 //
 // Bound by its bytes: 4 read and 2 written per value of a row, each once.  A
-// CTA takes kRopeTokens (or one, where there are few) tokens: its threads
+// CTA takes up to kRopeTokens tokens (one, where there are few): its threads
 // first compute the tokens' cosines and sines into shared memory, one pair
-// each, which all the heads then share; a row of D values is D / 4 lanes of
-// one float4 each, so a warp's access is 512 contiguous bytes, and the RMS
-// sum and the partner of a pair are shuffles inside that group of lanes.
+// each, which all the heads then share.  A lane takes 8 neighbouring values, so
+// a head is D / 8 lanes, and the RMS sum and the partner of a pair are shuffles
+// among them; a thread's next rows are loaded while it works on these.  q and k
+// rows and v rows are two loops, and the kinds of rotation and norm are template
+// arguments: with one loop of 4-value lanes the rows cost 136 instructions a
+// warp, and 32800 tokens of 48 heads of 64 took 200 us.
 //
 // The angle is formed in double and reduced to a fraction of a turn before it
 // is rounded to fp32: in fp32 the product of a position of 10^4 and a frequency
@@ -27,20 +30,40 @@ namespace b2q {
 namespace {
 
 constexpr int kRopeThreads = 256;
+constexpr int kRopeTokens = 8;  // most tokens of a CTA
+constexpr int kRopeBatch = 2;   // rows of a thread whose loads are under way together
+enum { kInterleaved = 0, kHalves = 1, kHalvesOdd = 2 };  // pairs (2i, 2i + 1); (i, i + R), R % 8 == 0; any R
 
+struct F8 {
+  float v[8];
+};
+__device__ __forceinline__ F8 load8(const float* p) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
 template <bool BF16>
-__device__ __forceinline__ uint2 pack4(float4 v) {
-  uint2 r;
-  if constexpr (BF16) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    r.x = *reinterpret_cast<const uint32_t*>(&a);
-    r.y = *reinterpret_cast<const uint32_t*>(&b);
-  } else {
-    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
-    r.x = *reinterpret_cast<const uint32_t*>(&a);
-    r.y = *reinterpret_cast<const uint32_t*>(&b);
+__device__ __forceinline__ uint4 pack8(const F8& f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&x);
+    } else {
+      const __half2 x = __floats2half2_rn(f.v[2 * i], f.v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
   }
-  return r;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// 16 bytes to a row that is 8-byte aligned at least
+__device__ __forceinline__ void store8(uint16_t* dst, uint4 w, bool wide) {
+  if (wide) {
+    __stcs(reinterpret_cast<uint4*>(dst), w);
+  } else {
+    __stcs(reinterpret_cast<uint2*>(dst), make_uint2(w.x, w.y));
+    __stcs(reinterpret_cast<uint2*>(dst) + 1, make_uint2(w.z, w.w));
+  }
 }
 
 // sum over the LPR lanes of a row
@@ -51,15 +74,37 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs a, int tokens_per_cta) {
-  constexpr int LPR = D / 4;            // lanes per row
+// A thread's rows (token, head) of n heads, `step` rows apart.
+struct RowWalk {
+  int tl, h, n, dt, dh;
+  __device__ __forceinline__ RowWalk(int first, int step, int heads) : n(heads) {
+    tl = first / n;
+    h = first - tl * n;
+    dt = step / n;
+    dh = step - dt * n;
+  }
+  __device__ __forceinline__ void next() {
+    tl += dt;
+    h += dh;
+    if (h >= n) h -= n, ++tl;
+  }
+};
+
+template <int D, bool BF16, bool NORM, int MODE>
+__global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs a, int tokens_per_cta, bool wide) {
+  constexpr int LPR = D / 8;               // lanes per row
   constexpr int RPP = kRopeThreads / LPR;  // rows per pass of the CTA
-  extern __shared__ float2 rope_cs[];   // [tokens_per_cta][R] (cos, sin)
+  extern __shared__ __align__(16) float2 rope_cs[];  // [tokens_per_cta][R] (cos, sin)
+  __shared__ int64_t rope_at[kRopeTokens];           // a token's place in kv head 0 of the cache, or -1
   const int tid = threadIdx.x;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens_per_cta;
   const int nt = static_cast<int>(min(static_cast<int64_t>(tokens_per_cta), a.T - t0));
   const int R = a.rot;
+  // this CTA's heads: lo .. hi - 1 of q, k, v heads in a row
+  const int heads = a.Hq + 2 * a.Hkv, n_qk = a.Hq + a.Hkv;
+  const int lo = static_cast<int>(static_cast<int64_t>(heads) * blockIdx.y / gridDim.y);
+  const int hi = static_cast<int>(static_cast<int64_t>(heads) * (blockIdx.y + 1) / gridDim.y);
+  const int l = tid % LPR;
   for (int i = tid; i < nt * R; i += kRopeThreads) {
     const int t = i / R, p = i - t * R;
     const int axis = p >= a.sec1 ? (p >= a.sec2 ? 2 : 1) : 0;
@@ -69,97 +114,129 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
     sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
     rope_cs[i] = make_float2(cs, sn);
   }
+  if (tid < nt && a.Hkv > 0) {
+    const int64_t slot = a.slots[t0 + tid];
+    const int64_t page = slot >> a.page_shift, off = slot & ((int64_t{1} << a.page_shift) - 1);
+    rope_at[tid] = slot >= 0 && slot < a.n_slots ? ((page * a.Hkv << a.page_shift) + off) * D : -1;
+  }
   __syncthreads();
+  const int64_t head_step = static_cast<int64_t>(D) << a.page_shift;
 
-  const int heads = a.Hq + 2 * a.Hkv;
-  const int h_lo = static_cast<int>(static_cast<int64_t>(heads) * blockIdx.y / gridDim.y);
-  const int h_n = static_cast<int>(static_cast<int64_t>(heads) * (blockIdx.y + 1) / gridDim.y) - h_lo;
-  const int l = tid % LPR, r0 = tid / LPR;
-  const int n_rows = nt * h_n;
-  const unsigned group = (LPR == 32) ? 0 : (tid & 31) / LPR * LPR;  // first lane of this row's group
-  // Every lane runs every pass (the shuffles name the whole warp); rows past
-  // the end reload the last row and store nothing.
-  for (int r = r0; r - r0 < n_rows; r += RPP) {
-    const int rc = min(r, n_rows - 1);
-    const int tl = rc / h_n, h = h_lo + (rc - tl * h_n);
-    const int64_t t = t0 + tl;
-    const float* row = a.qkv + t * a.ldqkv + static_cast<int64_t>(h) * D;
-    float4 v = __ldg(reinterpret_cast<const float4*>(row) + l);
-    const bool is_v = h >= a.Hq + a.Hkv;
-    // (the shuffles below run for v rows too: a warp may hold both kinds)
-    float scale = 1.0f;
-    if (a.norm) {
-      const float ss = row_sum<LPR>((v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w));
-      if (!is_v) scale = rsqrtf(ss * (1.0f / D) + a.eps);
-    }
-    const float* gamma = is_v ? nullptr : (h < a.Hq ? a.gamma_q : a.gamma_k);
-    const int64_t g0 = static_cast<int64_t>(h < a.Hq ? h : h - a.Hq) * D;
-    if (a.norm && !is_v) {
-      v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
-      if (gamma) {
-        const float4 g = __ldg(reinterpret_cast<const float4*>(gamma + g0) + l);
-        v.x *= g.x, v.y *= g.y, v.z *= g.z, v.w *= g.w;
-      }
-    }
-    const int d0 = 4 * l;
-    const float2* cs = rope_cs + tl * R;
-    if (a.interleaved) {
-      if (!is_v) {
-        if (d0 < 2 * R) {
-          const float2 c = cs[2 * l];
-          const float x = v.x * c.x - v.y * c.y;
-          v.y = v.y * c.x + v.x * c.y;
-          v.x = x;
-        }
-        if (d0 + 2 < 2 * R) {
-          const float2 c = cs[2 * l + 1];
-          const float x = v.z * c.x - v.w * c.y;
-          v.w = v.w * c.x + v.z * c.y;
-          v.z = x;
-        }
-      }
-    } else if (R % 4 == 0) {  // the four partners sit in one lane
-      const bool second = d0 >= R;
-      const int src = static_cast<int>(group) + (second ? (l - R / 4 + LPR) % LPR : (l + R / 4) % LPR);
-      float4 o;
-      o.x = __shfl_sync(0xffffffffu, v.x, src);
-      o.y = __shfl_sync(0xffffffffu, v.y, src);
-      o.z = __shfl_sync(0xffffffffu, v.z, src);
-      o.w = __shfl_sync(0xffffffffu, v.w, src);
-      if (!is_v && d0 < 2 * R) {
-        const float4* c4 = reinterpret_cast<const float4*>(cs + (second ? d0 - R : d0));
-        const float4 c01 = c4[0], c23 = c4[1];
-        const float sg = second ? 1.0f : -1.0f;
-        v.x = v.x * c01.x + sg * (o.x * c01.y);
-        v.y = v.y * c01.z + sg * (o.y * c01.w);
-        v.z = v.z * c23.x + sg * (o.z * c23.y);
-        v.w = v.w * c23.z + sg * (o.w * c23.w);
-      }
-    } else if (!is_v) {  // partners across lanes: read them from the row itself
-      float* e = reinterpret_cast<float*>(&v);
+  // Every lane runs every pass (the shuffles name the whole warp); rows past the
+  // end repeat the CTA's last token and store nothing.
+  if (lo < min(hi, n_qk)) {
+    const int n = min(hi, n_qk) - lo, rows = nt * n;
+    RowWalk w(tid / LPR, RPP, n);
+    const unsigned group = (tid & 31) / LPR * LPR;  // first lane of this row's group
+    for (int r = 0; r < rows; r += kRopeBatch * RPP) {
+      F8 x[kRopeBatch];
+      int xt[kRopeBatch], xh[kRopeBatch];
+      float scale[kRopeBatch];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = d0 + i;
-        if (d >= 2 * R) continue;
-        const bool second = d >= R;
-        const int dp = second ? d - R : d + R;
-        float o = __ldg(row + dp) * scale;
-        if (a.norm && gamma) o *= __ldg(gamma + g0 + dp);
-        const float2 c = cs[second ? dp : d];
-        e[i] = e[i] * c.x + (second ? o * c.y : -(o * c.y));
+      for (int u = 0; u < kRopeBatch; ++u) {
+        xt[u] = w.tl;
+        xh[u] = lo + w.h;
+        x[u] = load8(a.qkv + (t0 + min(w.tl, nt - 1)) * a.ldqkv + static_cast<int64_t>(xh[u]) * D + 8 * l);
+        w.next();
+      }
+      if constexpr (NORM) {
+#pragma unroll
+        for (int u = 0; u < kRopeBatch; ++u) {
+          float ss = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss = fmaf(x[u].v[i], x[u].v[i], ss);
+          scale[u] = ss;
+        }
+#pragma unroll
+        for (int u = 0; u < kRopeBatch; ++u) scale[u] = rsqrtf(row_sum<LPR>(scale[u]) * (1.0f / D) + a.eps);
+      }
+#pragma unroll
+      for (int u = 0; u < kRopeBatch; ++u) {
+        const int h = xh[u], tt = min(xt[u], nt - 1);
+        const float* gamma = h < a.Hq ? a.gamma_q : a.gamma_k;
+        const int64_t g0 = static_cast<int64_t>(h < a.Hq ? h : h - a.Hq) * D;
+        F8& v = x[u];
+        if constexpr (NORM) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v.v[i] *= scale[u];
+          if (gamma) {
+            const F8 g = load8(gamma + g0 + 8 * l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v.v[i] *= g.v[i];
+          }
+        }
+        const float2* cs = rope_cs + tt * R;
+        if constexpr (MODE == kInterleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (4 * l + i < R) {
+              const float2 c = cs[4 * l + i];
+              const float y = v.v[2 * i] * c.x - v.v[2 * i + 1] * c.y;
+              v.v[2 * i + 1] = v.v[2 * i + 1] * c.x + v.v[2 * i] * c.y;
+              v.v[2 * i] = y;
+            }
+        } else if constexpr (MODE == kHalves) {  // the eight partners sit in one lane
+          const bool second = 8 * l >= R;
+          const int src = static_cast<int>(group) + (second ? (l - R / 8 + LPR) % LPR : (l + R / 8) % LPR);
+          F8 o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.v[i] = __shfl_sync(0xffffffffu, v.v[i], src);
+          if (8 * l < 2 * R) {
+            const float4* c4 = reinterpret_cast<const float4*>(cs + (second ? 8 * l - R : 8 * l));
+            const float sg = second ? 1.0f : -1.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 c = c4[i];
+              v.v[2 * i] = v.v[2 * i] * c.x + sg * (o.v[2 * i] * c.y);
+              v.v[2 * i + 1] = v.v[2 * i + 1] * c.z + sg * (o.v[2 * i + 1] * c.w);
+            }
+          }
+        } else {  // partners across lanes: read them from the row itself
+          const float* row = a.qkv + (t0 + tt) * a.ldqkv + static_cast<int64_t>(h) * D;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int d = 8 * l + i;
+            if (d >= 2 * R) continue;
+            const bool second = d >= R;
+            const int dp = second ? d - R : d + R;
+            float o = __ldg(row + dp);
+            if constexpr (NORM) {
+              o *= scale[u];
+              if (gamma) o *= __ldg(gamma + g0 + dp);
+            }
+            const float2 c = cs[second ? dp : d];
+            v.v[i] = v.v[i] * c.x + (second ? o * c.y : -(o * c.y));
+          }
+        }
+        if (xt[u] >= nt) continue;
+        const uint4 p = pack8<BF16>(v);
+        if (h < a.Hq) {
+          store8(a.q + (t0 + tt) * a.ldq + static_cast<int64_t>(h) * D + 8 * l, p, wide);
+        } else {
+          const int64_t at = rope_at[tt];
+          if (at >= 0) store8(a.k_cache + at + (h - a.Hq) * head_step + 8 * l, p, wide);
+        }
       }
     }
-    if (r >= n_rows) continue;
-    const uint2 w = pack4<BF16>(v);
-    if (h < a.Hq) {
-      *(reinterpret_cast<uint2*>(a.q + t * a.ldq + static_cast<int64_t>(h) * D) + l) = w;
-    } else {
-      const int64_t slot = a.slots[t];
-      if (slot >= 0 && slot < a.n_slots) {
-        const int hk = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
-        const int64_t page = slot >> a.page_shift, off = slot & ((int64_t{1} << a.page_shift) - 1);
-        uint16_t* cache = is_v ? a.v_cache : a.k_cache;
-        *(reinterpret_cast<uint2*>(cache + ((((page * a.Hkv + hk) << a.page_shift) + off) * D)) + l) = w;
+  }
+  if (max(lo, n_qk) < hi) {
+    const int h0 = max(lo, n_qk), n = hi - h0, rows = nt * n;
+    RowWalk w(tid / LPR, RPP, n);
+    for (int r = 0; r < rows; r += 2 * kRopeBatch * RPP) {
+      F8 x[2 * kRopeBatch];
+      int xt[2 * kRopeBatch], xh[2 * kRopeBatch];
+#pragma unroll
+      for (int u = 0; u < 2 * kRopeBatch; ++u) {
+        xt[u] = w.tl;
+        xh[u] = h0 + w.h;
+        if (w.tl < nt) x[u] = load8(a.qkv + (t0 + w.tl) * a.ldqkv + static_cast<int64_t>(xh[u]) * D + 8 * l);
+        w.next();
+      }
+#pragma unroll
+      for (int u = 0; u < 2 * kRopeBatch; ++u) {
+        if (xt[u] >= nt) continue;
+        const int64_t at = rope_at[xt[u]];
+        if (at >= 0) store8(a.v_cache + at + (xh[u] - n_qk) * head_step + 8 * l, pack8<BF16>(x[u]), wide);
       }
     }
   }
@@ -169,12 +246,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
 
 cudaError_t launch_rope_cache(const RopeArgs& a, int D, bool bf16, int num_sms, cudaStream_t s) {
   const int heads = a.Hq + 2 * a.Hkv;
-  const int rows_per_pass = kRopeThreads / (D / 4);
+  const int rows_per_pass = kRopeThreads / (D / 8);
   // Tokens per CTA: as many as fill the threads with one pair each, while that
   // still gives every SM two CTAs; with fewer tokens, one per CTA and the heads
   // shared out over grid.y, down to one pass of rows each.
   int tpc = a.rot > 0 ? kRopeThreads / a.rot : kRopeThreads / (D / 2);
-  if (tpc > 8) tpc = 8;
+  if (tpc > kRopeTokens) tpc = kRopeTokens;
   if (a.T < static_cast<int64_t>(tpc) * num_sms * 2) tpc = 1;
   const int64_t gx = (a.T + tpc - 1) / tpc;
   if (gx > INT32_MAX) return cudaErrorInvalidValue;
@@ -186,12 +263,28 @@ cudaError_t launch_rope_cache(const RopeArgs& a, int D, bool bf16, int num_sms, 
   }
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
   const int smem = tpc * (a.rot > 0 ? a.rot : 1) * 8;
-#define B2Q_ROPE(DD, BF) rope_cache_kernel<DD, BF><<<grid, kRopeThreads, smem, s>>>(a, tpc)
+  const auto odd = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+  const bool wide = !odd(a.q) && a.ldq % 8 == 0 && !odd(a.k_cache) && !odd(a.v_cache);
+  const int mode = a.interleaved ? kInterleaved : a.rot % 8 == 0 ? kHalves : kHalvesOdd;
+#define B2Q_ROPE(DD, BF, NO, MO) rope_cache_kernel<DD, BF, NO, MO><<<grid, kRopeThreads, smem, s>>>(a, tpc, wide)
+#define B2Q_ROPE_M(DD, BF, NO)                                        \
+  do {                                                                \
+    if (mode == kInterleaved) B2Q_ROPE(DD, BF, NO, kInterleaved);     \
+    else if (mode == kHalves) B2Q_ROPE(DD, BF, NO, kHalves);          \
+    else B2Q_ROPE(DD, BF, NO, kHalvesOdd);                            \
+  } while (0)
+#define B2Q_ROPE_N(DD, BF)                 \
+  do {                                     \
+    if (a.norm) B2Q_ROPE_M(DD, BF, true);  \
+    else B2Q_ROPE_M(DD, BF, false);        \
+  } while (0)
   if (D == 64) {
-    if (bf16) B2Q_ROPE(64, true); else B2Q_ROPE(64, false);
+    if (bf16) B2Q_ROPE_N(64, true); else B2Q_ROPE_N(64, false);
   } else {
-    if (bf16) B2Q_ROPE(128, true); else B2Q_ROPE(128, false);
+    if (bf16) B2Q_ROPE_N(128, true); else B2Q_ROPE_N(128, false);
   }
+#undef B2Q_ROPE_N
+#undef B2Q_ROPE_M
 #undef B2Q_ROPE
   return cudaGetLastError();
 }

@@ -24,9 +24,10 @@
 // the warp's own ring: no barrier inside a tile.  The warps of a tile share out
 // its units (WK of them; the other factor, WR, is row tiles side by
 // side) and are summed at its end in a fixed order.
-//   up to 2 tokens (WIDE false): a token's columns are (p0, p1, -, p2), so a
-//     lane's pair of sums is 256 p0 + p1, or p2: one number to scale
-//   3 to 8 tokens (WIDE true): one product per digit, columns are tokens
+//   up to 4 tokens (NT 1 or 2 products a block, two tokens each): a token's
+//     columns are (p0, p1, -, p2), so a lane's pair of sums is 256 p0 + p1, or p2:
+//     one number to scale
+//   5 to 8 tokens (NT 3, WIDE): one product per digit, columns are tokens
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
 
@@ -44,18 +45,22 @@ constexpr int kMvUnitK = 256;
 // then meet all banks, and two rows' Q4_0 scales are one word.
 constexpr int kMvUnitBytes = 16 * kQ4KBytes;
 constexpr int kMvSmem = 227 * 1024;
-// The sums of 3 to 8 tokens take more registers a warp, so 16 warps and one more stage each.
-template <bool WIDE>
+// The sums of 5 to 8 tokens take more registers a warp, so 16 warps and one more stage each.
+template <int NT>
 struct MvShape {
+  static constexpr bool WIDE = NT == 3;
+  static constexpr int TOKENS = WIDE ? 8 : 2 * NT;           // at most
+  static constexpr int COLS = WIDE ? 8 : 4 * NT;             // of sums in a lane quad
   static constexpr int WARPS = WIDE ? 16 : 24, THREADS = WARPS * 32;
   static constexpr int STAGES = WIDE ? 3 : 2;
   static constexpr int TILES = 32;                           // row tiles whose sums a CTA keeps over the chunks
   static constexpr int RING = WARPS * STAGES * kMvUnitBytes;
   static constexpr int SCALES = WARPS * 8 * 16 * 4;          // Q4_K: a unit's d * sc per warp
-  static constexpr int RED = 2 * WARPS * 16 * (WIDE ? 8 : 4) * 4;
-  static constexpr int ACC = TILES * 16 * (WIDE ? 8 : 2) * 4;
+  static constexpr int RED = 2 * WARPS * 16 * COLS * 4;
+  static constexpr int ACC = TILES * 16 * TOKENS * 4;
   static constexpr int X = kMvSmem - RING - SCALES - RED - ACC;  // a chunk's activations
 };
+constexpr int kMvBatch = 4;              // blocks of activations that a group of lanes loads at a time
 constexpr int kMvMagic = 0x4B400000;     // bits of 1.5 * 2^23
 
 struct MvPlan {
@@ -63,7 +68,7 @@ struct MvPlan {
   int units;           // of 256 values along K
   int chunk_units;     // of one chunk
   int chunks;
-  int64_t supers;      // super-tiles of WR * 16 rows
+  int supers;          // super-tiles of WR * 16 rows; at least one per CTA
   int pitch;           // bytes of one digit row in shared memory
   int vec;             // x rows can be read four values at a time
 };
@@ -121,9 +126,10 @@ __device__ __forceinline__ void mv_cp16(uint32_t dst, const void* src, bool real
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-template <bool Q4K, bool WIDE, int XT>
-__global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(const MulVecArgs a, const MvPlan p) {
-  using S = MvShape<WIDE>;
+template <bool Q4K, int NT, int XT>
+__global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const MulVecArgs a, const MvPlan p) {
+  using S = MvShape<NT>;
+  constexpr bool WIDE = S::WIDE;
   extern __shared__ __align__(128) uint8_t mv_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -133,16 +139,16 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
   uint8_t* ring = mv_smem + warp * S::STAGES * kMvUnitBytes;
   const uint32_t ring_a = smem_u32(ring);
   float* scales = reinterpret_cast<float*>(mv_smem + S::RING) + warp * 128;  // [block % 4][block / 4][row]
-  float* red = reinterpret_cast<float*>(mv_smem + S::RING + S::SCALES);        // [2][warp][16][8 or 4]
+  float* red = reinterpret_cast<float*>(mv_smem + S::RING + S::SCALES);        // [2][warp][16][COLS]
   float* acc_s = reinterpret_cast<float*>(mv_smem + S::RING + S::SCALES + S::RED);  // [tile][16][M]
   uint8_t* digits = mv_smem + S::RING + S::SCALES + S::RED + S::ACC;  // [digit][token] (WIDE), [token][digit]; pitch
   // per token, the chunk's blocks: s; then (Q4_K) the sum of the block's x
   const int nb_pitch = p.chunk_units * (kMvUnitK / 32) + 4;  // floats; tokens meet different banks
   float* tab = reinterpret_cast<float*>(digits + 3 * a.M * p.pitch);
   float* sums = tab + a.M * nb_pitch;
-  constexpr int TC = WIDE ? 8 : 4;
+  constexpr int TC = S::COLS;
 
-  const int own = blockIdx.x < p.supers ? static_cast<int>((p.supers - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
+  const int own = (p.supers - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   const int group_n = p.chunks == 1 ? own : S::TILES / WR;  // super-tiles whose sums are kept at once
 
   // The warp's sequence of units: for each group, each chunk, each super-tile, its units of the chunk.
@@ -209,8 +215,14 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
 
   enter_tile();
   settle();
+  // The ring's first loads, behind the first activations' (which would wait for them to pass).
+  bool primed = false;
+  auto prime = [&] {
+    if (primed) return;
+    primed = true;
 #pragma unroll
-  for (int s = 0; s < S::STAGES - 1; ++s) load(s);
+    for (int s = 0; s < S::STAGES - 1; ++s) load(s);
+  };
   int stage = 0, fill = S::STAGES - 1, buf = 0;
 
   for (int g0 = 0; g0 < own; g0 += group_n) {
@@ -219,25 +231,46 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
       if (p.chunks > 1 || g0 == 0) {
         // ---- the chunk's activations: eight lanes per (token, block), four values each
         const int nb = (cu1 - cu0) * (kMvUnitK / 32);
-        for (int j = threadIdx.x >> 3; j < nb * a.M; j += S::THREADS / 8) {
-          const int m = j / nb, b = j - m * nb, i = threadIdx.x & 7;
-          const int64_t k0 = (static_cast<int64_t>(cu0) * (kMvUnitK / 32) + b) * 32 + i * 4;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (k0 < a.K) v = x4<XT>(a.x, m * a.ldx + k0, p.vec != 0);
-          float amax = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-          // a NaN counts as an infinity (fmaxf would drop it)
-          if (!(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) >= 0.0f)) amax = INFINITY;
-          const unsigned mask = 0xffu << (lane & 24);
+        constexpr int GROUPS = S::THREADS / 8;
+        const int gi = threadIdx.x >> 3, i = threadIdx.x & 7;
+        const unsigned mask = 0xffu << (lane & 24);
+        // (token, block) after (token, block), blocks of a token in a row, GROUPS apart
+        int t_m = gi / nb, t_b = gi - t_m * nb;
+        const int d_m = GROUPS / nb, d_b = GROUPS - d_m * nb;
+        while (t_m < a.M) {
+         float4 vb[kMvBatch];
+         int vm[kMvBatch], vk[kMvBatch];
 #pragma unroll
-          for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-          const bool fin = amax < INFINITY;
-          int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 22;  // amax in [2^(e+22), 2^(e+23)), or less
-          // s = 2^e, and what enters the table (for Q4_0 a sixteenth of it) is an fp32 number
+         for (int y = 0; y < kMvBatch; ++y) {  // loads under way together
+          vm[y] = t_m;
+          vk[y] = t_b;
+          const int64_t k0 = (static_cast<int64_t>(cu0) * (kMvUnitK / 32) + t_b) * 32 + i * 4;
+          vb[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (t_m < a.M && k0 < a.K) vb[y] = x4<XT>(a.x, t_m * a.ldx + k0, p.vec != 0);
+          t_m += d_m;
+          t_b += d_b;
+          if (t_b >= nb) t_b -= nb, ++t_m;
+         }
+         prime();
+#pragma unroll
+         for (int y = 0; y < kMvBatch; ++y) {
+          if (vm[y] >= a.M) break;
+          const int m = vm[y], b = vk[y];
+          const float4 v = vb[y];
+          // Magnitudes compare as their bits do, a NaN above infinity.
+          uint32_t amax = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+                              max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(mask, amax, o));
+          const bool fin = amax < 0x7f800000u;
+          // s = 2^e with the largest magnitude in [2^22, 8355711] of it: a mantissa past that
+          // number's takes the next power.  What enters the table (for Q4_0 a sixteenth of s)
+          // has to be an fp32 number, so e has a lowest value.
           constexpr int e_min = Q4K ? -149 : -145;
-          if (!fin) e = 0;
-          if (e >= e_min && amax * pow2(-e / 2) * pow2(-e - -e / 2) > 8355711.0f) ++e;
-          if (e < e_min) e = e_min;
-          const float i1 = pow2(-e / 2), i2 = pow2(-e - -e / 2);
+          const int e = max(static_cast<int>(amax >> 23) - 149 + ((amax & 0x7fffffu) > 0x7efefeu ? 1 : 0), e_min);
+          // 1 / s in two steps, for the sake of e below -126
+          const float i1 = __uint_as_float(static_cast<uint32_t>(127 - max(e, -126)) << 23);
+          const float i2 = __uint_as_float(static_cast<uint32_t>(127 + max(-126 - e, 0)) << 23);
           int q[4] = {0, 0, 0, 0};
           if (fin) {
             q[0] = __float2int_rn(v.x * i1 * i2);
@@ -245,16 +278,14 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
             q[2] = __float2int_rn(v.z * i1 * i2);
             q[3] = __float2int_rn(v.w * i1 * i2);
           }
-          uint32_t d0 = 0, d1 = 0, d2 = 0;
+          // Balanced digits: with 128 (65536 + 256 + 1) added every digit is 128 + p, and
+          // flipping its top bit makes the byte p; then bytes of four values into words.
+          uint32_t u[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int lo = static_cast<int8_t>(q[x]);
-            const int hi = (q[x] - lo) >> 8;
-            const int mid = static_cast<int8_t>(hi);
-            d2 |= (lo & 255u) << (8 * x);
-            d1 |= (mid & 255u) << (8 * x);
-            d0 |= (((hi - mid) >> 8) & 255u) << (8 * x);
-          }
+          for (int x = 0; x < 4; ++x) u[x] = (static_cast<uint32_t>(q[x]) + 0x808080u) ^ 0x808080u;
+          const uint32_t a01 = __byte_perm(u[0], u[1], 0x5140), a23 = __byte_perm(u[2], u[3], 0x5140);
+          const uint32_t d2 = __byte_perm(a01, a23, 0x5410), d1 = __byte_perm(a01, a23, 0x7632);
+          const uint32_t d0 = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410);
           // Lane c of the product has values 4c .. and 16 + 4c .. (Q4_0) or 8c .. 8c + 7 (Q4_K) of
           // a block; its pieces of two neighbouring blocks are one 16-byte word.
           const int lc = Q4K ? i >> 1 : i & 3, half = Q4K ? i & 1 : i >> 2;
@@ -275,58 +306,79 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
             tab[m * nb_pitch + b] = s;
             if constexpr (Q4K) sums[m * nb_pitch + b] = s * static_cast<float>(xsum);
           }
+         }
         }
+        prime();
         __syncthreads();
       }
 
-      // B operand: this lane's column is g
-      const int d_of_g = (g & 3) == 3 ? 2 : (g & 1);  // (p0, p1, p0 unused, p2)
-      const uint8_t* bcol =
-          digits + (WIDE ? min(g, a.M - 1) : 3 * min(g >> 2, a.M - 1) + d_of_g) * p.pitch + c * 16;
+      // B operand: this lane's column is g; narrow: of products 0 .. NT - 1, digits (p0, p1, p0 unused, p2).
+      // Columns past the tokens repeat the last one, unused.
+      constexpr int NB = WIDE ? 1 : NT;
+      const uint8_t* bcol[NB];
+      const float* tab0[NB];                    // s of this lane's token (WIDE: tokens 2c and 2c + 1)
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        const int digit = (g & 3) == 3 ? 2 : (g & 1);
+        bcol[x] = digits + (WIDE ? min(g, a.M - 1) : 3 * min(2 * x + (g >> 2), a.M - 1) + digit) * p.pitch + c * 16;
+        tab0[x] = tab + min(WIDE ? 2 * c : 2 * x + (c >> 1), a.M - 1) * nb_pitch;
+      }
+      const float* tab1 = tab + min(2 * c + 1, a.M - 1) * nb_pitch;
       const int dstep = a.M * p.pitch;          // WIDE: to the next digit
       const int mul = (c & 1) ? 0 : 256;        // narrow: weight of the first of the lane's two columns
-      // s of this lane's token (WIDE: tokens 2c and 2c + 1); columns past the tokens repeat the last one, unused
-      const float* tab0 = tab + min(WIDE ? 2 * c : c >> 1, a.M - 1) * nb_pitch;
-      const float* tab1 = tab + min(2 * c + 1, a.M - 1) * nb_pitch;
       for (int i = g0; i < min(own, g0 + group_n); ++i) {
-        // (the first row that this warp will finish: its bias is on its way while the units run)
-        const int64_t n_first = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * WR * 16 + warp;
-        const float bias_first = a.bias && n_first < a.N ? __ldg(a.bias + n_first) : 0.0f;
-        float macc[Q4K ? (WIDE ? kMulVecMaxM : 2) : 1] = {};  // Q4_K: minima, of row lane % 16, half of the blocks
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // WIDE: (row0, tokens 2c, 2c + 1), (row1, ..); else row0, row1
+        // A thread finishes outputs (row, token) threadIdx.x, + THREADS, .. of the super-tile, rows in a row;
+        // what the first one is added to is on its way while the units run.
+        const int64_t n_super = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * WR * 16;
+        const int outs = 16 * WR * a.M;
+        const int m_first = static_cast<int>(threadIdx.x) / (16 * WR);
+        const int64_t n_first = n_super + (static_cast<int>(threadIdx.x) - m_first * 16 * WR);
+        float bias_first = 0.0f, gate_first = 1.0f, resid_first = 0.0f;
+        if (static_cast<int>(threadIdx.x) < outs && n_first < a.N && chunk == p.chunks - 1) {
+          if (a.bias) bias_first = __ldg(a.bias + n_first);
+          if (a.gate) gate_first = __ldg(a.gate + n_first);
+          if (a.resid) resid_first = a.resid[m_first * a.ldr + n_first];
+        }
+        float macc[Q4K ? S::TOKENS : 1] = {};  // Q4_K: minima, of row lane % 16, half of the blocks
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // WIDE: (row0, tokens 2c, 2c + 1), (row1, ..); else (row0, row1) per product
         for (int u = cu0 + wk; u < cu1; u += WK) {
           asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
           __syncwarp();
           load(fill);
           const uint8_t* st = ring + stage * kMvUnitBytes;
-          const uint8_t* bu = bcol + (u - cu0) * kMvUnitK;
+          const int bu = (u - cu0) * kMvUnitK;
           const int kb0 = (u - cu0) * 8;
           // two blocks: A operands, scales of (row0, row1), s of the token(s) -> acc
-          auto fold = [&](const uint32_t (&af)[2][4], int pair, const float2 (&sr)[2], const float (&t0)[2],
+          auto fold = [&](const uint32_t (&af)[2][4], int pair, const float2 (&sr)[2], const float (&t0)[NB][2],
                           const float (&t1)[2]) {
-            const uint4 b0 = *reinterpret_cast<const uint4*>(bu + pair * 64);
-            uint4 b1, b2;
             if constexpr (WIDE) {
-              b1 = *reinterpret_cast<const uint4*>(bu + dstep + pair * 64);
-              b2 = *reinterpret_cast<const uint4*>(bu + 2 * dstep + pair * 64);
-            }
+              const uint4 b0 = *reinterpret_cast<const uint4*>(bcol[0] + bu + pair * 64);
+              const uint4 b1 = *reinterpret_cast<const uint4*>(bcol[0] + dstep + bu + pair * 64);
+              const uint4 b2 = *reinterpret_cast<const uint4*>(bcol[0] + 2 * dstep + bu + pair * 64);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              int x0[4];
-              mma_i8_16832<Q4K>(x0, af[h], h ? make_uint2(b0.z, b0.w) : make_uint2(b0.x, b0.y), WIDE ? kMvMagic : 0);
-              if constexpr (WIDE) {
-                int x1[4], x2[4];
+              for (int h = 0; h < 2; ++h) {
+                int x0[4], x1[4], x2[4];
+                mma_i8_16832<Q4K>(x0, af[h], h ? make_uint2(b0.z, b0.w) : make_uint2(b0.x, b0.y), kMvMagic);
                 mma_i8_16832<Q4K>(x1, af[h], h ? make_uint2(b1.z, b1.w) : make_uint2(b1.x, b1.y), 0);
                 mma_i8_16832<Q4K>(x2, af[h], h ? make_uint2(b2.z, b2.w) : make_uint2(b2.x, b2.y), 0);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                   const float v = fmaf(__int_as_float(x0[x]) - 12582912.0f, 65536.0f,
                                        static_cast<float>(x1[x] * 256 + x2[x]));
-                  acc[x] = fmaf(v * ((x & 1) ? t1[h] : t0[h]), x < 2 ? sr[h].x : sr[h].y, acc[x]);
+                  acc[x] = fmaf(v * ((x & 1) ? t1[h] : t0[0][h]), x < 2 ? sr[h].x : sr[h].y, acc[x]);
                 }
-              } else {
-                acc[0] = fmaf(static_cast<float>(x0[0] * mul + x0[1]) * t0[h], sr[h].x, acc[0]);
-                acc[1] = fmaf(static_cast<float>(x0[2] * mul + x0[3]) * t0[h], sr[h].y, acc[1]);
+              }
+            } else {
+#pragma unroll
+              for (int n = 0; n < NB; ++n) {
+                const uint4 b0 = *reinterpret_cast<const uint4*>(bcol[n] + bu + pair * 64);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  int x[4];
+                  mma_i8_16832<Q4K>(x, af[h], h ? make_uint2(b0.z, b0.w) : make_uint2(b0.x, b0.y), 0);
+                  acc[2 * n] = fmaf(static_cast<float>(x[0] * mul + x[1]) * t0[n][h], sr[h].x, acc[2 * n]);
+                  acc[2 * n + 1] = fmaf(static_cast<float>(x[2] * mul + x[3]) * t0[n][h], sr[h].y, acc[2 * n + 1]);
+                }
               }
             }
           };
@@ -343,7 +395,7 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
             const float m0 = static_cast<float>(mn & 255u), m1 = static_cast<float>((mn >> 8) & 255u),
                         m2 = static_cast<float>((mn >> 16) & 255u), m3 = static_cast<float>(mn >> 24);
 #pragma unroll
-            for (int m = 0; m < (WIDE ? kMulVecMaxM : 2); ++m) {
+            for (int m = 0; m < S::TOKENS; ++m) {
               if (m >= a.M) break;
               const float4 sx = *reinterpret_cast<const float4*>(sums + m * nb_pitch + kb0 + half * 4);
               macc[m] = fmaf(-dd.y, fmaf(m0, sx.x, fmaf(m1, sx.y, fmaf(m2, sx.z, m3 * sx.w))), macc[m]);
@@ -352,8 +404,10 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
           }
 #pragma unroll
           for (int q = 0; q < 2; ++q) {  // four blocks
-            const float4 ta = *reinterpret_cast<const float4*>(tab0 + kb0 + 4 * q);
-            float4 tb = ta;
+            float4 ta[NB], tb;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) ta[n] = *reinterpret_cast<const float4*>(tab0[n] + kb0 + 4 * q);
+            tb = ta[0];
             if constexpr (WIDE) tb = *reinterpret_cast<const float4*>(tab1 + kb0 + 4 * q);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -385,7 +439,10 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
                   sr[h] = __half22float2(reinterpret_cast<const __half2*>(st + 2048)[bi * 8 + g]);
                 }
               }
-              const float t0[2] = {r ? ta.z : ta.x, r ? ta.w : ta.y}, t1[2] = {r ? tb.z : tb.x, r ? tb.w : tb.y};
+              float t0[NB][2];
+#pragma unroll
+              for (int n = 0; n < NB; ++n) t0[n][0] = r ? ta[n].z : ta[n].x, t0[n][1] = r ? ta[n].w : ta[n].y;
+              const float t1[2] = {r ? tb.z : tb.x, r ? tb.w : tb.y};
               fold(af, j, sr, t0, t1);
             }
           }
@@ -399,43 +456,48 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
           *reinterpret_cast<float2*>(mine + row1 * TC + 2 * c) = make_float2(acc[2], acc[3]);
         } else {
           const float f = (c & 1) ? 1.0f : 256.0f;
-          mine[row0 * TC + c] = acc[0] * f;
-          mine[row1 * TC + c] = acc[1] * f;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            mine[row0 * TC + 4 * n + c] = acc[2 * n] * f;
+            mine[row1 * TC + 4 * n + c] = acc[2 * n + 1] * f;
+          }
         }
         if constexpr (Q4K) {
           __syncwarp();
 #pragma unroll
-          for (int m = 0; m < (WIDE ? kMulVecMaxM : 2); ++m) {
+          for (int m = 0; m < S::TOKENS; ++m) {
             const float v = macc[m] + __shfl_xor_sync(0xffffffffu, macc[m], 16);
             if (lane < 16 && m < a.M) mine[lane * TC + (WIDE ? m : 2 * m + 1)] += v;
           }
         }
         __syncthreads();  // and the other buffer's readers are done before it is written again
-        // Warp w sums rows w, w + 16, .. of the super-tile: lanes over (warp of the tile, column).
-        for (int r = warp; r < 16 * WR; r += S::WARPS) {
+        for (int x = threadIdx.x; x < outs; x += S::THREADS) {
+          const int m = x / (16 * WR), r = x - m * 16 * WR;
+          const int64_t n = n_super + r;
           const float* part = red + ((buf * S::WARPS + ((r >> 4) << p.wk_shift)) * 16 + (r & 15)) * TC;
           float v = 0.0f;
-          for (int x = lane / TC; x < WK; x += 32 / TC) v += part[x * 16 * TC + lane % TC];
-#pragma unroll
-          for (int o = TC; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          int m = lane;  // lane's token
-          if constexpr (!WIDE) {
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            m = (lane & 1) ? kMulVecMaxM : lane >> 1;
-          }
-          const int64_t n = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * WR * 16 + r;
-          if (m < a.M && n < a.N) {
-            if (p.chunks > 1) {
-              float* slot = acc_s + ((i - g0) * 16 * WR + r) * a.M + m;
-              if (chunk > 0) v += *slot;
-              *slot = v;
-            }
-            if (chunk == p.chunks - 1) {
-              if (a.bias) v = __fadd_rn(v, r == warp ? bias_first : __ldg(a.bias + n));
-              if (a.resid) v = __fadd_rn(a.resid[m * a.ldr + n], a.gate ? __fmul_rn(v, a.gate[n]) : v);
-              a.y[m * a.ldy + n] = v;
+          for (int w = 0; w < WK; ++w) {
+            if constexpr (WIDE) {
+              v += part[w * 16 * TC + m];
+            } else {
+              const float2 d = *reinterpret_cast<const float2*>(part + w * 16 * TC + 2 * m);
+              v += d.x + d.y;
             }
           }
+          if (n >= a.N) continue;
+          if (p.chunks > 1) {
+            float* slot = acc_s + (i - g0) * outs + x;
+            if (chunk > 0) v += *slot;
+            *slot = v;
+            if (chunk < p.chunks - 1) continue;
+          }
+          const bool first = x == static_cast<int>(threadIdx.x);
+          if (a.bias) v = __fadd_rn(v, first ? bias_first : __ldg(a.bias + n));
+          if (a.resid) {
+            if (a.gate) v = __fmul_rn(v, first ? gate_first : __ldg(a.gate + n));
+            v = __fadd_rn(first ? resid_first : a.resid[m * a.ldr + n], v);
+          }
+          a.y[m * a.ldy + n] = v;
         }
         buf ^= 1;
       }
@@ -444,10 +506,10 @@ __global__ void __launch_bounds__(MvShape<WIDE>::THREADS, 1) mul_vec_kernel(cons
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool Q4K, bool WIDE, int XT>
+template <bool Q4K, int NT, int XT>
 cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
-  using S = MvShape<WIDE>;
-  auto kern = mul_vec_kernel<Q4K, WIDE, XT>;
+  using S = MvShape<NT>;
+  auto kern = mul_vec_kernel<Q4K, NT, XT>;
   MvPlan p{};
   p.units = static_cast<int>((a.K + kMvUnitK - 1) / kMvUnitK);
   // Shared memory per unit: the digits, and per block s and the sum.
@@ -459,19 +521,21 @@ cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
   p.pitch = p.chunk_units * kMvUnitK + 64;
   const int64_t tiles = (a.N + 15) / 16;
   // WK, the warps that share a tile's units: what finishes first when a tile's
-  // end costs as much as 0.75 units and the super-tiles go round the SMs.
-  // Measured at 49152 x 8192, Q4_K, one token: WK 1 67 us, 2 68, 4 69.5, 8 68.5.
+  // end costs as much as 0.75 units and the super-tiles go round the SMs; the
+  // larger of equals, which spreads few rows over more SMs.  Measured, WK 1, 2,
+  // 4, 8: 49152 x 8192 Q4_K, one token 52.6, 54.3, 56.8, 57.1 us; 8192 x 4096 Q4_0,
+  // four tokens 38.5, 23.4, 16.1, 17.1; 6144 x 1024 Q4_0, one token 9.9, 7.1, 5.6, 4.8.
   int sh = 0;
   double best = 0.0;
-  for (int x = 0; x <= 3 && (1 << x) <= p.chunk_units; ++x) {
+  for (int x = 0; x <= 3; ++x) {
     const int64_t super = (tiles + (S::WARPS >> x) - 1) / (S::WARPS >> x);
     const double cost = static_cast<double>((super + num_sms - 1) / num_sms) *
                         ((p.units + (1 << x) - 1) / (1 << x) + 0.75 * p.chunks);
-    if (x == 0 || cost < best) best = cost, sh = x;
+    if (x == 0 || cost <= best) best = cost, sh = x;
   }
   p.wk_shift = sh;
   const int wr = S::WARPS >> sh;
-  p.supers = (tiles + wr - 1) / wr;
+  p.supers = static_cast<int>((tiles + wr - 1) / wr);
   const uintptr_t xa = reinterpret_cast<uintptr_t>(a.x);
   p.vec = XT == kXF32 ? (xa % 16 == 0 && a.ldx % 4 == 0) : (xa % 8 == 0 && a.ldx % 4 == 0);
   const int smem = kMvSmem;
@@ -483,7 +547,7 @@ cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     attr_set[dev] = true;
   }
-  const int64_t grid = p.supers < num_sms ? p.supers : num_sms;
+  const int grid = p.supers < num_sms ? p.supers : num_sms;
   kern<<<static_cast<unsigned>(grid), S::THREADS, smem, s>>>(a, p);
   return cudaGetLastError();
 }
@@ -491,12 +555,11 @@ cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_mul_vec(const MulVecArgs& a, bool q4k, int xt, int num_sms, cudaStream_t s) {
-  const bool wide = a.M > 2;
-#define B2Q_MV(Q, W)                                                                     \
-  (xt == kXF32 ? launch_mv<Q, W, kXF32>(a, num_sms, s)                                   \
-               : xt == kXF16 ? launch_mv<Q, W, kXF16>(a, num_sms, s) : launch_mv<Q, W, kXBF16>(a, num_sms, s))
-  if (q4k) return wide ? B2Q_MV(true, true) : B2Q_MV(true, false);
-  return wide ? B2Q_MV(false, true) : B2Q_MV(false, false);
+#define B2Q_MV(Q, N)                                                                     \
+  (xt == kXF32 ? launch_mv<Q, N, kXF32>(a, num_sms, s)                                   \
+               : xt == kXF16 ? launch_mv<Q, N, kXF16>(a, num_sms, s) : launch_mv<Q, N, kXBF16>(a, num_sms, s))
+  if (q4k) return a.M <= 2 ? B2Q_MV(true, 1) : a.M <= 4 ? B2Q_MV(true, 2) : B2Q_MV(true, 3);
+  return a.M <= 2 ? B2Q_MV(false, 1) : a.M <= 4 ? B2Q_MV(false, 2) : B2Q_MV(false, 3);
 #undef B2Q_MV
 }
 

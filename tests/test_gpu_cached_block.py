@@ -1,0 +1,99 @@
+"""The block over a paged cache (cached_block.py): prompts and single tokens of
+several requests, against a 64-bit recomputation of each whole request without
+a cache."""
+import numpy as np
+import pytest
+import torch
+
+import cached_block as cb
+import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+
+
+def layer_norm(x):
+    d = x - x.mean(-1, keepdim=True)
+    return d / torch.sqrt(d.square().mean(-1, keepdim=True) + EPS)
+
+
+def reference(block, weights, x, grid):
+    """One request's tokens x [n, C] (fp64) through the block, causal, no cache."""
+    dev = x.device
+    w = {n: torch.from_numpy(O.dequantize(weights[n], O.TYPE_Q4_0, k)).double().to(dev) for n, (_, k) in block.shape.items()}
+    v = {n: t.double() for n, t in block.vec.items()}
+    n, H, Hk, D = x.shape[0], block.H, block.Hk, block.D
+    qkv = layer_norm(x) @ w["qkv"].t() + v["b_qkv"]
+    q, k, vv = qkv.view(n, H + 2 * Hk, D).split([H, Hk, Hk], 1)
+    rms = lambda t, g: t / torch.sqrt(t.square().mean(-1, keepdim=True) + EPS) * g.view(-1, D)  # noqa: E731
+    axis = torch.repeat_interleave(torch.arange(3, device=dev), torch.tensor(block.sections, device=dev))
+    th = grid.double()[axis].t() * block.inv_freq.double()
+    c, s = torch.cos(th)[:, None], torch.sin(th)[:, None]
+
+    def turn(t):
+        a, b = t[..., :D // 2], t[..., D // 2:]
+        return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+    q, k = turn(rms(q, v["gq"])), turn(rms(k, v["gk"]))
+    i, j = torch.arange(n, device=dev)[:, None], torch.arange(n, device=dev)[None]
+    see = j <= i
+    if block.window:
+        see &= (j > i - block.window) | (j < block.sinks)
+    o = []
+    for h in range(H):
+        sc = (q[:, h] @ k[:, h // (H // Hk)].t()) / D ** 0.5
+        o.append(torch.softmax(sc.masked_fill(~see, float("-inf")), -1) @ vv[:, h // (H // Hk)])
+    x = x + torch.cat(o, 1) @ w["out"].t() + v["b_out"]
+    h = layer_norm(x) @ w["fc1"].t() + v["b1"]
+    h = 0.5 * h * (1 + torch.tanh(0.7978845608028654 * (h + 0.044715 * h ** 3)))
+    return x + h @ w["fc2"].t() + v["b2"]
+
+
+def coords(p):
+    return torch.stack([p // 64, p // 8 % 8, p % 8]).int()
+
+
+@pytest.mark.parametrize("heads,kv_heads,D,window,sinks", [(4, 4, 64, 0, 0), (6, 2, 64, 20, 3), (4, 1, 128, 0, 0)])
+@pytest.mark.parametrize("steps,bound", [
+    # Steps of at most 8 tokens in all: q, k, v and o are rounded to fp16 (2^-11 each) and gelu
+    # runs on fp16 inputs and outputs as ggml's does; everything else is fp32.
+    ([[3, 5], [1, 1], [1, 1], [2, 6], [1, 0], [4, 4], [0, 1], [1, 1]], 4e-3),
+    # Chunks too: their linears round the activations to Q8_0, half of 1/127 of a block's largest value.
+    ([[70, 133], [1, 1], [1, 1], [40, 3], [1, 1]], 2e-2),
+])
+def test_cached_steps_match_full_recomputation(dev, heads, kv_heads, D, window, sinks, steps, bound):
+    C, hidden = 256, 512
+    sections = (D // 2 - 2 * (D // 8), D // 8, D // 8)
+    block, weights = cb.random_block(dev, C, heads, kv_heads, D, hidden, sections, seed=3, window=window, sinks=sinks)
+    total = [sum(s[b] for s in steps) for b in range(2)]
+    g = torch.Generator(device=dev).manual_seed(1)
+    xs = [torch.randn(n, C, generator=g, device=dev) for n in total]
+    refs = [reference(block, weights, x.double(), coords(torch.arange(x.shape[0], device=dev))) for x in xs]
+    cache = cb.PagedCache(dev, 1, 2, kv_heads, D, pages=40, page_size=16, max_len=320)
+    at = [0, 0]
+    for new in steps:
+        step = cache.plan(new)
+        x = torch.cat([xs[b][at[b]:at[b] + new[b]] for b in range(2)])
+        y = block.forward(x.clone(), cache, 0, step, coords(step["pos"]))
+        ref = torch.cat([refs[b][at[b]:at[b] + new[b]] for b in range(2)])
+        err = (y.double() - ref).norm() / (ref - x.double()).norm()
+        assert float(err) <= bound, (new, float(err))
+        at = [at[b] + new[b] for b in range(2)]
+
+
+def test_full_cache_is_refused(dev):
+    cache = cb.PagedCache(dev, 1, 1, 1, 64, pages=2, page_size=16, max_len=64)
+    cache.plan([30])
+    with pytest.raises(RuntimeError):
+        cache.plan([3])
+    cache = cb.PagedCache(dev, 1, 1, 1, 64, pages=20, page_size=16, max_len=32)
+    with pytest.raises(RuntimeError):
+        cache.plan([33])
+
+
+def test_example_runs(dev, capsys):
+    cb.main()
+    out = capsys.readouterr().out.splitlines()
+    assert len(out) == 9 and out[-1].endswith("cached 308")
+    assert all(np.isfinite(float(line.split("rms ")[1].split(",")[0])) for line in out)

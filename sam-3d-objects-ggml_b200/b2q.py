@@ -763,10 +763,9 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
     ldt, ldc = block_table.stride()
     assert ldc == 1 or W <= 1 or B == 0
     if out is None:
-        dev = block_table.device
-        out = (torch.empty(max_tokens, dtype=torch.int64, device=dev), torch.empty(max_tokens, dtype=i32, device=dev),
-               torch.empty(B + 1, dtype=i32, device=dev), torch.empty(B, dtype=i32, device=dev),
-               torch.empty(2, dtype=i32, device=dev))
+        dev = block_table.device  # two allocations, not five: the int32 results are parts of one
+        out = (torch.empty(max_tokens, dtype=torch.int64, device=dev),
+               *torch.empty(max_tokens + 2 * B + 3, dtype=i32, device=dev).split((max_tokens, B + 1, B, 2)))
     slots, positions, cu, kv_len, counts = out
     rc = (_lib or _lib_obj()).b2q_kv_cache_plan(
         cached.data_ptr(), new.data_ptr(), B, page_size, free_pages.data_ptr(), free_pages.numel(),

@@ -104,7 +104,14 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   const int u0 = static_cast<int>(min(static_cast<int64_t>(split) * a.split_units, static_cast<int64_t>(u_all)));
   const int u1 =
       split == a.splits - 1 ? u_all : static_cast<int>(min(static_cast<int64_t>(u_all), u0 + a.split_units));
-  if (split > 0 && u0 >= u_all) return;  // the joining kernel knows
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may get ready
+  if (split > 0 && u0 >= u_all) {  // no keys in this stretch
+    const int64_t r = r0 + threadIdx.x;
+    if (threadIdx.x < 16 && r < rows)
+      a.part_ml[((rq.t0 + r / a.G) * a.Hq + static_cast<int64_t>(hk) * a.G + r % a.G) * a.splits + split] =
+          make_float2(-INFINITY, 0.0f);
+    return;
+  }
   const int su = static_cast<int>(un.su), gap = static_cast<int>(un.wu - un.su);
   auto unit_at = [&](int i) { return i < su ? i : i + gap; };
 
@@ -391,55 +398,77 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   }
 }
 
-// One warp per (token, query head): o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s
-// over the splits that hold keys, in their order.
+// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits, in their
+// order, for one (token, query head) a CTA.  The splits' weights are worked out
+// once, side by side; then every thread adds up its values, loads ahead.  Launched
+// with the attention kernel still running (it waits before it reads): 94 -> 83 us
+// for one request of 120k keys, with the warp-wide loop over 37 splits before.
+constexpr int kJoinMax = 1024;  // splits
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int tile_rows, int unit) {
-  const int lane = threadIdx.x & 31;
-  const int b = blockIdx.y;
-  const Request rq = request_of(a, b);
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (token, head) of the request
-  if (idx >= rq.n * a.Hq) return;
-  const int64_t i = idx / a.Hq, h = idx % a.Hq;
-  // the split count of the row's tile
-  const int64_t r0 = (i * a.G + h % a.G) / tile_rows * tile_rows;
-  const int64_t p_lo = rq.first + r0 / a.G, p_hi = rq.first + min(rq.n * a.G - 1, r0 + tile_rows - 1) / a.G;
-  const int64_t units = units_of(a, rq.len, p_lo, p_hi, unit).count();
-  const int ns = static_cast<int>(
-      min(static_cast<int64_t>(a.splits), max(int64_t{1}, (units + a.split_units - 1) / a.split_units)));
+__global__ void __launch_bounds__(D / 2) paged_join_kernel(const PagedArgs a) {
+  __shared__ float f[kJoinMax];
+  __shared__ float red[2][D / 64];
+  const int tid = threadIdx.x, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Request rq = request_of(a, blockIdx.y);
+  const int i = blockIdx.x / a.Hq, h = blockIdx.x - i * a.Hq;
+  if (i >= rq.n) return;
   const int64_t pi = ((rq.t0 + i) * a.Hq + h) * a.splits;
-  float M = -INFINITY;
-  for (int s = lane; s < ns; s += 32) M = fmaxf(M, a.part_ml[pi + s].x);
+  float m = -INFINITY;
+  for (int s = tid; s < a.splits; s += D / 2) m = fmaxf(m, a.part_ml[pi + s].x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  constexpr int E = D / 32;
-  float acc[E] = {}, sum = 0.0f;
-  {
-    for (int s = 0; s < ns; ++s) {
-      const float2 ml = a.part_ml[pi + s];
-      if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key
-      const float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - M);  // (only NaN scores: NaN)
-      sum = fmaf(f, ml.y, sum);
-      const float* src = a.part_o + (pi + s) * D + lane * E;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (D == 128) {
+    if (lane == 0) red[0][tid >> 5] = m;
+    __syncthreads();
+    m = fmaxf(red[0][0], red[0][D / 64 - 1]);
+  }
+  float sum = 0.0f;
+  for (int s = tid; s < a.splits; s += D / 2) {
+    const float2 ml = a.part_ml[pi + s];
+    // no key: 0, with nothing read; only NaN scores: NaN
+    const float w = ml.x == -INFINITY ? ml.y : ex2(ml.x - m);
+    f[s] = w;
+    sum = fmaf(w, ml.y, sum);
+  }
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + e);
-        acc[e] = fmaf(f, v.x, acc[e]);
-        acc[e + 1] = fmaf(f, v.y, acc[e + 1]);
-      }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (D == 128) {
+    if (lane == 0) red[1][tid >> 5] = sum;
+    __syncthreads();
+    sum = red[1][0] + red[1][D / 64 - 1];
+  } else {
+    __syncwarp();
+  }
+  float x = 0.0f, y = 0.0f;
+  const float2* src = reinterpret_cast<const float2*>(a.part_o + pi * D) + tid;
+#pragma unroll 8
+  for (int s = 0; s < a.splits; ++s) {
+    const float w = f[s];
+    if (w != 0.0f) {
+      const float2 v = src[s * (D / 2)];
+      x = fmaf(w, v.x, x);
+      y = fmaf(w, v.y, y);
     }
   }
-  const float inv = M == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo + h * D + lane * E);
-#pragma unroll
-  for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
+  const float inv = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
+  *(reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo + static_cast<int64_t>(h) * D) + tid) =
+      pack2<BF16>(x * inv, y * inv);
 }
 
 template <int D, bool BF16>
-cudaError_t launch_join(const PagedArgs& a, int tile_rows, int unit, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((a.max_q * a.Hq + 3) / 4), static_cast<unsigned>(a.B));
-  paged_join_kernel<D, BF16><<<grid, 128, 0, s>>>(a, tile_rows, unit);
-  return cudaGetLastError();
+cudaError_t launch_join(const PagedArgs& a, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.max_q * a.Hq), static_cast<unsigned>(a.B));
+  cfg.blockDim = dim3(D / 2);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, BF16>, a);
 }
 
 template <int D, bool BF16>
@@ -459,7 +488,7 @@ cudaError_t launch_rows(const PagedArgs& a, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles * a.splits), static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.B));
   kern<<<grid, kRowsThreads, RowsShape<D>::BYTES, s>>>(a, static_cast<int>(tiles));
   const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess || a.splits == 1 ? e : launch_join<D, BF16>(a, 16, kUnit, s);
+  return e != cudaSuccess || a.splits == 1 ? e : launch_join<D, BF16>(a, s);
 }
 
 }  // namespace
@@ -479,20 +508,23 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
   if (causal && window > 0 && window + tile_rows + sinks < span) span = window + tile_rows + sinks;
   const int64_t units = span / unit + 3;
   const int64_t ctas = B * Hkv * ((rows + tile_rows - 1) / tile_rows);
-  // Rows kernel: the 148 SMs hold two CTAs each.  One request is cut into as many
-  // stretches as make that one wave; several, whose lengths differ, into finer
-  // ones, up to eight waves where all are as long as announced (64 requests of 1k
-  // to 24k keys: 901 us with one wave, 662 with four, 631 with eight; one of 120k:
-  // 111, 142 and 187).  None is shorter than 1024 keys, or joining costs more than
-  // it saves.  Tile kernel (one CTA per SM): split only while CTAs are fewer than
-  // SMs, into stretches of 512 keys or more.
-  const int64_t goal = p.tiles ? 148 : 296 * (B < 8 ? (B > 0 ? B : 1) : 8), least = p.tiles ? 512 / kTileKeys : 1024 / kUnit;
-  const int64_t want = ctas >= goal ? 1 : p.tiles ? goal / (ctas > 0 ? ctas : 1) : (goal + ctas - 1) / (ctas > 0 ? ctas : 1);
-  int64_t per = (units + want - 1) / want;
-  if (per < least) per = least;
-  if (units <= per) per = units;
-  p.split_units = per;
-  p.splits = (units + per - 1) / per;
+  // Rows kernel: the 148 SMs hold two CTAs each.  Requests whose rows all see about
+  // as many keys (one request, or a window shorter than they are) are cut into as
+  // many stretches as make one wave; others, whose lengths differ, into finer ones,
+  // up to eight waves where all are as long as announced (64 requests of 1k to 24k
+  // keys: 901 us with one wave, 662 with four, 631 with eight; one of 120k: 111,
+  // 142 and 187).  None is shorter than 1024 keys, or joining costs more than it
+  // saves.  Tile kernel (one CTA per SM): split only while CTAs are fewer than SMs,
+  // into stretches of 512 keys or more.
+  const bool alike = B == 1 || span < max_kv;
+  const int64_t goal = p.tiles ? 148 : alike ? 296 : 296 * (B < 8 ? (B > 0 ? B : 1) : 8);
+  const int64_t least = p.tiles ? 512 / kTileKeys : 1024 / kUnit;
+  int64_t splits = ctas >= goal ? 1 : (goal + (p.tiles ? 0 : ctas / 2)) / (ctas > 0 ? ctas : 1);
+  if (splits > units / least) splits = units / least;
+  if (splits > kJoinMax) splits = kJoinMax;
+  if (splits < 1) splits = 1;
+  p.split_units = (units + splits - 1) / splits;
+  p.splits = (units + p.split_units - 1) / p.split_units;
   if (p.splits > 1) {
     p.part_o_bytes = round_up(T * Hq * p.splits * D * 4, 256);
     p.part_ml_bytes = round_up(T * Hq * p.splits * 8, 256);
@@ -500,9 +532,9 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
   return p;
 }
 
-cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, int tile_rows, int unit, cudaStream_t s) {
-  if (D == 64) return bf16 ? launch_join<64, true>(a, tile_rows, unit, s) : launch_join<64, false>(a, tile_rows, unit, s);
-  return bf16 ? launch_join<128, true>(a, tile_rows, unit, s) : launch_join<128, false>(a, tile_rows, unit, s);
+cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, cudaStream_t s) {
+  if (D == 64) return bf16 ? launch_join<64, true>(a, s) : launch_join<64, false>(a, s);
+  return bf16 ? launch_join<128, true>(a, s) : launch_join<128, false>(a, s);
 }
 
 cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, bool tiles, cudaStream_t s) {

@@ -149,7 +149,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const int u0 = static_cast<int>(min(static_cast<int64_t>(split) * a.split_units, static_cast<int64_t>(u_all)));
   const int u1 = split == a.splits - 1 ? u_all
                                        : static_cast<int>(min(static_cast<int64_t>(u_all), u0 + a.split_units));
-  if (split > 0 && u0 >= u_all) return;  // the joining kernel knows
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may get ready
+  if (split > 0 && u0 >= u_all) {  // no keys in this stretch
+    for (int64_t r = threadIdx.x; r < (i_end - i0) * a.G; r += kPtThreads)
+      a.part_ml[((rq.t0 + i0 + r / a.G) * a.Hq + static_cast<int64_t>(hk) * a.G + r % a.G) * a.splits + split] =
+          make_float2(-INFINITY, 0.0f);
+    return;
+  }
   TileList own[2];  // of the whole range of keys
   int j0[2], j1[2];  // and those of the stretch
 #pragma unroll
@@ -638,7 +644,7 @@ cudaError_t launch_tiles(const PagedArgs& a, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles * a.splits), static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.B));
   kern<<<grid, kPtThreads, S::BYTES, s>>>(maps, a, tok);
   const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess || a.splits == 1 ? e : launch_paged_join(a, D, BF16, 2 * tok * a.G, kTileKeys, s);
+  return e != cudaSuccess || a.splits == 1 ? e : launch_paged_join(a, D, BF16, s);
 }
 
 }  // namespace

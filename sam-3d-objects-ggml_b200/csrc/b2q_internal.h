@@ -355,7 +355,7 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
                      bool causal, int64_t window, int64_t sinks);
 cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, bool tiles, cudaStream_t s);
 cudaError_t launch_paged_tiles(const PagedArgs& a, int D, bool bf16, cudaStream_t s);
-cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, int tile_rows, int unit, cudaStream_t s);
+cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, cudaStream_t s);
 // Status word of the tile kernel's bounded waits (its own translation unit).
 cudaError_t read_paged_status(unsigned int* value, bool clear);
 

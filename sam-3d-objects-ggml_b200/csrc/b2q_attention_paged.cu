@@ -12,15 +12,17 @@
 // major: a key is read once for all of them.
 //
 // Few rows (paged_rows_kernel): bound by the cache's bytes.  A CTA of four
-// warps takes 16 rows and one stretch of the keys; its warps take the
-// stretch's units of 16 keys in turn, each with its own ring of cp.async stages
-// (no barrier inside the loop), its own running maxima, sums and outputs, and
-// they join at the end.  A unit lies inside one page (pages are multiples of
-// 16), keys that no row of the CTA sees are not loaded but filled with zeros.
-// More rows are more CTAs, side by side so that the second one's keys come from
-// the L2.  Products are m16n8k16; P is fed to the second product as two 16-bit
-// numbers, P and what rounding it left: the tensor pipe idles behind the loads,
-// and a single rounding of P would cost as much accuracy as the output's own.
+// warps takes 16 rows, or 32 (RT 2), and one stretch of the keys.  With 16 rows
+// every warp takes units of 16 keys in turn, with a ring of cp.async stages of its
+// own (no barrier inside the loop), its own running maxima, sums and outputs, and
+// they join at the end.  With 32, two warps share a ring, each copies half of a
+// unit and works on 16 of the rows, and a barrier of the two stands where a warp
+// alone has none.  (Two CTAs of 16 rows instead read the keys twice, and the L2 did
+// not make up for it: 24 rows over 120k keys took 192 us.)  A unit lies inside one
+// page (pages are multiples of 16), keys that no row of the CTA sees are not loaded
+// but filled with zeros.  Products are m16n8k16; P is fed to the second product as
+// two 16-bit numbers, P and what rounding it left: the tensor pipe idles behind the
+// loads, and a single rounding of P would cost as much accuracy as the output's own.
 // Stretches are split over CTAs when the rows alone do not fill the GPU; a
 // second kernel then joins their outputs by their maxima and sums.
 #include "b2q_internal.h"
@@ -75,29 +77,32 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-template <int D>
+template <int D, int RT>
 struct RowsShape {
-  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int GROUPS = kRowsWarps / RT;         // of RT warps with a ring each
+  static constexpr int STAGES = RT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 8 : 4);
   static constexpr int KV = kUnit * D * 2;               // bytes of one unit's keys (or values)
-  static constexpr int RING = STAGES * 2 * KV;           // per warp
-  static constexpr int BYTES = kRowsWarps * RING;
+  static constexpr int RING = STAGES * 2 * KV;           // per group
+  static constexpr int BYTES = GROUPS * RING;
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, int RT>
 __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArgs a, const int tiles) {
-  using S = RowsShape<D>;
+  using S = RowsShape<D, RT>;
   constexpr int CH = D / 8;         // 16-byte chunks of a row
   constexpr int RPI = 32 / CH;      // rows that a warp copies at a time
-  constexpr int COPIES = kUnit / RPI;
+  constexpr int COPIES = kUnit / RT / RPI;
+  constexpr int ROWS = 16 * RT;     // of the CTA
   extern __shared__ __align__(128) uint8_t rows_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = warp / RT, rt = warp % RT;
   const int b = blockIdx.z, hk = blockIdx.y;
   const int split = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   const Request rq = request_of(a, b);
   const int64_t rows = rq.n * a.G;
-  const int64_t r0 = static_cast<int64_t>(tile) * 16;
+  const int64_t r0 = static_cast<int64_t>(tile) * ROWS;
   if (r0 >= rows) return;
-  const int64_t p_lo = rq.first + r0 / a.G, p_hi = rq.first + min(rows - 1, r0 + 15) / a.G;
+  const int64_t p_lo = rq.first + r0 / a.G, p_hi = rq.first + min(rows - 1, r0 + ROWS - 1) / a.G;
   const Units un = units_of(a, rq.len, p_lo, p_hi, kUnit);
   // the last stretch takes what a longer request than announced has left
   const int u_all = static_cast<int>(un.count());
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may get ready
   if (split > 0 && u0 >= u_all) {  // no keys in this stretch
     const int64_t r = r0 + threadIdx.x;
-    if (threadIdx.x < 16 && r < rows)
+    if (threadIdx.x < ROWS && r < rows)
       a.part_ml[((rq.t0 + r / a.G) * a.Hq + static_cast<int64_t>(hk) * a.G + r % a.G) * a.splits + split] =
           make_float2(-INFINITY, 0.0f);
     return;
@@ -123,14 +128,14 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   const int full_lo = a.window > 0 ? static_cast<int>(max(int64_t{0}, p_hi - a.window + 1)) : 0;
   const int sinks = a.window > 0 ? static_cast<int>(a.sinks) : 0;
 
-  // Rows of this thread: g and g + 8; each sees [lo, hi) and the sinks below hi.
+  // Rows of this thread: g and g + 8 of its warp's 16; each sees [lo, hi) and the sinks below hi.
   const int g = lane >> 2, c = lane & 3;
   int lo[2], hi[2];
   uint32_t qf[D / 16][4];
   const uint16_t* qp = static_cast<const uint16_t*>(a.q);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int64_t r = r0 + g + 8 * e;
+    const int64_t r = r0 + rt * 16 + g + 8 * e;
     const bool real = r < rows;
     const int64_t i = real ? r / a.G : 0, pos = rq.first + i;
     hi[e] = real ? static_cast<int>(max(int64_t{0}, a.causal ? min(rq.len, pos + 1) : rq.len)) : 0;
@@ -147,16 +152,23 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
 #pragma unroll
   for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
 
-  uint8_t* ring = rows_smem + warp * S::RING;
+  const bool idle = r0 + rt * 16 >= rows;  // copies its half, and has no row of its own
+  auto together = [&] {  // the warps of a ring
+    if constexpr (RT == 1)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * RT) : "memory");
+  };
+  uint8_t* ring = rows_smem + group * S::RING;
   const uint32_t ring_a = smem_u32(ring);
   const int32_t* table = a.table + static_cast<int64_t>(b) * a.ldt;
   const int64_t page_elems = static_cast<int64_t>(a.Hkv) * D << a.page_shift;
-  const int64_t lane_elems = (static_cast<int64_t>(hk) * D << a.page_shift) + lane * 8;
+  const int64_t lane_elems = (static_cast<int64_t>(hk) * D << a.page_shift) + rt * (kUnit / RT) * D + lane * 8;
   const int page_mask = (1 << a.page_shift) - 1;
   // Chunk ch of row r sits at chunk ch ^ (r % 8) of its 128 bytes.  A lane copies
-  // chunk lane % CH of rows lane / CH + RPI x; reads keys (lane & 7) + 8 (lane / 16)
+  // chunk lane % CH of rows lane / CH + RPI x of its warp's share; reads keys (lane & 7) + 8 (lane / 16)
   // of K, (lane & 7) + 8 (lane / 8 % 2) of V.
-  const int cr = lane / CH, cc = lane % CH;
+  const int cr = rt * (kUnit / RT) + lane / CH, cc = lane % CH;
   uint32_t cp_off[COPIES < 4 ? COPIES : 4];
 #pragma unroll
   for (int x = 0; x < (COPIES < 4 ? COPIES : 4); ++x) {
@@ -201,22 +213,33 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
     cp_commit();  // an empty group keeps the count
   };
 
-  // Ring: the warp's units are u0 + warp, + 4, ..
-  int next = u0 + warp;
+  // Ring: the group's units are u0 + group, + GROUPS, ..
+  int next = u0 + group;
 #pragma unroll
-  for (int s = 0; s < S::STAGES - 1; ++s, next += kRowsWarps) load(next, s, page_of(next));
+  for (int s = 0; s < S::STAGES - 1; ++s, next += S::GROUPS) load(next, s, page_of(next));
   int32_t next_page = page_of(next);
   int stage = 0, fill = S::STAGES - 1;
-  for (int i = u0 + warp; i < u1; i += kRowsWarps) {
+  for (int i = u0 + group; i < u1; i += S::GROUPS) {
     cp_wait<S::STAGES - 2>();
-    __syncwarp();
-    const int32_t pg = next_page;
-    next_page = page_of(next + kRowsWarps);
-    load(next, fill, pg);
-    next += kRowsWarps;
+    together();  // the unit is there, and the stage before it has been read by all
     const uint32_t ka = ring_a + stage * 2 * S::KV, va = ka + S::KV;
     const int k0 = unit_at(i) * kUnit;
 
+    const bool page_in = (present >> stage) & 1u;
+    const bool full = page_in && k0 + kUnit <= full_hi && (k0 >= full_lo || k0 + kUnit <= sinks);
+    const bool mixed = !full && page_in && p_lo < p_hi;
+    auto refill = [&] {  // the stage before this one
+      const int32_t pg = next_page;
+      next_page = page_of(next + S::GROUPS);
+      load(next, fill, pg);
+      next += S::GROUPS;
+    };
+    if (RT > 1 && idle && !mixed) {
+      refill();
+      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+      fill = fill + 1 == S::STAGES ? 0 : fill + 1;
+      continue;
+    }
     float s[2][2][4];  // two accumulation chains per 8 keys
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -229,8 +252,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
       mma16816<BF16>(s[ks & 1][0], qf[ks], kf[0], kf[1]);
       mma16816<BF16>(s[ks & 1][1], qf[ks], kf[2], kf[3]);
     }
-    const bool page_in = (present >> stage) & 1u;
-    const bool full = page_in && k0 + kUnit <= full_hi && (k0 >= full_lo || k0 + kUnit <= sinks);
+    refill();  // (its instructions fill the time that the products take)
     float mx[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -287,7 +309,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
         pl[2 * t + e] = pack2<BF16>(x - h.x, y - h.y);
       }
     }
-    if (!full && page_in && p_lo < p_hi) {
+    if (mixed) {
       // Rows of this unit see different keys.  A key that some row does not see
       // may hold an infinity or a NaN, and 0 times that is no 0: such keys leave
       // the tensor product (their values are zeroed in the stage) and are added
@@ -295,17 +317,17 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
       uint8_t* vs = ring + stage * 2 * S::KV + S::KV;
       uint32_t bad = 0;
 #pragma unroll
-      for (int x = 0; x < COPIES; ++x) {
+      for (int x = 0; x < kUnit / RPI; ++x) {
         const uint4 u = *reinterpret_cast<const uint4*>(vs + (lane + 32 * x) * 16);
         if (nonfinite2<BF16>(u.x) || nonfinite2<BF16>(u.y) || nonfinite2<BF16>(u.z) || nonfinite2<BF16>(u.w))
-          bad |= 1u << (cr + RPI * x);
+          bad |= 1u << (lane / CH + RPI * x);
       }
       bad = __reduce_or_sync(0xffffffffu, bad);
-      while (bad) {
-        const int r = __ffs(bad) - 1, j = k0 + r;
-        bad &= bad - 1;
+      if (RT > 1) together();  // all have looked
+      for (uint32_t left = bad; left; left &= left - 1) {
+        const int r = __ffs(left) - 1, j = k0 + r;
         const int src = (lane & ~3) | ((r & 7) >> 1);
-        uint8_t* vr = vs + r * (D * 2);
+        const uint8_t* vr = vs + r * (D * 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float q0 = __shfl_sync(0xffffffffu, r < 8 ? s[0][0][2 * e] : s[0][1][2 * e], src);
@@ -321,9 +343,13 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
             }
           }
         }
-        __syncwarp();
-        if (lane < CH) *reinterpret_cast<uint4*>(vr + lane * 16) = make_uint4(0, 0, 0, 0);
-        __syncwarp();
+      }
+      if (bad) {
+        together();  // all have added
+        for (uint32_t left = bad; left; left &= left - 1)
+          if (lane < CH && rt == 0)
+            *reinterpret_cast<uint4*>(vs + (__ffs(left) - 1) * (D * 2) + lane * 16) = make_uint4(0, 0, 0, 0);
+        together();
       }
     }
 #pragma unroll
@@ -335,7 +361,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
       mma16816<BF16>(o[2 * j], pl, vf[0], vf[1]);
       mma16816<BF16>(o[2 * j + 1], pl, vf[2], vf[3]);
     }
-    __syncwarp();  // every lane has read the stage before it is refilled
+    if (RT == 1) __syncwarp();  // every lane has read the stage before it is refilled
     stage = stage + 1 == S::STAGES ? 0 : stage + 1;
     fill = fill + 1 == S::STAGES ? 0 : fill + 1;
   }
@@ -357,17 +383,17 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
       *reinterpret_cast<float2*>(ow + (warp * 16 + row) * D + j * 8 + 2 * c) = make_float2(o[j][2 * e], o[j][2 * e + 1]);
   }
   __syncthreads();
-  constexpr int TPR = kRowsThreads / 16;  // threads per row
-  const int row = threadIdx.x / TPR, part = threadIdx.x % TPR;
-  const int64_t r = r0 + row;
+  constexpr int TPR = kRowsThreads / ROWS;  // threads per row
+  const int part = threadIdx.x % TPR, row = threadIdx.x / TPR % 16, own = threadIdx.x / TPR / 16;  // row of tile `own`
+  const int64_t r = r0 + own * 16 + row;
   if (r >= rows) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, ml[w * 16 + row].x);
-  float f[kRowsWarps], sum = 0.0f;
+  for (int w = 0; w < S::GROUPS; ++w) M = fmaxf(M, ml[(w * RT + own) * 16 + row].x);
+  float f[S::GROUPS], sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kRowsWarps; ++w) {
-    const float2 x = ml[w * 16 + row];
+  for (int w = 0; w < S::GROUPS; ++w) {
+    const float2 x = ml[(w * RT + own) * 16 + row];
     f[w] = x.x == -INFINITY ? x.y * 0.0f : ex2(x.x - M);  // (no finite score: 0, or NaN where one was NaN)
     sum += f[w] * x.y;
   }
@@ -383,8 +409,8 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
     float x = 0.0f, y = 0.0f;
     if (!empty) {
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
-        const float2 v = *reinterpret_cast<const float2*>(ow + (w * 16 + row) * D + d);
+      for (int w = 0; w < S::GROUPS; ++w) {
+        const float2 v = *reinterpret_cast<const float2*>(ow + ((w * RT + own) * 16 + row) * D + d);
         if (f[w] != 0.0f) {  // a warp without keys adds nothing, whatever it holds
           x = fmaf(f[w], v.x, x);
           y = fmaf(f[w], v.y, y);
@@ -471,55 +497,65 @@ cudaError_t launch_join(const PagedArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, BF16>, a);
 }
 
-template <int D, bool BF16>
-cudaError_t launch_rows(const PagedArgs& a, cudaStream_t s) {
-  auto kern = paged_rows_kernel<D, BF16>;
+template <int D, bool BF16, int RT>
+cudaError_t launch_rows_t(const PagedArgs& a, cudaStream_t s) {
+  using S = RowsShape<D, RT>;
+  auto kern = paged_rows_kernel<D, BF16, RT>;
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!attr_set[dev]) {
     const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsShape<D>::BYTES);
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
     if (e != cudaSuccess) return e;
+    // all of the SM's memory as shared memory: three CTAs of 32 rows need it
+    const cudaError_t e2 = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e2 != cudaSuccess) return e2;
     attr_set[dev] = true;
   }
-  const int64_t tiles = (a.max_q * a.G + 15) / 16;
+  const int64_t tiles = (a.max_q * a.G + 16 * RT - 1) / (16 * RT);
   if (tiles * a.splits > INT32_MAX) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(tiles * a.splits), static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.B));
-  kern<<<grid, kRowsThreads, RowsShape<D>::BYTES, s>>>(a, static_cast<int>(tiles));
+  kern<<<grid, kRowsThreads, S::BYTES, s>>>(a, static_cast<int>(tiles));
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess || a.splits == 1 ? e : launch_join<D, BF16>(a, s);
+}
+
+template <int D, bool BF16>
+cudaError_t launch_rows(const PagedArgs& a, cudaStream_t s) {
+  return a.max_q * a.G <= 16 ? launch_rows_t<D, BF16, 1>(a, s) : launch_rows_t<D, BF16, 2>(a, s);
 }
 
 }  // namespace
 
 // Which kernel, and how the keys are split.  Up to 32 rows a (request, kv head)
-// the rows kernel; above, its tiles would read the keys from the L2 once more for
-// every 16 rows, and the tile kernel takes 256 rows at a time.
+// the rows kernel; above, its CTAs would read the keys from the L2 once more for
+// every 32 rows, and the tile kernel takes 256 rows at a time.
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,
                      bool causal, int64_t window, int64_t sinks) {
   PagedPlan p;
   const int64_t G = Hq / Hkv, rows = max_q * G;
   p.tiles = rows > 32 && G <= kTileRows;
   const int unit = p.tiles ? kTileKeys : kUnit;
-  const int64_t tile_rows = p.tiles ? 2 * (kTileRows / G) * G : 16;
+  const int64_t tile_rows = p.tiles ? 2 * (kTileRows / G) * G : rows <= 16 ? 16 : 32;
   // Keys that the rows of one CTA can see, in units.
   int64_t span = max_kv;
   if (causal && window > 0 && window + tile_rows + sinks < span) span = window + tile_rows + sinks;
   const int64_t units = span / unit + 3;
   const int64_t ctas = B * Hkv * ((rows + tile_rows - 1) / tile_rows);
-  // Rows kernel: the 148 SMs hold two CTAs each.  Requests whose rows all see about
+  // Rows kernel: the 148 SMs hold two CTAs of 16 rows each, or three of 32.  Requests whose rows all see about
   // as many keys (one request, or a window shorter than they are) are cut into as
   // many stretches as make one wave; others, whose lengths differ, into finer ones,
   // up to eight waves where all are as long as announced (64 requests of 1k to 24k
   // keys: 901 us with one wave, 662 with four, 631 with eight; one of 120k: 111,
-  // 142 and 187).  None is shorter than 1024 keys, or joining costs more than it
-  // saves.  Tile kernel (one CTA per SM): split only while CTAs are fewer than SMs,
+  // 142 and 187).  None is shorter than 1024 keys (512 with 32 rows, which are
+  // slower work), or joining costs more than it saves.  Tile kernel (one CTA per SM): split only while CTAs are fewer than SMs,
   // into stretches of 512 keys or more.
   const bool alike = B == 1 || span < max_kv;
-  const int64_t goal = p.tiles ? 148 : alike ? 296 : 296 * (B < 8 ? (B > 0 ? B : 1) : 8);
-  const int64_t least = p.tiles ? 512 / kTileKeys : 1024 / kUnit;
-  int64_t splits = ctas >= goal ? 1 : (goal + (p.tiles ? 0 : ctas / 2)) / (ctas > 0 ? ctas : 1);
+  const int64_t wave = p.tiles ? 148 : 148 * (rows <= 16 ? 2 : 3);
+  const int64_t goal = p.tiles || alike ? wave : wave * (B < 8 ? (B > 0 ? B : 1) : 8);
+  const int64_t least = p.tiles ? 512 / kTileKeys : (rows <= 16 ? 1024 : 512) / kUnit;
+  int64_t splits = ctas >= goal ? 1 : goal / (ctas > 0 ? ctas : 1);  // (one CTA more than a wave would be two waves)
   if (splits > units / least) splits = units / least;
   if (splits > kJoinMax) splits = kJoinMax;
   if (splits < 1) splits = 1;

@@ -603,7 +603,7 @@ B2Q_API int b2q_qkv_rope_cache(const float* qkv, int64_t T, int64_t Hq, int64_t 
  * are, only slower); nothing is read back.  q, o 16-byte aligned with strides
  * multiples of 16 bytes; workspace 256-byte aligned, at least
  * b2q_attention_paged_workspace_bytes of the same sizes (0: may be NULL).
- * D is 64 or 128.  Results do not depend on timing. */
+ * T * Hq < 2^31; D is 64 or 128.  Results do not depend on timing. */
 B2Q_API size_t b2q_attention_paged_workspace_bytes(int64_t B, int64_t T, int64_t max_new, int64_t max_kv, int64_t Hq,
                                                    int64_t Hkv, int64_t D, int causal, int64_t window, int64_t sinks);
 B2Q_API int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_bytes, const int32_t* cu_new, int64_t B,

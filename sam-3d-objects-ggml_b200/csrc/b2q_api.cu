@@ -1263,7 +1263,7 @@ static int paged_sizes(int64_t B, int64_t T, int64_t max_new, int64_t max_kv, in
     return B2Q_ERR_INVALID_ARG;
   if (D != 64 && D != 128) return B2Q_ERR_UNSUPPORTED;
   if (B > 65535 || Hkv > 65535 || Hq > 65535 || T > INT_MAX || max_new > INT_MAX || max_kv > INT_MAX ||
-      window > INT_MAX || sinks > INT_MAX || max_new * Hq > INT_MAX)
+      window > INT_MAX || sinks > INT_MAX || max_new * Hq > INT_MAX || T * Hq > INT_MAX)
     return B2Q_ERR_TOO_LARGE;
   return B2Q_OK;
 }

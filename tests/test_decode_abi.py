@@ -94,6 +94,13 @@ def test_attention_workspace_size(b2q_mod):
     assert f(-1, 2, 1, 100000, 8, 2, 128) == 0
 
 
+def test_attention_rows_times_heads_are_bounded(b2q_mod):
+    # T * Hq past 2^31: the partial outputs of such a call would not fit the byte counts
+    f = b2q.attention_paged_workspace_bytes
+    assert f(1, 1 << 26, 1, 1 << 30, 64, 1, 128) == 0
+    assert attn(T=1 << 26, mn=1, Hq=64, Hkv=1, ldq=1 << 14, ldo=1 << 14) == TOO
+
+
 def vec(**kw):
     a = dict(wt=2, w=FAKE, n=64, k=1024, xt=0, x=FAKE, m=4, ldx=4096, bias=None, gate=None, resid=None, ldr=0, y=FAKE,
              ldy=256)

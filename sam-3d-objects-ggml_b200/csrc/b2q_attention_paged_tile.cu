@@ -49,7 +49,7 @@ constexpr int kPtThreads = 384;
 constexpr int kPtLaunchRegs = 168, kPtRegsControl = 56, kPtRegsSoftmax = 224;
 static_assert(128 * kPtRegsControl + 256 * kPtRegsSoftmax <= kPtThreads * kPtLaunchRegs, "register split");
 constexpr int kQHalf = 128 * 128, kHalf = kTileKeys * 128;  // bytes of 64 columns of Q, and of K or V
-constexpr int kPolyPairs = 1;     // of every 4 pairs of exps, on the FMA pipe (0: 1076 us on the listed chunk, 1: 993, 2: 1005)
+constexpr int kPolyPairs = 1;     // of every 4 pairs of exps, on the FMA pipe (the chunks above: 0 1076 us, 1 993, 2 1005)
 constexpr int kMaxEdges = 24;     // edge tiles of a CTA that can hold non-finite keys
 
 template <int D>

@@ -15,8 +15,7 @@
 // balanced base-256 digits), x = s (65536 p0 + 256 p1 + p2) with signed 8-bit
 // digits, an absolute error of at most s / 2 <= 2^-23 of the block's largest
 // magnitude -- half an ulp of an fp32 number of that size.  The block sums are
-// exact in int32; they are read as fp32 through an accumulator that starts at
-// the bits of 1.5 * 2^23 (|sum| < 2^22), scaled and added in fp32.
+// exact in int32, converted, scaled and added in fp32.
 //
 // One CTA per SM, 16 or 24 warps.  The activations of a run of K ("chunk") are split
 // into digits once per CTA and stay in shared memory; then the CTA walks its
@@ -27,7 +26,15 @@
 //   up to 4 tokens (NT 1 or 2 products a block, two tokens each): a token's
 //     columns are (p0, p1, -, p2), so a lane's pair of sums is 256 p0 + p1, or p2:
 //     one number to scale
-//   5 to 8 tokens (NT 3, WIDE): one product per digit, columns are tokens
+//   5 to 8 tokens (NT 3, WIDE): one product per digit, columns are tokens; the
+//     sums of the highest digit (|sum| < 2^22) are read as fp32 through an
+//     accumulator that starts at the bits of 1.5 * 2^23
+// Three or four products of the first kind instead, for 5 to 8 tokens, of a
+// 49152 x 8192 weight: 157 us against 125 (8 tokens, Q4_K), 111 against 111 (6).
+// Measured: that weight in Q4_K, one token: 51 us, 4450 GB/s, bound by the issue
+// of 2.7 lane instructions a value; 8192 x 4096 Q4_0, 4 tokens: 14.4 us, of which
+// the digits of the activations are a third; 6144 x 1024 Q4_0, one token: 4.7 us,
+// a launch and one CTA's chain (the weight's bytes are 0.6 us).
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
 

@@ -12,22 +12,27 @@
 // major: a key is read once for all of them.
 //
 // Few rows (paged_rows_kernel): bound by the cache's bytes.  A CTA of four
-// warps takes 16 rows, or 32 (RT 2), and one stretch of the keys.  With 16 rows
-// every warp takes units of 16 keys in turn, with a ring of cp.async stages of its
-// own (no barrier inside the loop), its own running maxima, sums and outputs, and
-// they join at the end.  With 32, two warps share a ring, each copies half of a
-// unit and works on 16 of the rows, and a barrier of the two stands where a warp
-// alone has none.  (Two CTAs of 16 rows instead read the keys twice, and the L2 did
-// not make up for it: 24 rows over 120k keys took 192 us.)  A unit lies inside one
+// warps takes 16 rows, or 32 (RT 2), and one stretch of the keys.  Every warp takes
+// units of 16 keys in turn, with a ring of cp.async stages of its own (no barrier
+// inside the loop), its own running maxima, sums and outputs for all the rows, and
+// they join at the end.  With 32 rows an operand of keys serves two products, and q
+// comes from shared memory: outputs take the registers.  (Two warps with 16 rows each
+// and a shared ring instead, a barrier of the two per unit: 104 us against 88 for 24
+// rows over 120k keys, 143 against 117 for 64 requests with heads of 64.  Two CTAs of
+// 16 rows read the keys twice: 192 us.)  A unit lies inside one
 // page (pages are multiples of 16), keys that no row of the CTA sees are not loaded
 // but filled with zeros.  Products are m16n8k16; P is fed to the second product as
 // two 16-bit numbers, P and what rounding it left: the tensor pipe idles behind the
 // loads, and a single rounding of P would cost as much accuracy as the output's own.
+// Before the first products stand three loads that need one another (lengths, page,
+// keys), so the pages of a whole ring are asked for at once, ahead of q: with one
+// after the other, and 64-bit row numbers, a CTA took 7 us to its first unit, now 4.5.
 // Stretches are split over CTAs when the rows alone do not fill the GPU; a
 // second kernel then joins their outputs by their maxima and sums.
-// Measured (32 / 8 heads of 128): 64 requests of 0.9k to 24k keys 480 us,
-// 6800 GB/s; one of 120k keys 85 us, 5800 GB/s; 3 requests of 16 heads of 64
-// over at most 900 keys 10.5 us, two launches and one CTA's chain of units.
+// Measured (32 / 8 heads of 128): 64 requests of 0.9k to 24k keys 475 us,
+// 6850 GB/s; one of 120k keys 81 us, 6080 GB/s; 16 requests, 24 / 4 heads, a window of
+// 4096 keys, 1 to 5 tokens 37 us, 3630 GB/s; 3 requests of 16 heads of 64
+// over at most 900 keys 8.6 us, a launch and one CTA's chain of units.
 #include "b2q_internal.h"
 #include "b2q_paged.cuh"
 #include "b2q_ptx.cuh"
@@ -82,30 +87,29 @@ __device__ __forceinline__ void cp_wait() {
 }
 template <int D, int RT>
 struct RowsShape {
-  static constexpr int GROUPS = kRowsWarps / RT;         // of RT warps with a ring each
-  static constexpr int STAGES = RT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 8 : 4);
+  static constexpr int STAGES = D == 64 ? 4 : 3;
   static constexpr int KV = kUnit * D * 2;               // bytes of one unit's keys (or values)
-  static constexpr int RING = STAGES * 2 * KV;           // per group
-  static constexpr int BYTES = GROUPS * RING;
+  static constexpr int RING = STAGES * 2 * KV;           // per warp
+  static constexpr int Q = RT == 1 ? 0 : 16 * RT * D * 2;  // q rows, where the registers do not hold them
+  static constexpr int BYTES = kRowsWarps * RING + Q;
 };
 
 template <int D, bool BF16, int RT>
-__global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArgs a, const int tiles) {
+__global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const PagedArgs a, const int tiles) {
   using S = RowsShape<D, RT>;
   constexpr int CH = D / 8;         // 16-byte chunks of a row
   constexpr int RPI = 32 / CH;      // rows that a warp copies at a time
-  constexpr int COPIES = kUnit / RT / RPI;
+  constexpr int COPIES = kUnit / RPI;
   constexpr int ROWS = 16 * RT;     // of the CTA
   extern __shared__ __align__(128) uint8_t rows_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = warp / RT, rt = warp % RT;
   const int b = blockIdx.z, hk = blockIdx.y;
   const int split = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   const Request rq = request_of(a, b);
-  const int64_t rows = rq.n * a.G;
-  const int64_t r0 = static_cast<int64_t>(tile) * ROWS;
+  // (max_q * Hq is below 2^31: row numbers fit 32 bits, whose divisions cost far less)
+  const uint32_t G = a.G, rows = static_cast<uint32_t>(rq.n) * G, r0 = static_cast<uint32_t>(tile) * ROWS;
   if (r0 >= rows) return;
-  const int64_t p_lo = rq.first + r0 / a.G, p_hi = rq.first + min(rows - 1, r0 + ROWS - 1) / a.G;
+  const int64_t p_lo = rq.first + r0 / G, p_hi = rq.first + min(rows - 1, r0 + ROWS - 1) / G;
   const Units un = units_of(a, rq.len, p_lo, p_hi, kUnit);
   // the last stretch takes what a longer request than announced has left
   const int u_all = static_cast<int>(un.count());
@@ -114,14 +118,24 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
       split == a.splits - 1 ? u_all : static_cast<int>(min(static_cast<int64_t>(u_all), u0 + a.split_units));
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may get ready
   if (split > 0 && u0 >= u_all) {  // no keys in this stretch
-    const int64_t r = r0 + threadIdx.x;
+    const uint32_t r = r0 + threadIdx.x;
     if (threadIdx.x < ROWS && r < rows)
-      a.part_ml[((rq.t0 + r / a.G) * a.Hq + static_cast<int64_t>(hk) * a.G + r % a.G) * a.splits + split] =
+      a.part_ml[((rq.t0 + r / G) * a.Hq + static_cast<int64_t>(hk) * G + r % G) * a.splits + split] =
           make_float2(-INFINITY, 0.0f);
     return;
   }
   const int su = static_cast<int>(un.su), gap = static_cast<int>(un.wu - un.su);
   auto unit_at = [&](int i) { return i < su ? i : i + gap; };
+  const int32_t* table = a.table + static_cast<int64_t>(b) * a.ldt;
+  // The page of unit i of the stretch (-1: none).
+  auto page_of = [&](int i) -> int32_t {
+    return i < u1 ? __ldg(table + ((unit_at(i) * kUnit) >> a.page_shift)) : -1;
+  };
+  // The warp's units are u0 + warp, + kRowsWarps, ..; the first pages are asked for before all else.
+  int next = u0 + warp;
+  int32_t first_pages[S::STAGES];
+#pragma unroll
+  for (int s = 0; s < S::STAGES; ++s) first_pages[s] = page_of(next + s * kRowsWarps);
 
   // Keys: rows of the CTA see [win_lo, key_end) and [0, sinks); every one sees
   // [full_lo, full_hi) and the sinks below full_hi.
@@ -131,47 +145,49 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   const int full_lo = a.window > 0 ? static_cast<int>(max(int64_t{0}, p_hi - a.window + 1)) : 0;
   const int sinks = a.window > 0 ? static_cast<int>(a.sinks) : 0;
 
-  // Rows of this thread: g and g + 8 of its warp's 16; each sees [lo, hi) and the sinks below hi.
+  // Rows of this thread: g and g + 8 of each 16; each sees [lo, hi) and the sinks below hi.
   const int g = lane >> 2, c = lane & 3;
-  int lo[2], hi[2];
-  uint32_t qf[D / 16][4];
+  int lo[RT][2], hi[RT][2];
+  uint32_t qf[RT == 1 ? D / 16 : 1][4];  // RT 1: the q operand; else it is read from shared memory
   const uint16_t* qp = static_cast<const uint16_t*>(a.q);
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int64_t r = r0 + rt * 16 + g + 8 * e;
-    const bool real = r < rows;
-    const int64_t i = real ? r / a.G : 0, pos = rq.first + i;
-    hi[e] = real ? static_cast<int>(max(int64_t{0}, a.causal ? min(rq.len, pos + 1) : rq.len)) : 0;
-    lo[e] = a.window > 0 ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
-    const uint16_t* src = qp + (rq.t0 + i) * a.ldq + (static_cast<int64_t>(hk) * a.G + (real ? r % a.G : 0)) * D;
+  for (int y = 0; y < RT; ++y)
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      qf[ks][e] = real ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * c) : 0u;
-      qf[ks][2 + e] = real ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + 2 * c) : 0u;
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t r = r0 + y * 16 + g + 8 * e;
+      const bool real = r < rows;
+      const uint32_t i = real ? r / G : 0;
+      const int64_t pos = rq.first + i;
+      hi[y][e] = real ? static_cast<int>(max(int64_t{0}, a.causal ? min(rq.len, pos + 1) : rq.len)) : 0;
+      lo[y][e] = a.window > 0 ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
+      if constexpr (RT == 1) {
+        const uint16_t* src = qp + (rq.t0 + i) * a.ldq + (static_cast<int64_t>(hk) * G + (real ? r - i * G : 0)) * D;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          qf[ks][e] = real ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * c) : 0u;
+          qf[ks][2 + e] = real ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + 2 * c) : 0u;
+        }
+      }
     }
+
+  float m[RT][2], l[RT][2], o[RT][D / 8][4];
+#pragma unroll
+  for (int y = 0; y < RT; ++y) {
+    m[y][0] = m[y][1] = -INFINITY;
+    l[y][0] = l[y][1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[y][j][0] = o[y][j][1] = o[y][j][2] = o[y][j][3] = 0.0f;
   }
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[D / 8][4];
-#pragma unroll
-  for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-
-  const bool idle = r0 + rt * 16 >= rows;  // copies its half, and has no row of its own
-  auto together = [&] {  // the warps of a ring
-    if constexpr (RT == 1)
-      __syncwarp();
-    else
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * RT) : "memory");
-  };
-  uint8_t* ring = rows_smem + group * S::RING;
+  uint8_t* ring = rows_smem + warp * S::RING;
   const uint32_t ring_a = smem_u32(ring);
-  const int32_t* table = a.table + static_cast<int64_t>(b) * a.ldt;
   const int64_t page_elems = static_cast<int64_t>(a.Hkv) * D << a.page_shift;
-  const int64_t lane_elems = (static_cast<int64_t>(hk) * D << a.page_shift) + rt * (kUnit / RT) * D + lane * 8;
+  const int64_t lane_elems = (static_cast<int64_t>(hk) * D << a.page_shift) + lane * 8;
   const int page_mask = (1 << a.page_shift) - 1;
   // Chunk ch of row r sits at chunk ch ^ (r % 8) of its 128 bytes.  A lane copies
-  // chunk lane % CH of rows lane / CH + RPI x of its warp's share; reads keys (lane & 7) + 8 (lane / 16)
+  // chunk lane % CH of rows lane / CH + RPI x; reads keys (lane & 7) + 8 (lane / 16)
   // of K, (lane & 7) + 8 (lane / 8 % 2) of V.
-  const int cr = rt * (kUnit / RT) + lane / CH, cc = lane % CH;
+  const int cr = lane / CH, cc = lane % CH;
   uint32_t cp_off[COPIES < 4 ? COPIES : 4];
 #pragma unroll
   for (int x = 0; x < (COPIES < 4 ? COPIES : 4); ++x) {
@@ -183,10 +199,6 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   const uint32_t v_off = vrow * (D * 2) + (((lane >> 4) ^ vrow) & 7) * 16;
 
   uint32_t present = 0;  // bit s: stage s holds a page's keys
-  // The page of unit i of the stretch (-1: none).
-  auto page_of = [&](int i) -> int32_t {
-    return i < u1 ? __ldg(table + ((unit_at(i) * kUnit) >> a.page_shift)) : -1;
-  };
   auto load = [&](int i, int stage, int32_t page) {
     present &= ~(1u << stage);
     if (i < u1) {
@@ -216,102 +228,131 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
     cp_commit();  // an empty group keeps the count
   };
 
-  // Ring: the group's units are u0 + group, + GROUPS, ..
-  int next = u0 + group;
+  uint32_t q_a = 0;
+  if constexpr (RT > 1) {  // q rows, chunks placed as the keys' are
+    uint8_t* qs = rows_smem + kRowsWarps * S::RING;
 #pragma unroll
-  for (int s = 0; s < S::STAGES - 1; ++s, next += S::GROUPS) load(next, s, page_of(next));
-  int32_t next_page = page_of(next);
+    for (int x = 0; x < ROWS * CH / kRowsThreads; ++x) {
+      const uint32_t row = (threadIdx.x + x * kRowsThreads) / CH, ch = threadIdx.x % CH, r = r0 + row, i = r / G;
+      const bool real = r < rows;
+      cp16(smem_u32(qs) + row * (D * 2) + ((ch & ~7) | ((ch ^ row) & 7)) * 16,
+           real ? qp + (rq.t0 + i) * a.ldq + (static_cast<int64_t>(hk) * G + (r - i * G)) * D + ch * 8 : qp, real);
+    }
+    cp_commit();
+    q_a = smem_u32(qs) + (lane & 15) * (D * 2) + (((lane >> 4) ^ lane) & 7) * 16;
+  }
+#pragma unroll
+  for (int s = 0; s < S::STAGES - 1; ++s, next += kRowsWarps) load(next, s, first_pages[s]);
+  int32_t next_page = first_pages[S::STAGES - 1];
+  if constexpr (RT > 1) {
+    cp_wait<S::STAGES - 1>();
+    __syncthreads();
+  }
   int stage = 0, fill = S::STAGES - 1;
-  for (int i = u0 + group; i < u1; i += S::GROUPS) {
+  for (int i = u0 + warp; i < u1; i += kRowsWarps) {
     cp_wait<S::STAGES - 2>();
-    together();  // the unit is there, and the stage before it has been read by all
+    __syncwarp();  // the unit is there
     const uint32_t ka = ring_a + stage * 2 * S::KV, va = ka + S::KV;
     const int k0 = unit_at(i) * kUnit;
 
     const bool page_in = (present >> stage) & 1u;
     const bool full = page_in && k0 + kUnit <= full_hi && (k0 >= full_lo || k0 + kUnit <= sinks);
     const bool mixed = !full && page_in && p_lo < p_hi;
-    auto refill = [&] {  // the stage before this one
-      const int32_t pg = next_page;
-      next_page = page_of(next + S::GROUPS);
-      load(next, fill, pg);
-      next += S::GROUPS;
-    };
-    if (RT > 1 && idle && !mixed) {
-      refill();
-      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-      fill = fill + 1 == S::STAGES ? 0 : fill + 1;
-      continue;
-    }
-    float s[2][2][4];  // two accumulation chains per 8 keys
+    float s[2][RT][2][4];  // (RT 1) two accumulation chains per 8 keys
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int y = 0; y < RT; ++y)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[0][t][x] = s[1][t][x] = 0.0f;
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[0][y][t][x] = s[1][y][t][x] = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
       uint32_t kf[4];
       ldsm4(((ka + k_off) ^ ((ks & 3) * 32)) + (ks >> 2) * 128, kf);
-      mma16816<BF16>(s[ks & 1][0], qf[ks], kf[0], kf[1]);
-      mma16816<BF16>(s[ks & 1][1], qf[ks], kf[2], kf[3]);
+      if constexpr (RT == 1) {
+        mma16816<BF16>(s[ks & 1][0][0], qf[ks], kf[0], kf[1]);
+        mma16816<BF16>(s[ks & 1][0][1], qf[ks], kf[2], kf[3]);
+      } else {
+#pragma unroll
+        for (int y = 0; y < RT; ++y) {
+            uint32_t qq[4];
+          ldsm4((q_a ^ ((ks & 3) * 32)) + (ks >> 2) * 128 + y * 16 * (D * 2), qq);
+          mma16816<BF16>(s[0][y][0], qq, kf[0], kf[1]);
+          mma16816<BF16>(s[0][y][1], qq, kf[2], kf[3]);
+        }
+      }
     }
-    refill();  // (its instructions fill the time that the products take)
-    float mx[2];
+    {  // refill the stage before this one (its instructions fill the time that the products take)
+      const int32_t pg = next_page;
+      next_page = page_of(next + kRowsWarps);
+      load(next, fill, pg);
+      next += kRowsWarps;
+    }
+    float mx[RT][2];
+    bool grow = false;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int y = 0; y < RT; ++y)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) s[0][t][2 * e + x] = (s[0][t][2 * e + x] + s[1][t][2 * e + x]) * a.c2;
-      if (!full) {
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int j = k0 + t * 8 + 2 * c + x;
-            if (!(page_in && j < hi[e] && (j >= lo[e] || j < sinks))) s[0][t][2 * e + x] = -INFINITY;
+            float& v = s[0][y][t][2 * e + x];
+            v = (RT == 1 ? v + s[1][y][t][2 * e + x] : v) * a.c2;
           }
+        if (!full) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int j = k0 + t * 8 + 2 * c + x;
+              if (!(page_in && j < hi[y][e] && (j >= lo[y][e] || j < sinks))) s[0][y][t][2 * e + x] = -INFINITY;
+            }
+        }
+        float v = fmaxf(fmaxf(s[0][y][0][2 * e], s[0][y][0][2 * e + 1]), fmaxf(s[0][y][1][2 * e], s[0][y][1][2 * e + 1]));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        mx[y][e] = v;
+        // The maximum in use is raised only when a unit exceeds it by 2^8: P stays
+        // below 2^8, which 16-bit floats hold as exactly as values below 1.
+        grow |= v > m[y][e] + 8.0f || (m[y][e] == -INFINITY && v != -INFINITY);
       }
-      float v = fmaxf(fmaxf(s[0][0][2 * e], s[0][0][2 * e + 1]), fmaxf(s[0][1][2 * e], s[0][1][2 * e + 1]));
-      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-      mx[e] = v;
-    }
-    // The maximum in use is raised only when a unit exceeds it by 2^8: P stays
-    // below 2^8, which 16-bit floats hold as exactly as values below 1.
-    const bool grow = mx[0] > m[0] + 8.0f || (m[0] == -INFINITY && mx[0] != -INFINITY) || mx[1] > m[1] + 8.0f ||
-                      (m[1] == -INFINITY && mx[1] != -INFINITY);
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float nm = fmaxf(m[e], mx[e]);
-        const float al = m[e] == -INFINITY ? 0.0f : ex2(m[e] - nm);
-        m[e] = nm;
-        l[e] *= al;
+      for (int y = 0; y < RT; ++y)
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[j][2 * e] *= al;
-          o[j][2 * e + 1] *= al;
+        for (int e = 0; e < 2; ++e) {
+          const float nm = fmaxf(m[y][e], mx[y][e]);
+          const float al = m[y][e] == -INFINITY ? 0.0f : ex2(m[y][e] - nm);
+          m[y][e] = nm;
+          l[y][e] *= al;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            o[y][j][2 * e] *= al;
+            o[y][j][2 * e + 1] *= al;
+          }
+        }
+    }
+    uint32_t ph[RT][4], pl[RT][4];
+#pragma unroll
+    for (int y = 0; y < RT; ++y)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float base = m[y][e] == -INFINITY ? 0.0f : m[y][e];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float& x = s[0][y][t][2 * e];
+          float& z = s[0][y][t][2 * e + 1];
+          x = ex2(x - base);
+          z = ex2(z - base);
+          l[y][e] += x + z;
+          const uint32_t h2 = pack2<BF16>(x, z);
+          const float2 h = unpack2<BF16>(h2);
+          ph[y][2 * t + e] = h2;
+          pl[y][2 * t + e] = pack2<BF16>(x - h.x, z - h.y);
         }
       }
-    }
-    uint32_t ph[4], pl[4];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float base = m[e] == -INFINITY ? 0.0f : m[e];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float& x = s[0][t][2 * e];
-        float& y = s[0][t][2 * e + 1];
-        x = ex2(x - base);
-        y = ex2(y - base);
-        l[e] += x + y;
-        const uint32_t h2 = pack2<BF16>(x, y);
-        const float2 h = unpack2<BF16>(h2);
-        ph[2 * t + e] = h2;
-        pl[2 * t + e] = pack2<BF16>(x - h.x, y - h.y);
-      }
-    }
     if (mixed) {
       // Rows of this unit see different keys.  A key that some row does not see
       // may hold an infinity or a NaN, and 0 times that is no 0: such keys leave
@@ -326,82 +367,88 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
           bad |= 1u << (lane / CH + RPI * x);
       }
       bad = __reduce_or_sync(0xffffffffu, bad);
-      if (RT > 1) together();  // all have looked
       for (uint32_t left = bad; left; left &= left - 1) {
         const int r = __ffs(left) - 1, j = k0 + r;
         const int src = (lane & ~3) | ((r & 7) >> 1);
         const uint8_t* vr = vs + r * (D * 2);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float q0 = __shfl_sync(0xffffffffu, r < 8 ? s[0][0][2 * e] : s[0][1][2 * e], src);
-          const float q1 = __shfl_sync(0xffffffffu, r < 8 ? s[0][0][2 * e + 1] : s[0][1][2 * e + 1], src);
+        for (int ye = 0; ye < 2 * RT; ++ye) {
+          const int y = ye >> 1, e = ye & 1;
+          const float q0 = __shfl_sync(0xffffffffu, r < 8 ? s[0][y][0][2 * e] : s[0][y][1][2 * e], src);
+          const float q1 = __shfl_sync(0xffffffffu, r < 8 ? s[0][y][0][2 * e + 1] : s[0][y][1][2 * e + 1], src);
           const float p = (r & 1) ? q1 : q0;
-          if (j < hi[e] && (j >= lo[e] || j < sinks)) {
+          if (j < hi[y][e] && (j >= lo[y][e] || j < sinks)) {
 #pragma unroll
             for (int d = 0; d < D / 8; ++d) {
               const float2 v =
                   unpack2<BF16>(*reinterpret_cast<const uint32_t*>(vr + ((d & ~7) | ((d ^ r) & 7)) * 16 + c * 4));
-              o[d][2 * e] = fmaf(p, v.x, o[d][2 * e]);
-              o[d][2 * e + 1] = fmaf(p, v.y, o[d][2 * e + 1]);
+              o[y][d][2 * e] = fmaf(p, v.x, o[y][d][2 * e]);
+              o[y][d][2 * e + 1] = fmaf(p, v.y, o[y][d][2 * e + 1]);
             }
           }
         }
       }
       if (bad) {
-        together();  // all have added
+        __syncwarp();  // all have added
         for (uint32_t left = bad; left; left &= left - 1)
-          if (lane < CH && rt == 0)
+          if (lane < CH)
             *reinterpret_cast<uint4*>(vs + (__ffs(left) - 1) * (D * 2) + lane * 16) = make_uint4(0, 0, 0, 0);
-        together();
+        __syncwarp();
       }
     }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       uint32_t vf[4];
       ldsm4_t(((va + v_off) ^ ((j & 3) * 32)) + (j >> 2) * 128, vf);
-      mma16816<BF16>(o[2 * j], ph, vf[0], vf[1]);
-      mma16816<BF16>(o[2 * j + 1], ph, vf[2], vf[3]);
-      mma16816<BF16>(o[2 * j], pl, vf[0], vf[1]);
-      mma16816<BF16>(o[2 * j + 1], pl, vf[2], vf[3]);
+#pragma unroll
+      for (int y = 0; y < RT; ++y) {
+        mma16816<BF16>(o[y][2 * j], ph[y], vf[0], vf[1]);
+        mma16816<BF16>(o[y][2 * j + 1], ph[y], vf[2], vf[3]);
+        mma16816<BF16>(o[y][2 * j], pl[y], vf[0], vf[1]);
+        mma16816<BF16>(o[y][2 * j + 1], pl[y], vf[2], vf[3]);
+      }
     }
-    if (RT == 1) __syncwarp();  // every lane has read the stage before it is refilled
+    __syncwarp();  // every lane has read the stage before it is refilled
     stage = stage + 1 == S::STAGES ? 0 : stage + 1;
     fill = fill + 1 == S::STAGES ? 0 : fill + 1;
   }
   cp_wait<0>();
   __syncthreads();
 
-  // Join the four warps: [warp][row] (max, sum), then [warp][row][D].
+  // Join the four warps: [warp][row] (max, sum), then [warp][row][D], rows 8 banks apart.
+  constexpr int OP = D + 8;
   float2* ml = reinterpret_cast<float2*>(rows_smem);
-  float* ow = reinterpret_cast<float*>(rows_smem) + kRowsWarps * 16 * 2;
+  float* ow = reinterpret_cast<float*>(rows_smem) + kRowsWarps * ROWS * 2;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    float v = l[e];
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    v += __shfl_xor_sync(0xffffffffu, v, 2);
-    const int row = g + 8 * e;
-    if (c == 0) ml[warp * 16 + row] = make_float2(m[e], v);
+  for (int y = 0; y < RT; ++y)
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j)
-      *reinterpret_cast<float2*>(ow + (warp * 16 + row) * D + j * 8 + 2 * c) = make_float2(o[j][2 * e], o[j][2 * e + 1]);
-  }
+    for (int e = 0; e < 2; ++e) {
+      float v = l[y][e];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      const int row = warp * ROWS + y * 16 + g + 8 * e;
+      if (c == 0) ml[row] = make_float2(m[y][e], v);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2*>(ow + row * OP + j * 8 + 2 * c) = make_float2(o[y][j][2 * e], o[y][j][2 * e + 1]);
+    }
   __syncthreads();
   constexpr int TPR = kRowsThreads / ROWS;  // threads per row
-  const int part = threadIdx.x % TPR, row = threadIdx.x / TPR % 16, own = threadIdx.x / TPR / 16;  // row of tile `own`
-  const int64_t r = r0 + own * 16 + row;
+  const int part = threadIdx.x % TPR, row = threadIdx.x / TPR;
+  const uint32_t r = r0 + row;
   if (r >= rows) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < S::GROUPS; ++w) M = fmaxf(M, ml[(w * RT + own) * 16 + row].x);
-  float f[S::GROUPS], sum = 0.0f;
+  for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, ml[w * ROWS + row].x);
+  float f[kRowsWarps], sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < S::GROUPS; ++w) {
-    const float2 x = ml[(w * RT + own) * 16 + row];
+  for (int w = 0; w < kRowsWarps; ++w) {
+    const float2 x = ml[w * ROWS + row];
     f[w] = x.x == -INFINITY ? x.y * 0.0f : ex2(x.x - M);  // (no finite score: 0, or NaN where one was NaN)
     sum += f[w] * x.y;
   }
-  const int64_t t = rq.t0 + r / a.G;
-  const int64_t h = static_cast<int64_t>(hk) * a.G + r % a.G;
+  const int64_t t = rq.t0 + r / G;
+  const int64_t h = static_cast<int64_t>(hk) * G + r % G;
   const bool whole = a.splits == 1;
   const bool empty = M == -INFINITY && sum == 0.0f;
   const float inv = whole ? (empty ? 0.0f : 1.0f / sum) : 1.0f;
@@ -412,8 +459,8 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
     float x = 0.0f, y = 0.0f;
     if (!empty) {
 #pragma unroll
-      for (int w = 0; w < S::GROUPS; ++w) {
-        const float2 v = *reinterpret_cast<const float2*>(ow + ((w * RT + own) * 16 + row) * D + d);
+      for (int w = 0; w < kRowsWarps; ++w) {
+        const float2 v = *reinterpret_cast<const float2*>(ow + (w * ROWS + row) * OP + d);
         if (f[w] != 0.0f) {  // a warp without keys adds nothing, whatever it holds
           x = fmaf(f[w], v.x, x);
           y = fmaf(f[w], v.y, y);
@@ -427,70 +474,72 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedArg
   }
 }
 
-// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits, in their
-// order, for one (token, query head) a CTA.  The splits' weights are worked out
-// once, side by side; then every thread adds up its values, loads ahead.  Launched
-// with the attention kernel still running (it waits before it reads): 94 -> 83 us
-// for one request of 120k keys, with the warp-wide loop over 37 splits before.
+// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits for one
+// (token, query head) a CTA: every warp works out M and the sum, adds up its share of the
+// splits (one warp a split, a lane's values side by side, loads ahead), and the warps' sums
+// are added in their order.  One warp per two values looping over all the splits instead
+// took 25 us for 148 splits of 48 rows, as long as the attention itself.
+// Launched with the attention kernel still running (it waits before it reads).
 constexpr int kJoinMax = 1024;  // splits
+constexpr int kJoinWarps = 8;   // of a CTA, at most
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(D / 2) paged_join_kernel(const PagedArgs a) {
-  __shared__ float f[kJoinMax];
-  __shared__ float red[2][D / 64];
-  const int tid = threadIdx.x, lane = tid & 31;
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedArgs a) {
+  constexpr int V = D / 32;  // values of a lane
+  __shared__ __align__(16) float red[kJoinWarps][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Request rq = request_of(a, blockIdx.y);
   const int i = blockIdx.x / a.Hq, h = blockIdx.x - i * a.Hq;
   if (i >= rq.n) return;
   const int64_t pi = ((rq.t0 + i) * a.Hq + h) * a.splits;
+  const float2* ml = a.part_ml + pi;
+  const float* src = a.part_o + pi * D + lane * V;
   float m = -INFINITY;
-  for (int s = tid; s < a.splits; s += D / 2) m = fmaxf(m, a.part_ml[pi + s].x);
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[s].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (D == 128) {
-    if (lane == 0) red[0][tid >> 5] = m;
-    __syncthreads();
-    m = fmaxf(red[0][0], red[0][D / 64 - 1]);
-  }
+  // no key: 0, with nothing read; only NaN scores: NaN
+  auto weight = [&](float2 x) { return x.x == -INFINITY ? x.y : ex2(x.x - m); };
   float sum = 0.0f;
-  for (int s = tid; s < a.splits; s += D / 2) {
-    const float2 ml = a.part_ml[pi + s];
-    // no key: 0, with nothing read; only NaN scores: NaN
-    const float w = ml.x == -INFINITY ? ml.y : ex2(ml.x - m);
-    f[s] = w;
-    sum = fmaf(w, ml.y, sum);
-  }
+  for (int s = lane; s < a.splits; s += 32) sum = fmaf(weight(ml[s]), ml[s].y, sum);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (D == 128) {
-    if (lane == 0) red[1][tid >> 5] = sum;
-    __syncthreads();
-    sum = red[1][0] + red[1][D / 64 - 1];
-  } else {
-    __syncwarp();
-  }
-  float x = 0.0f, y = 0.0f;
-  const float2* src = reinterpret_cast<const float2*>(a.part_o + pi * D) + tid;
-#pragma unroll 8
-  for (int s = 0; s < a.splits; ++s) {
-    const float w = f[s];
+  float acc[V] = {};
+#pragma unroll 4
+  for (int s = warp; s < a.splits; s += warps) {
+    const float w = weight(ml[s]);
     if (w != 0.0f) {
-      const float2 v = src[s * (D / 2)];
-      x = fmaf(w, v.x, x);
-      y = fmaf(w, v.y, y);
+      float v[V];
+      if constexpr (V == 4)
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D);
+      else
+        *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src + static_cast<int64_t>(s) * D);
+#pragma unroll
+      for (int x = 0; x < V; ++x) acc[x] = fmaf(w, v[x], acc[x]);
     }
   }
+#pragma unroll
+  for (int x = 0; x < V; ++x) red[warp][lane * V + x] = acc[x];
+  __syncthreads();
   const float inv = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
-  *(reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo + static_cast<int64_t>(h) * D) + tid) =
-      pack2<BF16>(x * inv, y * inv);
+  uint16_t* to = static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo + static_cast<int64_t>(h) * D;
+  for (int d = 2 * threadIdx.x; d < D; d += 2 * blockDim.x) {
+    float x = 0.0f, y = 0.0f;
+    for (int w = 0; w < warps; ++w) {
+      const float2 v = *reinterpret_cast<const float2*>(&red[w][d]);
+      x += v.x;
+      y += v.y;
+    }
+    *reinterpret_cast<uint32_t*>(to + d) = pack2<BF16>(x * inv, y * inv);
+  }
 }
 
 template <int D, bool BF16>
 cudaError_t launch_join(const PagedArgs& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.max_q * a.Hq), static_cast<unsigned>(a.B));
-  cfg.blockDim = dim3(D / 2);
+  cfg.blockDim = dim3(32 * (a.splits >= 4 * kJoinWarps ? kJoinWarps : (a.splits + 3) / 4));
   cfg.stream = s;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -511,7 +560,7 @@ cudaError_t launch_rows_t(const PagedArgs& a, cudaStream_t s) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
     if (e != cudaSuccess) return e;
-    // all of the SM's memory as shared memory: three CTAs of 32 rows need it
+    // all of the SM's memory as shared memory: two CTAs of 32 rows need it
     const cudaError_t e2 = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     if (e2 != cudaSuccess) return e2;
     attr_set[dev] = true;
@@ -546,16 +595,16 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
   if (causal && window > 0 && window + tile_rows + sinks < span) span = window + tile_rows + sinks;
   const int64_t units = span / unit + 3;
   const int64_t ctas = B * Hkv * ((rows + tile_rows - 1) / tile_rows);
-  // Rows kernel: the 148 SMs hold two CTAs of 16 rows each, or three of 32.  Requests whose rows all see about
+  // Rows kernel: the 148 SMs hold two CTAs each.  Requests whose rows all see about
   // as many keys (one request, or a window shorter than they are) are cut into as
   // many stretches as make one wave; others, whose lengths differ, into finer ones,
   // up to eight waves where all are as long as announced (64 requests of 1k to 24k
   // keys: 901 us with one wave, 662 with four, 631 with eight; one of 120k: 111,
   // 142 and 187).  None is shorter than 1024 keys (512 with 32 rows, which are
-  // slower work), or joining costs more than it saves.  Tile kernel (one CTA per SM): split only while CTAs are fewer than SMs,
-  // into stretches of 512 keys or more.
+  // slower work), or joining costs more than it saves.  Tile kernel (one CTA per
+  // SM): split only while CTAs are fewer than SMs, into stretches of 512 keys or more.
   const bool alike = B == 1 || span < max_kv;
-  const int64_t wave = p.tiles ? 148 : 148 * (rows <= 16 ? 2 : 3);
+  const int64_t wave = p.tiles ? 148 : 148 * 2;
   const int64_t goal = p.tiles || alike ? wave : wave * (B < 8 ? (B > 0 ? B : 1) : 8);
   const int64_t least = p.tiles ? 512 / kTileKeys : (rows <= 16 ? 1024 : 512) / kUnit;
   int64_t splits = ctas >= goal ? 1 : goal / (ctas > 0 ? ctas : 1);  // (one CTA more than a wave would be two waves)

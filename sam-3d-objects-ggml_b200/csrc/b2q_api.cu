@@ -1328,6 +1328,7 @@ int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_bytes, con
   a.o = o;
   a.ldo = o_row_stride_bytes / 2;
   a.splits = static_cast<int>(p.splits);
+  a.cluster = p.cluster;
   a.split_units = p.split_units;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.part_o_bytes);

@@ -28,11 +28,12 @@
 // keys), so the pages of a whole ring are asked for at once, ahead of q: with one
 // after the other, and 64-bit row numbers, a CTA took 7 us to its first unit, now 4.5.
 // Stretches are split over CTAs when the rows alone do not fill the GPU; a
-// second kernel then joins their outputs by their maxima and sums.
+// second kernel, or the cluster that they form, then joins their outputs by their
+// maxima and sums.
 // Measured (32 / 8 heads of 128): 64 requests of 0.9k to 24k keys 475 us,
 // 6850 GB/s; one of 120k keys 81 us, 6080 GB/s; 16 requests, 24 / 4 heads, a window of
-// 4096 keys, 1 to 5 tokens 37 us, 3630 GB/s; 3 requests of 16 heads of 64
-// over at most 900 keys 8.6 us, a launch and one CTA's chain of units.
+// 4096 keys, 1 to 5 tokens 35.5 us, 3800 GB/s; 3 requests of 16 heads of 64
+// over at most 900 keys 6.1 us, a launch and one CTA's chain of units.
 #include "b2q_internal.h"
 #include "b2q_paged.cuh"
 #include "b2q_ptx.cuh"
@@ -40,6 +41,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 namespace b2q {
@@ -49,6 +51,7 @@ namespace {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kUnit = 16;  // keys
+constexpr int kClusterMax = 8;
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -85,6 +88,14 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// Two floats of the cluster's CTA `rank`, at this CTA's address of them.
+__device__ __forceinline__ float2 ld_cluster(uint32_t addr, int rank) {
+  uint32_t there;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(there) : "memory");
+  return v;
+}
 template <int D, int RT>
 struct RowsShape {
   static constexpr int STAGES = D == 64 ? 4 : 3;
@@ -104,7 +115,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
   extern __shared__ __align__(128) uint8_t rows_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, hk = blockIdx.y;
-  const int split = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+  // (the stretches of a cluster are neighbours)
+  const int split = a.cluster ? blockIdx.x % a.splits : blockIdx.x / tiles;
+  const int tile = a.cluster ? blockIdx.x / a.splits : blockIdx.x % tiles;
   const Request rq = request_of(a, b);
   // (max_q * Hq is below 2^31: row numbers fit 32 bits, whose divisions cost far less)
   const uint32_t G = a.G, rows = static_cast<uint32_t>(rq.n) * G, r0 = static_cast<uint32_t>(tile) * ROWS;
@@ -117,7 +130,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
   const int u1 =
       split == a.splits - 1 ? u_all : static_cast<int>(min(static_cast<int64_t>(u_all), u0 + a.split_units));
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may get ready
-  if (split > 0 && u0 >= u_all) {  // no keys in this stretch
+  if (split > 0 && u0 >= u_all && !a.cluster) {  // no keys in this stretch
     const uint32_t r = r0 + threadIdx.x;
     if (threadIdx.x < ROWS && r < rows)
       a.part_ml[((rq.t0 + r / G) * a.Hq + static_cast<int64_t>(hk) * G + r % G) * a.splits + split] =
@@ -436,7 +449,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
   constexpr int TPR = kRowsThreads / ROWS;  // threads per row
   const int part = threadIdx.x % TPR, row = threadIdx.x / TPR;
   const uint32_t r = r0 + row;
-  if (r >= rows) return;
+  if (r >= rows && !a.cluster) return;
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, ml[w * ROWS + row].x);
@@ -447,30 +460,77 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
     f[w] = x.x == -INFINITY ? x.y * 0.0f : ex2(x.x - M);  // (no finite score: 0, or NaN where one was NaN)
     sum += f[w] * x.y;
   }
-  const int64_t t = rq.t0 + r / G;
-  const int64_t h = static_cast<int64_t>(hk) * G + r % G;
-  const bool whole = a.splits == 1;
   const bool empty = M == -INFINITY && sum == 0.0f;
-  const float inv = whole ? (empty ? 0.0f : 1.0f / sum) : 1.0f;
-  const int64_t pi = (t * a.Hq + h) * a.splits + split;
-  if (!whole && part == 0) a.part_ml[pi] = make_float2(M, sum);
-#pragma unroll
-  for (int d = part * 2; d < D; d += TPR * 2) {
-    float x = 0.0f, y = 0.0f;
+  auto joined = [&](int d) {  // values d and d + 1 of the row
+    float2 x = make_float2(0.0f, 0.0f);
     if (!empty) {
 #pragma unroll
       for (int w = 0; w < kRowsWarps; ++w) {
         const float2 v = *reinterpret_cast<const float2*>(ow + (w * ROWS + row) * OP + d);
         if (f[w] != 0.0f) {  // a warp without keys adds nothing, whatever it holds
-          x = fmaf(f[w], v.x, x);
-          y = fmaf(f[w], v.y, y);
+          x.x = fmaf(f[w], v.x, x.x);
+          x.y = fmaf(f[w], v.y, x.y);
         }
       }
     }
+    return x;
+  };
+  if (a.cluster) {
+    // Each CTA leaves its rows where its first warp's were; then the CTAs share out the
+    // values and read them from each other.
+    __shared__ float2 done[ROWS];
+    if (part == 0) done[row] = make_float2(M, sum);
+#pragma unroll
+    for (int d = part * 2; d < D; d += TPR * 2) *reinterpret_cast<float2*>(ow + row * OP + d) = joined(d);
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    const int pairs = static_cast<int>(min(rows - r0, static_cast<uint32_t>(ROWS))) * (D / 2);
+    for (int p = split * kRowsThreads + threadIdx.x; p < pairs; p += a.splits * kRowsThreads) {
+      const int prow = p / (D / 2), d = p % (D / 2) * 2;
+      const uint32_t at_ml = smem_u32(&done[prow]), at_o = smem_u32(ow + prow * OP + d);
+      float2 sm[kClusterMax], so[kClusterMax];
+#pragma unroll
+      for (int w = 0; w < kClusterMax; ++w) {
+        sm[w] = make_float2(-INFINITY, 0.0f);
+        so[w] = make_float2(0.0f, 0.0f);
+        if (w < a.splits) sm[w] = ld_cluster(at_ml, w), so[w] = ld_cluster(at_o, w);
+      }
+      float m_all = -INFINITY, l_all = 0.0f;
+      float2 x = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kClusterMax; ++w) m_all = fmaxf(m_all, sm[w].x);
+#pragma unroll
+      for (int w = 0; w < kClusterMax; ++w) {
+        const float u = sm[w].x == -INFINITY ? sm[w].y * 0.0f : ex2(sm[w].x - m_all);  // (as above)
+        l_all = fmaf(u, sm[w].y, l_all);
+        if (u != 0.0f) {
+          x.x = fmaf(u, so[w].x, x.x);
+          x.y = fmaf(u, so[w].y, x.y);
+        }
+      }
+      const float inv = m_all == -INFINITY && l_all == 0.0f ? 0.0f : 1.0f / l_all;
+      const uint32_t rr = r0 + prow, i = rr / G;
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo +
+                                   (static_cast<int64_t>(hk) * G + (rr - i * G)) * D + d) =
+          pack2<BF16>(x.x * inv, x.y * inv);
+    }
+    // none may go while others read from it
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    return;
+  }
+  const int64_t t = rq.t0 + r / G;
+  const int64_t h = static_cast<int64_t>(hk) * G + r % G;
+  const bool whole = a.splits == 1;
+  const float inv = whole ? (empty ? 0.0f : 1.0f / sum) : 1.0f;
+  const int64_t pi = (t * a.Hq + h) * a.splits + split;
+  if (!whole && part == 0) a.part_ml[pi] = make_float2(M, sum);
+#pragma unroll
+  for (int d = part * 2; d < D; d += TPR * 2) {
+    const float2 x = joined(d);
     if (whole)
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + t * a.ldo + h * D + d) = pack2<BF16>(x * inv, y * inv);
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + t * a.ldo + h * D + d) =
+          pack2<BF16>(x.x * inv, x.y * inv);
     else
-      *reinterpret_cast<float2*>(a.part_o + pi * D + d) = make_float2(x, y);
+      *reinterpret_cast<float2*>(a.part_o + pi * D + d) = x;
   }
 }
 
@@ -568,6 +628,20 @@ cudaError_t launch_rows_t(const PagedArgs& a, cudaStream_t s) {
   const int64_t tiles = (a.max_q * a.G + 16 * RT - 1) / (16 * RT);
   if (tiles * a.splits > INT32_MAX) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(tiles * a.splits), static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.B));
+  if (a.cluster) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = static_cast<unsigned>(a.splits);
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, a, static_cast<int>(tiles));
+  }
   kern<<<grid, kRowsThreads, S::BYTES, s>>>(a, static_cast<int>(tiles));
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess || a.splits == 1 ? e : launch_join<D, BF16>(a, s);
@@ -600,20 +674,41 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_
   // many stretches as make one wave; others, whose lengths differ, into finer ones,
   // up to eight waves where all are as long as announced (64 requests of 1k to 24k
   // keys: 901 us with one wave, 662 with four, 631 with eight; one of 120k: 111,
-  // 142 and 187).  None is shorter than 1024 keys (512 with 32 rows, which are
-  // slower work), or joining costs more than it saves.  Tile kernel (one CTA per
-  // SM): split only while CTAs are fewer than SMs, into stretches of 512 keys or more.
+  // 142 and 187).  Past one wave none is shorter than 512 keys, or joining
+  // costs more than it saves (16 requests of up to 2000 keys, 8 kv heads: 24.8 us in
+  // stretches of 1024, 18.2 of 512; 24 rows each: 30 us of 256, 26 of 512).  Up to one
+  // wave 128 keys are enough where there are 512 or more (one request, 8 kv heads of
+  // 128, 4k keys: 21.1 us in stretches of 1024, 13.8 of 512, 10.3 of 128, 11.0 of 64;
+  // 700 keys: 10.9 whole, 8.3 of 128; 300 keys: 6.8 whole, 8.0 of 128).
+  // Up to eight stretches of 64 keys or more that leave an eighth of a wave free (clusters
+  // do not fill it to the last CTA) are a cluster that joins in its own memory, from
+  // 256 keys on: one launch, which saves a caller 4.5 us of host time and the GPU 2 (300
+  // keys: 6.0 us, 700: 6.2 against 8.6 with the joining kernel, 1500: 7.0 and 8.9, 4k: 10.5
+  // and 10.6).  Eight stretches are kept although one wave has room for more as long as
+  // they have at most 640 keys, 256 with 32 rows (8k keys: 15.8 us and 13.0; 24 rows of 4k
+  // keys: 15.2 and 11.3).  Past one wave clusters wait for their slowest CTA (64 requests
+  // of up to 24k keys: 576 us against 477).  Tile kernel
+  // (one CTA per SM): split only while CTAs are fewer than SMs, into stretches of 512
+  // keys or more.
   const bool alike = B == 1 || span < max_kv;
   const int64_t wave = p.tiles ? 148 : 148 * 2;
   const int64_t goal = p.tiles || alike ? wave : wave * (B < 8 ? (B > 0 ? B : 1) : 8);
-  const int64_t least = p.tiles ? 512 / kTileKeys : (rows <= 16 ? 1024 : 512) / kUnit;
+  const int64_t least = 512 / unit;
   int64_t splits = ctas >= goal ? 1 : goal / (ctas > 0 ? ctas : 1);  // (one CTA more than a wave would be two waves)
   if (splits > units / least) splits = units / least;
+  if (!p.tiles && units >= 512 / kUnit && ctas > 0)
+    splits = std::max(splits, std::min(wave / ctas, units / (128 / kUnit)));
+  if (!p.tiles && ctas > 0 && units >= 256 / kUnit) {
+    const int64_t f = std::min({wave * 7 / 8 / ctas, units / (64 / kUnit), int64_t{kClusterMax}});
+    if (f >= splits || (f == kClusterMax && units <= f * (rows <= 16 ? 640 : 256) / kUnit))
+      splits = f, p.cluster = f > 1;
+  }
   if (splits > kJoinMax) splits = kJoinMax;
   if (splits < 1) splits = 1;
   p.split_units = (units + splits - 1) / splits;
   p.splits = (units + p.split_units - 1) / p.split_units;
-  if (p.splits > 1) {
+  if (p.splits <= 1) p.cluster = false;
+  if (p.splits > 1 && !p.cluster) {
     p.part_o_bytes = round_up(T * Hq * p.splits * D * 4, 256);
     p.part_ml_bytes = round_up(T * Hq * p.splits * 8, 256);
   }
@@ -628,7 +723,7 @@ cudaError_t launch_paged_join(const PagedArgs& a, int D, bool bf16, cudaStream_t
 cudaError_t launch_attention_paged(const PagedArgs& a, int D, bool bf16, bool tiles, cudaStream_t s) {
   if (tiles && a.n_pages > 0) return launch_paged_tiles(a, D, bf16, s);
   PagedArgs r = a;
-  if (a.n_pages == 0) r.splits = 1;  // no keys at all
+  if (a.n_pages == 0) r.splits = 1, r.cluster = 0;  // no keys at all
   if (D == 64) return bf16 ? launch_rows<64, true>(r, s) : launch_rows<64, false>(r, s);
   return bf16 ? launch_rows<128, true>(r, s) : launch_rows<128, false>(r, s);
 }

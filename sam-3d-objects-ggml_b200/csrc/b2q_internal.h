@@ -342,6 +342,7 @@ struct PagedArgs {
   int64_t ldo;
   // Keys split into stretches of split_units units, joined afterwards (splits 1: not split).
   int splits;
+  int cluster;            // 1: the CTAs of a run's stretches are a cluster and join by themselves
   int64_t split_units;
   float* part_o;          // [T][Hq][splits][D]
   float2* part_ml;        // [T][Hq][splits] (max, sum)
@@ -349,6 +350,7 @@ struct PagedArgs {
 constexpr int kTileRows = 128, kTileKeys = 64;  // of the tensor-memory kernel
 struct PagedPlan {
   bool tiles = false;  // the tile kernel (b2q_attention_paged_tile.cu), else the rows kernel
+  bool cluster = false; // the stretches of a run are a thread block cluster
   int64_t splits = 1, split_units = 0, part_o_bytes = 0, part_ml_bytes = 0;
 };
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,

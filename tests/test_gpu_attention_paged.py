@@ -278,3 +278,46 @@ def test_capture_and_new_lengths(dev):
         g.replay()
         ref, mag = reference(q, kc, vc, table, L, cu, Hq)
         check(out, ref, mag, dt)
+
+
+# Lengths at which a call has two to eight stretches that join in one launch, one more or less, and requests that
+# fill none, one or part of them; 16 rows of a kv head and 17 to 32; a share of rows that does not divide evenly.
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16")])
+@pytest.mark.parametrize("Hq,Hkv,news", [(2, 2, [1, 1, 1, 0]), (16, 1, [1, 1, 1, 1]), (21, 3, [3, 1, 4, 0]), (64, 2, [1, 1, 1, 1])])
+@pytest.mark.parametrize("top", [207, 208, 256, 300, 471, 512, 1100, 2047, 5100])
+def test_few_stretches(dev, D, dt, Hq, Hkv, news, top):
+    assert b2q.attention_paged_workspace_bytes(4, sum(news), max(news), 1100, Hq, Hkv, D) == 0
+    run(dev, [top, 4, top // 2 + 1, 0 if news[3] == 0 else 1], news, Hq, Hkv, D, dt, 16, seed=top, stale=float("nan"))
+    run(dev, [top, 40, 1, 7], news, Hq, Hkv, D, dt, 32, seed=top + 1, causal=False)
+
+
+@pytest.mark.parametrize("D,dt", [(64, "bf16"), (128, "f16")])
+@pytest.mark.parametrize("window,sinks", [(300, 0), (700, 4), (700, 40)])
+def test_few_stretches_window(dev, D, dt, window, sinks):
+    run(dev, [3000, 650, 20], [5, 1, 3], 12, 2, D, dt, 64, seed=window, window=window, sinks=sinks, stale=float("inf"))
+
+
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16")])
+def test_few_stretches_without_pages(dev, D, dt):
+    """Pages of whole stretches are missing; a request whose pages are all missing gives rows of 0."""
+    q, kc, vc, table, L, cu = make(dev, [1500, 900, 600], [2, 1, 1], 8, 2, D, DT[dt], 16, seed=5)
+    table[0, 10:60] = -1
+    table[1, :] = -1
+    table[2, 30:] = 1 << 30
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, 2, 1500, 8)
+    ref, mag = reference(q, kc, vc, table, L, cu, 8)
+    assert not bool(o[2].any())
+    check(o, ref, mag, DT[dt])
+
+
+def test_few_stretches_nonfinite_keys(dev):
+    """An infinity among the values reaches the rows that see it and no other; NaN scores give NaN rows."""
+    q, kc, vc, table, L, cu = make(dev, [1200, 800], [3, 1], 8, 2, 64, torch.float16, 32, seed=6)
+    vc[table[0, 1199 // 32].long(), :, 1199 % 32, 3] = math.inf   # seen by the last token only
+    vc[table[1, 5].long(), 0, 2, 7] = -math.inf
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, 3, 1200, 8)
+    ref, mag = reference(q, kc, vc, table, L, cu, 8)
+    check(o, ref, mag, torch.float16)
+    q[3] = math.nan
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, 3, 1200, 8)
+    assert bool(torch.isnan(o[3]).all()) and bool(torch.isfinite(o[:2]).all())

@@ -22,7 +22,9 @@
 // row tiles.  A warp's unit is 16 rows x 256 values, fetched with cp.async into
 // the warp's own ring: no barrier inside a tile.  The warps of a tile share out
 // its units (WK of them; the other factor, WR, is row tiles side by
-// side) and are summed at its end in a fixed order.
+// side) and are summed at its end in a fixed order.  Where rows are long and
+// few, the CTAs of a cluster share out K, so that each splits its part of the
+// activations only, and add up their sums out of each other's shared memory.
 //   up to 4 tokens (NT 1 or 2 products a block, two tokens each): a token's
 //     columns are (p0, p1, -, p2), so a lane's pair of sums is 256 p0 + p1, or p2:
 //     one number to scale
@@ -40,6 +42,8 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 namespace b2q {
 
@@ -67,6 +71,7 @@ struct MvShape {
   static constexpr int ACC = TILES * 16 * TOKENS * 4;
   static constexpr int X = kMvSmem - RING - SCALES - RED - ACC;  // a chunk's activations
 };
+constexpr int kMvRanks = 8;              // CTAs of a cluster, at most
 constexpr int kMvBatch = 4;              // blocks of activations that a group of lanes loads at a time
 constexpr int kMvMagic = 0x4B400000;     // bits of 1.5 * 2^23
 
@@ -75,7 +80,8 @@ struct MvPlan {
   int units;           // of 256 values along K
   int chunk_units;     // of one chunk
   int chunks;
-  int supers;          // super-tiles of WR * 16 rows; at least one per CTA
+  int supers;          // super-tiles of WR * 16 rows; at least one per cluster
+  int rank_shift;      // log2 of the CTAs of a cluster
   int pitch;           // bytes of one digit row in shared memory
   int vec;             // x rows can be read four values at a time
 };
@@ -133,7 +139,17 @@ __device__ __forceinline__ void mv_cp16(uint32_t dst, const void* src, bool real
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-template <bool Q4K, int NT, int XT>
+// A float of the cluster's CTA `rank`, at this CTA's address of it.
+__device__ __forceinline__ float mv_peer(uint32_t addr, int rank) {
+  uint32_t there;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+  return v;
+}
+
+// CLUSTER: the CTAs of a cluster share out K and add up their sums.
+template <bool Q4K, int NT, int XT, bool CLUSTER>
 __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const MulVecArgs a, const MvPlan p) {
   using S = MvShape<NT>;
   constexpr bool WIDE = S::WIDE;
@@ -155,16 +171,22 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
   float* sums = tab + a.M * nb_pitch;
   constexpr int TC = S::COLS;
 
-  const int own = (p.supers - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  const int group_n = p.chunks == 1 ? own : S::TILES / WR;  // super-tiles whose sums are kept at once
+  const int rs = CLUSTER ? p.rank_shift : 0, ranks = 1 << rs;
+  const int rank = static_cast<int>(blockIdx.x) & (ranks - 1), cid = static_cast<int>(blockIdx.x) >> rs;
+  const int clusters = static_cast<int>(gridDim.x) >> rs;
+  const int u_lo = rank * p.units >> rs, u_hi = (rank + 1) * p.units >> rs;  // this CTA's units
+
+  const int own = (p.supers - cid + clusters - 1) / clusters;
+  const int group_n = p.chunks == 1 && !CLUSTER ? own : S::TILES / WR;  // super-tiles whose sums are kept at once
+  const int outs = 16 * WR * a.M;                                           // of a super-tile
 
   // The warp's sequence of units: for each group, each chunk, each super-tile, its units of the chunk.
-  int q_g0 = 0, q_i = 0, q_chunk = 0, q_u = wk, q_end = min(p.units, p.chunk_units);
+  int q_g0 = 0, q_i = 0, q_chunk = 0, q_u = u_lo + wk, q_end = min(u_hi, u_lo + p.chunk_units);
   const uint8_t* q_src = nullptr;  // the warp's tile
   int64_t q_n0 = 0;
   uint32_t src_off[5];             // this lane's 16-byte pieces of a unit
   auto enter_tile = [&] {
-    q_n0 = ((blockIdx.x + static_cast<int64_t>(q_i) * gridDim.x) * WR + wr) * 16;
+    q_n0 = ((cid + static_cast<int64_t>(q_i) * clusters) * WR + wr) * 16;
     q_n0 = min(q_n0, (a.N - 1) / 16 * 16);  // (a tile past the end repeats the last one, unused)
     q_src = a.w + q_n0 * a.row_bytes;
     const int last = static_cast<int>(min(a.N - 1 - q_n0, int64_t{15}));
@@ -185,9 +207,9 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
           q_g0 += group_n;
         }
         q_i = q_g0;
-        q_end = min(p.units, (q_chunk + 1) * p.chunk_units);
+        q_end = min(u_hi, u_lo + (q_chunk + 1) * p.chunk_units);
       }
-      q_u = q_chunk * p.chunk_units + wk;
+      q_u = u_lo + q_chunk * p.chunk_units + wk;
       enter_tile();
     }
   };
@@ -234,7 +256,7 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
 
   for (int g0 = 0; g0 < own; g0 += group_n) {
     for (int chunk = 0; chunk < p.chunks; ++chunk) {
-      const int cu0 = chunk * p.chunk_units, cu1 = min(p.units, cu0 + p.chunk_units);
+      const int cu0 = u_lo + chunk * p.chunk_units, cu1 = min(u_hi, cu0 + p.chunk_units);
       if (p.chunks > 1 || g0 == 0) {
         // ---- the chunk's activations: eight lanes per (token, block), four values each
         const int nb = (cu1 - cu0) * (kMvUnitK / 32);
@@ -336,12 +358,11 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
       for (int i = g0; i < min(own, g0 + group_n); ++i) {
         // A thread finishes outputs (row, token) threadIdx.x, + THREADS, .. of the super-tile, rows in a row;
         // what the first one is added to is on its way while the units run.
-        const int64_t n_super = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * WR * 16;
-        const int outs = 16 * WR * a.M;
+        const int64_t n_super = (cid + static_cast<int64_t>(i) * clusters) * WR * 16;
         const int m_first = static_cast<int>(threadIdx.x) / (16 * WR);
         const int64_t n_first = n_super + (static_cast<int>(threadIdx.x) - m_first * 16 * WR);
         float bias_first = 0.0f, gate_first = 1.0f, resid_first = 0.0f;
-        if (static_cast<int>(threadIdx.x) < outs && n_first < a.N && chunk == p.chunks - 1) {
+        if (static_cast<int>(threadIdx.x) < outs && n_first < a.N && chunk == p.chunks - 1 && !CLUSTER) {
           if (a.bias) bias_first = __ldg(a.bias + n_first);
           if (a.gate) gate_first = __ldg(a.gate + n_first);
           if (a.resid) resid_first = a.resid[m_first * a.ldr + n_first];
@@ -492,11 +513,11 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
             }
           }
           if (n >= a.N) continue;
-          if (p.chunks > 1) {
+          if (CLUSTER || p.chunks > 1) {
             float* slot = acc_s + (i - g0) * outs + x;
             if (chunk > 0) v += *slot;
             *slot = v;
-            if (chunk < p.chunks - 1) continue;
+            if (CLUSTER || chunk < p.chunks - 1) continue;
           }
           const bool first = x == static_cast<int>(threadIdx.x);
           if (a.bias) v = __fadd_rn(v, first ? bias_first : __ldg(a.bias + n));
@@ -509,6 +530,29 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
         buf ^= 1;
       }
     }
+    if constexpr (CLUSTER) {  // the sums of the cluster, in the order of its CTAs, which share out the outputs
+      asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+      const int n_here = (min(own, g0 + group_n) - g0) * outs;
+      for (int x = rank * S::THREADS + threadIdx.x; x < n_here; x += ranks * S::THREADS) {
+        const int i = x / outs, y = x - i * outs, m = y / (16 * WR);
+        const int64_t n = (cid + static_cast<int64_t>(g0 + i) * clusters) * WR * 16 + (y - m * 16 * WR);
+        if (n >= a.N) continue;
+        const float bias = a.bias ? __ldg(a.bias + n) : 0.0f, gate = a.gate ? __ldg(a.gate + n) : 1.0f;
+        const float resid = a.resid ? a.resid[m * a.ldr + n] : 0.0f;
+        float v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kMvRanks; ++r)
+          if (r < ranks) v += mv_peer(smem_u32(acc_s + x), r);
+        if (a.bias) v = __fadd_rn(v, bias);
+        if (a.resid) {
+          if (a.gate) v = __fmul_rn(v, gate);
+          v = __fadd_rn(resid, v);
+        }
+        a.y[m * a.ldy + n] = v;
+      }
+      // none may go on while others read from it
+      asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -516,47 +560,91 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
 template <bool Q4K, int NT, int XT>
 cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
   using S = MvShape<NT>;
-  auto kern = mul_vec_kernel<Q4K, NT, XT>;
+  auto kern = mul_vec_kernel<Q4K, NT, XT, false>;
+  auto kern_cl = mul_vec_kernel<Q4K, NT, XT, true>;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = kMvSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  // Clusters of 1, 2, 4 and 8 CTAs that the device runs at a time (B200: 148, 74, 33, 15).
+  static int fit[64][4] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (fit[dev][0] == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern_cl, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem);
+    if (e != cudaSuccess) return e;
+    for (int c = 3; c >= 0; --c) {
+      int n = num_sms;
+      cfg.gridDim = dim3(num_sms << c);
+      cluster.val.clusterDim.x = 1 << c;
+      if (c > 0 && cudaOccupancyMaxActiveClusters(&n, kern_cl, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      fit[dev][c] = n;
+    }
+  }
+
   MvPlan p{};
   p.units = static_cast<int>((a.K + kMvUnitK - 1) / kMvUnitK);
   // Shared memory per unit: the digits, and per block s and the sum.
   const int per_unit = a.M * (3 * kMvUnitK + (Q4K ? 64 : 32));
   const int most = (S::X - a.M * (3 * 64 + 32)) / per_unit;
-  p.chunks = (p.units + most - 1) / most;
-  p.chunk_units = (p.units + p.chunks - 1) / p.chunks;
-  p.chunks = (p.units + p.chunk_units - 1) / p.chunk_units;
-  p.pitch = p.chunk_units * kMvUnitK + 64;
-  const int64_t tiles = (a.N + 15) / 16;
-  // WK, the warps that share a tile's units: what finishes first when a tile's
-  // end costs as much as 0.75 units and the super-tiles go round the SMs; the
-  // larger of equals, which spreads few rows over more SMs.  Measured, WK 1, 2,
-  // 4, 8: 49152 x 8192 Q4_K, one token 52.6, 54.3, 56.8, 57.1 us; 8192 x 4096 Q4_0,
-  // four tokens 38.5, 23.4, 16.1, 17.1; 6144 x 1024 Q4_0, one token 9.9, 7.1, 5.6, 4.8.
-  int sh = 0;
-  double best = 0.0;
-  for (int x = 0; x <= 3; ++x) {
-    const int64_t super = (tiles + (S::WARPS >> x) - 1) / (S::WARPS >> x);
-    const double cost = static_cast<double>((super + num_sms - 1) / num_sms) *
-                        ((p.units + (1 << x) - 1) / (1 << x) + 0.75 * p.chunks);
-    if (x == 0 || cost <= best) best = cost, sh = x;
+  // The CTAs of a cluster (2^c) that share out K, and the warps of a CTA that share a
+  // tile's units (2^x = WK): what finishes first when the super-tiles go round the
+  // clusters that run at a time; the larger of equals, which spreads few rows over more
+  // SMs.  In units' time, fitted to 41 sizes: a tile's end costs 0.75 between values of
+  // WK and 1.5 between sizes of clusters, a round of activation blocks 0.2, a cluster's
+  // first join 0.7 and a later one 1.  One CTA, and clusters of 2, 4 and 8 with their best WK, us:
+  //   6144 x 1024 Q4_0, 1 token 5.0, 7.0, 7.1, -; 8192 x 4096 Q4_0, 4 tokens 14.8, 14.7, 15.0, 20.9;
+  //   49152 x 8192 Q4_K, 1 token 54, 61, 105, 148; 1500 x 4096 Q4_0, 8 tokens 14.6, 9.5, 8.4, 7.8;
+  //   200 x 16384 Q4_0, 1 token 19.1, 12.6, 9.3, 7.3, 8 tokens 50, -, -, 9.3.
+  // WK 1, 2, 4, 8 of one CTA: 49152 x 8192 Q4_K, one token 52.6, 54.3, 56.8, 57.1 us; 8192 x 4096
+  // Q4_0, four tokens 38.5, 23.4, 16.1, 17.1; 6144 x 1024 Q4_0, one token 9.9, 7.1, 5.6, 4.8.
+  const int tiles = static_cast<int>((a.N + 15) / 16);
+  float best = 0.0f;
+  for (int c = 0; c <= 3; ++c) {
+    const int per = (p.units + (1 << c) - 1) >> c, chunks = (per + most - 1) / most;
+    // (a rank without units, or with fewer chunks than another, is not provided for)
+    if (c > 0 && (fit[dev][c] == 0 || p.units < 1 << c || chunks > 1)) continue;
+    const float stage = 0.2f * static_cast<float>((static_cast<int64_t>(per) * 8 * a.M + S::THREADS / 8 - 1) / (S::THREADS / 8));
+    int shift = 0, rounds = 0;
+    float run = 0.0f;
+    for (int x = 0; x <= 3; ++x) {
+      const int wr = S::WARPS >> x, turns = ((tiles + wr - 1) / wr + fit[dev][c] - 1) / fit[dev][c];
+      const float r = static_cast<float>(turns) * (((per + (1 << x) - 1) >> x) + 0.75f * chunks);
+      if (x == 0 || r <= run) run = r, shift = x, rounds = turns;
+    }
+    const int keep = S::TILES / (S::WARPS >> shift);
+    const float join = c == 0 ? 0.0f : static_cast<float>((rounds + keep - 1) / keep) - 0.3f;
+    const float cost = run + 0.75f * rounds * chunks + stage + join;
+    if (best == 0.0f || cost <= best) {
+      best = cost;
+      p.wk_shift = shift;
+      p.rank_shift = c;
+      p.chunk_units = (per + chunks - 1) / chunks;
+      p.chunks = (per + p.chunk_units - 1) / p.chunk_units;
+    }
   }
-  p.wk_shift = sh;
-  const int wr = S::WARPS >> sh;
-  p.supers = static_cast<int>((tiles + wr - 1) / wr);
+  const int wr = S::WARPS >> p.wk_shift;
+  p.supers = (tiles + wr - 1) / wr;
+  p.pitch = p.chunk_units * kMvUnitK + 64;
   const uintptr_t xa = reinterpret_cast<uintptr_t>(a.x);
   p.vec = XT == kXF32 ? (xa % 16 == 0 && a.ldx % 4 == 0) : (xa % 8 == 0 && a.ldx % 4 == 0);
-  const int smem = kMvSmem;
-  static bool attr_set[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    attr_set[dev] = true;
+  const int clusters = std::min(p.supers, fit[dev][p.rank_shift]);
+  if (p.rank_shift == 0) {
+    kern<<<static_cast<unsigned>(clusters), S::THREADS, kMvSmem, s>>>(a, p);
+    return cudaGetLastError();
   }
-  const int grid = p.supers < num_sms ? p.supers : num_sms;
-  kern<<<static_cast<unsigned>(grid), S::THREADS, smem, s>>>(a, p);
-  return cudaGetLastError();
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters << p.rank_shift));
+  cluster.val.clusterDim.x = 1u << p.rank_shift;
+  return cudaLaunchKernelEx(&cfg, kern_cl, a, p);
 }
 
 }  // namespace

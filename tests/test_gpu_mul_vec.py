@@ -158,3 +158,40 @@ def test_repeats_bit_for_bit_and_empty(dev):
     for _ in range(3):
         assert torch.equal(b2q.mul_vec(b2q.TYPE_Q4_K, packed, 3000, 2048, x), y)
     assert b2q.mul_vec(b2q.TYPE_Q4_K, packed, 3000, 2048, x[:0]).shape == (0, 3000)
+
+
+@pytest.mark.parametrize("wtype", [b2q.TYPE_Q4_0, b2q.TYPE_Q4_K])
+@pytest.mark.parametrize("n,k,m,xt", [
+    (200, 4096, 1, "f16"), (41, 2048, 8, "bf16"), (1500, 4352, 4, "f32"), (1, 16384, 3, "f32"), (6000, 4096, 8, "f32"),
+    (3001, 8448, 6, "bf16"), (1000, 16128, 2, "f32"), (2500, 11264, 5, "f16"), (12001, 4096, 7, "f32"),
+])
+def test_long_rows_shared_out(dev, wtype, n, k, m, xt):
+    """Rows long beside their number: several CTAs share them out.  Bias, gate and the residual in place are added
+    once, the result repeats bit for bit, and a captured call on another stream gives it too."""
+    _, packed, w, mag = make(dev, wtype, n, k, n + k + 1)
+    g = torch.Generator(device=dev).manual_seed(m)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    x, bias, gate, base = rand(m, k).to(DT[xt]), rand(n), rand(n), rand(m, n + 5)
+    ref, tol = x.double() @ w.t(), bound(x, mag, k)
+    r1 = ref + bias.double()
+    r2 = base[:, :n].double() + gate.double() * r1
+    lim = tol * gate.double().abs() + 2.0 ** -22 * ((gate.double() * r1).abs() + r2.abs())
+    outs = []
+    for _ in range(3):
+        y = base.clone()
+        b2q.mul_vec(wtype, packed, n, k, x, bias=bias, gate=gate, resid=y[:, :n], out=y[:, :n])
+        outs.append(y)
+    assert bool(((outs[0][:, :n].double() - r2).abs() <= lim).all())
+    assert torch.equal(outs[0][:, n:], base[:, n:])
+    assert torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])
+    plain = b2q.mul_vec(wtype, packed, n, k, x)
+    assert bool(((plain.double() - ref).abs() <= tol).all())
+    side = torch.cuda.Stream()
+    y = torch.zeros(m, n, device=dev)
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        b2q.mul_vec(wtype, packed, n, k, x, out=y)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, plain)

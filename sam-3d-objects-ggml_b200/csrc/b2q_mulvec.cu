@@ -33,10 +33,10 @@
 //     accumulator that starts at the bits of 1.5 * 2^23
 // Three or four products of the first kind instead, for 5 to 8 tokens, of a
 // 49152 x 8192 weight: 157 us against 125 (8 tokens, Q4_K), 111 against 111 (6).
-// Measured: that weight in Q4_K, one token: 51 us, 4450 GB/s, bound by the issue
-// of 2.7 lane instructions a value; 8192 x 4096 Q4_0, 4 tokens: 14.4 us, of which
-// the digits of the activations are a third; 6144 x 1024 Q4_0, one token: 4.7 us,
-// a launch and one CTA's chain (the weight's bytes are 0.6 us).
+// Measured: that weight in Q4_K, one token: 50 us, 4500 GB/s, bound by the issue
+// of 2.7 lane instructions a value; 8192 x 4096 Q4_0, 4 tokens: 11.8 us, digits,
+// units and a launch in equal parts; 6144 x 1024 Q4_0, one token: 4.6 us, a launch
+// and one CTA's chain (the weight's bytes are 0.6 us).
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
 
@@ -76,7 +76,8 @@ constexpr int kMvBatch = 4;              // blocks of activations that a group o
 constexpr int kMvMagic = 0x4B400000;     // bits of 1.5 * 2^23
 
 struct MvPlan {
-  int wk_shift;        // log2(WK)
+  int wk, wr;          // warps that share a tile's units, and tiles side by side: WK * WR warps work
+  int wk_inv;          // 2^16 / WK rounded up
   int units;           // of 256 values along K
   int chunk_units;     // of one chunk
   int chunks;
@@ -156,8 +157,8 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
   extern __shared__ __align__(128) uint8_t mv_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int WK = 1 << p.wk_shift, WR = S::WARPS >> p.wk_shift;
-  const int wk = warp & (WK - 1), wr = warp >> p.wk_shift;
+  const int WK = p.wk, WR = p.wr;
+  const int wr = warp * p.wk_inv >> 16, wk = warp - wr * WK;  // warp / WK
   const int row0 = 2 * g, row1 = 2 * g + 1;  // of a tile
   uint8_t* ring = mv_smem + warp * S::STAGES * kMvUnitBytes;
   const uint32_t ring_a = smem_u32(ring);
@@ -180,6 +181,8 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
   const int group_n = p.chunks == 1 && !CLUSTER ? own : S::TILES / WR;  // super-tiles whose sums are kept at once
   const int outs = 16 * WR * a.M;                                           // of a super-tile
 
+  const int mine_n = wr < WR ? own : 0;  // super-tiles that this warp works on
+
   // The warp's sequence of units: for each group, each chunk, each super-tile, its units of the chunk.
   int q_g0 = 0, q_i = 0, q_chunk = 0, q_u = u_lo + wk, q_end = min(u_hi, u_lo + p.chunk_units);
   const uint8_t* q_src = nullptr;  // the warp's tile
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
     }
   };
   auto settle = [&] {  // to the next unit that exists
-    while (q_u >= q_end && q_g0 < own) {
+    while (q_u >= q_end && q_g0 < mine_n) {
       if (++q_i >= min(own, q_g0 + group_n)) {
         if (++q_chunk == p.chunks) {
           q_chunk = 0;
@@ -214,7 +217,7 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
     }
   };
   auto load = [&](int stage) {
-    if (q_g0 < own) {
+    if (q_g0 < mine_n) {
       const uint32_t dst = ring_a + stage * kMvUnitBytes;
       if constexpr (Q4K) {
         const uint8_t* src = q_src + static_cast<int64_t>(q_u) * kQ4KBytes;
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
         }
         float macc[Q4K ? S::TOKENS : 1] = {};  // Q4_K: minima, of row lane % 16, half of the blocks
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // WIDE: (row0, tokens 2c, 2c + 1), (row1, ..); else (row0, row1) per product
-        for (int u = cu0 + wk; u < cu1; u += WK) {
+        for (int u = wr < WR ? cu0 + wk : cu1; u < cu1; u += WK) {
           asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
           __syncwarp();
           load(fill);
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(MvShape<NT>::THREADS, 1) mul_vec_kernel(const 
         for (int x = threadIdx.x; x < outs; x += S::THREADS) {
           const int m = x / (16 * WR), r = x - m * 16 * WR;
           const int64_t n = n_super + r;
-          const float* part = red + ((buf * S::WARPS + ((r >> 4) << p.wk_shift)) * 16 + (r & 15)) * TC;
+          const float* part = red + ((buf * S::WARPS + (r >> 4) * WK) * 16 + (r & 15)) * TC;
           float v = 0.0f;
           for (int w = 0; w < WK; ++w) {
             if constexpr (WIDE) {
@@ -596,44 +599,47 @@ cudaError_t launch_mv(const MulVecArgs& a, int num_sms, cudaStream_t s) {
   // Shared memory per unit: the digits, and per block s and the sum.
   const int per_unit = a.M * (3 * kMvUnitK + (Q4K ? 64 : 32));
   const int most = (S::X - a.M * (3 * 64 + 32)) / per_unit;
-  // The CTAs of a cluster (2^c) that share out K, and the warps of a CTA that share a
-  // tile's units (2^x = WK): what finishes first when the super-tiles go round the
-  // clusters that run at a time; the larger of equals, which spreads few rows over more
-  // SMs.  In units' time, fitted to 41 sizes: a tile's end costs 0.75 between values of
-  // WK and 1.5 between sizes of clusters, a round of activation blocks 0.2, a cluster's
-  // first join 0.7 and a later one 1.  One CTA, and clusters of 2, 4 and 8 with their best WK, us:
-  //   6144 x 1024 Q4_0, 1 token 5.0, 7.0, 7.1, -; 8192 x 4096 Q4_0, 4 tokens 14.8, 14.7, 15.0, 20.9;
-  //   49152 x 8192 Q4_K, 1 token 54, 61, 105, 148; 1500 x 4096 Q4_0, 8 tokens 14.6, 9.5, 8.4, 7.8;
-  //   200 x 16384 Q4_0, 1 token 19.1, 12.6, 9.3, 7.3, 8 tokens 50, -, -, 9.3.
-  // WK 1, 2, 4, 8 of one CTA: 49152 x 8192 Q4_K, one token 52.6, 54.3, 56.8, 57.1 us; 8192 x 4096
-  // Q4_0, four tokens 38.5, 23.4, 16.1, 17.1; 6144 x 1024 Q4_0, one token 9.9, 7.1, 5.6, 4.8.
+  // The CTAs of a cluster (2^c) that share out K, the warps of a CTA that share a tile's
+  // units (WK) and the tiles side by side (WR): what finishes first when the super-tiles
+  // go round the clusters that run at a time; the larger of equals, which spreads few
+  // rows over more SMs.  In units' time with all warps at work (0.6 of it and less work,
+  // with fewer: latency), fitted to 39 sizes x 4 clusters x 8 WK, of which it takes 0.7%
+  // more than the best: a tile's end costs 0.5, a round of activation blocks 0.15, a
+  // cluster's first join 0.5 and a later one 0.7.  One CTA, and clusters of 2, 4 and 8 with their best WK, us:
+  //   6144 x 1024 Q4_0, 1 token 4.6, 5.8, 6.0, -; 8192 x 4096 Q4_0, 4 tokens 12.3, 12.0, 12.2, 16.3;
+  //   49152 x 8192 Q4_K, 1 token 50, 53, 63, 86; 200 x 16384 Q4_0, 8 tokens 44, -, -, 8.5.
+  // WK 1, 2, 4, 8 of one CTA: 49152 x 8192 Q4_K, 1 token 50.9, 50.7, 55.1, 54.1 us; 8192 x 4096
+  // Q4_0, 4 tokens 15.5, 13.3, 12.4, 13.3; 6144 x 1024 Q4_0, 1 token 5.4, 4.8, 4.6, 4.6.
   const int tiles = static_cast<int>((a.N + 15) / 16);
+  const auto over = [](int x, int y) { return (x + y - 1) / y; };
   float best = 0.0f;
   for (int c = 0; c <= 3; ++c) {
-    const int per = (p.units + (1 << c) - 1) >> c, chunks = (per + most - 1) / most;
+    const int per = (p.units + (1 << c) - 1) >> c, chunks = over(per, most);
+    // Activations of one round are not worth sharing out (nor the host's time to weigh it).
+    if (c > 0 && p.units * 8 * a.M <= S::THREADS / 8) break;
     // (a rank without units, or with fewer chunks than another, is not provided for)
     if (c > 0 && (fit[dev][c] == 0 || p.units < 1 << c || chunks > 1)) continue;
-    const float stage = 0.2f * static_cast<float>((static_cast<int64_t>(per) * 8 * a.M + S::THREADS / 8 - 1) / (S::THREADS / 8));
-    int shift = 0, rounds = 0;
-    float run = 0.0f;
-    for (int x = 0; x <= 3; ++x) {
-      const int wr = S::WARPS >> x, turns = ((tiles + wr - 1) / wr + fit[dev][c] - 1) / fit[dev][c];
-      const float r = static_cast<float>(turns) * (((per + (1 << x) - 1) >> x) + 0.75f * chunks);
-      if (x == 0 || r <= run) run = r, shift = x, rounds = turns;
-    }
-    const int keep = S::TILES / (S::WARPS >> shift);
-    const float join = c == 0 ? 0.0f : static_cast<float>((rounds + keep - 1) / keep) - 0.3f;
-    const float cost = run + 0.75f * rounds * chunks + stage + join;
-    if (best == 0.0f || cost <= best) {
-      best = cost;
-      p.wk_shift = shift;
-      p.rank_shift = c;
-      p.chunk_units = (per + chunks - 1) / chunks;
-      p.chunks = (per + p.chunk_units - 1) / p.chunk_units;
+    const float stage = 0.15f * static_cast<float>((static_cast<int64_t>(per) * 8 * a.M + S::THREADS / 8 - 1) / (S::THREADS / 8));
+    for (const int wk : {1, 2, 3, 4, 6, 8, 12}) {
+      if (wk > S::WARPS / 2) break;
+      // as few tiles side by side as the same number of rounds allows: they reach more SMs
+      const int rounds = over(over(tiles, S::WARPS / wk), fit[dev][c]);
+      const int wr = over(tiles, rounds * fit[dev][c]);
+      const float busy = std::max(0.6f, static_cast<float>(wk * wr) / S::WARPS);
+      const float join = c == 0 ? 0.0f : 0.7f * over(rounds, S::TILES / wr) - 0.2f;
+      const float cost = rounds * (busy * over(per, wk) + 0.5f * chunks) + stage + join;
+      if (best == 0.0f || cost <= best) {
+        best = cost;
+        p.wk = wk;
+        p.wr = wr;
+        p.rank_shift = c;
+        p.chunk_units = over(per, chunks);
+        p.chunks = over(per, p.chunk_units);
+      }
     }
   }
-  const int wr = S::WARPS >> p.wk_shift;
-  p.supers = (tiles + wr - 1) / wr;
+  p.wk_inv = (65536 + p.wk - 1) / p.wk;
+  p.supers = over(tiles, p.wr);
   p.pitch = p.chunk_units * kMvUnitK + 64;
   const uintptr_t xa = reinterpret_cast<uintptr_t>(a.x);
   p.vec = XT == kXF32 ? (xa % 16 == 0 && a.ldx % 4 == 0) : (xa % 8 == 0 && a.ldx % 4 == 0);

@@ -10,14 +10,15 @@
 // Bound by its bytes: 4 read and 2 written per value of a row, each once.  A
 // CTA takes up to kRopeTokens tokens (one, where there are few): its threads
 // first compute the tokens' cosines and sines into shared memory, one pair
-// each, which all the heads then share.  A lane takes 8 neighbouring values, so
-// a head is D / 8 lanes, and the RMS sum and the partner of a pair are shuffles
-// among them; a thread's next rows are loaded while it works on these.  q and k
-// rows and v rows are two loops, and the kinds of rotation and norm are template
-// arguments: with one loop of 4-value lanes the rows cost 136 instructions a
-// warp, and 32800 tokens of 48 heads of 64 took 200 us where this takes 101
-// (5990 GB/s).  24 tokens of 40 heads of 128: 3.7 us, a launch and one round of
-// loads and stores.
+// each, which all the heads then share.  A lane takes 8 values that hold whole pairs (8 neighbours, or for pairs
+// (i, i + R) four neighbours and their four partners), so a head is D / 8 lanes
+// and the RMS sum is shuffles among them; a thread's next rows are loaded while it
+// works on these.  q and k rows and v rows are two loops, and the kinds of rotation
+// and norm are template arguments: with one loop of 4-value lanes the rows cost 136
+// instructions a warp, and 32800 tokens of 48 heads of 64 took 200 us where this
+// takes 101 (5970 GB/s).  With pairs (i, i + R) and 40 heads of 128: 160 us, 6290
+// GB/s, and 207 when the partners came by shuffles.  24 tokens of 40 heads of 128:
+// 3.2 us, a launch and one round of loads and stores.
 //
 // The angle is formed in double and reduced to a fraction of a turn before it
 // is rounded to fp32: in fp32 the product of a position of 10^4 and a frequency
@@ -34,13 +35,18 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTokens = 8;  // most tokens of a CTA
 constexpr int kRopeBatch = 2;   // rows of a thread whose loads are under way together
-enum { kInterleaved = 0, kHalves = 1, kHalvesOdd = 2 };  // pairs (2i, 2i + 1); (i, i + R), R % 8 == 0; any R
+enum { kInterleaved = 0, kHalves = 1, kHalvesOdd = 2 };  // pairs (2i, 2i + 1); (i, i + R), R % 4 == 0; any R
 
 struct F8 {
   float v[8];
 };
 __device__ __forceinline__ F8 load8(const float* p) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+// four values and four more
+__device__ __forceinline__ F8 load44(const float* p, const float* q) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(q));
   return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 template <bool BF16>
@@ -92,8 +98,9 @@ struct RowWalk {
   }
 };
 
+// (four CTAs an SM: with registers for fewer the 32800 tokens above take 112 us, for five 109)
 template <int D, bool BF16, bool NORM, int MODE>
-__global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs a, int tokens_per_cta, bool wide) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_cache_kernel(const RopeArgs a, int tokens_per_cta, bool wide) {
   constexpr int LPR = D / 8;               // lanes per row
   constexpr int RPP = kRopeThreads / LPR;  // rows per pass of the CTA
   extern __shared__ __align__(16) float2 rope_cs[];  // [tokens_per_cta][R] (cos, sin)
@@ -129,7 +136,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
   if (lo < min(hi, n_qk)) {
     const int n = min(hi, n_qk) - lo, rows = nt * n;
     RowWalk w(tid / LPR, RPP, n);
-    const unsigned group = (tid & 31) / LPR * LPR;  // first lane of this row's group
+    // A lane's values: four from da and four from db, neighbours but for pairs of halves,
+    // where the second four are the partners of the first (past the pairs, neighbours again).
+    int da = 8 * l, db = 8 * l + 4;
+    if (MODE == kHalves && 4 * l < R) da = 4 * l, db = R + 4 * l;
     for (int r = 0; r < rows; r += kRopeBatch * RPP) {
       F8 x[kRopeBatch];
       int xt[kRopeBatch], xh[kRopeBatch];
@@ -138,7 +148,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
       for (int u = 0; u < kRopeBatch; ++u) {
         xt[u] = w.tl;
         xh[u] = lo + w.h;
-        x[u] = load8(a.qkv + (t0 + min(w.tl, nt - 1)) * a.ldqkv + static_cast<int64_t>(xh[u]) * D + 8 * l);
+        const float* row = a.qkv + (t0 + min(w.tl, nt - 1)) * a.ldqkv + static_cast<int64_t>(xh[u]) * D;
+        x[u] = load44(row + da, row + db);
         w.next();
       }
       if constexpr (NORM) {
@@ -162,7 +173,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
 #pragma unroll
           for (int i = 0; i < 8; ++i) v.v[i] *= scale[u];
           if (gamma) {
-            const F8 g = load8(gamma + g0 + 8 * l);
+            const F8 g = load44(gamma + g0 + da, gamma + g0 + db);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v.v[i] *= g.v[i];
           }
@@ -177,20 +188,18 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
               v.v[2 * i + 1] = v.v[2 * i + 1] * c.x + v.v[2 * i] * c.y;
               v.v[2 * i] = y;
             }
-        } else if constexpr (MODE == kHalves) {  // the eight partners sit in one lane
-          const bool second = 8 * l >= R;
-          const int src = static_cast<int>(group) + (second ? (l - R / 8 + LPR) % LPR : (l + R / 8) % LPR);
-          F8 o;
+        } else if constexpr (MODE == kHalves) {
+          if (4 * l < R) {
+            const float4* c4 = reinterpret_cast<const float4*>(cs + 4 * l);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o.v[i] = __shfl_sync(0xffffffffu, v.v[i], src);
-          if (8 * l < 2 * R) {
-            const float4* c4 = reinterpret_cast<const float4*>(cs + (second ? 8 * l - R : 8 * l));
-            const float sg = second ? 1.0f : -1.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
               const float4 c = c4[i];
-              v.v[2 * i] = v.v[2 * i] * c.x + sg * (o.v[2 * i] * c.y);
-              v.v[2 * i + 1] = v.v[2 * i + 1] * c.z + sg * (o.v[2 * i + 1] * c.w);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float x0 = v.v[2 * i + k], x1 = v.v[4 + 2 * i + k], cc = k ? c.z : c.x, sn = k ? c.w : c.y;
+                v.v[2 * i + k] = x0 * cc - x1 * sn;
+                v.v[4 + 2 * i + k] = x1 * cc + x0 * sn;
+              }
             }
           }
         } else {  // partners across lanes: read them from the row itself
@@ -212,11 +221,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_kernel(const RopeArgs
         }
         if (xt[u] >= nt) continue;
         const uint4 p = pack8<BF16>(v);
+        const auto put = [&](uint16_t* row) {
+          if constexpr (MODE == kHalves) {
+            __stcs(reinterpret_cast<uint2*>(row + da), make_uint2(p.x, p.y));
+            __stcs(reinterpret_cast<uint2*>(row + db), make_uint2(p.z, p.w));
+          } else {
+            store8(row + 8 * l, p, wide);
+          }
+        };
         if (h < a.Hq) {
-          store8(a.q + (t0 + tt) * a.ldq + static_cast<int64_t>(h) * D + 8 * l, p, wide);
+          put(a.q + (t0 + tt) * a.ldq + static_cast<int64_t>(h) * D);
         } else {
           const int64_t at = rope_at[tt];
-          if (at >= 0) store8(a.k_cache + at + (h - a.Hq) * head_step + 8 * l, p, wide);
+          if (at >= 0) put(a.k_cache + at + (h - a.Hq) * head_step);
         }
       }
     }
@@ -267,7 +284,7 @@ cudaError_t launch_rope_cache(const RopeArgs& a, int D, bool bf16, int num_sms, 
   const int smem = tpc * (a.rot > 0 ? a.rot : 1) * 8;
   const auto odd = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
   const bool wide = !odd(a.q) && a.ldq % 8 == 0 && !odd(a.k_cache) && !odd(a.v_cache);
-  const int mode = a.interleaved ? kInterleaved : a.rot % 8 == 0 ? kHalves : kHalvesOdd;
+  const int mode = a.interleaved ? kInterleaved : a.rot % 4 == 0 ? kHalves : kHalvesOdd;
 #define B2Q_ROPE(DD, BF, NO, MO) rope_cache_kernel<DD, BF, NO, MO><<<grid, kRopeThreads, smem, s>>>(a, tpc, wide)
 #define B2Q_ROPE_M(DD, BF, NO)                                        \
   do {                                                                \

@@ -260,3 +260,11 @@ def test_rope_offsets_past_32_bits(dev):
     page, off = slots // ps, slots % ps
     assert torch.equal(kc[page, :, off], x[:, :Hkv]) and torch.equal(vc[page, :, off], x[:, Hkv:])
     assert int((kc[:4] != 0).sum()) == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R", [2, 4, 6, 8, 12, 20, 24, 28, 30, 32])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rope_cache_numbers_of_pairs(dev, D, R, norm):
+    """Halves of every kind of length: multiples of 4 and 8, others, and values past the pairs."""
+    test_rope_cache(dev, 70, 3, 2, D, (R // 2, R - R // 2), False, norm, "bf16" if R % 8 else "f16", 16)

@@ -34,7 +34,7 @@
 // Three or four products of the first kind instead, for 5 to 8 tokens, of a
 // 49152 x 8192 weight: 157 us against 125 (8 tokens, Q4_K), 111 against 111 (6).
 // Measured: that weight in Q4_K, one token: 50 us, 4500 GB/s, bound by the issue
-// of 2.7 lane instructions a value; 8192 x 4096 Q4_0, 4 tokens: 11.8 us, digits,
+// of 2.5 lane instructions a value; 8192 x 4096 Q4_0, 4 tokens: 11.8 us, digits,
 // units and a launch in equal parts; 6144 x 1024 Q4_0, one token: 4.6 us, a launch
 // and one CTA's chain (the weight's bytes are 0.6 us).
 #include "b2q_internal.h"

@@ -656,12 +656,19 @@ cudaError_t launch_rows(const PagedArgs& a, cudaStream_t s) {
 
 // Which kernel, and how the keys are split.  Up to 32 rows a (request, kv head)
 // the rows kernel; above, its CTAs would read the keys from the L2 once more for
-// every 32 rows, and the tile kernel takes 256 rows at a time.
+// every 32 rows, and the tile kernel takes 256 rows at a time.  But that one starts
+// slower and has one CTA an SM: up to 128 rows over at most 1280 keys stay with the rows
+// kernel where one wave holds them (us, rows and tile kernel, 16 heads of 64 and 3
+// requests: 40 to 60 rows over 1000 keys 12.5, 24.0; 100 to 120 rows 17.4, 28.1; 40 to 60
+// rows over 2900 keys 29.1, 26.1; 3 heads of 128 and 10 requests, 24 to 96 rows over up to
+// 2000 keys 25.2, 21.0; 16 requests, 48 to 72 rows in a window of 1000 31.5, 31.0).
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t max_q, int64_t max_kv, int64_t Hq, int64_t Hkv, int64_t D,
                      bool causal, int64_t window, int64_t sinks) {
   PagedPlan p;
   const int64_t G = Hq / Hkv, rows = max_q * G;
-  p.tiles = rows > 32 && G <= kTileRows;
+  const bool brief = rows <= 128 && B * Hkv * ((rows + 31) / 32) <= 148 * 2 &&
+                     std::min(max_kv, causal && window > 0 ? window + 32 + sinks : max_kv) <= 1280;
+  p.tiles = rows > 32 && G <= kTileRows && !brief;
   const int unit = p.tiles ? kTileKeys : kUnit;
   const int64_t tile_rows = p.tiles ? 2 * (kTileRows / G) * G : rows <= 16 ? 16 : 32;
   // Keys that the rows of one CTA can see, in units.

@@ -321,3 +321,16 @@ def test_few_stretches_nonfinite_keys(dev):
     q[3] = math.nan
     o = b2q.attention_paged(q, kc, vc, table, L, cu, 3, 1200, 8)
     assert bool(torch.isnan(o[3]).all()) and bool(torch.isfinite(o[:2]).all())
+
+
+# 33 to 128 rows of a kv head: few keys announced, and the same requests announced as long ones.
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16")])
+@pytest.mark.parametrize("Hq,Hkv,news,lens", [
+    (2, 2, [33, 1, 64, 0], [33, 700, 1000, 5]), (8, 1, [5, 16, 9, 12], [900, 16, 2000, 333]), (20, 2, [12, 1, 4, 7], [2036, 3, 40, 7]),
+    (100, 1, [1, 1, 1, 1], [800, 1, 64, 65]),
+])
+@pytest.mark.parametrize("max_kv", [None, 2500])
+def test_middle_numbers_of_rows(dev, D, dt, Hq, Hkv, news, lens, max_kv):
+    run(dev, lens, news, Hq, Hkv, D, dt, 16, seed=Hq, max_kv=max_kv, stale=float("nan"))
+    run(dev, lens, news, Hq, Hkv, D, dt, 64, seed=Hq + 1, max_kv=max_kv, window=70, sinks=3, stale=float("inf"))
+    run(dev, lens, news, Hq, Hkv, D, dt, 32, seed=Hq + 2, max_kv=max_kv, causal=False)

@@ -13,6 +13,7 @@ every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import re
 import subprocess
@@ -739,6 +740,16 @@ def _raw_stream(stream, t) -> int:
     return _torch()._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def _empty_on(stream, size, dtype, device):
+    """Memory that `stream` is the first to use: from its own pool, since what the
+    current stream's pool gives may still be in use there."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(size, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(size, dtype=dtype, device=device)
+
+
 def _type16(dtype) -> int:
     torch = _torch()
     if dtype is torch.float16:
@@ -764,8 +775,8 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
     assert ldc == 1 or W <= 1 or B == 0
     if out is None:
         dev = block_table.device  # two allocations, not five: the int32 results are parts of one
-        out = (torch.empty(max_tokens, dtype=torch.int64, device=dev),
-               *torch.empty(max_tokens + 2 * B + 3, dtype=i32, device=dev).split((max_tokens, B + 1, B, 2)))
+        out = (_empty_on(stream, max_tokens, torch.int64, dev),
+               *_empty_on(stream, max_tokens + 2 * B + 3, i32, dev).split((max_tokens, B + 1, B, 2)))
     slots, positions, cu, kv_len, counts = out
     rc = (_lib or _lib_obj()).b2q_kv_cache_plan(
         cached.data_ptr(), new.data_ptr(), B, page_size, free_pages.data_ptr(), free_pages.numel(),
@@ -805,7 +816,7 @@ def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq
         if axes == 1:
             pos_stride = T
     if out is None:
-        out = torch.empty((T, Hq * D), dtype=dt, device=qkv.device)
+        out = _empty_on(stream, (T, Hq * D), dt, qkv.device)
     assert out.dtype is dt
     sec = (ctypes.c_int32 * 3)(*sections)
     rc = (_lib or _lib_obj()).b2q_qkv_rope_cache(
@@ -821,6 +832,10 @@ def attention_paged_workspace_bytes(B: int, T: int, max_new: int, max_kv: int, H
                                     causal: bool = True, window: int = 0, sinks: int = 0) -> int:
     return lib().b2q_attention_paged_workspace_bytes(B, T, max_new, max_kv, Hq, Hkv, D, 1 if causal else 0, window,
                                                      sinks)
+
+
+# (the layers of a step ask for the same sizes)
+_paged_ws_bytes = functools.lru_cache(maxsize=256)(attention_paged_workspace_bytes)
 
 
 def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: int, max_kv: int, Hq: int,
@@ -846,14 +861,14 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
     if scale is None:
         scale = D ** -0.5
     if out is None:
-        out = torch.empty((T, width), dtype=dt, device=q.device)
+        out = _empty_on(stream, (T, width), dt, q.device)
     ws_ptr, ws_bytes = None, 0
     if ws is not None:
         ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
     else:
-        ws_bytes = L.b2q_attention_paged_workspace_bytes(B, T, max_new, max_kv, Hq, Hkv, D, 1 if causal else 0, window, sinks)
+        ws_bytes = _paged_ws_bytes(B, T, max_new, max_kv, Hq, Hkv, D, causal, window, sinks)
         if ws_bytes:  # the allocator's blocks are 512-byte aligned
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            ws = _empty_on(stream, ws_bytes, torch.uint8, q.device)
             ws_ptr = ws.data_ptr()
     rc = L.b2q_attention_paged(
         _type16(dt), q.data_ptr(), ldq * 2, cu_new.data_ptr(), B, T, max_new, k_cache.data_ptr(), v_cache.data_ptr(),
@@ -886,7 +901,7 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
         assert dt is torch.bfloat16
         xtype, size = TYPE_BF16, 2
     if out is None:
-        out = torch.empty((m, n), dtype=torch.float32, device=x.device)
+        out = _empty_on(stream, (m, n), torch.float32, x.device)
     rc = (_lib or _lib_obj()).b2q_mul_vec(
         wtype, packed.data_ptr(), n, k, xtype, x.data_ptr(), m, ld * size, _ptr(bias), _ptr(gate), _ptr(resid),
         0 if resid is None else resid.stride(0) * 4, out.data_ptr(), out.stride(0) * 4, _raw_stream(stream, x))

@@ -1,10 +1,13 @@
 """The block over a paged cache (cached_block.py): prompts and single tokens of
 several requests, against a 64-bit recomputation of each whole request without
 a cache."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
+import b2q
 import cached_block as cb
 import oracle as O
 
@@ -97,3 +100,29 @@ def test_example_runs(dev, capsys):
     out = capsys.readouterr().out.splitlines()
     assert len(out) == 9 and out[-1].endswith("cached 308")
     assert all(np.isfinite(float(line.split("rms ")[1].split(",")[0])) for line in out)
+
+
+def test_results_on_another_stream_come_from_its_pool(dev):
+    """Outputs and workspaces of a call on a given stream are allocated for it: memory that the current stream
+    has freed, and still works on, is not handed to the other one."""
+    D, n = 128, 30011
+    kc = torch.randn(n // 16 + 1, 1, 16, D, device=dev).half()
+    vc = torch.randn_like(kc)
+    table = torch.arange(kc.shape[0], dtype=torch.int32, device=dev)[None]
+    kv_len = torch.tensor([n], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    q = torch.randn(1, 2 * D, device=dev).half()
+    assert b2q.attention_paged_workspace_bytes(1, 1, 1, n, 2, 1, D) > 0
+    ref = b2q.attention_paged(q, kc, vc, table, kv_len, cu, 1, n, 2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    big = torch.randn(8192, 8192, device=dev)
+    for _ in range(4):
+        for _ in range(4):
+            big = torch.tanh(big @ big)                              # the current stream is busy,
+        scrap = torch.full((1 << 20,), math.nan, device=dev)         # and then writes what it has freed by now
+        del scrap
+        o = b2q.attention_paged(q, kc, vc, table, kv_len, cu, 1, n, 2, stream=side)
+        side.synchronize()
+        assert torch.equal(o, ref)
+    torch.cuda.synchronize()

@@ -92,7 +92,9 @@ __device__ __forceinline__ uint64_t pt_desc_v(uint32_t addr, uint32_t lbo) {
 
 // exp2 of a pair on the FMA pipe (the dense F16 attention has the derivation:
 // Cody-Waite, cubic of least maximum relative error 7.5e-5); the others go to
-// the MUFU.
+// the MUFU.  Below -125, so for masked scores too, it is exactly 0: the cubic gives
+// its constant term times 2^-125 there, which is subtracted.  bf16 holds 2^-125, and a
+// row that sees no key would have become a mean of values that it must not see.
 __device__ __forceinline__ float2 pt_ex2_poly(float2 x) {
   constexpr float kRound = 12582912.0f;
   const float2 one = make_float2(1.0f, 1.0f), neg = make_float2(-1.0f, -1.0f);
@@ -102,9 +104,11 @@ __device__ __forceinline__ float2 pt_ex2_poly(float2 x) {
   const float2 f = ffma2(n, neg, x);
   float2 q = ffma2(make_float2(0.0551716685f, 0.0551716685f), f, make_float2(0.242611140f, 0.242611140f));
   q = ffma2(q, f, make_float2(0.693260968f, 0.693260968f));
-  q = ffma2(q, f, make_float2(0.999928057f, 0.999928057f));
-  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(r.x) << 23)),
-                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(r.y) << 23)));
+  constexpr float c0 = 0.999928057f, least = -c0 * 0x1p-125f;
+  q = ffma2(q, f, make_float2(c0, c0));
+  q = make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(r.x) << 23)),
+                  __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(r.y) << 23)));
+  return ffma2(q, one, make_float2(least, least));
 }
 
 __device__ __forceinline__ float pt_max3(float a, float b, float c) {

@@ -1,0 +1,59 @@
+"""Paged attention (b2q_attention_paged) where rows and keys are unusual: rows without a key beside rows with some,
+values near the type's limits, infinities, scores far below a row's largest."""
+import math
+
+import pytest
+import torch
+
+import b2q
+from test_gpu_attention_paged import DT, check, make, reference
+
+pytestmark = pytest.mark.gpu
+
+
+# 4 / 2 heads: two rows a token; up to 32 and 128 rows (rows kernel), more (tile kernel); announced lengths that give
+# one stretch of the keys and several
+@pytest.mark.parametrize("news", [[1, 1, 1, 1], [3, 2, 20, 6], [150, 130, 40, 300], [70, 64, 65, 200]])
+@pytest.mark.parametrize("D,dt", [(64, "bf16"), (128, "bf16"), (64, "f16"), (128, "f16")])
+@pytest.mark.parametrize("max_kv", [700, 20000])
+def test_rows_without_keys_are_zero(dev, news, D, dt, max_kv):
+    """No keys, fewer keys than new tokens (rows before the first key beside rows that see some), absent pages at the
+    front, in the middle and everywhere: rows that see nothing are exactly 0."""
+    lens = [0, max(1, news[1] // 2), 500, 700]
+    q, kc, vc, table, L, cu = make(dev, lens, news, 4, 2, D, DT[dt], 32, seed=7)
+    table[2] = -1
+    table[3, 2:5] = -1
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, max(news), max_kv, 4)
+    ref, mag = reference(q, kc, vc, table, L, cu, 4)
+    check(o, ref, mag, DT[dt])
+    blind = mag.sum(1) == 0
+    assert int(blind.sum()) >= news[0] + news[2] + news[1] - lens[1]
+    assert bool((o[blind] == 0).all())
+
+
+@pytest.mark.parametrize("D,dt", [(64, "bf16"), (128, "bf16"), (128, "f16")])
+@pytest.mark.parametrize("max_kv", [700, 20000])
+def test_window_without_pages(dev, D, dt, max_kv):
+    """A window whose pages are absent for some rows of a chunk and present for others."""
+    q, kc, vc, table, L, cu = make(dev, [700, 460], [300, 200], 4, 2, D, DT[dt], 32, seed=8)
+    table[0, 12:17] = -1   # keys 384 to 543: rows at 450 to 543 with a window of 64 see none
+    table[1, 10:] = -1
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, 300, max_kv, 4, window=64)
+    ref, mag = reference(q, kc, vc, table, L, cu, 4, window=64)
+    check(o, ref, mag, DT[dt])
+    blind = mag.sum(1) == 0
+    assert int(blind.sum()) > 100 and bool((o[blind] == 0).all())
+
+
+@pytest.mark.parametrize("news,lens", [([5, 3], [300, 64]), ([200, 131], [500, 131]), ([300, 40], [3000, 900])])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("max_kv", [None, 20000])
+def test_huge_values_of_unseen_keys(dev, news, lens, D, max_kv):
+    """Finite bf16 values of 1e36 in later tokens' keys do not reach the rows before them (2^-125 of them would)."""
+    q, kc, vc, table, L, cu = make(dev, lens, news, 4, 2, D, torch.bfloat16, 32, seed=9)
+    for b in range(2):
+        for key in (lens[b] - 1, lens[b] - news[b] // 2):
+            vc[int(table[b, key // 32]), :, key % 32] = 1e36
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, max(news), max(lens) if max_kv is None else max_kv, 4)
+    ref, mag = reference(q, kc, vc, table, L, cu, 4)
+    check(o, ref, mag, torch.bfloat16)

@@ -38,19 +38,27 @@ class PagedCache:
         self.v = [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(layers)]
         self.page_size, self.dev = page_size, dev
         self.table = torch.full((requests, -(-max_len // page_size)), -1, dtype=torch.int32, device=dev)
-        self.free = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.free = torch.arange(pages, dtype=torch.int32, device=dev)  # entries `taken` and on are the free pages
+        self.taken = 0
         self.lengths = [0] * requests
 
-    def plan(self, new: list) -> dict:
-        """Room for new[b] tokens of every request b; the step's slots, positions and lengths."""
+    def plan(self, new: list, stream=None) -> dict:
+        """Room for new[b] tokens of every request b; the step's slots, positions and lengths.  A step that
+        runs on a given stream is planned on it too (the table and the free list are never reallocated)."""
+        import torch
+        with torch.cuda.stream(stream):
+            return self._plan(new)
+
+    def _plan(self, new: list) -> dict:
         import torch
         ps = self.page_size
         pages = sum(-(-(c + n) // ps) - -(-c // ps) for c, n in zip(self.lengths, new))
-        if pages > self.free.numel() or max(c + n for c, n in zip(self.lengths, new)) > self.table.shape[1] * ps:
+        if pages > self.free.numel() - self.taken or max(c + n for c, n in zip(self.lengths, new)) > self.table.shape[1] * ps:
             raise RuntimeError("the cache is full")
         i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=self.dev)  # noqa: E731
-        slots, pos, cu, kv_len, _ = b2q.kv_cache_plan(i32(self.lengths), i32(new), ps, self.free, self.table, sum(new))
-        self.free = self.free[pages:].clone()
+        slots, pos, cu, kv_len, _ = b2q.kv_cache_plan(i32(self.lengths), i32(new), ps, self.free[self.taken:], self.table,
+                                                      sum(new))
+        self.taken += pages
         self.lengths = [c + n for c, n in zip(self.lengths, new)]
         return {"slots": slots, "pos": pos, "cu": cu, "kv_len": kv_len, "max_new": max(new), "max_kv": max(self.lengths)}
 
@@ -73,27 +81,33 @@ class CachedBlock:
         self.packed = {n: b2q.weight_pack_q4_0(torch.from_numpy(weights[n]).to(dev), k) for n, (_, k) in self.shape.items()}
         self.vec = vectors
 
-    def _linear(self, name: str, x, bias, resid=None, stream=None):
+    def _linear(self, name: str, x, bias, resid=None):
         n, k = self.shape[name]
         m = x.shape[0]
         if m <= b2q.MUL_VEC_MAX_M:
-            return b2q.mul_vec(b2q.TYPE_Q4_0, self.packed[name], n, k, x, bias=bias, resid=resid, out=resid, stream=stream)
-        act = b2q.act_prepare(x.float(), stream=stream)
-        return b2q.mul_mat_prepared_q4_0(self.packed[name], n, k, act, m, bias=bias, resid=resid, out=resid, stream=stream)
+            return b2q.mul_vec(b2q.TYPE_Q4_0, self.packed[name], n, k, x, bias=bias, resid=resid, out=resid)
+        act = b2q.act_prepare(x.float())
+        return b2q.mul_mat_prepared_q4_0(self.packed[name], n, k, act, m, bias=bias, resid=resid, out=resid)
 
     def forward(self, x, cache: PagedCache, layer: int, step: dict, positions, stream=None):
-        """x: fp32 [tokens, C], updated in place and returned; positions int32 [axes, tokens]."""
+        """x: fp32 [tokens, C], updated in place and returned; positions int32 [axes, tokens].  With a stream the
+        whole pass belongs to it: its casts, and the pool that its temporaries come from and go back to."""
+        import torch
+        with torch.cuda.stream(stream):
+            return self._forward(x, cache, layer, step, positions)
+
+    def _forward(self, x, cache: PagedCache, layer: int, step: dict, positions):
         v = self.vec
-        h = b2q.norm_modulate(x, stream=stream)
-        qkv = self._linear("qkv", h, v["b_qkv"], stream=stream)
+        h = b2q.norm_modulate(x)
+        qkv = self._linear("qkv", h, v["b_qkv"])
         k, vv = cache.k[layer], cache.v[layer]
         q = b2q.qkv_rope_cache(qkv, self.H, self.Hk, self.D, positions, self.sections, self.inv_freq, step["slots"], k, vv,
-                               norm=True, gamma_q=v["gq"], gamma_k=v["gk"], stream=stream)
+                               norm=True, gamma_q=v["gq"], gamma_k=v["gk"])
         o = b2q.attention_paged(q, k, vv, cache.table, step["kv_len"], step["cu"], step["max_new"], step["max_kv"], self.H,
-                                window=self.window, sinks=self.sinks, stream=stream)
-        self._linear("out", o, v["b_out"], resid=x, stream=stream)
-        h = b2q.gelu(self._linear("fc1", b2q.norm_modulate(x, stream=stream), v["b1"], stream=stream), stream=stream)
-        self._linear("fc2", h, v["b2"], resid=x, stream=stream)
+                                window=self.window, sinks=self.sinks)
+        self._linear("out", o, v["b_out"], resid=x)
+        h = b2q.gelu(self._linear("fc1", b2q.norm_modulate(x), v["b1"]))
+        self._linear("fc2", h, v["b2"], resid=x)
         return x
 
 

@@ -126,3 +126,46 @@ def test_results_on_another_stream_come_from_its_pool(dev):
         side.synchronize()
         assert torch.equal(o, ref)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("news", [[[40, 30], [2, 1], [1, 1]]])
+def test_forward_on_another_stream(dev, news):
+    """Steps of more than eight tokens and of few, plan and forward on a given stream, while the current stream is
+    busy: the results of the same steps on the current stream."""
+    C, heads, D, hidden = 256, 4, 64, 512
+    block, _ = cb.random_block(dev, C, heads, heads, D, hidden, (12, 10, 10), seed=4)
+    g = torch.Generator(device=dev).manual_seed(2)
+    xs = [torch.randn(sum(n), C, generator=g, device=dev) for n in news]
+    grids = []
+
+    def steps(stream=None, before=lambda: None):
+        cache = cb.PagedCache(dev, 1, 2, heads, D, pages=16, page_size=16, max_len=64)
+        torch.cuda.synchronize()
+        out = []
+        for i, (n, x0) in enumerate(zip(news, xs)):
+            x = x0.clone()
+            torch.cuda.synchronize()
+            before()
+            step = cache.plan(n, stream=stream)
+            if stream is None:
+                grids.append(coords(step["pos"]))
+            out.append(block.forward(x, cache, 0, step, grids[i], stream=stream))
+            if stream is not None:
+                stream.synchronize()
+        torch.cuda.synchronize()
+        return [y.clone() for y in out]
+
+    ref = steps()
+    side = torch.cuda.Stream()
+    big = torch.randn(8192, 8192, device=dev)
+
+    def busy():  # what the current stream's pool hands out from here on holds NaN, and the stream has work for long
+        nonlocal big
+        held = [torch.full((rows * cols,), math.nan, device=dev) for rows in (70, 3, 2) for cols in (C, 768, hidden) for _ in range(40)]
+        torch.cuda.synchronize()
+        del held
+        for _ in range(8):
+            big = torch.tanh(big @ big)
+
+    for a, b in zip(steps(side, busy), ref):
+        assert torch.equal(a, b)

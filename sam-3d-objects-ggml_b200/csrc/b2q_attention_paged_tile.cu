@@ -452,6 +452,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
       for (int x = 0; x < kTileKeys; x += 32) tmem_ld_32x32b_x32(ts + x, *reinterpret_cast<uint32_t(*)[32]>(&sr[x]));
       tmem_wait_ld();
+      if (!positive) {  // rare: the order of the scaled scores is another one (before the masks: -inf is a score too)
+#pragma unroll
+        for (int x = 0; x < kTileKeys; ++x) sr[x] = __float_as_uint(__uint_as_float(sr[x]) * a.c2);
+      }
       const int kt = mine.at(j);
       if (holes || kt >= plain_hi || (kt < plain_lo && kt >= plain_sk)) {
         uint32_t pages = 0xffffffffu;
@@ -470,11 +474,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
         for (int x = 0; x < kTileKeys; ++x)
           if (!(x < hi && (x >= lo || x < sk) && ((pages >> (x >> row_bit)) & 1u))) sr[x] = __float_as_uint(-INFINITY);
-      }
-      if (!positive) {  // rare: the order of the scaled scores is another one
-#pragma unroll
-        for (int x = 0; x < kTileKeys; ++x)
-          if (sr[x] != __float_as_uint(-INFINITY)) sr[x] = __float_as_uint(__uint_as_float(sr[x]) * a.c2);
       }
       float mx8[8];  // row max: three-input max, eight chains
 #pragma unroll

@@ -57,3 +57,16 @@ def test_huge_values_of_unseen_keys(dev, news, lens, D, max_kv):
     o = b2q.attention_paged(q, kc, vc, table, L, cu, max(news), max(lens) if max_kv is None else max_kv, 4)
     ref, mag = reference(q, kc, vc, table, L, cu, 4)
     check(o, ref, mag, torch.bfloat16)
+
+
+@pytest.mark.parametrize("news,lens", [([1, 1], [400, 77]), ([70, 150], [400, 150])])
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16")])
+def test_infinite_scores_under_a_negative_scale(dev, news, lens, D, dt):
+    """A product of -infinity is a score of +infinity when the scale is negative, and rows that see it are NaN."""
+    q, kc, vc, table, L, cu = make(dev, lens, news, 4, 2, D, DT[dt], 16, seed=2)
+    q.abs_().add_(0.25)  # (no zeros: they would give NaN themselves)
+    kc[int(table[0, 1]), :, 3, 9] = -math.inf
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, max(news), max(lens), 4, scale=-0.1)
+    assert bool(torch.isnan(o[:int(cu[1])]).all())
+    ref, mag = reference(q, kc, vc, table, L, cu, 4, scale=-0.1)
+    check(o[int(cu[1]):], ref[int(cu[1]):], mag[int(cu[1]):], DT[dt])

@@ -475,6 +475,19 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
     }
     return x;
   };
+  // Values d and d + 1 of row rr, of sum `total`, once their NaN are settled.
+  auto settle = [&](float2 x, float total, uint32_t rr, int d) {
+    if ((x.x != x.x || x.y != x.y) && total == total) {
+      const int64_t pos = rq.first + rr / G;
+      const int row_hi = static_cast<int>(max(int64_t{0}, a.causal ? min(rq.len, pos + 1) : rq.len));
+      const int row_lo = a.window > 0 ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
+      const uint2 seen = nonfinite_seen<1, BF16>(a.v + ((static_cast<int64_t>(hk) * D) << a.page_shift) + d, table, a.n_pages,
+                                                 a.page_shift, page_elems, D, row_lo, row_hi, sinks);
+      if (x.x != x.x) x.x = settled(seen, 0);
+      if (x.y != x.y) x.y = settled(seen, 1);
+    }
+    return x;
+  };
   if (a.cluster) {
     // Each CTA leaves its rows where its first warp's were; then the CTAs share out the
     // values and read them from each other.
@@ -509,6 +522,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
       }
       const float inv = m_all == -INFINITY && l_all == 0.0f ? 0.0f : 1.0f / l_all;
       const uint32_t rr = r0 + prow, i = rr / G;
+      x = settle(x, l_all, rr, d);
       *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (rq.t0 + i) * a.ldo +
                                    (static_cast<int64_t>(hk) * G + (rr - i * G)) * D + d) =
           pack2<BF16>(x.x * inv, x.y * inv);
@@ -525,7 +539,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
   if (!whole && part == 0) a.part_ml[pi] = make_float2(M, sum);
 #pragma unroll
   for (int d = part * 2; d < D; d += TPR * 2) {
-    const float2 x = joined(d);
+    const float2 x = settle(joined(d), sum, r, d);
     if (whole)
       *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + t * a.ldo + h * D + d) =
           pack2<BF16>(x.x * inv, x.y * inv);

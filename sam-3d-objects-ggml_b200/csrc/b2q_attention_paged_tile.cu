@@ -579,6 +579,21 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 }
               }
         }
+        if (l == l) {  // (an empty row is 0 by now)
+          bool lost = false;
+#pragma unroll
+          for (int x = 0; x < 32; ++x) lost |= o[x] != o[x];
+          if (lost) {  // an infinite value met a weight of 0
+            const int hi = static_cast<int>(max(int64_t{0}, a.causal ? min(rq.len, pos + 1) : rq.len));
+            const int lo = a.window > 0 ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
+            const uint2 seen = nonfinite_seen<16, BF16>(
+                a.v + ((static_cast<int64_t>(hk) * D) << a.page_shift) + d, table, a.n_pages, a.page_shift,
+                (static_cast<int64_t>(a.Hkv) * D) << a.page_shift, D, lo, hi, a.window > 0 ? static_cast<int>(a.sinks) : 0);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (o[x] != o[x]) o[x] = settled(seen, x);
+          }
+        }
         if (whole_keys) {
           uint16_t* dst = static_cast<uint16_t*>(a.o) + tr * a.ldo + h * D + d;
 #pragma unroll

@@ -82,4 +82,42 @@ __device__ __forceinline__ bool sees(const PagedArgs& a, int64_t p, int64_t j, i
   return j < len && (!a.causal || j <= p) && (a.window <= 0 || j > p - a.window || j < a.sinks);
 }
 
+// A key's infinite value makes the outputs of the rows that see it infinite, but in the tensor
+// products it meets weights that are 0 where they have no bits left (an fp16 weight below 2^-25 of
+// the largest, the rounding error of a weight that is exact) or negative (other rounding errors),
+// and gives NaN.  So an output that is NaN although its row's sum is not is settled from the
+// values themselves: a NaN, or infinities of both signs, among the keys that the row sees is NaN,
+// else the infinity (none: the sums overflowed, NaN as before).  A row sees keys [lo, hi) and those
+// of [0, sinks) below hi.  v: the kv head's values of page 0 at the first of 2 W columns; the
+// result's bits x say that column x has an infinity or NaN of positive (.x) or negative (.y) sign,
+// a NaN counting as both.  Rare, so the loop over the keys is plain.
+template <int W, bool BF16>
+__device__ __noinline__ uint2 nonfinite_seen(const uint16_t* v, const int32_t* table, int64_t n_pages, int page_shift,
+                                             int64_t page_elems, int D, int lo, int hi, int sinks) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  uint2 seen = make_uint2(0u, 0u);
+  for (int j = sinks > 0 ? 0 : lo; j < hi; j = j + 1 >= sinks && j + 1 < lo ? lo : j + 1) {
+    const int32_t page = __ldg(table + (j >> page_shift));
+    if (page < 0 || page >= n_pages) continue;
+    const uint16_t* row = v + page * page_elems + static_cast<int64_t>(j & ((1 << page_shift) - 1)) * D;
+    for (int w = 0; w < W; ++w) {
+      const uint32_t u = __ldg(reinterpret_cast<const uint32_t*>(row) + w);
+      if (!nonfinite2<BF16>(u)) continue;
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t h = x ? u >> 16 : u & 0xffffu;
+        if ((h & kExp) != kExp) continue;
+        const bool nan = (h & 0x7fffu) != kExp;
+        if (nan || h == kExp) seen.x |= 1u << (2 * w + x);
+        if (nan || h != kExp) seen.y |= 1u << (2 * w + x);
+      }
+    }
+  }
+  return seen;
+}
+// What column x of a row with those bits is, where its sum gave NaN.
+__device__ __forceinline__ float settled(uint2 seen, int x) {
+  const bool up = (seen.x >> x) & 1u, down = (seen.y >> x) & 1u;
+  return up == down ? NAN : up ? INFINITY : -INFINITY;
+}
+
 }  // namespace b2q

@@ -70,3 +70,52 @@ def test_infinite_scores_under_a_negative_scale(dev, news, lens, D, dt):
     assert bool(torch.isnan(o[:int(cu[1])]).all())
     ref, mag = reference(q, kc, vc, table, L, cu, 4, scale=-0.1)
     check(o[int(cu[1]):], ref[int(cu[1]):], mag[int(cu[1]):], DT[dt])
+
+
+def same_kind(got, ref):
+    """NaN, +infinity and -infinity in the same places."""
+    return all(torch.equal(f(got), f(ref)) for f in (torch.isnan, torch.isposinf, torch.isneginf))
+
+
+# rows kernel (one stretch, a cluster, stretches joined afterwards; 16 and 32 rows), tile kernel (whole and split)
+@pytest.mark.parametrize("Hq,news,lens,max_kv", [
+    (4, [1, 1], [100, 33], None), (4, [1, 1], [900, 333], None), (4, [1, 1], [9000, 333], None), (24, [2, 1], [100, 40], None),
+    (24, [2, 1], [5000, 40], None), (4, [150, 140], [400, 140], None), (4, [150, 140], [400, 140], 20000),
+])
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16"), (128, "f16"), (64, "bf16")])
+@pytest.mark.parametrize("scale", [0.125, 0.4])
+def test_infinite_values_reach_rows_that_see_them(dev, Hq, news, lens, max_kv, D, dt, scale):
+    """An infinite value of a key that a row sees makes that output the infinity, however small the key's weight;
+    infinities of both signs, or a NaN, make it NaN.  Weights stay above 2^-126 of a row's largest."""
+    q, kc, vc, table, L, cu = make(dev, lens, news, Hq, 2, D, DT[dt], 16, seed=Hq + D)
+    q *= 0.5
+    at = lambda b, key: (int(table[b, key // 16]), slice(None), key % 16)  # noqa: E731
+    for b in range(2):
+        vc[at(b, 3)][:, 5] = math.inf
+        vc[at(b, lens[b] // 2)][:, 6] = -math.inf
+        vc[at(b, 1)][:, 7] = math.inf
+        vc[at(b, lens[b] // 3)][:, 7] = -math.inf
+        vc[at(b, 2)][:, 8] = math.nan
+        vc[at(b, lens[b] - 1)][:, 9] = math.inf
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, max(news), max(lens) if max_kv is None else max_kv, Hq, scale=scale)
+    ref, mag = reference(q, kc, vc, table, L, cu, Hq, scale=scale)
+    assert bool(torch.isposinf(ref).any()) and bool(torch.isneginf(ref).any()) and bool(torch.isnan(ref).any())
+    assert same_kind(o, ref.to(DT[dt]))
+    fin = torch.isfinite(ref)
+    check(torch.where(fin, o, 0), torch.where(fin, ref, 0.0), torch.where(fin, mag, 0.0), DT[dt])
+
+
+@pytest.mark.parametrize("Hq,news,lens", [(4, [1], [700]), (24, [2], [5000]), (4, [150], [400])])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_infinite_value_of_a_light_key(dev, Hq, news, lens, dt):
+    """The key with the infinity weighs 2^-60 of the others: still the infinity."""
+    D = 64
+    q, kc, vc, table, L, cu = make(dev, lens, news, Hq, 2, D, DT[dt], 16, seed=3)
+    q.fill_(1.0)
+    kc.zero_()
+    pg, off = int(table[0, 1]), 4
+    kc[pg, :, off] = -5.25     # 64 * 5.25 / 8 = 42 below the others: 2^-60.6
+    vc[pg, :, off, 11] = -math.inf
+    o = b2q.attention_paged(q, kc, vc, table, L, cu, max(news), max(lens), Hq)
+    ref, _ = reference(q, kc, vc, table, L, cu, Hq)
+    assert bool(torch.isneginf(ref).any()) and same_kind(o, ref.to(DT[dt]))

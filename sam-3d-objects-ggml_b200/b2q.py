@@ -772,7 +772,7 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
     assert cached.numel() == B and new.numel() == B
     assert cached.is_contiguous() and new.is_contiguous() and free_pages.is_contiguous()
     ldt, ldc = block_table.stride()
-    assert ldc == 1 or W <= 1 or B == 0
+    assert (ldc == 1 or W <= 1 or B == 0) and (ldt >= W or B <= 1)  # (rows of an expanded table would be taken W apart)
     if out is None:
         dev = block_table.device  # two allocations, not five: the int32 results are parts of one
         out = (_empty_on(stream, max_tokens, torch.int64, dev),
@@ -853,7 +853,7 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
     ldq, ldc = q.stride()
     ldt, ldtc = block_table.stride()
     assert k_cache.dtype is dt and v_cache.dtype is dt and v_cache.shape == k_cache.shape
-    assert width == Hq * D and (ldc == 1 or T == 0) and (ldtc == 1 or W <= 1 or B == 0)
+    assert width == Hq * D and (ldc == 1 or T == 0) and (ldtc == 1 or W <= 1 or B == 0) and (ldt >= W or B <= 1)
     assert k_cache.is_contiguous() and v_cache.is_contiguous()
     assert block_table.dtype is i32 and kv_len.dtype is i32 and cu_new.dtype is i32
     assert kv_len.numel() == B and cu_new.numel() == B + 1 and kv_len.is_contiguous() and cu_new.is_contiguous()

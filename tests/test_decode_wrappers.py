@@ -1,0 +1,90 @@
+"""What the Python wrappers of the cached-decoding calls refuse before anything reaches the library: operands whose
+size, type or strides are not those that the kernels would read and write.  The library is a stand-in that records the
+calls; no GPU needed."""
+import types
+
+import pytest
+import torch
+
+import b2q
+
+F32, F16, BF16, I32, I64 = torch.float32, torch.float16, torch.bfloat16, torch.int32, torch.int64
+
+
+@pytest.fixture
+def lib_calls(monkeypatch):
+    calls = []
+    fake = lambda name: lambda *a: (calls.append((name, a)), 0)[1]  # noqa: E731
+    names = ("b2q_kv_cache_plan", "b2q_qkv_rope_cache", "b2q_attention_paged", "b2q_mul_vec")
+    monkeypatch.setattr(b2q, "_lib", types.SimpleNamespace(**{n: fake(n) for n in names}))
+    monkeypatch.setattr(b2q, "_raw_stream", lambda *a: 0)
+    monkeypatch.setattr(b2q, "_paged_ws_bytes", lambda *a: 0)
+    return calls
+
+
+def plan(B=3, W=8, T=40, **kw):
+    a = dict(cached=torch.zeros(B, dtype=I32), new=torch.zeros(B, dtype=I32), page_size=16,
+             free_pages=torch.zeros(9, dtype=I32), block_table=torch.zeros(B, W, dtype=I32), max_tokens=T)
+    a.update(kw)
+    return b2q.kv_cache_plan(**a)
+
+
+def rope(T=4, Hq=4, Hkv=2, D=64, **kw):
+    a = dict(qkv=torch.zeros(T, (Hq + 2 * Hkv) * D), Hq=Hq, Hkv=Hkv, D=D, positions=torch.zeros(2, T, dtype=I32),
+             sections=(8, 8), inv_freq=torch.zeros(16), slots=torch.zeros(T, dtype=I64),
+             k_cache=torch.zeros(5, Hkv, 16, D, dtype=F16), v_cache=torch.zeros(5, Hkv, 16, D, dtype=F16))
+    a.update(kw)
+    return b2q.qkv_rope_cache(**a)
+
+
+def attention(T=6, B=3, W=8, Hq=4, Hkv=2, D=64, **kw):
+    a = dict(q=torch.zeros(T, Hq * D, dtype=F16), k_cache=torch.zeros(5, Hkv, 16, D, dtype=F16),
+             v_cache=torch.zeros(5, Hkv, 16, D, dtype=F16), block_table=torch.zeros(B, W, dtype=I32),
+             kv_len=torch.zeros(B, dtype=I32), cu_new=torch.zeros(B + 1, dtype=I32), max_new=2, max_kv=128, Hq=Hq)
+    a.update(kw)
+    return b2q.attention_paged(**a)
+
+
+def accepted(lib_calls, name, call, **kw):
+    call(**kw)
+    assert len(lib_calls) == 1 and lib_calls[0][0] == name
+    return lib_calls[0][1]
+
+
+def refused(lib_calls, call, **kw):
+    with pytest.raises(AssertionError):
+        call(**kw)
+    assert not lib_calls
+
+
+# ------------------------------------------------------------------------------------------------- block tables
+def table(kind, B=3, W=8):
+    if kind == "expanded":          # one row for all requests: rows 0 bytes apart
+        return torch.zeros(W, dtype=I32).expand(B, W)
+    if kind == "overlapping":       # rows that begin inside one another
+        return torch.zeros(B * W, dtype=I32).as_strided((B, W), (W - 3, 1))
+    if kind == "columns":
+        return torch.zeros(W, B, dtype=I32).t()
+    if kind == "wide":
+        return torch.zeros(B, W + 5, dtype=I32)[:, 2:2 + W]
+    return torch.zeros(B, W, dtype=I32)
+
+
+@pytest.mark.parametrize("kind", ["expanded", "overlapping", "columns"])
+@pytest.mark.parametrize("call", [plan, attention])
+def test_tables_whose_rows_overlap_are_refused(lib_calls, call, kind):
+    refused(lib_calls, call, block_table=table(kind))
+
+
+@pytest.mark.parametrize("kind,stride", [("plain", 32), ("wide", 52)])
+def test_tables_that_are_taken(lib_calls, kind, stride):
+    assert accepted(lib_calls, "b2q_kv_cache_plan", plan, block_table=table(kind))[8] == stride
+    lib_calls.clear()
+    assert accepted(lib_calls, "b2q_attention_paged", attention, block_table=table(kind))[13] == stride
+
+
+def test_a_table_of_one_request_may_have_any_stride(lib_calls):
+    t = torch.zeros(8, dtype=I32).expand(1, 8)
+    assert accepted(lib_calls, "b2q_kv_cache_plan", plan, B=1, block_table=t)[8] >= 32
+    lib_calls.clear()
+    assert accepted(lib_calls, "b2q_attention_paged", attention, B=1, block_table=t)[13] >= 32

@@ -750,6 +750,16 @@ def _empty_on(stream, size, dtype, device):
         return torch.empty(size, dtype=dtype, device=device)
 
 
+def _are_rows(t, rows: int, cols: int, dtype) -> bool:
+    """t is a matrix whose rows lie in memory as the kernels read and write them."""
+    return t.dtype is dtype and t.shape == (rows, cols) and (t.stride(1) == 1 or cols <= 1 or rows == 0)
+
+
+def _are_floats(t, n: int) -> bool:
+    """t is absent, or n fp32 values one after another."""
+    return t is None or (t.dtype is _torch().float32 and t.numel() == n and t.is_contiguous())
+
+
 def _type16(dtype) -> int:
     torch = _torch()
     if dtype is torch.float16:
@@ -793,7 +803,7 @@ def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq
     """fused qkv rows fp32 [T, (Hq + 2 Hkv) * D] -> q rows [T, Hq * D] of the
     cache's type, with rotary positions (int32 [axes, T]; sections: pairs per
     axis; inv_freq fp32 [sum(sections)]) on q and k after an optional per-head
-    RMS norm; k and v go to slots (int64 [T]) of k_cache, v_cache
+    RMS norm (gamma_q fp32 [Hq * D], gamma_k [Hkv * D]); k and v go to slots (int64 [T]) of k_cache, v_cache
     [pages, Hkv, page size, D], in place."""
     torch = _torch()
     T, width = qkv.shape
@@ -815,9 +825,11 @@ def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq
         assert step == 1 or T <= 1
         if axes == 1:
             pos_stride = T
+    if norm:
+        assert _are_floats(gamma_q, Hq * D) and _are_floats(gamma_k, Hkv * D)
     if out is None:
         out = _empty_on(stream, (T, Hq * D), dt, qkv.device)
-    assert out.dtype is dt
+    assert _are_rows(out, T, Hq * D, dt)
     sec = (ctypes.c_int32 * 3)(*sections)
     rc = (_lib or _lib_obj()).b2q_qkv_rope_cache(
         qkv.data_ptr(), T, Hq, Hkv, D, ld * 4, 1 if norm else 0, _ptr(gamma_q), _ptr(gamma_k), eps, pos_ptr, pos_stride,

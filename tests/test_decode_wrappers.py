@@ -88,3 +88,28 @@ def test_a_table_of_one_request_may_have_any_stride(lib_calls):
     assert accepted(lib_calls, "b2q_kv_cache_plan", plan, B=1, block_table=t)[8] >= 32
     lib_calls.clear()
     assert accepted(lib_calls, "b2q_attention_paged", attention, B=1, block_table=t)[13] >= 32
+
+
+# ------------------------------------------------------------------------------------------- operands of the rope call
+D_, HQ, HKV = 64, 4, 2
+
+
+@pytest.mark.parametrize("kw", [
+    dict(gamma_q=torch.ones(D_)), dict(gamma_k=torch.ones(D_)),                          # one head's gamma for all
+    dict(gamma_q=torch.ones(HQ * D_ + 1)), dict(gamma_k=torch.ones(HKV * D_).half()), dict(gamma_q=torch.ones(HQ * D_, dtype=BF16)),
+    dict(gamma_q=torch.ones(HQ * D_, 2)[:, 0]), dict(gamma_k=torch.ones(D_).expand(HKV, D_)),
+    dict(out=torch.zeros(3, HQ * D_, dtype=F16)), dict(out=torch.zeros(4, HQ * D_ - 8, dtype=F16)),
+    dict(out=torch.zeros(HQ * D_, 4, dtype=F16).t()), dict(out=torch.zeros(4, HQ * D_)),
+])
+def test_rope_operands_that_do_not_fit_are_refused(lib_calls, kw):
+    refused(lib_calls, rope, norm=True, **kw)
+
+
+def test_rope_operands_that_fit(lib_calls):
+    kw = dict(gamma_q=torch.ones(HQ, D_), gamma_k=torch.ones(HKV * D_), out=torch.zeros(4, HQ * D_ + 8, dtype=F16)[:, :HQ * D_])
+    args = accepted(lib_calls, "b2q_qkv_rope_cache", rope, norm=True, **kw)
+    assert args[7] == kw["gamma_q"].data_ptr() and args[8] == kw["gamma_k"].data_ptr() and args[18] == 2 * (HQ * D_ + 8)
+    lib_calls.clear()
+    accepted(lib_calls, "b2q_qkv_rope_cache", rope, norm=False, gamma_q=torch.ones(3))  # not read without the norm
+    lib_calls.clear()
+    accepted(lib_calls, "b2q_qkv_rope_cache", rope, T=1, out=torch.zeros(1, HQ * D_, dtype=F16))

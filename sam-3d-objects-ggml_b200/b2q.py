@@ -895,6 +895,11 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
 MUL_VEC_MAX_M = 8
 
 
+@functools.lru_cache(maxsize=1024)
+def _packed4_bytes(wtype: int, n: int, k: int) -> int:
+    return lib().b2q_weight_packed_q4_0_bytes(n, k) if wtype == TYPE_Q4_0 else weight_packed_bytes(wtype, n, k)
+
+
 def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=None, out=None, stream=None):
     """At most 8 rows x [m, k] (fp32, fp16 or bf16) times a 4-bit weight
     (TYPE_Q4_0 from weight_pack_q4_0, TYPE_Q4_K from weight_pack) taken at its
@@ -914,6 +919,9 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
         xtype, size = TYPE_BF16, 2
     if out is None:
         out = _empty_on(stream, (m, n), torch.float32, x.device)
+    assert packed.numel() * packed.element_size() >= _packed4_bytes(wtype, n, k) and packed.is_contiguous()
+    assert _are_floats(bias, n) and _are_floats(gate, n) and _are_rows(out, m, n, torch.float32)
+    assert resid is None or resid is out or _are_rows(resid, m, n, torch.float32)
     rc = (_lib or _lib_obj()).b2q_mul_vec(
         wtype, packed.data_ptr(), n, k, xtype, x.data_ptr(), m, ld * size, _ptr(bias), _ptr(gate), _ptr(resid),
         0 if resid is None else resid.stride(0) * 4, out.data_ptr(), out.stride(0) * 4, _raw_stream(stream, x))

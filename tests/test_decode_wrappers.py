@@ -113,3 +113,41 @@ def test_rope_operands_that_fit(lib_calls):
     accepted(lib_calls, "b2q_qkv_rope_cache", rope, norm=False, gamma_q=torch.ones(3))  # not read without the norm
     lib_calls.clear()
     accepted(lib_calls, "b2q_qkv_rope_cache", rope, T=1, out=torch.zeros(1, HQ * D_, dtype=F16))
+
+
+# ---------------------------------------------------------------------------------------------- operands of mul_vec
+def vec(m=3, n=40, k=512, wtype=b2q.TYPE_Q4_0, packed=None, x=None, **kw):
+    size = b2q.lib_packed_bytes(wtype, n, k)
+    packed = torch.zeros(size, dtype=torch.uint8) if packed is None else packed(size)
+    return b2q.mul_vec(wtype, packed, n, k, torch.zeros(m, k) if x is None else x, **kw)
+
+
+@pytest.fixture
+def packed_sizes(monkeypatch):
+    """Sizes of the packed layouts as the library gives them (on the stand-in they are what a test says)."""
+    sizes = lambda wtype, n, k: n * k // 2 + n * k // 32 * 2 + (256 if wtype == b2q.TYPE_Q4_0 else 0)  # noqa: E731
+    monkeypatch.setattr(b2q, "_packed4_bytes", sizes, raising=False)
+    monkeypatch.setattr(b2q, "lib_packed_bytes", sizes, raising=False)
+
+
+@pytest.mark.parametrize("wtype", [b2q.TYPE_Q4_0, b2q.TYPE_Q4_K])
+@pytest.mark.parametrize("kw", [
+    dict(bias=torch.zeros(39)), dict(bias=torch.zeros(40, dtype=F16)), dict(bias=torch.zeros(40, 2)[:, 0]),
+    dict(bias=torch.zeros(3, 40)), dict(gate=torch.zeros(1), resid=torch.zeros(3, 40)),
+    dict(gate=torch.zeros(40, dtype=BF16), resid=torch.zeros(3, 40)), dict(resid=torch.zeros(40)), dict(resid=torch.zeros(2, 40)),
+    dict(resid=torch.zeros(3, 40, dtype=F16)), dict(resid=torch.zeros(40, 3).t()), dict(out=torch.zeros(3, 39)),
+    dict(out=torch.zeros(3, 40, dtype=F16)), dict(out=torch.zeros(40, 3).t()), dict(out=torch.zeros(120)),
+    dict(packed=lambda size: torch.zeros(size - 1, dtype=torch.uint8)), dict(packed=lambda size: torch.zeros(2 * size, dtype=torch.uint8)[::2]),
+])
+def test_vec_operands_that_do_not_fit_are_refused(lib_calls, packed_sizes, wtype, kw):
+    refused(lib_calls, vec, wtype=wtype, **kw)
+
+
+def test_vec_operands_that_fit(lib_calls, packed_sizes):
+    wide = torch.zeros(3, 50)
+    args = accepted(lib_calls, "b2q_mul_vec", vec, bias=torch.zeros(40), gate=torch.zeros(1, 40), resid=wide[:, 1:41], out=wide[:, 1:41])
+    assert args[11] == args[13] == 200
+    for kw in (dict(m=0, resid=torch.zeros(0, 40)), dict(m=1, out=torch.zeros(1, 40)), dict(x=torch.zeros(3, 512, dtype=BF16)),
+               dict(packed=lambda size: torch.zeros(size + 9, dtype=torch.uint8))):
+        lib_calls.clear()
+        accepted(lib_calls, "b2q_mul_vec", vec, **kw)

@@ -787,6 +787,9 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
         dev = block_table.device  # two allocations, not five: the int32 results are parts of one
         out = (_empty_on(stream, max_tokens, torch.int64, dev),
                *_empty_on(stream, max_tokens + 2 * B + 3, i32, dev).split((max_tokens, B + 1, B, 2)))
+    else:  # (each as long as its part of the plan, or longer)
+        for t, n, dt in zip(out, (max_tokens, max_tokens, B + 1, B, 2), (torch.int64, i32, i32, i32, i32), strict=True):
+            assert t.dtype is dt and t.numel() >= n and t.is_contiguous()
     slots, positions, cu, kv_len, counts = out
     rc = (_lib or _lib_obj()).b2q_kv_cache_plan(
         cached.data_ptr(), new.data_ptr(), B, page_size, free_pages.data_ptr(), free_pages.numel(),

@@ -151,3 +151,30 @@ def test_vec_operands_that_fit(lib_calls, packed_sizes):
                dict(packed=lambda size: torch.zeros(size + 9, dtype=torch.uint8))):
         lib_calls.clear()
         accepted(lib_calls, "b2q_mul_vec", vec, **kw)
+
+
+# ------------------------------------------------------------------------------------------------ outputs of the plan
+def plan_out(**kw):
+    """The five outputs for 3 requests and 40 tokens."""
+    o = dict(slots=torch.zeros(40, dtype=I64), positions=torch.zeros(40, dtype=I32), cu=torch.zeros(4, dtype=I32),
+             kv_len=torch.zeros(3, dtype=I32), counts=torch.zeros(2, dtype=I32))
+    o.update(kw)
+    return tuple(o.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(slots=torch.zeros(39, dtype=I64)), dict(slots=torch.zeros(40, dtype=I32)), dict(slots=torch.zeros(80, dtype=I64)[::2]),
+    dict(positions=torch.zeros(39, dtype=I32)), dict(positions=torch.zeros(40, dtype=torch.int16)), dict(cu=torch.zeros(3, dtype=I32)),
+    dict(cu=torch.zeros(8, dtype=I32)[::2]), dict(kv_len=torch.zeros(2, dtype=I32)), dict(counts=torch.zeros(1, dtype=I32)),
+    dict(kv_len=torch.zeros(3, dtype=torch.int8)),
+])
+def test_plan_outputs_that_do_not_fit_are_refused(lib_calls, kw):
+    refused(lib_calls, plan, out=plan_out(**kw))
+
+
+def test_plan_outputs_that_fit(lib_calls):
+    out = plan_out()
+    args = accepted(lib_calls, "b2q_kv_cache_plan", plan, out=out)
+    assert args[10:15] == tuple(t.data_ptr() for t in out)
+    lib_calls.clear()
+    accepted(lib_calls, "b2q_kv_cache_plan", plan, out=plan_out(slots=torch.zeros(50, dtype=I64)))  # room to spare

@@ -751,8 +751,11 @@ def _empty_on(stream, size, dtype, device):
 
 
 def _are_rows(t, rows: int, cols: int, dtype) -> bool:
-    """t is a matrix whose rows lie in memory as the kernels read and write them."""
-    return t.dtype is dtype and t.shape == (rows, cols) and (t.stride(1) == 1 or cols <= 1 or rows == 0)
+    """t is a matrix of that many rows and columns, or more, whose rows lie in memory as the kernels read and write them."""
+    if t.dtype is not dtype or t.dim() != 2:
+        return False
+    have, wide = t.shape
+    return have >= rows and wide >= cols and (t.stride(1) == 1 or wide <= 1 or rows == 0)
 
 
 def _are_floats(t, n: int) -> bool:
@@ -877,9 +880,11 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
         scale = D ** -0.5
     if out is None:
         out = _empty_on(stream, (T, width), dt, q.device)
+    assert _are_rows(out, T, width, dt)
     ws_ptr, ws_bytes = None, 0
     if ws is not None:
-        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
+        assert ws.is_contiguous()
+        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
     else:
         ws_bytes = _paged_ws_bytes(B, T, max_new, max_kv, Hq, Hkv, D, causal, window, sinks)
         if ws_bytes:  # the allocator's blocks are 512-byte aligned

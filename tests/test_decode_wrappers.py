@@ -178,3 +178,30 @@ def test_plan_outputs_that_fit(lib_calls):
     assert args[10:15] == tuple(t.data_ptr() for t in out)
     lib_calls.clear()
     accepted(lib_calls, "b2q_kv_cache_plan", plan, out=plan_out(slots=torch.zeros(50, dtype=I64)))  # room to spare
+
+
+# --------------------------------------------------------------------------------- output and workspace of the attention
+@pytest.mark.parametrize("kw", [
+    dict(out=torch.zeros(6, 256)), dict(out=torch.zeros(6, 256, dtype=BF16)), dict(out=torch.zeros(5, 256, dtype=F16)),
+    dict(out=torch.zeros(6, 128, dtype=F16)), dict(out=torch.zeros(256, 6, dtype=F16).t()),
+    dict(ws=torch.zeros(4096, dtype=torch.uint8)[::2]),
+])
+def test_attention_operands_that_do_not_fit_are_refused(lib_calls, kw):
+    refused(lib_calls, attention, **kw)
+
+
+def test_attention_operands_that_fit(lib_calls):
+    out, ws = torch.zeros(9, 280, dtype=F16)[:6, 8:264], torch.zeros(512, dtype=torch.uint8)
+    args = accepted(lib_calls, "b2q_attention_paged", attention, out=out, ws=ws)
+    assert args[23:27] == (out.data_ptr(), 560, ws.data_ptr(), 512)
+    lib_calls.clear()
+    assert accepted(lib_calls, "b2q_attention_paged", attention, ws=torch.zeros(64))[26] == 256
+
+
+def test_outputs_may_have_rows_and_columns_to_spare(lib_calls, packed_sizes):
+    """What lies past them is left alone."""
+    accepted(lib_calls, "b2q_attention_paged", attention, out=torch.zeros(9, 264, dtype=F16))
+    lib_calls.clear()
+    accepted(lib_calls, "b2q_qkv_rope_cache", rope, out=torch.zeros(9, HQ * D_ + 8, dtype=F16))
+    lib_calls.clear()
+    accepted(lib_calls, "b2q_mul_vec", vec, out=torch.zeros(8, 44), resid=torch.zeros(4, 40))

@@ -758,9 +758,9 @@ def _are_rows(t, rows: int, cols: int, dtype) -> bool:
     return have >= rows and wide >= cols and (t.stride(1) == 1 or wide <= 1 or rows == 0)
 
 
-def _are_floats(t, n: int) -> bool:
-    """t is absent, or n fp32 values one after another."""
-    return t is None or (t.dtype is _torch().float32 and t.numel() == n and t.is_contiguous())
+def _are_floats(t, n: int, f32) -> bool:
+    """t is absent, or n values of type f32 one after another."""
+    return t is None or (t.dtype is f32 and t.numel() == n and t.is_contiguous())
 
 
 def _type16(dtype) -> int:
@@ -832,10 +832,11 @@ def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq
         if axes == 1:
             pos_stride = T
     if norm:
-        assert _are_floats(gamma_q, Hq * D) and _are_floats(gamma_k, Hkv * D)
+        assert _are_floats(gamma_q, Hq * D, torch.float32) and _are_floats(gamma_k, Hkv * D, torch.float32)
     if out is None:
         out = _empty_on(stream, (T, Hq * D), dt, qkv.device)
-    assert _are_rows(out, T, Hq * D, dt)
+    else:
+        assert _are_rows(out, T, Hq * D, dt)
     sec = (ctypes.c_int32 * 3)(*sections)
     rc = (_lib or _lib_obj()).b2q_qkv_rope_cache(
         qkv.data_ptr(), T, Hq, Hkv, D, ld * 4, 1 if norm else 0, _ptr(gamma_q), _ptr(gamma_k), eps, pos_ptr, pos_stride,
@@ -880,7 +881,8 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
         scale = D ** -0.5
     if out is None:
         out = _empty_on(stream, (T, width), dt, q.device)
-    assert _are_rows(out, T, width, dt)
+    else:
+        assert _are_rows(out, T, width, dt)
     ws_ptr, ws_bytes = None, 0
     if ws is not None:
         assert ws.is_contiguous()
@@ -917,8 +919,8 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
     m, width = x.shape
     ld, ldc = x.stride()
     assert width == k and (ldc == 1 or k <= 1 or m == 0)
-    dt = x.dtype
-    if dt is torch.float32:
+    dt, f32 = x.dtype, torch.float32
+    if dt is f32:
         xtype, size = TYPE_F32, 4
     elif dt is torch.float16:
         xtype, size = TYPE_F16, 2
@@ -926,10 +928,14 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
         assert dt is torch.bfloat16
         xtype, size = TYPE_BF16, 2
     if out is None:
-        out = _empty_on(stream, (m, n), torch.float32, x.device)
-    assert packed.numel() * packed.element_size() >= _packed4_bytes(wtype, n, k) and packed.is_contiguous()
-    assert _are_floats(bias, n) and _are_floats(gate, n) and _are_rows(out, m, n, torch.float32)
-    assert resid is None or resid is out or _are_rows(resid, m, n, torch.float32)
+        out = _empty_on(stream, (m, n), f32, x.device)
+    else:
+        assert _are_rows(out, m, n, f32)
+    assert packed.numel() >= _packed4_bytes(wtype, n, k) and packed.is_contiguous()
+    if bias is not None:
+        assert _are_floats(bias, n, f32)
+    if resid is not None:
+        assert (resid is out or _are_rows(resid, m, n, f32)) and _are_floats(gate, n, f32)
     rc = (_lib or _lib_obj()).b2q_mul_vec(
         wtype, packed.data_ptr(), n, k, xtype, x.data_ptr(), m, ld * size, _ptr(bias), _ptr(gate), _ptr(resid),
         0 if resid is None else resid.stride(0) * 4, out.data_ptr(), out.stride(0) * 4, _raw_stream(stream, x))

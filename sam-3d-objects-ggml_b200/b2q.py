@@ -146,6 +146,7 @@ def _check(fn: str, rc: int) -> None:
 
 
 # ----------------------------------------------------------------- torch glue
+@functools.cache
 def _torch():
     import torch
     return torch
@@ -734,10 +735,14 @@ def mul_mat_q_simt(wtype: int, w, a, k: int, stream=None):
 # The cached-decoding calls below are a few microseconds of device work at small
 # sizes, so their wrappers read each tensor property once and take the current
 # stream's handle without building a Stream object.
-def _raw_stream(stream, t) -> int:
-    if stream is not None:
-        return stream.cuda_stream
-    return _torch()._C._cuda_getCurrentRawStream(t.get_device())
+def _raw_stream(stream, t, *others) -> int:
+    """The handle of the stream to run on, once all operands are found on one CUDA device: an address of the host's
+    memory, or of another device's, would fault in the kernel."""
+    dev = t.get_device()
+    assert dev >= 0
+    for o in others:
+        assert o is None or o.get_device() == dev
+    return _torch()._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
 
 
 def _empty_on(stream, size, dtype, device):
@@ -786,6 +791,7 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
     assert cached.is_contiguous() and new.is_contiguous() and free_pages.is_contiguous()
     ldt, ldc = block_table.stride()
     assert (ldc == 1 or W <= 1 or B == 0) and (ldt >= W or B <= 1)  # (rows of an expanded table would be taken W apart)
+    given = ()
     if out is None:
         dev = block_table.device  # two allocations, not five: the int32 results are parts of one
         out = (_empty_on(stream, max_tokens, torch.int64, dev),
@@ -793,11 +799,13 @@ def kv_cache_plan(cached, new, page_size: int, free_pages, block_table, max_toke
     else:  # (each as long as its part of the plan, or longer)
         for t, n, dt in zip(out, (max_tokens, max_tokens, B + 1, B, 2), (torch.int64, i32, i32, i32, i32), strict=True):
             assert t.dtype is dt and t.numel() >= n and t.is_contiguous()
+        given = out
     slots, positions, cu, kv_len, counts = out
     rc = (_lib or _lib_obj()).b2q_kv_cache_plan(
         cached.data_ptr(), new.data_ptr(), B, page_size, free_pages.data_ptr(), free_pages.numel(),
         block_table.data_ptr(), W, 4 * (ldt if ldt > W else W), max_tokens, slots.data_ptr(), positions.data_ptr(),
-        cu.data_ptr(), kv_len.data_ptr(), counts.data_ptr(), _raw_stream(stream, block_table))
+        cu.data_ptr(), kv_len.data_ptr(), counts.data_ptr(),
+        _raw_stream(stream, block_table, cached, new, free_pages, *given))
     if rc:
         _check("b2q_kv_cache_plan", rc)
     return out
@@ -841,7 +849,9 @@ def qkv_rope_cache(qkv, Hq: int, Hkv: int, D: int, positions, sections, inv_freq
     rc = (_lib or _lib_obj()).b2q_qkv_rope_cache(
         qkv.data_ptr(), T, Hq, Hkv, D, ld * 4, 1 if norm else 0, _ptr(gamma_q), _ptr(gamma_k), eps, pos_ptr, pos_stride,
         axes, sec, freq_ptr, 1 if interleaved else 0, _type16(dt), out.data_ptr(), out.stride(0) * 2, k_cache.data_ptr(),
-        v_cache.data_ptr(), slots.data_ptr(), n_pages, page_size, _raw_stream(stream, qkv))
+        v_cache.data_ptr(), slots.data_ptr(), n_pages, page_size,
+        _raw_stream(stream, qkv, slots, k_cache, v_cache, out, *((positions, inv_freq) if axes else ()),
+                    *((gamma_q, gamma_k) if norm else ())))
     if rc:
         _check("b2q_qkv_rope_cache", rc)
     return out
@@ -896,7 +906,7 @@ def attention_paged(q, k_cache, v_cache, block_table, kv_len, cu_new, max_new: i
         _type16(dt), q.data_ptr(), ldq * 2, cu_new.data_ptr(), B, T, max_new, k_cache.data_ptr(), v_cache.data_ptr(),
         n_pages, page_size, block_table.data_ptr(), W, 4 * (ldt if ldt > W else W), kv_len.data_ptr(), max_kv, Hq, Hkv, D,
         scale, 1 if causal else 0, window, sinks, out.data_ptr(), out.stride(0) * 2, ws_ptr, ws_bytes,
-        _raw_stream(stream, q))
+        _raw_stream(stream, q, k_cache, v_cache, block_table, kv_len, cu_new, out, ws))
     if rc:
         _check("b2q_attention_paged", rc)
     return out
@@ -938,7 +948,7 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
         assert (resid is out or _are_rows(resid, m, n, f32)) and _are_floats(gate, n, f32)
     rc = (_lib or _lib_obj()).b2q_mul_vec(
         wtype, packed.data_ptr(), n, k, xtype, x.data_ptr(), m, ld * size, _ptr(bias), _ptr(gate), _ptr(resid),
-        0 if resid is None else resid.stride(0) * 4, out.data_ptr(), out.stride(0) * 4, _raw_stream(stream, x))
+        0 if resid is None else resid.stride(0) * 4, out.data_ptr(), out.stride(0) * 4, _raw_stream(stream, x, packed, bias, gate, resid, out))
     if rc:
         _check("b2q_mul_vec", rc)
     return out

@@ -205,3 +205,35 @@ def test_outputs_may_have_rows_and_columns_to_spare(lib_calls, packed_sizes):
     accepted(lib_calls, "b2q_qkv_rope_cache", rope, out=torch.zeros(9, HQ * D_ + 8, dtype=F16))
     lib_calls.clear()
     accepted(lib_calls, "b2q_mul_vec", vec, out=torch.zeros(8, 44), resid=torch.zeros(4, 40))
+
+
+# --------------------------------------------------------------------------------------------------------- devices
+class On:
+    """A tensor as far as its device goes."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+@pytest.mark.parametrize("devices", [(-1,), (0, -1), (0, 0, 1), (1, 0)])
+def test_operands_on_the_host_or_on_several_devices_are_refused(devices):
+    with pytest.raises(AssertionError):
+        b2q._raw_stream(types.SimpleNamespace(cuda_stream=7), *(On(d) for d in devices))
+
+
+def test_operands_on_one_device_are_taken():
+    assert b2q._raw_stream(types.SimpleNamespace(cuda_stream=7), On(1), None, On(1)) == 7
+
+
+@pytest.mark.parametrize("call,device_operands", [
+    (plan, 4), (lambda **kw: plan(out=plan_out(), **kw), 9), (rope, 7), (lambda **kw: rope(norm=True, gamma_k=torch.ones(128), **kw), 8),
+    (attention, 7), (lambda **kw: attention(ws=torch.zeros(64), **kw), 8), (lambda **kw: vec(bias=torch.zeros(40), **kw), 4),
+])
+def test_every_operand_is_looked_at(lib_calls, packed_sizes, monkeypatch, call, device_operands):
+    looked = []
+    monkeypatch.setattr(b2q, "_raw_stream", lambda stream, *t: looked.extend(x for x in t if x is not None) or 0)
+    call()
+    assert len(looked) == device_operands

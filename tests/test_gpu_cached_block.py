@@ -169,3 +169,28 @@ def test_forward_on_another_stream(dev, news):
 
     for a, b in zip(steps(side, busy), ref):
         assert torch.equal(a, b)
+
+
+def test_operands_on_the_host_are_refused(dev):
+    """Addresses of the host's memory never reach a kernel."""
+    i32 = lambda n, d=dev: torch.zeros(n, dtype=torch.int32, device=d)  # noqa: E731
+    table, pool = i32((2, 4)), torch.zeros(4, 1, 16, 64, dtype=torch.float16, device=dev)
+    for bad in range(3):
+        lens = [i32(2, "cpu" if bad == i else dev) for i in range(3)]
+        with pytest.raises(AssertionError):
+            b2q.kv_cache_plan(lens[0], lens[1], 16, lens[2], table, 2)
+    qkv, inv = torch.zeros(2, 3 * 64, device=dev), torch.zeros(32, device=dev)
+    for bad in range(3):
+        pos, f, slots = i32((1, 2)), inv, torch.zeros(2, dtype=torch.int64, device=dev)
+        pos, f, slots = (t.cpu() if bad == i else t for i, t in enumerate((pos, f, slots)))
+        with pytest.raises(AssertionError):
+            b2q.qkv_rope_cache(qkv, 1, 1, 64, pos, (32,), f, slots, pool, pool.clone())
+    q = torch.zeros(2, 64, dtype=torch.float16, device=dev)
+    for bad in range(3):
+        ops = [t.cpu() if bad == i else t for i, t in enumerate((table, i32(2), i32(3)))]
+        with pytest.raises(AssertionError):
+            b2q.attention_paged(q, pool, pool, *ops, 1, 16, 1)
+    packed = b2q.weight_pack_q4_0(torch.zeros(16, 18, dtype=torch.uint8, device=dev), 32)
+    with pytest.raises(AssertionError):
+        b2q.mul_vec(b2q.TYPE_Q4_0, packed, 16, 32, torch.zeros(1, 32, device=dev), bias=torch.zeros(16))
+    assert b2q.device_status() == 0

@@ -195,3 +195,35 @@ def test_long_rows_shared_out(dev, wtype, n, k, m, xt):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, plain)
+
+
+# Activations that do not fit a CTA's shared memory (split into digits chunk by chunk, the sums kept in between), with
+# one and with several row tiles a CTA; CTAs that own more row tiles than they keep sums of, with and without chunks; and
+# the same for the CTAs of a cluster.
+@pytest.mark.parametrize("wtype,n,k,m,xt", [
+    (b2q.TYPE_Q4_0, 53, 65536, 3, "f32"), (b2q.TYPE_Q4_0, 53, 65536, 8, "f16"), (b2q.TYPE_Q4_0, 40, 65568, 5, "bf16"),
+    (b2q.TYPE_Q4_0, 17, 131104, 8, "f32"), (b2q.TYPE_Q4_K, 53, 65536, 4, "f32"), (b2q.TYPE_Q4_K, 70, 65536, 8, "bf16"),
+    (b2q.TYPE_Q4_K, 1, 22784, 8, "f32"), (b2q.TYPE_Q4_0, 20000, 6432, 8, "f32"), (b2q.TYPE_Q4_K, 20000, 6400, 7, "f16"),
+    (b2q.TYPE_Q4_0, 79000, 3360, 8, "f32"), (b2q.TYPE_Q4_K, 78506, 3328, 8, "f32"),
+    (b2q.TYPE_Q4_0, 38419, 1888, 7, "f32"), (b2q.TYPE_Q4_0, 38419, 1888, 8, "bf16"), (b2q.TYPE_Q4_K, 37927, 2048, 6, "f32"),
+    (b2q.TYPE_Q4_K, 56881, 6400, 2, "bf16"), (b2q.TYPE_Q4_0, 56881, 5408, 4, "f32"),
+])
+def test_chunks_and_groups_of_tiles(dev, wtype, n, k, m, xt):
+    rows = torch.arange(n, device=dev) % 1009  # (1009 rows over and over: quick to make)
+    raw, _, w, mag = make(dev, wtype, min(n, 1009), k, n + k + 2)
+    raw = raw[rows].contiguous()
+    packed = b2q.weight_pack_q4_0(raw, k) if wtype == b2q.TYPE_Q4_0 else b2q.weight_pack(wtype, raw, k)
+    g = torch.Generator(device=dev).manual_seed(m + 1)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    x, bias, gate, base = rand(m, k).to(DT[xt]), rand(n), rand(n), rand(m, n + 3)
+    ref, tol = (x.double() @ w.t())[:, rows], bound(x, mag, k)[:, rows]
+    plain = b2q.mul_vec(wtype, packed, n, k, x)
+    assert bool(((plain.double() - ref).abs() <= tol).all())
+    r1 = ref + bias.double()
+    r2 = base[:, :n].double() + gate.double() * r1
+    lim = tol * gate.double().abs() + 2.0 ** -22 * ((gate.double() * r1).abs() + r2.abs())
+    y = base.clone()
+    b2q.mul_vec(wtype, packed, n, k, x, bias=bias, gate=gate, resid=y[:, :n], out=y[:, :n])
+    assert bool(((y[:, :n].double() - r2).abs() <= lim).all())
+    assert torch.equal(y[:, n:], base[:, n:])
+    assert torch.equal(b2q.mul_vec(wtype, packed, n, k, x), plain)

@@ -52,6 +52,8 @@ class PagedCache:
     def _plan(self, new: list) -> dict:
         import torch
         ps = self.page_size
+        if min(new) < 0:
+            raise ValueError("a step adds tokens")
         pages = sum(-(-(c + n) // ps) - -(-c // ps) for c, n in zip(self.lengths, new))
         if pages > self.free.numel() - self.taken or max(c + n for c, n in zip(self.lengths, new)) > self.table.shape[1] * ps:
             raise RuntimeError("the cache is full")

@@ -194,3 +194,13 @@ def test_operands_on_the_host_are_refused(dev):
     with pytest.raises(AssertionError):
         b2q.mul_vec(b2q.TYPE_Q4_0, packed, 16, 32, torch.zeros(1, 32, device=dev), bias=torch.zeros(16))
     assert b2q.device_status() == 0
+
+
+def test_negative_counts_are_refused(dev):
+    """The device takes a negative count for none; the host's lengths must not shrink beside it."""
+    cache = cb.PagedCache(dev, 1, 2, 1, 64, pages=8, page_size=16, max_len=64)
+    cache.plan([20, 3])
+    with pytest.raises(ValueError):
+        cache.plan([-4, 1])
+    assert cache.lengths == [20, 3]
+    assert cache.plan([1, 0])["kv_len"].tolist() == [21, 3]

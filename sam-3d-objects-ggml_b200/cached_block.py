@@ -57,9 +57,9 @@ class PagedCache:
         pages = sum(-(-(c + n) // ps) - -(-c // ps) for c, n in zip(self.lengths, new))
         if pages > self.free.numel() - self.taken or max(c + n for c, n in zip(self.lengths, new)) > self.table.shape[1] * ps:
             raise RuntimeError("the cache is full")
-        i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=self.dev)  # noqa: E731
-        slots, pos, cu, kv_len, _ = b2q.kv_cache_plan(i32(self.lengths), i32(new), ps, self.free[self.taken:], self.table,
-                                                      sum(new))
+        # (from pinned memory: a copy from pageable memory would wait for all that the stream has to do)
+        counts = torch.tensor([self.lengths, new], dtype=torch.int32).pin_memory().to(self.dev, non_blocking=True)
+        slots, pos, cu, kv_len, _ = b2q.kv_cache_plan(counts[0], counts[1], ps, self.free[self.taken:], self.table, sum(new))
         self.taken += pages
         self.lengths = [c + n for c, n in zip(self.lengths, new)]
         return {"slots": slots, "pos": pos, "cu": cu, "kv_len": kv_len, "max_new": max(new), "max_kv": max(self.lengths)}

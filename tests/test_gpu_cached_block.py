@@ -204,3 +204,18 @@ def test_negative_counts_are_refused(dev):
         cache.plan([-4, 1])
     assert cache.lengths == [20, 3]
     assert cache.plan([1, 0])["kv_len"].tolist() == [21, 3]
+
+
+def test_plan_does_not_wait_for_the_device(dev):
+    cache = cb.PagedCache(dev, 1, 2, 1, 64, pages=8, page_size=16, max_len=64)
+    for _ in range(3):
+        cache.plan([1, 2])  # memory of these sizes is at hand from here on
+    torch.cuda.synchronize()
+    big = torch.randn(8192, 8192, device=dev)
+    done = torch.cuda.Event()
+    for _ in range(8):
+        big = torch.tanh(big @ big)
+    done.record()
+    step = cache.plan([2, 1])
+    assert not done.query()
+    assert step["kv_len"].tolist() == [5, 7] and step["pos"].tolist() == [3, 4, 6]

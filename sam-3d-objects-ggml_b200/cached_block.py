@@ -16,7 +16,7 @@ the same compact Q4_0 weights, which rounds the activations to Q8_0 as ggml's
 CPU mul_mat does.
 
 `PagedCache` keeps the pools, the block tables and the free pages of a set of
-requests; the host knows the lengths it asked for, the device builds the rest
+requests, and takes back the pages of those that end; the host knows the lengths it asked for, the device builds the rest
 (b2q_kv_cache_plan), so a step never waits for the device.
 
     python cached_block.py       # a prompt of 300 tokens, then 8 single tokens
@@ -63,6 +63,16 @@ class PagedCache:
         self.taken += pages
         self.lengths = [c + n for c, n in zip(self.lengths, new)]
         return {"slots": slots, "pos": pos, "cu": cu, "kv_len": kv_len, "max_new": max(new), "max_kv": max(self.lengths)}
+
+    def release(self, request: int, stream=None) -> None:
+        """Ends a request: its pages are free again, and its number is there for another one."""
+        import torch
+        with torch.cuda.stream(stream):
+            pages = -(-self.lengths[request] // self.page_size)
+            self.free[self.taken - pages:self.taken].copy_(self.table[request, :pages])
+            self.table[request].fill_(-1)
+        self.taken -= pages
+        self.lengths[request] = 0
 
 
 class CachedBlock:

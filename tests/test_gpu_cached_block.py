@@ -219,3 +219,42 @@ def test_plan_does_not_wait_for_the_device(dev):
     step = cache.plan([2, 1])
     assert not done.query()
     assert step["kv_len"].tolist() == [5, 7] and step["pos"].tolist() == [3, 4, 6]
+
+
+def test_released_pages_serve_other_requests(dev):
+    """More requests than the pool could hold, one after another: every page has one owner, and steps on pages that
+    others have left match a recomputation without a cache."""
+    C, heads, D, hidden = 256, 4, 64, 512
+    block, weights = cb.random_block(dev, C, heads, heads, D, hidden, (12, 10, 10), seed=5)
+    cache = cb.PagedCache(dev, 1, 3, heads, D, pages=9, page_size=16, max_len=64)
+    g = torch.Generator(device=dev).manual_seed(6)
+    rng = np.random.default_rng(7)
+    xs = [torch.zeros(0, C, device=dev) for _ in range(3)]
+    for turn in range(12):
+        new = [int(n) for n in rng.integers(0, 4, 3)]  # at most 8 tokens a step, as mul_vec takes them
+        new = [min(n, 44 - cache.lengths[b]) for b, n in enumerate(new)] if sum(new) <= 8 else [1, 1, 1]
+        if sum(new) == 0:
+            continue
+        step = cache.plan(new)
+        add = [torch.randn(n, C, generator=g, device=dev) for n in new]
+        xs = [torch.cat(p) for p in zip(xs, add)]
+        y = block.forward(torch.cat(add), cache, 0, step, coords(step["pos"]))
+        full = [reference(block, weights, x.double(), coords(torch.arange(x.shape[0], device=dev))) for x in xs]
+        ref = torch.cat([f[f.shape[0] - n:] for f, n in zip(full, new)])
+        assert float((y.double() - ref).norm() / (ref - torch.cat(add).double()).norm()) <= 4e-3
+        owned = cache.table[cache.table >= 0].tolist()
+        left = cache.free[cache.taken:].tolist()
+        assert sorted(owned + left) == list(range(9))
+        b = turn % 3
+        if turn % 2:
+            cache.release(b)
+            assert cache.lengths[b] == 0 and int(cache.table[b].max()) == -1
+            assert sorted(cache.table[cache.table >= 0].tolist() + cache.free[cache.taken:].tolist()) == list(range(9))
+            xs[b] = xs[b][:0]
+    for _ in range(5):  # a full pool, again and again
+        for b in range(3):
+            cache.release(b)
+        cache.plan([48, 48, 48])
+        with pytest.raises(RuntimeError):
+            cache.plan([1, 0, 0])
+        assert sorted(cache.table[cache.table >= 0].tolist()) == list(range(9))

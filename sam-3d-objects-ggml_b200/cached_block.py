@@ -10,14 +10,17 @@ step (a prompt's chunks, then single tokens) runs per layer.
     x = x + (o . W_out + b_out)                        b2q_mul_vec, or the Q4_0 GEMM
     x = x + (gelu(norm(x) . W1 + b1) . W2 + b2)        same, with b2q_gelu between
 
-Up to MUL_VEC_MAX_M rows the linears are b2q_mul_vec's (the 4-bit weight's
-values against unrounded activations); more rows go to the tensor-core GEMM on
-the same compact Q4_0 weights, which rounds the activations to Q8_0 as ggml's
-CPU mul_mat does.
+Up to `unrounded_rows` rows (MUL_VEC_MAX_M unless the block is told more) the
+linears are b2q_mul_vec's, eight rows at a time: the 4-bit weight's values
+against unrounded activations.  More rows go to the tensor-core GEMM on the same
+compact Q4_0 weights, which rounds the activations to Q8_0 as ggml's CPU mul_mat
+does: a token's result depends, by that rounding, on which side of the number its
+step is.
 
 `PagedCache` keeps the pools, the block tables and the free pages of a set of
-requests, and takes back the pages of those that end; the host knows the lengths it asked for, the device builds the rest
-(b2q_kv_cache_plan), so a step never waits for the device.
+requests, and takes back the pages of those that end; the host knows the lengths
+it asked for, the device builds the rest (b2q_kv_cache_plan), so a step never
+waits for the device.
 
     python cached_block.py       # a prompt of 300 tokens, then 8 single tokens
 """
@@ -83,10 +86,12 @@ class CachedBlock:
         return {"qkv": ((heads + 2 * kv_heads) * D, C), "out": (C, heads * D), "fc1": (hidden, C), "fc2": (C, hidden)}
 
     def __init__(self, dev, weights: dict, vectors: dict, C: int, heads: int, kv_heads: int, D: int, hidden: int,
-                 sections, inv_freq, window: int = 0, sinks: int = 0):
+                 sections, inv_freq, window: int = 0, sinks: int = 0, unrounded_rows: int = b2q.MUL_VEC_MAX_M):
         """weights: GGUF Q4_0 rows (uint8 numpy [out, row bytes]); vectors: fp32 device tensors
-        b_qkv, b_out, b1, b2 and the RMS gammas gq [heads * D], gk [kv_heads * D]."""
+        b_qkv, b_out, b1, b2 and the RMS gammas gq [heads * D], gk [kv_heads * D].  Steps of up to
+        unrounded_rows tokens keep the activations of the linears as they are, more round them to Q8_0."""
         import torch
+        self.unrounded_rows = unrounded_rows
         self.C, self.H, self.Hk, self.D, self.hidden = C, heads, kv_heads, D, hidden
         self.sections, self.inv_freq, self.window, self.sinks = tuple(sections), inv_freq, window, sinks
         self.shape = self.shapes(C, heads, kv_heads, D, hidden)
@@ -96,8 +101,16 @@ class CachedBlock:
     def _linear(self, name: str, x, bias, resid=None):
         n, k = self.shape[name]
         m = x.shape[0]
-        if m <= b2q.MUL_VEC_MAX_M:
+        if m <= min(self.unrounded_rows, b2q.MUL_VEC_MAX_M):
             return b2q.mul_vec(b2q.TYPE_Q4_0, self.packed[name], n, k, x, bias=bias, resid=resid, out=resid)
+        if m <= self.unrounded_rows:
+            import torch
+            y = resid if resid is not None else torch.empty((m, n), dtype=torch.float32, device=x.device)
+            for i in range(0, m, b2q.MUL_VEC_MAX_M):
+                part = slice(i, i + b2q.MUL_VEC_MAX_M)
+                b2q.mul_vec(b2q.TYPE_Q4_0, self.packed[name], n, k, x[part], bias=bias,
+                            resid=None if resid is None else resid[part], out=y[part])
+            return y
         act = b2q.act_prepare(x.float())
         return b2q.mul_mat_prepared_q4_0(self.packed[name], n, k, act, m, bias=bias, resid=resid, out=resid)
 

@@ -258,3 +258,17 @@ def test_released_pages_serve_other_requests(dev):
         with pytest.raises(RuntimeError):
             cache.plan([1, 0, 0])
         assert sorted(cache.table[cache.table >= 0].tolist()) == list(range(9))
+
+
+@pytest.mark.parametrize("requests", [9, 17])
+def test_larger_batches_can_keep_their_activations(dev, requests):
+    """Steps of more tokens than one product takes, with the accuracy of few: the bound for steps of at most eight."""
+    C, heads, D, hidden = 256, 4, 64, 512
+    block, weights = cb.random_block(dev, C, heads, heads, D, hidden, (12, 10, 10), seed=8, unrounded_rows=20)
+    cache = cb.PagedCache(dev, 1, requests, heads, D, pages=requests, page_size=16, max_len=16)
+    xs = torch.randn(3, requests, C, generator=torch.Generator(device=dev).manual_seed(9), device=dev)
+    for t in range(3):
+        step = cache.plan([1] * requests)
+        y = block.forward(xs[t].clone(), cache, 0, step, coords(step["pos"]))
+    ref = torch.stack([reference(block, weights, xs[:, b].double(), coords(torch.arange(3, device=dev)))[-1] for b in range(requests)])
+    assert float((y.double() - ref).norm() / (ref - xs[2].double()).norm()) <= 4e-3

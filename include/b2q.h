@@ -596,10 +596,14 @@ B2Q_API int b2q_qkv_rope_cache(const float* qkv, int64_t T, int64_t Hq, int64_t 
  * its page, j <= p (causal = 1) and, when window > 0 (causal only), j > p -
  * window or j < sinks.  Query head h reads kv head h / (Hq / Hkv).
  *   o[t][h*D + d] = sum_j softmax_j(scale * q . k_j) v_j
- * Scores, maxima and sums in fp32; a row that sees no key is 0; what keys that
- * a row does not see hold (infinities, NaN) does not reach it; an infinite value
- * of a key that it sees is its output (NaN with a NaN or infinities of both
- * signs; such rows cost another look at their keys).  Rows of o past
+ * Scores, maxima and sums in fp32.  The weights enter the product with v as two
+ * numbers of `type` (the weight and what rounding it left) up to 32 rows (tokens x
+ * Hq / Hkv) and for some more over few keys; beyond, rounded once, which is as
+ * large an error as the output's own rounding.  A row that sees no key, or no
+ * score above -infinity, is 0; what keys that a row does not see hold
+ * (infinities, NaN) does not reach it; an infinite value of a key that it sees
+ * is its output (NaN with a NaN or infinities of both signs; such rows cost
+ * another look at their keys).  Rows of o past
  * cu_new[B] are not written.  max_new and max_kv bound the requests' new tokens
  * and lengths on the host (tokens past max_new are not computed; longer lengths
  * are, only slower); nothing is read back.  q, o 16-byte aligned with strides

@@ -23,16 +23,17 @@
 // page (pages are multiples of 16), keys that no row of the CTA sees are not loaded
 // but filled with zeros.  Products are m16n8k16; P is fed to the second product as
 // two 16-bit numbers, P and what rounding it left: the tensor pipe idles behind the
-// loads, and a single rounding of P would cost as much accuracy as the output's own.
+// loads, and a single rounding of P would cost as much accuracy as the output's own (two
+// bf16 numbers hold P to 2^-17 of it, two fp16 ones to 2^-22).
 // Before the first products stand three loads that need one another (lengths, page,
 // keys), so the pages of a whole ring are asked for at once, ahead of q: with one
 // after the other, and 64-bit row numbers, a CTA took 7 us to its first unit, now 4.5.
 // Stretches are split over CTAs when the rows alone do not fill the GPU; a
 // second kernel, or the cluster that they form, then joins their outputs by their
 // maxima and sums.
-// Measured (32 / 8 heads of 128): 64 requests of 0.9k to 24k keys 475 us,
-// 6850 GB/s; one of 120k keys 81 us, 6080 GB/s; 16 requests, 24 / 4 heads, a window of
-// 4096 keys, 1 to 5 tokens 35.5 us, 3800 GB/s; 3 requests of 16 heads of 64
+// Measured (32 / 8 heads of 128): 64 requests of 0.9k to 24k keys 476 us,
+// 6850 GB/s; one of 120k keys 81 us, 6040 GB/s; 16 requests, 24 / 4 heads, a window of
+// 4096 keys, 1 to 5 tokens 35.0 us, 3850 GB/s; 3 requests of 16 heads of 64
 // over at most 900 keys 6.1 us, a launch and one CTA's chain of units.
 #include "b2q_internal.h"
 #include "b2q_paged.cuh"

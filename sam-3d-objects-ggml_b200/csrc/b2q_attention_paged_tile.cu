@@ -24,7 +24,8 @@
 // trip through the tensor pipe.  With tiles of 128 keys there is room for one S a
 // query tile only: S, softmax and P V then follow one another (1027 us).
 // Measured on two chunks of 3.9k tokens over 4k and 7.5k cached, 32 / 8 heads of
-// 128: 993 us, 1010 TFLOP/s, the tensor pipe active half of the time; the
+// 128: 985 us, 1020 TFLOP/s (1130 us at the clock that the power cap leaves in steady
+// calls), the tensor pipe active half of the time; the
 // softmax warps' own chain (loads from tensor memory, maximum, exps, stores) is
 // what a tile waits for.
 //

@@ -14,8 +14,8 @@
 // the CTAs share out the table rows (one warp a row) and the tokens (four
 // consecutive ones per thread, one search in the scanned offsets).  The work is
 // 12 bytes a token and 4 a table entry, all written once; bound by its latency
-// (the launch, two scans, one pass of writes): 5.8 us for 48 requests of one
-// token, 11.9 us for 1000 requests of 750k tokens in all, where the bytes are 1.5 us.
+// (the launch, two scans, one pass of writes): 5.3 us for 48 requests of one
+// token, 11.5 us for 1000 requests of 750k tokens in all, where the bytes are 1.5 us.
 #include "b2q_internal.h"
 
 namespace b2q {

@@ -32,10 +32,11 @@
 //     sums of the highest digit (|sum| < 2^22) are read as fp32 through an
 //     accumulator that starts at the bits of 1.5 * 2^23
 // Three or four products of the first kind instead, for 5 to 8 tokens, of a
-// 49152 x 8192 weight: 157 us against 125 (8 tokens, Q4_K), 111 against 111 (6).
-// Measured: that weight in Q4_K, one token: 50 us, 4500 GB/s, bound by the issue
-// of 2.5 lane instructions a value; 8192 x 4096 Q4_0, 4 tokens: 11.8 us, digits,
-// units and a launch in equal parts; 6144 x 1024 Q4_0, one token: 4.6 us, a launch
+// 49152 x 8192 weight, in steady calls: 157 us against 125 (8 tokens, Q4_K), 111 against 111 (6).
+// Measured: that weight in Q4_K, one token: 49 us, 4620 GB/s, 2.5 lane instructions
+// a value in 64% of the issue slots; 4 tokens 75 us, 8 tokens 112 us, each token's sums
+// to scale and add; 8192 x 4096 Q4_0, 4 tokens: 11.9 us, digits,
+// units and a launch in equal parts; 6144 x 1024 Q4_0, one token: 4.5 us, a launch
 // and one CTA's chain (the weight's bytes are 0.6 us).
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"

@@ -16,7 +16,7 @@
 // works on these.  q and k rows and v rows are two loops, and the kinds of rotation
 // and norm are template arguments: with one loop of 4-value lanes the rows cost 136
 // instructions a warp, and 32800 tokens of 48 heads of 64 took 200 us where this
-// takes 101 (5970 GB/s).  With pairs (i, i + R) and 40 heads of 128: 160 us, 6290
+// takes 102 (5950 GB/s).  With pairs (i, i + R) and 40 heads of 128: 160 us, 6290
 // GB/s, and 207 when the partners came by shuffles.  24 tokens of 40 heads of 128:
 // 3.2 us, a launch and one round of loads and stores.
 //

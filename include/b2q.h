@@ -45,7 +45,7 @@ extern "C" {
 #endif
 
 enum b2q_type { B2Q_TYPE_F32 = 0, B2Q_TYPE_F16 = 1, B2Q_TYPE_Q4_0 = 2, B2Q_TYPE_Q8_0 = 8, B2Q_TYPE_Q4_K = 12,
-                B2Q_TYPE_BF16 = 30 };  /* BF16: the cached-decoding entries only */
+                B2Q_TYPE_BF16 = 30 };  /* BF16: the cached-decoding entries and those below them */
 
 /* Activation-quantizer variant (fp32 -> Q8_0 rounding).
  *   B2Q_ACT_X86: the from_float of ggml's CPU backend on x86 (the host the
@@ -634,6 +634,95 @@ B2Q_API int b2q_attention_paged(int type, const void* q, int64_t q_row_stride_by
 B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, const void* x, int64_t m,
                         int64_t x_row_stride_bytes, const float* bias, const float* gate, const float* resid,
                         int64_t resid_row_stride_bytes, float* y, int64_t y_row_stride_bytes, void* stream);
+
+/* ------------------------------------------------------ rows that go by group
+ * Linears whose weight is chosen row by row: the experts of a mixture layer, and
+ * adapters that the requests of a batch bring along.  In ggml terms these take
+ * the place of ARGSORT / GET_ROWS of the router's scores, MUL_MAT_ID, the
+ * weighted sum behind it, and the two MUL_MATs of an adapter beside a linear; no
+ * counterpart in the reference, whose layers have one weight each.
+ *
+ * A slot is one row of such a product: (token, choice) pairs, token after token,
+ * for experts; tokens for adapters.  A plan of S slots over G groups (at most
+ * 1024; S at most 2^30):
+ *   offsets int32 [G + 1]  group g owns the sorted slots offsets[g] .. offsets[g + 1] - 1
+ *   order   int32 [S]      the slots by group, in slot order inside one; those of no group last
+ * Plans that the calls below did not make are clamped to their buffers, never
+ * trusted.  All results are the same from call to call: no atomics on floats.
+ *
+ * b2q_moe_route: logits [T][E] of type F32, F16 or BF16.  Each token's choices
+ * are its `top` largest of logit + bias (bias fp32 [E] or NULL; the sum in
+ * fp32), largest first, ties to the lower expert; -infinity and NaN are never
+ * chosen.  ids int32 [T][top] (-1 where nothing was left to choose), weights
+ * fp32 [T][top]: softmax over the E logits (NaN left out) or sigmoid of the
+ * chosen ones, divided by their sum if renorm (0 where that is 0), times scale;
+ * 0 for id -1.  order [T * top] and offsets [E + 1] are the plan of the slots
+ * token * top + choice.  top at most 32.  Workspace (4-byte aligned) of
+ * b2q_moe_route_workspace_bytes; 0 for a few tokens, which take one launch.
+ *
+ * b2q_group_rows: the plan of slots whose groups are given: ids int32 [S], any
+ * number outside 0 .. G - 1 is none.
+ *
+ * b2q_mul_mat_id: y[s][r] = sum_k w[e][r][k] x[s / per_row][k] (+ bias[e][r]) for
+ * every slot s of expert e, r < n; with glu = 1 the weight has 2 n rows and
+ *   y[s][r] = silu(z[r]) * z[n + r],  z the 2 n sums (bias included).
+ * Slots of no group get rows of 0.  wtype F16 or BF16: w [E][n or 2 n][k], rows
+ * and experts at the given strides (16-byte aligned, k % 8 == 0), x of the same
+ * type; wtype Q4_0: b2q_weight_pack_q4_0 of the E * (n or 2 n) rows one under
+ * another (strides ignored, k % 32 == 0), x F16 -- not rounded to 8 bits.  x has
+ * x_rows rows (at least ceil(slots / per_row)), 16-byte aligned.  ytype F32 or
+ * x's type.  fp32 sums.
+ *
+ * b2q_moe_combine: out[t] = resid[t] + sum_j weights[t][j] y[t * top + j], in
+ * fp32, choices in order; rows whose ids[t][j] is negative are not read (ids may
+ * be NULL).  resid is of out's type, NULL for none, and may be out.
+ *
+ * b2q_lora_add: y[t] = resid[t] + scales[g] * b[g] (a[g] x[t]), g the adapter
+ * that the plan gives row t; rows of no adapter: y[t] = resid[t].  a [G][rank][k]
+ * and b [G][n][rank] contiguous, of x's type (F16 or BF16; rank a multiple of 8,
+ * at most 128; k % 8 == 0), scales fp32 [G] or NULL for 1.  resid and y of type F32 or
+ * x's, the same buffer with the same stride, or disjoint.  The rank values
+ * between the two products are kept to more than 16 bits.
+ *
+ * b2q_draft_verify: which drafted tokens a target model keeps, from given random
+ * numbers.  Request b of B has the drafts cu_drafts[b] .. cu_drafts[b+1] - 1
+ * (int32 tokens; D in all) and one row more of target probabilities: row i + b
+ * of target [D + B][V] is what the target says of draft i, the row behind a
+ * request's last draft what follows it.  draft_probs [D][V] is what the draft
+ * model said (NULL: it named its token with probability 1).  Types F32, F16 or
+ * BF16.  Draft i stays while u[i] * draft_probs[i][token] < target[i + b][token];
+ * the first that does not is replaced by a draw from max(target - draft_probs, 0)
+ * of its row (from target where that is 0 everywhere), and when all stay, a draw
+ * from the last row follows.  A draw takes the first token at which the running
+ * sum passes v[b] times the sum (64-bit sums; rows need not add up to 1; NaN,
+ * infinities and negative values count as 0; -1 when nothing is left).
+ * accepted int32 [B]: drafts that stay; tokens int32 [D + B], laid out as
+ * target's rows: those drafts, the drawn token, -1 after it.  Tokens outside
+ * 0 .. V - 1 are turned down. */
+enum b2q_scoring { B2Q_SCORE_SOFTMAX = 0, B2Q_SCORE_SIGMOID = 1 };
+B2Q_API size_t b2q_moe_route_workspace_bytes(int64_t T, int64_t E, int64_t top);
+B2Q_API int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t row_stride_bytes,
+                          const float* bias, int64_t top, int scoring, int renorm, float scale, int32_t* ids,
+                          float* weights, int32_t* order, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                          void* stream);
+B2Q_API size_t b2q_group_rows_workspace_bytes(int64_t S, int64_t groups);
+B2Q_API int b2q_group_rows(const int32_t* ids, int64_t S, int64_t groups, int32_t* order, int32_t* offsets,
+                           void* workspace, size_t workspace_bytes, void* stream);
+B2Q_API int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t k, int64_t w_row_stride_bytes,
+                           int64_t w_expert_stride_bytes, const void* x, int64_t x_rows, int64_t x_row_stride_bytes,
+                           const int32_t* order, const int32_t* offsets, int64_t slots, int64_t per_row,
+                           const float* bias, int glu, int ytype, void* y, int64_t y_row_stride_bytes, void* stream);
+B2Q_API int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const float* weights,
+                            const int32_t* ids, int64_t T, int64_t top, int64_t n, int otype, const void* resid,
+                            int64_t resid_row_stride_bytes, void* out, int64_t out_row_stride_bytes, void* stream);
+B2Q_API int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
+                         const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales,
+                         const int32_t* order, const int32_t* offsets, int ytype, const void* resid,
+                         int64_t resid_row_stride_bytes, void* y, int64_t y_row_stride_bytes, void* stream);
+B2Q_API int b2q_draft_verify(int type, const void* target, int64_t target_row_stride_bytes, const void* draft_probs,
+                             int64_t draft_row_stride_bytes, const int32_t* drafts, const int32_t* cu_drafts,
+                             int64_t B, int64_t D, int64_t V, const float* u, const float* v, int32_t* accepted,
+                             int32_t* tokens, void* stream);
 
 /* Fault-free test of the failure path: launches the GEMM of
  * b2q_mul_mat_prepared with its TMA producer withholding every stage, so the

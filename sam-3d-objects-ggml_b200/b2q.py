@@ -121,6 +121,14 @@ def _lib_obj():
             "b2q_attention_paged": (I, [I, P, I64, P, I64, I64, I64, P, P, I64, I64, P, I64, I64, P, I64, I64, I64,
                                         I64, ctypes.c_float, I, I64, I64, P, I64, P, SZ, P]),
             "b2q_mul_vec": (I, [I, P, I64, I64, I, P, I64, I64, P, P, P, I64, P, I64, P]),
+            "b2q_moe_route_workspace_bytes": (SZ, [I64, I64, I64]),
+            "b2q_moe_route": (I, [I, P, I64, I64, I64, P, I64, I, I, ctypes.c_float, P, P, P, P, P, SZ, P]),
+            "b2q_group_rows_workspace_bytes": (SZ, [I64, I64]),
+            "b2q_group_rows": (I, [P, I64, I64, P, P, P, SZ, P]),
+            "b2q_mul_mat_id": (I, [I, P, I64, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, I, I, P, I64, P]),
+            "b2q_moe_combine": (I, [I, P, I64, P, P, I64, I64, I64, I, P, I64, P, I64, P]),
+            "b2q_lora_add": (I, [I, P, I64, I64, I64, P, P, I64, I64, I64, P, P, P, I, P, I64, P, I64, P]),
+            "b2q_draft_verify": (I, [I, P, I64, P, I64, P, P, I64, I64, I64, P, P, P, P, P]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -952,6 +960,188 @@ def mul_vec(wtype: int, packed, n: int, k: int, x, bias=None, gate=None, resid=N
     if rc:
         _check("b2q_mul_vec", rc)
     return out
+
+
+def _val_type(dtype):
+    """(B2Q_TYPE, bytes) of fp32, fp16 or bf16."""
+    torch = _torch()
+    if dtype is torch.float32:
+        return TYPE_F32, 4
+    return _type16(dtype), 2
+
+
+def _is_list(t, n: int, dtype) -> bool:
+    """t is n values of that type one after another."""
+    return t.dtype is dtype and t.numel() == n and t.is_contiguous()
+
+
+_route_ws_bytes = functools.lru_cache(maxsize=256)(lambda T, E, top: lib().b2q_moe_route_workspace_bytes(T, E, top))
+_group_ws_bytes = functools.lru_cache(maxsize=256)(lambda S, groups: lib().b2q_group_rows_workspace_bytes(S, groups))
+SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_route(logits, top: int, bias=None, scoring: str = "softmax", renorm: bool = True, scale: float = 1.0,
+              stream=None):
+    """The router of an expert layer, logits [T, E] (fp32, fp16 or bf16) -> (ids int32 [T, top], weights fp32
+    [T, top], order int32 [T * top], offsets int32 [E + 1]): every token's `top` largest of logit + bias (ties
+    to the lower expert, -infinity and NaN never; -1 where none is left), their softmax or sigmoid weights,
+    and the plan of the slots token * top + choice by expert."""
+    torch = _torch()
+    T, E = logits.shape
+    ld, ldc = logits.stride()
+    dtype, size = _val_type(logits.dtype)
+    assert (ldc == 1 or E <= 1 or T == 0) and (ld >= E or T <= 1) and 0 < top <= E
+    if bias is not None:
+        assert _are_floats(bias, E, torch.float32)
+    dev, S = logits.device, T * top
+    need = _route_ws_bytes(T, E, top)
+    ids, order, offsets, ws = _empty_on(stream, 2 * S + E + 1 + need // 4, torch.int32, dev).split((S, S, E + 1, need // 4))
+    weights = _empty_on(stream, (T, top), torch.float32, dev)
+    rc = (_lib or _lib_obj()).b2q_moe_route(
+        dtype, logits.data_ptr(), T, E, size * (ld if ld > E else E), _ptr(bias), top, SCORING[scoring],
+        1 if renorm else 0, scale, ids.data_ptr(), weights.data_ptr(), order.data_ptr(), offsets.data_ptr(),
+        ws.data_ptr() if need else None, need, _raw_stream(stream, logits, bias))
+    if rc:
+        _check("b2q_moe_route", rc)
+    return ids.view(T, top), weights, order, offsets
+
+
+def group_rows(ids, groups: int, stream=None):
+    """(order int32 [S], offsets int32 [groups + 1]): the plan of the slots whose groups are ids (int32, any
+    shape; -1 for none)."""
+    torch = _torch()
+    S = ids.numel()
+    assert ids.dtype is torch.int32 and ids.is_contiguous()
+    need = _group_ws_bytes(S, groups)
+    order, offsets, ws = _empty_on(stream, S + groups + 1 + need // 4, torch.int32, ids.device).split(
+        (S, groups + 1, need // 4))
+    rc = (_lib or _lib_obj()).b2q_group_rows(ids.data_ptr(), S, groups, order.data_ptr(), offsets.data_ptr(),
+                                             ws.data_ptr() if need else None, need, _raw_stream(stream, ids))
+    if rc:
+        _check("b2q_group_rows", rc)
+    return order, offsets
+
+
+def mul_mat_id(wtype: int, w, n: int, k: int, x, order, offsets, per_row: int = 1, bias=None, glu: bool = False,
+               out_dtype=None, out=None, stream=None):
+    """Row x[s // per_row] times the weight of slot s's expert, for every slot of the plan -> [slots, n] of x's
+    type (or fp32); with glu the weight has 2 n rows and the result is silu(first n) * last n.  w: [E, n or
+    2 n, k] of x's type (TYPE_F16, TYPE_BF16), or weight_pack_q4_0 of all experts' rows (TYPE_Q4_0, x fp16).
+    Slots without an expert give rows of 0."""
+    torch = _torch()
+    E, S = offsets.numel() - 1, order.numel()
+    x_rows, width = x.shape
+    ldx, ldxc = x.stride()
+    dt, rows = x.dtype, 2 * n if glu else n
+    assert width == k and (ldxc == 1 or x_rows == 0) and (ldx >= k or x_rows <= 1)
+    assert _is_list(order, S, torch.int32) and _is_list(offsets, E + 1, torch.int32)
+    ldw = lde = 0
+    if wtype == TYPE_Q4_0:
+        assert dt is torch.float16 and w.is_contiguous() and w.numel() * w.element_size() >= _packed4_bytes(wtype, E * rows, k)
+    else:
+        assert _type16(dt) == wtype and w.dtype is dt and w.shape == (E, rows, k)
+        lde, ldw, ldwc = w.stride()
+        assert ldwc == 1 and ldw >= k
+    if bias is not None:
+        assert _are_floats(bias, E * rows, torch.float32)
+    if out is None:
+        out = _empty_on(stream, (S, n), out_dtype or dt, x.device)
+    else:
+        assert _are_rows(out, S, n, out_dtype or out.dtype)
+    ytype, ysize = _val_type(out.dtype)
+    rc = (_lib or _lib_obj()).b2q_mul_mat_id(
+        wtype, w.data_ptr(), E, n, k, ldw * 2, lde * 2, x.data_ptr(), x_rows, 2 * (ldx if ldx > k else k),
+        order.data_ptr(), offsets.data_ptr(), S, per_row, _ptr(bias), 1 if glu else 0, ytype, out.data_ptr(),
+        ysize * max(out.stride(0), n), _raw_stream(stream, x, w, order, offsets, bias, out))
+    if rc:
+        _check("b2q_mul_mat_id", rc)
+    return out
+
+
+def moe_combine(y, weights, ids=None, resid=None, out_dtype=None, out=None, stream=None):
+    """[T, n]: resid + every token's weighted sum of its slots' rows y [T * top, n]; weights fp32 [T, top], rows
+    whose ids (int32 [T, top]) are negative left out.  Of resid's type, or y's without one, or out_dtype
+    (out=resid updates in place)."""
+    torch = _torch()
+    T, top = weights.shape
+    S, n = y.shape
+    assert S == T * top and _is_list(weights, S, torch.float32) and (ids is None or _is_list(ids, S, torch.int32))
+    assert _are_rows(y, S, n, y.dtype) and (y.stride(0) >= n or S <= 1)
+    if out is None:
+        out = _empty_on(stream, (T, n), out_dtype or (resid if resid is not None else y).dtype, y.device)
+    else:
+        assert _are_rows(out, T, n, out_dtype or out.dtype) and (out.stride(0) >= n or T <= 1)
+    if resid is not None:
+        assert resid is out or (_are_rows(resid, T, n, out.dtype) and resid.shape == (T, n))
+    (yt, ys), (ot, os_) = _val_type(y.dtype), _val_type(out.dtype)
+    rc = (_lib or _lib_obj()).b2q_moe_combine(
+        yt, y.data_ptr(), ys * max(y.stride(0), n), weights.data_ptr(), _ptr(ids), T, top, n, ot, _ptr(resid),
+        0 if resid is None else os_ * max(resid.stride(0), n), out.data_ptr(), os_ * max(out.stride(0), n),
+        _raw_stream(stream, y, weights, ids, resid, out))
+    if rc:
+        _check("b2q_moe_combine", rc)
+    return out
+
+
+LORA_MAX_RANK = 128
+
+
+def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
+    """resid + scales[g] * (x . a[g]^T) . b[g]^T row by row, g the adapter that the plan (group_rows of the rows'
+    adapters) gives the row; rows without one stay as they are.  resid [T, n] fp32 or of x's type, x [T, k]
+    fp16 or bf16, a [G, rank, k] and b [G, n, rank] of x's type, scales fp32 [G] or None
+    (out=resid updates in place)."""
+    torch = _torch()
+    T, k = x.shape
+    G, rank, ka = a.shape
+    n = resid.shape[1]
+    dt = x.dtype
+    ldx, ldxc = x.stride()
+    assert ka == k and a.dtype is dt and b.dtype is dt and b.shape == (G, n, rank)
+    assert a.is_contiguous() and b.is_contiguous() and (ldxc == 1 or T == 0) and (ldx >= k or T <= 1)
+    assert resid.shape[0] == T and _are_rows(resid, T, n, resid.dtype) and (resid.stride(0) >= n or T <= 1)
+    assert _is_list(order, T, torch.int32) and _is_list(offsets, G + 1, torch.int32)
+    if scales is not None:
+        assert _are_floats(scales, G, torch.float32)
+    if out is None:
+        out = _empty_on(stream, (T, n), resid.dtype, x.device)
+    else:
+        assert _are_rows(out, T, n, resid.dtype) and (out.stride(0) >= n or T <= 1)
+    ytype, ys = _val_type(resid.dtype)
+    rc = (_lib or _lib_obj()).b2q_lora_add(
+        _type16(dt), x.data_ptr(), T, k, 2 * (ldx if ldx > k else k), a.data_ptr(), b.data_ptr(), G, rank, n,
+        _ptr(scales), order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * max(resid.stride(0), n),
+        out.data_ptr(), ys * max(out.stride(0), n), _raw_stream(stream, x, a, b, scales, order, offsets, resid, out))
+    if rc:
+        _check("b2q_lora_add", rc)
+    return out
+
+
+def draft_verify(target, draft_probs, drafts, cu_drafts, u, v, stream=None):
+    """Which drafted tokens (int32 [D], request b's at cu_drafts[b] .. cu_drafts[b + 1]) stay, and the token after
+    them -> (accepted int32 [B], tokens int32 [D + B]: request b's kept drafts and its drawn token from
+    cu_drafts[b] + b on, -1 behind).  target [D + B, V] in that layout too, draft_probs [D, V] or None;
+    uniform numbers u fp32 [D] for the drafts and v fp32 [B] for the draws."""
+    torch = _torch()
+    i32, f32 = torch.int32, torch.float32
+    rows, V = target.shape
+    B, D = cu_drafts.numel() - 1, drafts.numel()
+    ldp, ldpc = target.stride()
+    dtype, size = _val_type(target.dtype)
+    assert rows == D + B and (ldpc == 1 or V <= 1 or rows == 0) and (ldp >= V or rows <= 1)
+    ldq = 0
+    if draft_probs is not None:
+        ldq = draft_probs.stride(0)
+        assert draft_probs.shape == (D, V) and _are_rows(draft_probs, D, V, target.dtype) and (ldq >= V or D <= 1)
+    assert _is_list(drafts, D, i32) and _is_list(cu_drafts, B + 1, i32) and _is_list(u, D, f32) and _is_list(v, B, f32)
+    accepted, tokens = _empty_on(stream, 2 * B + D, i32, target.device).split((B, B + D))
+    rc = (_lib or _lib_obj()).b2q_draft_verify(
+        dtype, target.data_ptr(), size * max(ldp, V), _ptr(draft_probs), size * max(ldq, V), drafts.data_ptr(),
+        cu_drafts.data_ptr(), B, D, V, u.data_ptr(), v.data_ptr(), accepted.data_ptr(), tokens.data_ptr(),
+        _raw_stream(stream, target, draft_probs, drafts, cu_drafts, u, v))
+    if rc:
+        _check("b2q_draft_verify", rc)
+    return accepted, tokens
 
 
 def device_status(clear: bool = True) -> int:

@@ -1384,4 +1384,255 @@ int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int xtype, 
   return from_cuda(launch_mul_vec(a, q4k, xt, sms, static_cast<cudaStream_t>(stream)));
 }
 
+// ------------------------------------------- rows that go by group, drafted tokens
+
+// kXF32 / kXF16 / kXBF16 of a B2Q_TYPE, -1 for others; and bytes of a value.
+static int val_type(int type) {
+  return type == B2Q_TYPE_F32 ? kXF32 : type == B2Q_TYPE_F16 ? kXF16 : type == B2Q_TYPE_BF16 ? kXBF16 : -1;
+}
+static int val_size(int vt) { return vt == kXF32 ? 4 : 2; }
+
+// The slots of a plan are numbered with 32 bits.
+constexpr int64_t kMaxSlots = 1 << 30;
+
+static int route_sizes(int64_t T, int64_t E, int64_t top) {
+  if (T < 0 || E <= 0 || top <= 0 || top > E) return B2Q_ERR_INVALID_ARG;
+  if (E > kMaxGroups || top > kRouteMaxTop || T > kMaxSlots / top) return B2Q_ERR_TOO_LARGE;
+  return B2Q_OK;
+}
+static size_t run_bytes(const RunPlan& p, int64_t groups) {
+  return p.runs > 1 ? static_cast<size_t>(p.runs) * (groups + 1) * 4 : 0;
+}
+
+size_t b2q_moe_route_workspace_bytes(int64_t T, int64_t E, int64_t top) {
+  return route_sizes(T, E, top) == B2Q_OK ? run_bytes(run_plan(T, static_cast<int>(top)), E) : 0;
+}
+
+int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t row_stride_bytes, const float* bias,
+                  int64_t top, int scoring, int renorm, float scale, int32_t* ids, float* weights, int32_t* order,
+                  int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream) {
+  const int vt = val_type(type);
+  if (vt < 0) return B2Q_ERR_UNSUPPORTED;
+  if (int rc = route_sizes(T, E, top)) return rc;
+  const int size = val_size(vt);
+  if ((scoring != B2Q_SCORE_SOFTMAX && scoring != B2Q_SCORE_SIGMOID) || (renorm != 0 && renorm != 1) ||
+      !std::isfinite(scale) || !offsets || (T > 0 && (!logits || !ids || !weights || !order)) ||
+      row_stride_bytes < E * size)
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(logits, size) || row_stride_bytes % size != 0 || !aligned(bias, 4) || !aligned(ids, 4) ||
+      !aligned(weights, 4) || !aligned(order, 4) || !aligned(offsets, 4) || !aligned(workspace, 4))
+    return B2Q_ERR_MISALIGNED;
+  const size_t need = run_bytes(run_plan(T, static_cast<int>(top)), E);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
+  if (int rc = check_device(nullptr)) return rc;
+  RouteArgs a{};
+  a.logits = logits;
+  a.T = T;
+  a.ld = row_stride_bytes / size;
+  a.E = static_cast<int>(E);
+  a.top = static_cast<int>(top);
+  a.bias = bias;
+  a.scoring = scoring;
+  a.renorm = renorm;
+  a.scale = scale;
+  a.ids = ids;
+  a.weights = weights;
+  a.order = order;
+  a.offsets = offsets;
+  a.run_counts = static_cast<int32_t*>(workspace);
+  return from_cuda(launch_route(a, vt, static_cast<cudaStream_t>(stream)));
+}
+
+static int group_sizes(int64_t S, int64_t groups) {
+  if (S < 0 || groups <= 0) return B2Q_ERR_INVALID_ARG;
+  if (S > kMaxSlots || groups > kMaxGroups) return B2Q_ERR_TOO_LARGE;
+  return B2Q_OK;
+}
+
+size_t b2q_group_rows_workspace_bytes(int64_t S, int64_t groups) {
+  return group_sizes(S, groups) == B2Q_OK ? run_bytes(run_plan(S, 1), groups) : 0;
+}
+
+int b2q_group_rows(const int32_t* ids, int64_t S, int64_t groups, int32_t* order, int32_t* offsets, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  if (int rc = group_sizes(S, groups)) return rc;
+  if (!offsets || (S > 0 && (!ids || !order))) return B2Q_ERR_INVALID_ARG;
+  if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || !aligned(workspace, 4))
+    return B2Q_ERR_MISALIGNED;
+  const size_t need = run_bytes(run_plan(S, 1), groups);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
+  if (int rc = check_device(nullptr)) return rc;
+  return from_cuda(launch_group_rows(ids, S, static_cast<int>(groups), order, offsets,
+                                     static_cast<int32_t*>(workspace), static_cast<cudaStream_t>(stream)));
+}
+
+int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t k, int64_t w_row_stride_bytes,
+                   int64_t w_expert_stride_bytes, const void* x, int64_t x_rows, int64_t x_row_stride_bytes,
+                   const int32_t* order, const int32_t* offsets, int64_t slots, int64_t per_row, const float* bias,
+                   int glu, int ytype, void* y, int64_t y_row_stride_bytes, void* stream) {
+  const bool q4 = wtype == B2Q_TYPE_Q4_0;
+  if (!q4 && wtype != B2Q_TYPE_F16 && wtype != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
+  const int xtype = wtype == B2Q_TYPE_BF16 ? B2Q_TYPE_BF16 : B2Q_TYPE_F16;
+  if (ytype != B2Q_TYPE_F32 && ytype != xtype) return B2Q_ERR_UNSUPPORTED;
+  const int ysize = ytype == B2Q_TYPE_F32 ? 4 : 2;
+  if (experts <= 0 || n < 0 || k <= 0 || k % (q4 ? kQK : 8) != 0 || x_rows < 0 || slots < 0 || per_row <= 0 ||
+      (glu != 0 && glu != 1))
+    return B2Q_ERR_INVALID_ARG;
+  const int64_t rows = glu ? 2 * n : n;
+  if (experts > kMaxGroups || n > (INT_MAX >> 1) || rows * experts > INT_MAX || k > (1 << 28) || x_rows > INT_MAX ||
+      slots > kMaxSlots || per_row > kMaxSlots)
+    return B2Q_ERR_TOO_LARGE;
+  if (x_rows < (slots + per_row - 1) / per_row) return B2Q_ERR_INVALID_ARG;
+  const bool any = slots > 0 && n > 0;
+  if (any && (!w || !x || !order || !offsets || !y)) return B2Q_ERR_INVALID_ARG;
+  if ((!q4 && (w_row_stride_bytes < k * 2 || (experts > 1 && w_expert_stride_bytes < 0))) || x_row_stride_bytes < k * 2 ||
+      y_row_stride_bytes < n * ysize)
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(w, q4 ? 256 : 16) || (!q4 && (w_row_stride_bytes % 16 != 0 || w_expert_stride_bytes % 16 != 0)) ||
+      !aligned(x, 16) || x_row_stride_bytes % 16 != 0 || !aligned(order, 4) || !aligned(offsets, 4) ||
+      !aligned(bias, 4) || !aligned(y, ysize) || y_row_stride_bytes % ysize != 0)
+    return B2Q_ERR_MISALIGNED;
+  if (!any) return B2Q_OK;
+  if (int rc = check_device(nullptr)) return rc;
+  MulMatIdArgs a{};
+  if (q4) {
+    const Q4cWeight c = q4c_at(static_cast<const uint8_t*>(w), experts * rows, k);
+    a.w = c.nibbles;
+    a.scales = c.scales;
+    a.lds = c.ld;
+  } else {
+    a.w = w;
+    a.ldw = w_row_stride_bytes / 2;
+    a.expert_stride = w_expert_stride_bytes / 2;
+  }
+  a.E = static_cast<int>(experts);
+  a.rows = rows;
+  a.n = n;
+  a.K = k;
+  a.x = x;
+  a.ldx = x_row_stride_bytes / 2;
+  a.x_rows = x_rows;
+  a.order = order;
+  a.offsets = offsets;
+  a.S = slots;
+  a.per_row = static_cast<int>(per_row);
+  a.bias = bias;
+  a.glu = glu;
+  a.y = y;
+  a.ldy = y_row_stride_bytes / ysize;
+  return from_cuda(launch_mul_mat_id(a, q4 ? kWQ4 : val_type(wtype), val_type(xtype), val_type(ytype),
+                                     static_cast<cudaStream_t>(stream)));
+}
+
+int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const float* weights, const int32_t* ids,
+                    int64_t T, int64_t top, int64_t n, int otype, const void* resid, int64_t resid_row_stride_bytes,
+                    void* out, int64_t out_row_stride_bytes, void* stream) {
+  const int yt = val_type(ytype), ot = val_type(otype);
+  if (yt < 0 || ot < 0) return B2Q_ERR_UNSUPPORTED;
+  if (T < 0 || top <= 0 || n < 0) return B2Q_ERR_INVALID_ARG;
+  if (top > kMaxSlots || T > kMaxSlots / top || n > INT_MAX) return B2Q_ERR_TOO_LARGE;
+  const bool any = T > 0 && n > 0;
+  const int ys = val_size(yt), os = val_size(ot);
+  if ((any && (!y || !weights || !out)) || y_row_stride_bytes < n * ys || out_row_stride_bytes < n * os ||
+      (resid && resid_row_stride_bytes < n * os) ||
+      (resid && resid == out && resid_row_stride_bytes != out_row_stride_bytes))
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(y, ys) || y_row_stride_bytes % ys != 0 || !aligned(weights, 4) || !aligned(ids, 4) ||
+      !aligned(out, os) || out_row_stride_bytes % os != 0 ||
+      (resid && (!aligned(resid, os) || resid_row_stride_bytes % os != 0)))
+    return B2Q_ERR_MISALIGNED;
+  if (!any) return B2Q_OK;
+  if (int rc = check_device(nullptr)) return rc;
+  CombineArgs a{};
+  a.y = y;
+  a.ldy = y_row_stride_bytes / ys;
+  a.T = T;
+  a.n = n;
+  a.top = static_cast<int>(top);
+  a.weights = weights;
+  a.ids = ids;
+  a.resid = resid;
+  a.ldr = resid ? resid_row_stride_bytes / os : 0;
+  a.out = out;
+  a.ldo = out_row_stride_bytes / os;
+  return from_cuda(launch_combine(a, yt, ot, static_cast<cudaStream_t>(stream)));
+}
+
+int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
+                 const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales, const int32_t* order,
+                 const int32_t* offsets, int ytype, const void* resid, int64_t resid_row_stride_bytes, void* y,
+                 int64_t y_row_stride_bytes, void* stream) {
+  if (xtype != B2Q_TYPE_F16 && xtype != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
+  if (ytype != B2Q_TYPE_F32 && ytype != xtype) return B2Q_ERR_UNSUPPORTED;
+  const int ys = ytype == B2Q_TYPE_F32 ? 4 : 2;
+  if (T < 0 || k <= 0 || k % 8 != 0 || adapters <= 0 || rank <= 0 || rank % 8 != 0 || n < 0) return B2Q_ERR_INVALID_ARG;
+  if (T > kMaxSlots || k > (1 << 28) || n > INT_MAX || adapters > kMaxGroups || rank > kLoraMaxRank)
+    return B2Q_ERR_TOO_LARGE;
+  const bool any = T > 0 && n > 0;
+  if (any && (!x || !a || !b || !order || !offsets || !resid || !y)) return B2Q_ERR_INVALID_ARG;
+  if (x_row_stride_bytes < k * 2 || y_row_stride_bytes < n * ys || resid_row_stride_bytes < n * ys ||
+      (resid == y && resid_row_stride_bytes != y_row_stride_bytes))
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(x, 16) || x_row_stride_bytes % 16 != 0 || !aligned(a, 16) || !aligned(b, 16) || !aligned(scales, 4) ||
+      !aligned(order, 4) || !aligned(offsets, 4) || !aligned(resid, ys) || resid_row_stride_bytes % ys != 0 ||
+      !aligned(y, ys) || y_row_stride_bytes % ys != 0)
+    return B2Q_ERR_MISALIGNED;
+  if (!any) return B2Q_OK;
+  int sms = 0;
+  if (int rc = check_device(&sms)) return rc;
+  LoraArgs p{};
+  p.x = x;
+  p.T = T;
+  p.K = k;
+  p.N = n;
+  p.ldx = x_row_stride_bytes / 2;
+  p.a = a;
+  p.b = b;
+  p.groups = static_cast<int>(adapters);
+  p.rank = static_cast<int>(rank);
+  p.scales = scales;
+  p.order = order;
+  p.offsets = offsets;
+  p.resid = resid;
+  p.ldr = resid_row_stride_bytes / ys;
+  p.y = y;
+  p.ldy = y_row_stride_bytes / ys;
+  return from_cuda(launch_lora(p, val_type(xtype), val_type(ytype), sms, static_cast<cudaStream_t>(stream)));
+}
+
+int b2q_draft_verify(int type, const void* target, int64_t target_row_stride_bytes, const void* draft_probs,
+                     int64_t draft_row_stride_bytes, const int32_t* drafts, const int32_t* cu_drafts, int64_t B,
+                     int64_t D, int64_t V, const float* u, const float* v, int32_t* accepted, int32_t* tokens,
+                     void* stream) {
+  const int vt = val_type(type);
+  if (vt < 0) return B2Q_ERR_UNSUPPORTED;
+  if (B < 0 || D < 0 || V <= 0) return B2Q_ERR_INVALID_ARG;
+  if (B > (1 << 20) || D > kMaxSlots || V > (1 << 28)) return B2Q_ERR_TOO_LARGE;
+  const int size = val_size(vt);
+  if ((B > 0 && (!target || !cu_drafts || !v || !accepted || !tokens)) || (B > 0 && D > 0 && (!drafts || !u)) ||
+      target_row_stride_bytes < V * size || (draft_probs && draft_row_stride_bytes < V * size))
+    return B2Q_ERR_INVALID_ARG;
+  if (!aligned(target, size) || target_row_stride_bytes % size != 0 ||
+      (draft_probs && (!aligned(draft_probs, size) || draft_row_stride_bytes % size != 0)) || !aligned(drafts, 4) ||
+      !aligned(cu_drafts, 4) || !aligned(u, 4) || !aligned(v, 4) || !aligned(accepted, 4) || !aligned(tokens, 4))
+    return B2Q_ERR_MISALIGNED;
+  if (B == 0) return B2Q_OK;
+  if (int rc = check_device(nullptr)) return rc;
+  VerifyArgs a{};
+  a.target = target;
+  a.guess = draft_probs;
+  a.drafts = drafts;
+  a.cu = cu_drafts;
+  a.ldp = target_row_stride_bytes / size;
+  a.ldq = draft_probs ? draft_row_stride_bytes / size : 0;
+  a.B = B;
+  a.D = D;
+  a.V = V;
+  a.u = u;
+  a.v = v;
+  a.accepted = accepted;
+  a.tokens = tokens;
+  return from_cuda(launch_verify(a, vt, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -1,0 +1,84 @@
+// b2q_groups.cuh -- what the kernels share whose rows are sorted by group (an
+// expert, an adapter): 16-bit values, and the tile of a group that a CTA works on.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace b2q {
+
+// Values of type kXF32 / kXF16 / kXBF16 as fp32, and back with one rounding.
+template <int T>
+struct Val;
+template <>
+struct Val<0> {
+  using type = float;
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ float to(float v) { return v; }
+};
+template <>
+struct Val<1> {
+  using type = __half;
+  static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ __half to(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Val<2> {
+  using type = __nv_bfloat16;
+  static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ __nv_bfloat16 to(float v) { return __float2bfloat16_rn(v); }
+};
+
+// The sorted slots of a group, from offsets that are not trusted: a stale or
+// broken plan must not lead outside the S slots.  Group `groups` is the slots
+// that have none, behind the last group's.
+__device__ __forceinline__ int group_begin(const int32_t* offsets, int g, int64_t S) {
+  return static_cast<int>(min(max(static_cast<int64_t>(__ldg(offsets + g)), int64_t{0}), S));
+}
+__device__ __forceinline__ int group_end(const int32_t* offsets, int g, int groups, int64_t S, int begin) {
+  if (g >= groups) return static_cast<int>(S);
+  return max(begin, group_begin(offsets, g + 1, S));
+}
+
+struct GroupTile {
+  int group;  // -1: no such tile
+  int begin, end;
+};
+
+// Tile number `tile` of all groups' tiles of at most `rows` sorted slots, group
+// after group, the slots of no group last.  All lanes of a warp call it.
+__device__ __forceinline__ GroupTile find_group_tile(const int32_t* offsets, int groups, int64_t S, int tile, int rows) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int g0 = 0; g0 <= groups; g0 += 32) {
+    const int g = g0 + lane;
+    int lo = 0, hi = 0;
+    if (g <= groups) {
+      lo = group_begin(offsets, g, S);
+      hi = group_end(offsets, g, groups, S, lo);
+    }
+    const int n = (hi - lo + rows - 1) / rows;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    const unsigned found = __ballot_sync(0xffffffffu, before + inc > tile);
+    if (found) {
+      const int src = __ffs(found) - 1;
+      const int first = __shfl_sync(0xffffffffu, before + inc - n, src);
+      GroupTile t;
+      t.group = g0 + src;
+      t.begin = __shfl_sync(0xffffffffu, lo, src) + (tile - first) * rows;
+      t.end = min(t.begin + rows, __shfl_sync(0xffffffffu, hi, src));
+      return t;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return {-1, 0, 0};
+}
+
+}  // namespace b2q

@@ -378,4 +378,88 @@ struct MulVecArgs {
 };
 cudaError_t launch_mul_vec(const MulVecArgs& a, bool q4k, int xt, int num_sms, cudaStream_t s);
 
+// ---- rows that go by group: router and plan, experts' products, adapters; drafted tokens ----
+constexpr int64_t kMaxGroups = 1024;  // experts or adapters of one plan (their counts are in shared memory)
+constexpr int64_t kRouteMaxTop = 32;  // choices of one token (one a lane)
+// The slots of a plan, cut into runs of one CTA each; one run: one launch, no workspace.
+struct RunPlan {
+  int runs = 1, run_units = 0;
+};
+RunPlan run_plan(int64_t units, int per_unit);
+struct RouteArgs {
+  const void* logits;  // [T] rows of E, ld elements apart
+  int64_t T, ld;
+  int E, top;
+  const float* bias;   // [E] or nullptr
+  int scoring;         // 0 softmax, 1 sigmoid
+  int renorm;
+  float scale;
+  int32_t* ids;        // [T][top]
+  float* weights;      // [T][top]
+  int32_t *order, *offsets;
+  int32_t* run_counts; // [runs][E + 1]
+  int64_t run_rows;
+};
+cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s);
+cudaError_t launch_group_rows(const int32_t* ids, int64_t S, int groups, int32_t* order, int32_t* offsets,
+                              int32_t* run_counts, cudaStream_t s);
+struct CombineArgs {
+  const void* y;  // [T * top] rows, ldy elements apart
+  int64_t ldy, T, n;
+  int top;
+  const float* weights;  // [T][top]
+  const int32_t* ids;    // [T][top] or nullptr
+  const void* resid;
+  int64_t ldr;
+  void* out;
+  int64_t ldo;
+};
+cudaError_t launch_combine(const CombineArgs& a, int ytype, int otype, cudaStream_t s);
+
+struct MulMatIdArgs {
+  const void* w;          // 16-bit [E][rows][K], or Q4_0 nibbles [E * rows][K / 2]
+  const uint16_t* scales; // Q4_0: fp16 [K / 32][lds]
+  int64_t lds, ldw, expert_stride;  // elements
+  int E;
+  int64_t rows, n, K;     // rows: n, or 2 n with glu
+  const void* x;          // rows of K, ldx elements apart
+  int64_t ldx, x_rows;
+  const int32_t *order, *offsets;
+  int64_t S;
+  int per_row;
+  const float* bias;      // [E][rows] or nullptr
+  int glu;
+  void* y;                // [S] rows of n, ldy elements apart
+  int64_t ldy;
+};
+constexpr int kWQ4 = 3;  // beside kXF16, kXBF16
+cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int ytype, cudaStream_t s);
+
+constexpr int kLoraMaxRank = 128;
+struct LoraArgs {
+  const void* x;  // [T] rows of K, ldx elements apart
+  int64_t T, K, N, ldx;
+  const void *a, *b;  // [groups][rank][K], [groups][N][rank]
+  int groups, rank;
+  const float* scales;  // [groups] or nullptr
+  const int32_t *order, *offsets;
+  const void* resid;
+  int64_t ldr;
+  void* y;
+  int64_t ldy;
+};
+cudaError_t launch_lora(const LoraArgs& a, int xtype, int ytype, int num_sms, cudaStream_t s);
+
+constexpr int kVerifyRanks = 8;  // CTAs of one request
+struct VerifyArgs {
+  const void* target;  // [D + B] rows of V, ldp elements apart
+  const void* guess;   // [D] rows of V, ldq apart, or nullptr
+  const int32_t *drafts, *cu;
+  int64_t ldp, ldq, B, D, V;
+  const float *u, *v;
+  int32_t *accepted, *tokens;
+  int ranks;
+};
+cudaError_t launch_verify(VerifyArgs a, int type, cudaStream_t s);
+
 }  // namespace b2q

@@ -1,0 +1,333 @@
+// b2q_route.cu -- the router of an expert layer and the plan of rows that go by
+// group.
+//
+//   key_e = logit_e + bias_e; the `top` largest keys, ties to the lower expert
+//   w_j   = softmax or sigmoid of the chosen logits, times scale
+//   order   = the slots (token * top + choice) sorted by expert, stable
+//   offsets = where each expert's slots begin
+//
+// A row's experts are spread over the lanes of one warp, as unsigned numbers
+// that order as the keys do (-0 as 0, NaN as -infinity).  Each choice is one
+// warp maximum (redux) and, among the lanes that hold it, one minimum of the
+// index.
+//
+// The sort is a counting sort without float work or global atomics: every CTA
+// counts the experts of its run of slots; then every CTA adds up the counts of
+// all runs itself (the L2 serves them), so none waits for another, and places
+// its slots: the warps take consecutive parts of the run, ranks inside a warp
+// come from the lanes that hold the same expert.  The second launch is made
+// early (programmatic dependent launch).  Where one CTA can do it all, it does:
+// one launch.
+#include "b2q_groups.cuh"
+#include "b2q_internal.h"
+
+#include <algorithm>
+
+namespace b2q {
+
+namespace {
+
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kRunSlots = 1024;      // of one CTA, at least
+constexpr int kMaxRuns = 296;
+constexpr int kOneSlots = 2048;      // up to these many slots one CTA does everything
+
+__device__ __forceinline__ uint32_t key_bits(float v) {
+  if (v != v) v = -INFINITY;
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 becomes 0
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+constexpr uint32_t kKeyNone = 0x007fffffu;  // of -infinity; all others are larger
+
+// Counts the groups of slots [s0, s1) warp by warp into counts[warp][groups + 1].
+__device__ __forceinline__ void warp_part(int s0, int s1, int* lo, int* hi) {
+  const int each = ((s1 - s0 + kWarps - 1) / kWarps + 31) / 32 * 32;
+  *lo = min(s1, s0 + static_cast<int>(threadIdx.x >> 5) * each);
+  *hi = min(s1, *lo + each);
+}
+
+__device__ __forceinline__ int group_of(const int32_t* ids, int s, int groups) {
+  const int g = ids[s];
+  return (g < 0 || g >= groups) ? groups : g;
+}
+
+// Exclusive scan over the block of the sums that thread t holds of its `n`
+// consecutive values; `sums` has kWarps + 1 ints.
+__device__ __forceinline__ int block_exclusive(int v, int* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+  __syncthreads();
+  return before + inc - v;
+}
+
+// Places the slots of run `run` of `runs`; run_counts [runs][groups + 1] of all
+// runs, or nullptr when this run is all there is.  smem: (kWarps + 1) * (groups
+// + 1) + kWarps ints.
+__device__ void place_run(const int32_t* ids, int S, int groups, int run, int runs, int run_slots,
+                          const int32_t* run_counts, int32_t* order, int32_t* offsets, int* smem) {
+  const int G = groups + 1;
+  int* counts = smem;               // [kWarps][G]
+  int* base = smem + kWarps * G;    // [G]
+  int* sums = base + G;             // [kWarps]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int s0 = static_cast<int>(min(static_cast<int64_t>(run) * run_slots, static_cast<int64_t>(S)));
+  const int s1 = static_cast<int>(min(static_cast<int64_t>(s0) + run_slots, static_cast<int64_t>(S)));
+  int lo, hi;
+  warp_part(s0, s1, &lo, &hi);
+  for (int i = threadIdx.x; i < kWarps * G; i += kThreads) counts[i] = 0;
+  __syncthreads();
+  for (int s = lo + lane; s < hi; s += 32) atomicAdd(&counts[warp * G + group_of(ids, s, groups)], 1);
+  __syncthreads();
+  // Totals of every group, and of the runs before this one.
+  const int each = (G + kThreads - 1) / kThreads;
+  int mine = 0;
+  for (int i = 0; i < each; ++i) {
+    const int g = threadIdx.x * each + i;
+    if (g >= G) break;
+    int total = 0, before = 0;
+    if (run_counts) {
+      for (int r = 0; r < runs; ++r) {
+        const int c = run_counts[static_cast<int64_t>(r) * G + g];
+        total += c;
+        if (r < run) before += c;
+      }
+    } else {
+      for (int w = 0; w < kWarps; ++w) total += counts[w * G + g];
+    }
+    base[g] = before;
+    mine += total;
+    // the totals are needed once more below; keep them in the order's sums
+    sums[kWarps + g] = total;
+  }
+  int at = block_exclusive(mine, sums);
+  for (int i = 0; i < each; ++i) {
+    const int g = threadIdx.x * each + i;
+    if (g >= G) break;
+    if (run == 0) offsets[g] = at;
+    int place = at + base[g];
+    at += sums[kWarps + g];
+    for (int w = 0; w < kWarps; ++w) {  // where each warp's slots of this group begin
+      const int c = counts[w * G + g];
+      counts[w * G + g] = place;
+      place += c;
+    }
+  }
+  __syncthreads();
+  for (int s = lo; s < hi; s += 32) {
+    const bool there = s + lane < hi;
+    const int g = there ? group_of(ids, s + lane, groups) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    int place = 0;
+    if (there) place = counts[warp * G + g] + rank;
+    __syncwarp();
+    if (there && rank == 0) counts[warp * G + g] += __popc(same);
+    __syncwarp();
+    if (there) order[place] = s + lane;
+  }
+}
+
+size_t place_smem(int groups) { return (static_cast<size_t>(kWarps + 2) * (groups + 1) + kWarps) * 4; }
+
+template <int T, bool ONE>
+__global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
+  extern __shared__ int smem[];
+  using V = typename Val<T>::type;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int E = a.E;
+  if constexpr (!ONE) {
+    for (int i = threadIdx.x; i <= E; i += kThreads) smem[i] = 0;
+    __syncthreads();
+  }
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.run_rows;
+  const int64_t t1 = min(t0 + a.run_rows, a.T);
+  for (int64_t t = t0 + warp; t < t1; t += kWarps) {
+    const V* row = static_cast<const V*>(a.logits) + t * a.ld;
+    // Lane l holds experts l, l + 32, ...: the largest key that is left of them.
+    float mx = -INFINITY;
+    uint32_t last = 0xffffffffu;  // the key and expert of the last choice: what is left lies behind it
+    int last_e = -1;
+    float picked = 0.0f;  // lane j: the logit of choice j
+    int chosen = -1;
+    for (int j = 0; j < a.top; ++j) {
+      uint32_t best = 0;
+      int best_e = 0x7fffffff;
+      for (int e = lane; e < E; e += 32) {
+        const float x = Val<T>::load(row + e);
+        const uint32_t k = key_bits(a.bias ? x + __ldg(a.bias + e) : x);
+        if (j == 0 && x == x) mx = fmaxf(mx, x);
+        const bool left = k < last || (k == last && e > last_e);
+        if (left && k > best) best = k, best_e = e;
+      }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+      const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == top ? static_cast<unsigned>(best_e) : 0x7fffffffu));
+      if (top <= kKeyNone) break;  // only -infinity is left
+      last = top;
+      last_e = e;
+      if (lane == j) {
+        chosen = e;
+        picked = Val<T>::load(row + e);
+      }
+    }
+    const bool there = chosen >= 0;
+    float w = 0.0f;
+    if (a.scoring == 1) {
+      if (there) w = 1.0f / (1.0f + expf(-picked));
+    } else {
+      // the largest logit of all (of the choice, when only the choice counts); its own weight is e^0, also where it is infinite
+      float m = a.renorm ? (there ? picked : -INFINITY) : mx;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (there) w = picked == m ? 1.0f : expf(picked - m);
+      if (!a.renorm) {
+        float z = 0.0f;
+        for (int e = lane; e < E; e += 32) {
+          const float x = Val<T>::load(row + e);
+          if (x == x) z += x == m ? 1.0f : expf(x - m);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        if (there) w /= z;
+      }
+    }
+    if (a.renorm) {
+      float z = w;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      w = z > 0.0f ? w / z : 0.0f;
+    }
+    if (lane < a.top) {
+      a.ids[t * a.top + lane] = chosen;
+      a.weights[t * a.top + lane] = w * a.scale;
+      if constexpr (!ONE) atomicAdd(&smem[there ? chosen : E], 1);
+    }
+  }
+  __syncthreads();
+  if constexpr (ONE) {
+    place_run(a.ids, static_cast<int>(a.T * a.top), E, 0, 1, static_cast<int>(a.T * a.top), nullptr, a.order,
+              a.offsets, smem);
+  } else {
+    for (int i = threadIdx.x; i <= E; i += kThreads)
+      a.run_counts[static_cast<int64_t>(blockIdx.x) * (E + 1) + i] = smem[i];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) count_kernel(const int32_t* ids, int S, int groups, int run_slots,
+                                                         int32_t* run_counts) {
+  extern __shared__ int smem[];
+  for (int i = threadIdx.x; i <= groups; i += kThreads) smem[i] = 0;
+  __syncthreads();
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * run_slots;
+  const int64_t s1 = min(s0 + run_slots, static_cast<int64_t>(S));
+  for (int64_t s = s0 + threadIdx.x; s < s1; s += kThreads) atomicAdd(&smem[group_of(ids, static_cast<int>(s), groups)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i <= groups; i += kThreads)
+    run_counts[static_cast<int64_t>(blockIdx.x) * (groups + 1) + i] = smem[i];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kThreads) place_kernel(const int32_t* ids, int S, int groups, int run_slots,
+                                                         const int32_t* run_counts, int32_t* order, int32_t* offsets) {
+  extern __shared__ int smem[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  place_run(ids, S, groups, blockIdx.x, gridDim.x, run_slots, run_counts, order, offsets, smem);
+}
+
+cudaError_t set_smem(const void* f, size_t bytes) {
+  return bytes > 48 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes))
+                           : cudaSuccess;
+}
+
+cudaError_t launch_place(const int32_t* ids, int64_t S, int groups, int runs, int run_slots, const int32_t* run_counts,
+                         int32_t* order, int32_t* offsets, cudaStream_t s) {
+  const size_t smem = place_smem(groups);
+  if (cudaError_t e = set_smem(reinterpret_cast<const void*>(place_kernel), smem)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(runs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = run_counts ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, place_kernel, ids, static_cast<int>(S), groups, run_slots, run_counts, order, offsets);
+}
+
+// y [T * top] rows -> out [T] rows: out = resid + sum_j w_j y_j, choices in order.
+template <int Y, int O>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
+  using YV = typename Val<Y>::type;
+  using OV = typename Val<O>::type;
+  const int64_t t = blockIdx.x;
+  for (int64_t n = threadIdx.x; n < a.n; n += 256) {
+    float sum = 0.0f;
+    for (int j = 0; j < a.top; ++j) {
+      const int64_t s = t * a.top + j;
+      if (a.ids && __ldg(a.ids + s) < 0) continue;
+      sum = fmaf(__ldg(a.weights + s), Val<Y>::load(static_cast<const YV*>(a.y) + s * a.ldy + n), sum);
+    }
+    if (a.resid) sum += Val<O>::load(static_cast<const OV*>(a.resid) + t * a.ldr + n);
+    static_cast<OV*>(a.out)[t * a.ldo + n] = Val<O>::to(sum);
+  }
+}
+
+}  // namespace
+
+RunPlan run_plan(int64_t units, int per_unit) {
+  RunPlan p;
+  const int64_t slots = units * per_unit;
+  if (slots <= kOneSlots) return p;
+  int64_t runs = std::min<int64_t>(kMaxRuns, (slots + kRunSlots - 1) / kRunSlots);
+  p.run_units = static_cast<int>((units + runs - 1) / runs);
+  p.runs = static_cast<int>((units + p.run_units - 1) / p.run_units);
+  return p;
+}
+
+cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
+  const RunPlan p = run_plan(a.T, a.top);
+  const bool one = p.runs == 1;
+  a.run_rows = one ? a.T : p.run_units;
+  const size_t smem = one ? place_smem(a.E) : (a.E + 1) * 4;
+  void (*kernels[3][2])(const RouteArgs) = {{route_kernel<0, false>, route_kernel<0, true>},
+                                            {route_kernel<1, false>, route_kernel<1, true>},
+                                            {route_kernel<2, false>, route_kernel<2, true>}};
+  auto k = kernels[type][one];
+  if (cudaError_t e = set_smem(reinterpret_cast<const void*>(k), smem)) return e;
+  k<<<p.runs, kThreads, smem, s>>>(a);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  if (one) return cudaSuccess;
+  return launch_place(a.ids, a.T * a.top, a.E, p.runs, p.run_units * a.top, a.run_counts, a.order, a.offsets, s);
+}
+
+cudaError_t launch_group_rows(const int32_t* ids, int64_t S, int groups, int32_t* order, int32_t* offsets,
+                              int32_t* run_counts, cudaStream_t s) {
+  const RunPlan p = run_plan(S, 1);
+  if (p.runs == 1)
+    return launch_place(ids, S, groups, 1, static_cast<int>(std::max<int64_t>(S, 1)), nullptr, order, offsets, s);
+  count_kernel<<<p.runs, kThreads, (groups + 1) * 4, s>>>(ids, static_cast<int>(S), groups, p.run_units, run_counts);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  return launch_place(ids, S, groups, p.runs, p.run_units, run_counts, order, offsets, s);
+}
+
+cudaError_t launch_combine(const CombineArgs& a, int ytype, int otype, cudaStream_t s) {
+  void (*kernels[3][3])(const CombineArgs) = {
+      {combine_kernel<0, 0>, combine_kernel<0, 1>, combine_kernel<0, 2>},
+      {combine_kernel<1, 0>, combine_kernel<1, 1>, combine_kernel<1, 2>},
+      {combine_kernel<2, 0>, combine_kernel<2, 1>, combine_kernel<2, 2>}};
+  kernels[ytype][otype]<<<static_cast<unsigned>(a.T), 256, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace b2q

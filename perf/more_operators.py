@@ -249,7 +249,9 @@ def _own_experts(s):
 
 
 def _own_adapters(s):
-    return _b2q().lora_add(s["y"], s["x"], s["a"], s["b"], s["scales"], s["order"], s["offsets"])
+    # fp32 rows are updated where they are, as the plain form updates them
+    return _b2q().lora_add(s["y"], s["x"], s["a"], s["b"], s["scales"], s["order"], s["offsets"],
+                           out=s["y"] if s["y"].dtype is torch.float32 else None)
 
 
 def _own_verify(s):

@@ -1158,6 +1158,8 @@ int b2q_device_status(unsigned int* code, int clear) {
   if (!*code) *code = attn;
   if (read_paged_status(&attn, clear != 0) != cudaSuccess) return B2Q_ERR_CUDA;
   if (!*code) *code = attn;
+  if (read_id_status(&attn, clear != 0) != cudaSuccess) return B2Q_ERR_CUDA;
+  if (!*code) *code = attn;
   return *code ? B2Q_ERR_DEVICE : B2Q_OK;
 }
 

@@ -434,6 +434,8 @@ struct MulMatIdArgs {
 };
 constexpr int kWQ4 = 3;  // beside kXF16, kXBF16
 cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int ytype, cudaStream_t s);
+// Status word of its bounded waits (its own translation unit).
+cudaError_t read_id_status(unsigned int* value, bool clear);
 
 constexpr int kLoraMaxRank = 128;
 struct LoraArgs {

@@ -223,6 +223,10 @@ bool make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* ba
 bool make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t (&dims)[3],
                         const uint64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swz);
 
+// The same for four.
+bool make_tensor_map_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t (&dims)[4],
+                        const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swz);
+
 // Q4_K x Q8_K GEMM (b2q_gemm_q4k.cuh):
 //   weight: block_q4_K rows, ldw_bytes apart (16-byte aligned base and stride);
 //   activations: int8 Q8_K codes [M][K], fp32 d [K/256][lda].

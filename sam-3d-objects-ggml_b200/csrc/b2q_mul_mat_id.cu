@@ -56,14 +56,15 @@ struct IdShape {
   static constexpr int STAGES = Q4 ? 4 : 6, RAWS = Q4 ? 4 : 0;
   static constexpr int EPI = Q4 ? 8 : 16;   // epilogue warps
   static constexpr int CONV = Q4 ? 8 : 0;   // widening warps
-  static constexpr int WARPS = 2 + EPI + CONV + (Q4 ? 1 : 0), THREADS = WARPS * 32;
+  static constexpr int GATHER = 4;          // warps that fetch rows of x
+  static constexpr int WARPS = 2 + EPI + CONV + GATHER + 1, THREADS = WARPS * 32;
   static constexpr int CHUNK = GLU ? 16 : 32;  // accumulator columns that an epilogue warp has in registers
   static constexpr int OFF_RAW = STAGES * kStageBytes;
   static constexpr int OFF_SWAP = OFF_RAW + RAWS * kRawStride;
   static constexpr int SWAP = GLU ? EPI * 32 * 8 * 4 : 0;
   static constexpr int OFF_PRE = OFF_SWAP + SWAP;
   static constexpr int OFF_BARS = OFF_PRE + (static_cast<int>(kMaxGroups) + 2) * 4 + 8;
-  static constexpr int NBARS = 2 * STAGES + 2 * RAWS + 2 * kAccs + 1;
+  static constexpr int NBARS = 3 * STAGES + 2 * RAWS + 2 * kAccs + 1;
   static constexpr int SMEM = OFF_BARS + NBARS * 8 + 8 + 4 + 4 + 2 * EPI * 4 + THREADS / 32 * 4 + 1024;
 };
 static_assert(IdShape<1, true>::SMEM <= 227 * 1024 && IdShape<kWQ4, true>::SMEM <= 227 * 1024, "shared memory");
@@ -104,7 +105,7 @@ __device__ __forceinline__ IdTile id_tile(const MulMatIdArgs& a, const int* pre,
 }
 
 struct IdMaps {
-  CUtensorMap w, scales, x;
+  CUtensorMap w, scales;
 };
 
 __device__ __forceinline__ uint32_t hsub2_u(uint32_t a, uint32_t b) {
@@ -141,7 +142,8 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
   int* pre = reinterpret_cast<int*>(smem + Sh::OFF_PRE);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::OFF_BARS);  // used in the leader
   uint64_t* empty = full + ST;
-  uint64_t* raw_full = empty + ST;
+  uint64_t* x_full = empty + ST;  // rows of x have arrived in this CTA
+  uint64_t* raw_full = x_full + ST;
   uint64_t* raw_empty = raw_full + RS;
   uint64_t* acc_full = raw_empty + RS;
   uint64_t* acc_empty = acc_full + kAccs;  // used in the leader: both CTAs' epilogue warps
@@ -161,7 +163,8 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], 1 + 2 * Sh::CONV);
+      mbar_init(&full[s], (Q4 ? 0 : 1) + 2 * (Sh::CONV + 1));
+      mbar_init(&x_full[s], Sh::GATHER * 32);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < RS; ++s) {
@@ -176,7 +179,6 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
     *abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&maps.w);
-    tma_prefetch_desc(&maps.x);
     if constexpr (Q4) tma_prefetch_desc(&maps.scales);
   }
   if (warp == 1) {
@@ -216,44 +218,63 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
   const int num_tiles = pre[p.E];
 
   if (warp == 0) {
-    // ---------------------------- producer: rows of x, and the 16-bit weight tile
-    const uint32_t full0 = cluster_addr(full, 0);
-    uint32_t stage = 0, phase = 0, issued_mask = 0, issued_par = 0;
-    bool ok = true;
-    for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
-      const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
-      const int half = t.width >> 1;
-      int rows[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // the numbers behind the tile's last slot bring some row that exists; nobody looks at it
-        const int s = __ldg(p.order + max(0, min(t.begin + static_cast<int>(rank) * half + 4 * lane + i, t.end - 1)));
-        rows[i] = s < 0 || s >= p.S ? 0 : s / p.per_row;
-      }
-      for (int ks = 0; ks < kst; ++ks) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
-        if (!ok) break;
-        uint8_t* sb = smem + stage * kStageBytes;
-        const uint32_t fb = full0 + stage * 8;
-        if (lane == 0) {
-          if (leader) mbar_arrive_expect_tx(&full[stage], t.width * 128 + (Q4 ? 0 : 2 * kABytes));  // both CTAs' bytes
-          if constexpr (!Q4) {
-            tma_load_3d_pair(sb, &maps.w, fb, ks * kStageK, t.r0, t.e);
-            tma_load_3d_pair(sb + kABytes / 2, &maps.w, fb, ks * kStageK, t.r1, t.e);
+    // ------------------------------------- producer: the weights, as they are stored
+    if (elect_one()) {
+      if constexpr (!Q4) {
+        const uint32_t full0 = cluster_addr(full, 0);
+        uint32_t stage = 0, phase = 0, issued_mask = 0, issued_par = 0;
+        bool ok = true;
+        for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
+          const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
+          for (int ks = 0; ks < kst; ++ks) {
+            if (!mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag)) {
+              ok = false;
+              break;
+            }
+            uint8_t* sb = smem + stage * kStageBytes;
+            const uint32_t fb = full0 + stage * 8;
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kABytes);  // both CTAs' bytes
+            tma_load_4d_pair(sb, &maps.w, fb, ks * kStageK, t.r0, 0, t.e);
+            issued_mask |= 1u << stage;
+            issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
+            if (++stage == ST) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
-        if (4 * lane < half)
-          tma_gather4_pair(sb + kABytes + lane * 512, &maps.x, fb, ks * kStageK, rows[0], rows[1], rows[2], rows[3]);
-        issued_mask |= 1u << stage;
-        issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
-        if (++stage == ST) {
-          stage = 0;
-          phase ^= 1u;
+        if (leader)  // every issued copy of both CTAs lands before the pair may exit
+          for (int s = 0; s < ST; ++s)
+            if ((issued_mask >> s) & 1u) mbar_wait(&full[s], (issued_par >> s) & 1u, status, kDevWaitDrain, nullptr);
+      } else {
+        uint32_t raw = 0, phase = 0, issued_mask = 0, issued_par = 0;
+        bool ok = true;
+        for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
+          const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
+          const int y0 = static_cast<int>(t.e * p.rows + t.r0), y1 = static_cast<int>(t.e * p.rows + t.r1);
+          for (int rs = 0; rs * 4 < kst; ++rs) {
+            if (!mbar_wait(&raw_empty[raw], phase ^ 1u, status, kDevWaitProducer, abort_flag)) {
+              ok = false;
+              break;
+            }
+            uint8_t* rb = raws + raw * kRawStride;
+            mbar_arrive_expect_tx(&raw_full[raw], kRawBytes);
+            tma_load_2d(rb, &maps.w, &raw_full[raw], rs * (kRawK / 2), y0);
+            tma_load_2d(rb + kRawBox, &maps.w, &raw_full[raw], rs * (kRawK / 2), y1);
+            tma_load_2d(rb + 2 * kRawBox, &maps.scales, &raw_full[raw], y0 & ~7, rs * (kRawK / 32));
+            tma_load_2d(rb + 2 * kRawBox + kScaleBox, &maps.scales, &raw_full[raw], y1 & ~7, rs * (kRawK / 32));
+            issued_mask |= 1u << raw;
+            issued_par = (issued_par & ~(1u << raw)) | (phase << raw);
+            if (++raw == RS) {
+              raw = 0;
+              phase ^= 1u;
+            }
+          }
         }
+        for (int s = 0; s < RS; ++s)
+          if ((issued_mask >> s) & 1u) mbar_wait(&raw_full[s], (issued_par >> s) & 1u, status, kDevWaitDrain, nullptr);
       }
     }
-    if (leader)  // every issued copy of both CTAs lands before the pair may exit
-      for (int s = 0; s < ST; ++s)
-        if ((issued_mask >> s) & 1u) mbar_wait(&full[s], (issued_par >> s) & 1u, status, kDevWaitDrain, nullptr);
   } else if (warp == 1) {
     // ------------------------------------------------- MMA issuer (leader)
     if (leader && elect_one()) {
@@ -267,9 +288,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
         tc_fence_after();
         const uint32_t d = tmem_base + a * kBN;
         for (int ks = 0; ks < kst; ++ks) {
-          const bool got = Q4 ? mbar_wait_cluster(&full[stage], phase, status, kDevWaitMma, abort_flag)
-                              : mbar_wait(&full[stage], phase, status, kDevWaitMma, abort_flag);
-          if (!got) {
+          if (!mbar_wait(&full[stage], phase, status, kDevWaitMma, abort_flag)) {
             ok = false;
             break;
           }
@@ -422,7 +441,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(full0 + stage * 8);
+          if (lane == 0) mbar_arrive_remote(full0 + stage * 8);
           if (++stage == ST) {
             stage = 0;
             phase ^= 1u;
@@ -430,37 +449,59 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
         }
       }
     }
+  } else if (warp < 2 + Sh::EPI + Sh::CONV + Sh::GATHER) {
+    // -------------------------------------------------------- rows of x by their numbers
+    const int gw = warp - (2 + Sh::EPI + Sh::CONV);
+    const int chunk = lane & 7;  // 16 bytes of a row's 128; four rows a request of the warp
+    const int row0 = gw * 4 + (lane >> 3);
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
+      const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
+      const int half = t.width >> 1;
+      const uint8_t* src[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // the numbers behind the tile's last slot bring some row that exists; nobody looks at it
+        const int s = __ldg(p.order + max(0, min(t.begin + static_cast<int>(rank) * half + i * 16 + row0, t.end - 1)));
+        src[i] = static_cast<const uint8_t*>(p.x) + (s < 0 || s >= p.S ? 0 : s / p.per_row) * p.ldx * 2 + chunk * 16;
+      }
+      for (int ks = 0; ks < kst; ++ks) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
+        if (!ok) break;
+        const uint32_t dst = smem_u32(smem + stage * kStageBytes + kABytes) + ((chunk ^ (row0 & 7)) << 4) + row0 * 128;
+        const int bytes = ks * kStageK + chunk * 8 < p.K ? 16 : 0;  // zeros behind the row's end
+        const int64_t at = bytes ? static_cast<int64_t>(ks) * 128 : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i * 16 < half)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * 2048), "l"(src[i] + at), "r"(bytes)
+                         : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&x_full[stage])) : "memory");
+        if (++stage == ST) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    // ----------------------------------------- Q4_0: producer of nibbles and scales
-    if constexpr (Q4) {
-      if (elect_one()) {
-        uint32_t raw = 0, phase = 0, issued_mask = 0, issued_par = 0;
-        bool ok = true;
-        for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
-          const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
-          const int y0 = static_cast<int>(t.e * p.rows + t.r0), y1 = static_cast<int>(t.e * p.rows + t.r1);
-          for (int rs = 0; rs * 4 < kst; ++rs) {
-            if (!mbar_wait(&raw_empty[raw], phase ^ 1u, status, kDevWaitProducer, abort_flag)) {
-              ok = false;
-              break;
-            }
-            uint8_t* rb = raws + raw * kRawStride;
-            mbar_arrive_expect_tx(&raw_full[raw], kRawBytes);
-            tma_load_2d(rb, &maps.w, &raw_full[raw], rs * (kRawK / 2), y0);
-            tma_load_2d(rb + kRawBox, &maps.w, &raw_full[raw], rs * (kRawK / 2), y1);
-            tma_load_2d(rb + 2 * kRawBox, &maps.scales, &raw_full[raw], y0 & ~7, rs * (kRawK / 32));
-            tma_load_2d(rb + 2 * kRawBox + kScaleBox, &maps.scales, &raw_full[raw], y1 & ~7, rs * (kRawK / 32));
-            issued_mask |= 1u << raw;
-            issued_par = (issued_par & ~(1u << raw)) | (phase << raw);
-            if (++raw == RS) {
-              raw = 0;
-              phase ^= 1u;
-            }
+    // A thread with no copies of its own makes the arrived rows visible to the tensor core (the same fence in a
+    // gather warp would wait for all that the warp has asked for) and reports them to the leader.
+    if (elect_one()) {
+      const uint32_t full0 = cluster_addr(full, 0);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int tile = cluster; ok && tile < num_tiles; tile += nclusters)
+        for (int ks = 0; ks < kst; ++ks) {
+          ok = mbar_wait(&x_full[stage], phase, status, kDevWaitProducer, abort_flag);
+          if (!ok) break;
+          fence_proxy_async_smem();
+          mbar_arrive_remote(full0 + stage * 8);
+          if (++stage == ST) {
+            stage = 0;
+            phase ^= 1u;
           }
         }
-        for (int s = 0; s < RS; ++s)
-          if ((issued_mask >> s) & 1u) mbar_wait(&raw_full[s], (issued_par >> s) & 1u, status, kDevWaitDrain, nullptr);
-      }
     }
   }
 
@@ -513,18 +554,20 @@ cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int y
   const bool q4 = wtype == kWQ4, glu = a.glu != 0, out32 = ytype == kXF32;
   const CUtensorMapDataType dt = xtype == kXBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   IdMaps maps = {};
-  bool ok = make_tensor_map_2d(&maps.x, dt, a.x, a.K, a.x_rows, a.ldx * 2, kStageK, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+  bool ok;
   if (q4) {
-    ok = ok && make_tensor_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.K / 2, a.E * a.rows, a.K / 2, kRawK / 2, 64,
+    ok = make_tensor_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.K / 2, a.E * a.rows, a.K / 2, kRawK / 2, 64,
                                   CU_TENSOR_MAP_SWIZZLE_128B) &&
          make_tensor_map_2d(&maps.scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.scales, a.lds, a.K / 32, a.lds * 2,
                             kScaleCols, kRawK / 32, CU_TENSOR_MAP_SWIZZLE_NONE);
   } else {
-    const uint64_t dims[3] = {static_cast<uint64_t>(a.K), static_cast<uint64_t>(a.rows), static_cast<uint64_t>(a.E)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(a.ldw) * 2,
+    // [expert][gate / up][row][k]: one box has a CTA's rows, with GLU 64 of either half
+    const uint64_t dims[4] = {static_cast<uint64_t>(a.K), static_cast<uint64_t>(a.n), glu ? 2u : 1u,
+                              static_cast<uint64_t>(a.E)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(a.ldw) * 2, static_cast<uint64_t>(a.ldw * a.n) * 2,
                                  static_cast<uint64_t>(a.E > 1 ? a.expert_stride : a.ldw * a.rows) * 2};
-    const uint32_t box[3] = {kStageK, kBM / 2, 1};
-    ok = ok && make_tensor_map_3d(&maps.w, dt, a.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint32_t box[4] = {kStageK, static_cast<uint32_t>(glu ? kBM / 2 : kBM), glu ? 2u : 1u, 1};
+    ok = make_tensor_map_4d(&maps.w, dt, a.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   }
   if (!ok) return cudaErrorInvalidValue;
   // As many tiles as there can be at most, whatever the groups' sizes.

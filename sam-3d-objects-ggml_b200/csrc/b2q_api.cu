@@ -1495,7 +1495,8 @@ int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t
       !aligned(bias, 4) || !aligned(y, ysize) || y_row_stride_bytes % ysize != 0)
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
-  if (int rc = check_device(nullptr)) return rc;
+  int sms = 0;
+  if (int rc = check_device(&sms)) return rc;
   MulMatIdArgs a{};
   if (q4) {
     const Q4cWeight c = q4c_at(static_cast<const uint8_t*>(w), experts * rows, k);
@@ -1522,7 +1523,7 @@ int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t
   a.glu = glu;
   a.y = y;
   a.ldy = y_row_stride_bytes / ysize;
-  return from_cuda(launch_mul_mat_id(a, q4 ? kWQ4 : val_type(wtype), val_type(xtype), val_type(ytype),
+  return from_cuda(launch_mul_mat_id(a, q4 ? kWQ4 : val_type(wtype), val_type(xtype), val_type(ytype), sms,
                                      static_cast<cudaStream_t>(stream)));
 }
 
@@ -1532,7 +1533,7 @@ int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const 
   const int yt = val_type(ytype), ot = val_type(otype);
   if (yt < 0 || ot < 0) return B2Q_ERR_UNSUPPORTED;
   if (T < 0 || top <= 0 || n < 0) return B2Q_ERR_INVALID_ARG;
-  if (top > kMaxSlots || T > kMaxSlots / top || n > INT_MAX) return B2Q_ERR_TOO_LARGE;
+  if (top > kMaxSlots || T > kMaxSlots / top || n > kCombineMaxN) return B2Q_ERR_TOO_LARGE;
   const bool any = T > 0 && n > 0;
   const int ys = val_size(yt), os = val_size(ot);
   if ((any && (!y || !weights || !out)) || y_row_stride_bytes < n * ys || out_row_stride_bytes < n * os ||

@@ -407,6 +407,7 @@ struct RouteArgs {
 cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s);
 cudaError_t launch_group_rows(const int32_t* ids, int64_t S, int groups, int32_t* order, int32_t* offsets,
                               int32_t* run_counts, cudaStream_t s);
+constexpr int64_t kCombineMaxN = 1 << 21;  // columns (blocks of at least 32 in the grid's second dimension)
 struct CombineArgs {
   const void* y;  // [T * top] rows, ldy elements apart
   int64_t ldy, T, n;
@@ -437,7 +438,10 @@ struct MulMatIdArgs {
   int64_t ldy;
 };
 constexpr int kWQ4 = 3;  // beside kXF16, kXBF16
-cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int ytype, cudaStream_t s);
+cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int ytype, int num_sms, cudaStream_t s);
+// The kernel for 4-bit weights and few rows per expert (b2q_mul_mat_id_rows.cu), and whether rows of K fit its shared memory.
+bool id_rows_fits(int64_t K);
+cudaError_t launch_id_rows(const MulMatIdArgs& a, int ytype, int num_sms, cudaStream_t s);
 // Status word of its bounded waits (its own translation unit).
 cudaError_t read_id_status(unsigned int* value, bool clear);
 

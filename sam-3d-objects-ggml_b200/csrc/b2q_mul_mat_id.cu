@@ -10,17 +10,18 @@
 // a prompt's groups run at the tensor cores' rate.  The pairs are persistent and
 // find their tiles themselves from the plan's offsets, so that the host never
 // learns the groups' sizes.
-//   A   weight tile by TMA, two boxes of 64 rows per CTA: with GLU a box of gate
-//       rows and one of the up rows that belong to them, so both sums of an
-//       output end in one CTA
-//   B   rows of x by their numbers (TMA gather of four rows a request, issued by
-//       the lanes of one warp): no sorted copy of x is written or read
+//   A   weight tile by TMA, one box a stage: with GLU 64 gate rows and the 64 up
+//       rows that belong to them, so both sums of an output end in one CTA
+//   B   rows of x by their numbers, cp.async into the layout of the MMA; a thread
+//       of its own waits for them, makes them visible to the tensor core and
+//       reports them to the pair's leader: no sorted copy of x is written or read
 //   D   fp32 in tensor memory, two accumulators of 256 columns; the epilogue
 //       scatters rows to their slots
 // 4-bit weights (Q4_0): the nibble blocks come by TMA, 256 values of a row at a
-// time, and eight warps widen them to fp16, (q - 8) * d rounded once -- half a
-// step of fp16 on a weight that has 4 bits, as large as what rounding the
-// output does -- into the A tile.
+// time, and eight warps widen them into A.  A weight (q - 8) d has up to 15 bits,
+// so d is taken as a number of 7 bits and one of 4, whose products with q - 8 are
+// exact in fp16, and two MMAs add up to the weight as it is (|8 d| < 65504).
+// Few rows with such weights go to b2q_mul_mat_id_rows.cu.
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
@@ -39,8 +40,8 @@ constexpr int kBN = 256;              // slots per tile, at most
 constexpr int kStageK = 64;           // values of K per stage: 128 bytes
 constexpr int kABytes = kBM * kStageK * 2;
 constexpr int kBBytes = kBN / 2 * kStageK * 2;
-constexpr int kStageBytes = kABytes + kBBytes;
 constexpr int kAccs = 2;
+constexpr int kFewRows = 16;          // rows per expert, on average, up to which the rows kernel does it
 // Q4_0: a raw slot is 256 values of the CTA's 128 rows: nibbles in two boxes of
 // 64 rows, and each box's fp16 scales from the multiple of 8 rows below its first
 // (a TMA copy starts on 16 bytes).
@@ -53,13 +54,15 @@ static_assert(kScaleBox % 128 == 0, "TMA destinations");
 template <int W, bool GLU>
 struct IdShape {
   static constexpr bool Q4 = W == kWQ4;
-  static constexpr int STAGES = Q4 ? 4 : 6, RAWS = Q4 ? 4 : 0;
+  static constexpr int STAGES = Q4 ? 3 : 6, RAWS = Q4 ? 3 : 0;
+  static constexpr int A = Q4 ? 2 * kABytes : kABytes;  // 4 bits: the weights as sums of two numbers
+  static constexpr int STAGE = A + kBBytes;
   static constexpr int EPI = Q4 ? 8 : 16;   // epilogue warps
   static constexpr int CONV = Q4 ? 8 : 0;   // widening warps
   static constexpr int GATHER = 4;          // warps that fetch rows of x
   static constexpr int WARPS = 2 + EPI + CONV + GATHER + 1, THREADS = WARPS * 32;
   static constexpr int CHUNK = GLU ? 16 : 32;  // accumulator columns that an epilogue warp has in registers
-  static constexpr int OFF_RAW = STAGES * kStageBytes;
+  static constexpr int OFF_RAW = STAGES * STAGE;
   static constexpr int OFF_SWAP = OFF_RAW + RAWS * kRawStride;
   static constexpr int SWAP = GLU ? EPI * 32 * 8 * 4 : 0;
   static constexpr int OFF_PRE = OFF_SWAP + SWAP;
@@ -117,14 +120,14 @@ __device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Four 4-bit codes in the low halves of four bytes -> (q - 8) * d, two fp16 pairs.
+// Four 4-bit codes in the low halves of four bytes -> q - 8, two fp16 pairs.
 // 0x64 above a byte q is the fp16 number 1024 + q.
-__device__ __forceinline__ uint2 widen4(uint32_t q, uint32_t d2) {
+__device__ __forceinline__ uint2 codes4(uint32_t q) {
   uint32_t a, b;
   asm("prmt.b32 %0, %1, %2, 0x4140;" : "=r"(a) : "r"(q), "r"(0x64646464u));
   asm("prmt.b32 %0, %1, %2, 0x4342;" : "=r"(b) : "r"(q), "r"(0x64646464u));
   const uint32_t bias = 0x64086408u;  // 1032
-  return make_uint2(hmul2_u(hsub2_u(a, bias), d2), hmul2_u(hsub2_u(b, bias), d2));
+  return make_uint2(hsub2_u(a, bias), hsub2_u(b, bias));
 }
 
 template <int W, bool GLU, bool OUT32>
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
               ok = false;
               break;
             }
-            uint8_t* sb = smem + stage * kStageBytes;
+            uint8_t* sb = smem + stage * Sh::STAGE;
             const uint32_t fb = full0 + stage * 8;
             if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kABytes);  // both CTAs' bytes
             tma_load_4d_pair(sb, &maps.w, fb, ks * kStageK, t.r0, 0, t.e);
@@ -293,12 +296,17 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t a_base = smem_u32(smem + stage * kStageBytes);
-          const uint32_t b_base = a_base + kABytes;
+          const uint32_t a_base = smem_u32(smem + stage * Sh::STAGE);
+          const uint32_t b_base = a_base + Sh::A;
 #pragma unroll
           for (int j = 0; j < kStageK / 16; ++j)
             mma_f16_pair(d, smem_desc_k_sw128(a_base + j * 32), smem_desc_k_sw128(b_base + j * 32), idesc,
                          (ks | j) != 0 ? 1u : 0u);
+          if constexpr (Q4) {
+#pragma unroll
+            for (int j = 0; j < kStageK / 16; ++j)
+              mma_f16_pair(d, smem_desc_k_sw128(a_base + kABytes + j * 32), smem_desc_k_sw128(b_base + j * 32), idesc, 1u);
+          }
           mma_commit_pair(&empty[stage], 0x3);
           if (++stage == ST) {
             stage = 0;
@@ -419,7 +427,8 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
           const int block = (ks % 4) * 2 + b;
           const uint4 q = *reinterpret_cast<const uint4*>(rb + r * 128 + ((block ^ (r & 7)) << 4));
           const uint32_t d = *reinterpret_cast<const uint16_t*>(rb + scale_at + block * (kScaleCols * 2));
-          const uint32_t d2 = d | (d << 16);
+          // d as a number of 7 bits and one of 4: both times q - 8 are exact in fp16
+          const uint32_t hi2 = (d | (d << 16)) & 0xfff0fff0u, lo2 = hsub2_u(d | (d << 16), hi2);
           if (ks % 4 == 3 || ks == kst - 1) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&raw_empty[raw]);
@@ -430,14 +439,16 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
           }
           ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
           if (!ok) break;
-          uint8_t* ab = smem + stage * kStageBytes + r * 128;
+          uint8_t* ab = smem + stage * Sh::STAGE + r * 128;
           constexpr uint32_t m = 0x0f0f0f0fu;
           const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // values 8 j .. 8 j + 7: low nibbles of 8 bytes, then the high ones
             const uint32_t w0 = words[(j & 1) * 2], w1 = words[(j & 1) * 2 + 1];
-            const uint2 lo = widen4((j < 2 ? w0 : w0 >> 4) & m, d2), hi = widen4((j < 2 ? w1 : w1 >> 4) & m, d2);
-            *reinterpret_cast<uint4*>(ab + (((b * 4 + j) ^ (r & 7)) << 4)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            const uint2 u = codes4((j < 2 ? w0 : w0 >> 4) & m), v = codes4((j < 2 ? w1 : w1 >> 4) & m);
+            uint4* at = reinterpret_cast<uint4*>(ab + (((b * 4 + j) ^ (r & 7)) << 4));
+            at[0] = make_uint4(hmul2_u(u.x, hi2), hmul2_u(u.y, hi2), hmul2_u(v.x, hi2), hmul2_u(v.y, hi2));
+            at[kABytes / 16] = make_uint4(hmul2_u(u.x, lo2), hmul2_u(u.y, lo2), hmul2_u(v.x, lo2), hmul2_u(v.y, lo2));
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -468,7 +479,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
       for (int ks = 0; ks < kst; ++ks) {
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
         if (!ok) break;
-        const uint32_t dst = smem_u32(smem + stage * kStageBytes + kABytes) + ((chunk ^ (row0 & 7)) << 4) + row0 * 128;
+        const uint32_t dst = smem_u32(smem + stage * Sh::STAGE + Sh::A) + ((chunk ^ (row0 & 7)) << 4) + row0 * 128;
         const int bytes = ks * kStageK + chunk * 8 < p.K ? 16 : 0;  // zeros behind the row's end
         const int64_t at = bytes ? static_cast<int64_t>(ks) * 128 : 0;
 #pragma unroll
@@ -550,7 +561,8 @@ cudaError_t launch_shape(const MulMatIdArgs& a, const IdMaps& maps, int64_t tile
 
 }  // namespace
 
-cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int ytype, cudaStream_t s) {
+cudaError_t launch_mul_mat_id(const MulMatIdArgs& a, int wtype, int xtype, int ytype, int num_sms, cudaStream_t s) {
+  if (wtype == kWQ4 && a.S <= kFewRows * a.E && id_rows_fits(a.K)) return launch_id_rows(a, ytype, num_sms, s);
   const bool q4 = wtype == kWQ4, glu = a.glu != 0, out32 = ytype == kXF32;
   const CUtensorMapDataType dt = xtype == kXBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   IdMaps maps = {};

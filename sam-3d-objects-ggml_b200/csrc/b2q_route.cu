@@ -265,22 +265,40 @@ cudaError_t launch_place(const int32_t* ids, int64_t S, int groups, int runs, in
   return cudaLaunchKernelEx(&cfg, place_kernel, ids, static_cast<int>(S), groups, run_slots, run_counts, order, offsets);
 }
 
-// y [T * top] rows -> out [T] rows: out = resid + sum_j w_j y_j, choices in order.
-template <int Y, int O>
+// y [T * top] rows -> out [T] rows: out = resid + sum_j w_j y_j, choices in
+// order.  A thread has N columns of one token and asks for four choices' values
+// at a time.  Bound by the bytes of y.
+template <int Y, int O, int N>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   using YV = typename Val<Y>::type;
   using OV = typename Val<O>::type;
-  const int64_t t = blockIdx.x;
-  for (int64_t n = threadIdx.x; n < a.n; n += 256) {
-    float sum = 0.0f;
-    for (int j = 0; j < a.top; ++j) {
-      const int64_t s = t * a.top + j;
-      if (a.ids && __ldg(a.ids + s) < 0) continue;
-      sum = fmaf(__ldg(a.weights + s), Val<Y>::load(static_cast<const YV*>(a.y) + s * a.ldy + n), sum);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t n = (static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x) * N;
+  if (t >= a.T || n >= a.n) return;
+  float sum[N] = {}, more[N];
+  if (a.resid) load_vec<O>(static_cast<const OV*>(a.resid) + t * a.ldr + n, more);
+  const YV* y = static_cast<const YV*>(a.y) + t * a.top * a.ldy + n;
+  const float* w = a.weights + t * a.top;
+  const int32_t* ids = a.ids ? a.ids + t * a.top : nullptr;
+  for (int j0 = 0; j0 < a.top; j0 += 4) {
+    float v[4][N], share[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool there = j0 + j < a.top && !(ids && __ldg(ids + j0 + j) < 0);
+      share[j] = there ? __ldg(w + j0 + j) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[j][i] = 0.0f;
+      if (there) load_vec<Y>(y + (j0 + j) * a.ldy, v[j]);
     }
-    if (a.resid) sum += Val<O>::load(static_cast<const OV*>(a.resid) + t * a.ldr + n);
-    static_cast<OV*>(a.out)[t * a.ldo + n] = Val<O>::to(sum);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] = fmaf(share[j], v[j][i], sum[i]);
   }
+  if (a.resid)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] += more[i];
+  store_vec<O>(static_cast<OV*>(a.out) + t * a.ldo + n, sum);
 }
 
 }  // namespace
@@ -322,11 +340,32 @@ cudaError_t launch_group_rows(const int32_t* ids, int64_t S, int groups, int32_t
 }
 
 cudaError_t launch_combine(const CombineArgs& a, int ytype, int otype, cudaStream_t s) {
-  void (*kernels[3][3])(const CombineArgs) = {
-      {combine_kernel<0, 0>, combine_kernel<0, 1>, combine_kernel<0, 2>},
-      {combine_kernel<1, 0>, combine_kernel<1, 1>, combine_kernel<1, 2>},
-      {combine_kernel<2, 0>, combine_kernel<2, 1>, combine_kernel<2, 2>}};
-  kernels[ytype][otype]<<<static_cast<unsigned>(a.T), 256, 0, s>>>(a);
+  // N columns a thread where every row starts on them, else one.  8 of 16 bits; 4 where a type has 32.
+  const int wide = ytype == kXF32 || otype == kXF32 ? 4 : 8;
+  const int ys = ytype == kXF32 ? 4 : 2, os = otype == kXF32 ? 4 : 2;
+  auto on = [&](const void* p, int64_t ld, int size) {
+    return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * size)) % (wide * size) == 0;
+  };
+  const bool vec = a.n % wide == 0 && on(a.y, a.ldy, ys) && on(a.out, a.ldo, os) && (!a.resid || on(a.resid, a.ldr, os));
+  const int n = vec ? wide : 1;
+  const int64_t cols = (a.n + n - 1) / n;
+  int tx = 32;
+  while (tx < 128 && tx < cols) tx *= 2;
+  const dim3 block(tx, 256 / tx);
+  const dim3 grid(static_cast<unsigned>((a.T + block.y - 1) / block.y), static_cast<unsigned>((cols + tx - 1) / tx));
+  auto pick = [&](auto y, auto o) {
+    constexpr int Y = decltype(y)::value, O = decltype(o)::value, N = Y == 0 || O == 0 ? 4 : 8;
+    auto k = vec ? combine_kernel<Y, O, N> : combine_kernel<Y, O, 1>;
+    k<<<grid, block, 0, s>>>(a);
+  };
+  auto pick_o = [&](auto y) {
+    if (otype == kXF32) pick(y, std::integral_constant<int, 0>());
+    else if (otype == kXF16) pick(y, std::integral_constant<int, 1>());
+    else pick(y, std::integral_constant<int, 2>());
+  };
+  if (ytype == kXF32) pick_o(std::integral_constant<int, 0>());
+  else if (ytype == kXF16) pick_o(std::integral_constant<int, 1>());
+  else pick_o(std::integral_constant<int, 2>());
   return cudaGetLastError();
 }
 

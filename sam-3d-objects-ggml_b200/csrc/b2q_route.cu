@@ -6,10 +6,11 @@
 //   order   = the slots (token * top + choice) sorted by expert, stable
 //   offsets = where each expert's slots begin
 //
-// A row's experts are spread over the lanes of one warp, as unsigned numbers
-// that order as the keys do (-0 as 0, NaN as -infinity).  Each choice is one
-// warp maximum (redux) and, among the lanes that hold it, one minimum of the
-// index.
+// A row's experts are spread over the lanes of one warp and stay in registers,
+// as unsigned numbers that order as the keys do (-0 as 0, NaN as -infinity).  Each
+// choice is one warp maximum (redux) of the lanes' largest and, among the lanes
+// that hold it, one minimum of the expert's number; its lane then looks for its
+// next largest.
 //
 // The sort is a counting sort without float work or global atomics: every CTA
 // counts the experts of its run of slots; then every CTA adds up the counts of
@@ -27,10 +28,10 @@ namespace b2q {
 
 namespace {
 
-constexpr int kWarps = 16, kThreads = kWarps * 32;
-constexpr int kRunSlots = 1024;      // of one CTA, at least
-constexpr int kMaxRuns = 296;
-constexpr int kOneSlots = 2048;      // up to these many slots one CTA does everything
+constexpr int kWarps = 32, kThreads = kWarps * 32;
+constexpr int kRunSlots = 512;       // of one CTA, at least
+constexpr int kMaxRuns = 148;
+constexpr int kOneSlots = 512;       // up to these many slots one CTA does everything
 
 __device__ __forceinline__ uint32_t key_bits(float v) {
   if (v != v) v = -INFINITY;
@@ -87,26 +88,42 @@ __device__ void place_run(const int32_t* ids, int S, int groups, int run, int ru
   __syncthreads();
   for (int s = lo + lane; s < hi; s += 32) atomicAdd(&counts[warp * G + group_of(ids, s, groups)], 1);
   __syncthreads();
-  // Totals of every group, and of the runs before this one.
+  // Totals of every group, and of the runs before this one: a warp a run, its lanes the groups.
+  int* total = sums + kWarps;
+  for (int g = threadIdx.x; g < G; g += kThreads) {
+    int c = 0;
+    if (!run_counts)
+      for (int w = 0; w < kWarps; ++w) c += counts[w * G + g];
+    total[g] = c;
+    base[g] = 0;
+  }
+  __syncthreads();
+  if (run_counts) {
+    for (int g = lane; g < G; g += 32) {
+      int all = 0, before = 0;
+      for (int r0 = warp; r0 < runs; r0 += 5 * kWarps) {
+        int c[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          const int r = r0 + i * kWarps;
+          c[i] = r < runs ? __ldg(run_counts + static_cast<int64_t>(r) * G + g) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          all += c[i];
+          if (r0 + i * kWarps < run) before += c[i];
+        }
+      }
+      atomicAdd(&total[g], all);
+      atomicAdd(&base[g], before);
+    }
+    __syncthreads();
+  }
   const int each = (G + kThreads - 1) / kThreads;
   int mine = 0;
   for (int i = 0; i < each; ++i) {
     const int g = threadIdx.x * each + i;
-    if (g >= G) break;
-    int total = 0, before = 0;
-    if (run_counts) {
-      for (int r = 0; r < runs; ++r) {
-        const int c = run_counts[static_cast<int64_t>(r) * G + g];
-        total += c;
-        if (r < run) before += c;
-      }
-    } else {
-      for (int w = 0; w < kWarps; ++w) total += counts[w * G + g];
-    }
-    base[g] = before;
-    mine += total;
-    // the totals are needed once more below; keep them in the order's sums
-    sums[kWarps + g] = total;
+    if (g < G) mine += total[g];
   }
   int at = block_exclusive(mine, sums);
   for (int i = 0; i < each; ++i) {
@@ -114,7 +131,7 @@ __device__ void place_run(const int32_t* ids, int S, int groups, int run, int ru
     if (g >= G) break;
     if (run == 0) offsets[g] = at;
     int place = at + base[g];
-    at += sums[kWarps + g];
+    at += total[g];
     for (int w = 0; w < kWarps; ++w) {  // where each warp's slots of this group begin
       const int c = counts[w * G + g];
       counts[w * G + g] = place;
@@ -138,62 +155,78 @@ __device__ void place_run(const int32_t* ids, int S, int groups, int run, int ru
 
 size_t place_smem(int groups) { return (static_cast<size_t>(kWarps + 2) * (groups + 1) + kWarps) * 4; }
 
-template <int T, bool ONE>
+// NV: experts of a lane.
+template <int T, int NV>
 __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
   extern __shared__ int smem[];
   using V = typename Val<T>::type;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int E = a.E;
-  if constexpr (!ONE) {
+  const bool one = a.run_counts == nullptr;
+  if (!one) {
     for (int i = threadIdx.x; i <= E; i += kThreads) smem[i] = 0;
     __syncthreads();
   }
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.run_rows;
   const int64_t t1 = min(t0 + a.run_rows, a.T);
-  for (int64_t t = t0 + warp; t < t1; t += kWarps) {
+  float x[NV], next[NV];
+  auto fetch = [&](int64_t t) {
     const V* row = static_cast<const V*>(a.logits) + t * a.ld;
-    // Lane l holds experts l, l + 32, ...: the largest key that is left of them.
-    float mx = -INFINITY;
-    uint32_t last = 0xffffffffu;  // the key and expert of the last choice: what is left lies behind it
-    int last_e = -1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) next[i] = lane + 32 * i < E ? Val<T>::load(row + lane + 32 * i) : -INFINITY;
+  };
+  if (t0 + warp < t1) fetch(t0 + warp);
+  for (int64_t t = t0 + warp; t < t1; t += kWarps) {
+    uint32_t key[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = next[i];
+      const int e = lane + 32 * i;
+      key[i] = e < E ? key_bits(a.bias ? x[i] + __ldg(a.bias + e) : x[i]) : 0u;
+    }
+    if (t + kWarps < t1) fetch(t + kWarps);
     float picked = 0.0f;  // lane j: the logit of choice j
     int chosen = -1;
     for (int j = 0; j < a.top; ++j) {
-      uint32_t best = 0;
-      int best_e = 0x7fffffff;
-      for (int e = lane; e < E; e += 32) {
-        const float x = Val<T>::load(row + e);
-        const uint32_t k = key_bits(a.bias ? x + __ldg(a.bias + e) : x);
-        if (j == 0 && x == x) mx = fmaxf(mx, x);
-        const bool left = k < last || (k == last && e > last_e);
-        if (left && k > best) best = k, best_e = e;
-      }
+      uint32_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < NV; ++i) best = max(best, key[i]);
       const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == top ? static_cast<unsigned>(best_e) : 0x7fffffffu));
       if (top <= kKeyNone) break;  // only -infinity is left
-      last = top;
-      last_e = e;
-      if (lane == j) {
-        chosen = e;
-        picked = Val<T>::load(row + e);
-      }
+      unsigned mine = 0x7fffffffu;  // the lane's lowest expert with that key
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+        if (key[i] == top) mine = lane + 32 * i;
+      const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) key[i] = e == lane + 32 * i ? 0u : key[i];
+      chosen = lane == j ? e : chosen;
     }
     const bool there = chosen >= 0;
+    // lane j: the logit of choice j, from the lane that has it
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float v = __shfl_sync(0xffffffffu, x[i], chosen & 31);
+      if (chosen >> 5 == i) picked = v;
+    }
     float w = 0.0f;
     if (a.scoring == 1) {
       if (there) w = 1.0f / (1.0f + expf(-picked));
     } else {
       // the largest logit of all (of the choice, when only the choice counts); its own weight is e^0, also where it is infinite
-      float m = a.renorm ? (there ? picked : -INFINITY) : mx;
+      float m = there ? picked : -INFINITY;
+      if (!a.renorm) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) m = fmaxf(m, x[i]);  // (fmaxf passes over NaN)
+      }
 #pragma unroll
       for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (there) w = picked == m ? 1.0f : expf(picked - m);
       if (!a.renorm) {
         float z = 0.0f;
-        for (int e = lane; e < E; e += 32) {
-          const float x = Val<T>::load(row + e);
-          if (x == x) z += x == m ? 1.0f : expf(x - m);
-        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (lane + 32 * i < E && x[i] == x[i]) z += x[i] == m ? 1.0f : expf(x[i] - m);
 #pragma unroll
         for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
         if (there) w /= z;
@@ -208,11 +241,11 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
     if (lane < a.top) {
       a.ids[t * a.top + lane] = chosen;
       a.weights[t * a.top + lane] = w * a.scale;
-      if constexpr (!ONE) atomicAdd(&smem[there ? chosen : E], 1);
+      if (!one) atomicAdd(&smem[there ? chosen : E], 1);
     }
   }
   __syncthreads();
-  if constexpr (ONE) {
+  if (one) {
     place_run(a.ids, static_cast<int>(a.T * a.top), E, 0, 1, static_cast<int>(a.T * a.top), nullptr, a.order,
               a.offsets, smem);
   } else {
@@ -318,12 +351,28 @@ cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
   const bool one = p.runs == 1;
   a.run_rows = one ? a.T : p.run_units;
   const size_t smem = one ? place_smem(a.E) : (a.E + 1) * 4;
-  void (*kernels[3][2])(const RouteArgs) = {{route_kernel<0, false>, route_kernel<0, true>},
-                                            {route_kernel<1, false>, route_kernel<1, true>},
-                                            {route_kernel<2, false>, route_kernel<2, true>}};
-  auto k = kernels[type][one];
-  if (cudaError_t e = set_smem(reinterpret_cast<const void*>(k), smem)) return e;
-  k<<<p.runs, kThreads, smem, s>>>(a);
+  if (one) a.run_counts = nullptr;
+  auto run = [&](auto ty) {
+    constexpr int T = decltype(ty)::value;
+    const int nv = (a.E + 31) / 32;
+    auto go = [&](auto k) {
+      if (cudaError_t e = set_smem(reinterpret_cast<const void*>(k), smem)) return e;
+      k<<<p.runs, kThreads, smem, s>>>(a);
+      return cudaSuccess;
+    };
+    if (nv <= 1) return go(route_kernel<T, 1>);
+    if (nv <= 2) return go(route_kernel<T, 2>);
+    if (nv <= 3) return go(route_kernel<T, 3>);
+    if (nv <= 4) return go(route_kernel<T, 4>);
+    if (nv <= 5) return go(route_kernel<T, 5>);
+    if (nv <= 6) return go(route_kernel<T, 6>);
+    if (nv <= 8) return go(route_kernel<T, 8>);
+    if (nv <= 16) return go(route_kernel<T, 16>);
+    return go(route_kernel<T, 32>);
+  };
+  const cudaError_t err = type == kXF32 ? run(std::integral_constant<int, 0>())
+                          : type == kXF16 ? run(std::integral_constant<int, 1>()) : run(std::integral_constant<int, 2>());
+  if (err != cudaSuccess) return err;
   if (cudaError_t e = cudaGetLastError()) return e;
   if (one) return cudaSuccess;
   return launch_place(a.ids, a.T * a.top, a.E, p.runs, p.run_units * a.top, a.run_counts, a.order, a.offsets, s);

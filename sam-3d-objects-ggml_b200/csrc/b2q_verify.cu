@@ -8,10 +8,14 @@
 // tokens of a large vocabulary would move by more than a rare token is wide.
 //
 // A cluster of CTAs has one request: each looks at the drafts itself (a warp, a
-// draft a lane), sums its part of the one row that counts, and hands its sum to
-// the others; the CTA, and in it the warp, whose part holds the border goes
-// through that part again.  Every value is read from memory once, the drafts'
-// own probabilities and that last part apart.
+// draft a lane), sums its part of the one row that counts, a piece a warp, and
+// hands its sum to the others.  The CTA that finds the border in the piece of one
+// of its warps shares that piece out among all of them again, and so on, until
+// what is left is one warp's few values.  Every value is read from memory once,
+// those pieces apart.
+// Bound by that read; a thread asks for 8 values of each row at a time, and an SM
+// has 6 CTAs, so that enough are on their way (rows of any alignment: values are
+// read one by one, 32 neighbours a warp).
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
@@ -20,13 +24,15 @@ namespace b2q {
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kBatch = 8;  // values of a row that a thread asks for at a time
 
 // One weight of the draw: target probability p against draft probability q.
 // What is not a finite number above 0 counts as 0.
 __device__ __forceinline__ double weight(float p, float q) {
-  if (!(p > q) || !(p > 0.0f) || p == INFINITY) return 0.0;
-  return static_cast<double>(p) - static_cast<double>(q);
+  // (p > 0 and p > q, also where q is NaN, which is neither below nor above)
+  const bool counts = p > fmaxf(q, 0.0f) && q == q && p < INFINITY;
+  return counts ? static_cast<double>(p) - static_cast<double>(q) : 0.0;
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -36,7 +42,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 template <int T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a) {
   using V = typename Val<T>::type;
   __shared__ double sums[kWarps], totals[kVerifyRanks], mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -80,17 +86,49 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   const int64_t j0 = min(a.V, (static_cast<int64_t>(rank) * kWarps + warp) * part);
   const int64_t j1 = min(a.V, j0 + part);
   bool residual = down;
+  // The weights of the warp's values from j on, 32 a step.
+  auto fetch = [&](int64_t j, int64_t end, float (&pv)[kBatch], float (&qv)[kBatch]) {
+    const V* pp = p_row + j + lane;
+    const V* qq = q_row + j + lane;
+    const bool with_q = residual && q_row;
+    if (j + kBatch * 32 <= end) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) pv[i] = Val<T>::load(pp + i * 32);
+      if (with_q) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) qv[i] = Val<T>::load(qq + i * 32);
+        return;
+      }
+    } else {
+      const int left = static_cast<int>(end - j) - lane;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) pv[i] = i * 32 < left ? Val<T>::load(pp + i * 32) : 0.0f;
+      if (with_q) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) qv[i] = i * 32 < left ? Val<T>::load(qq + i * 32) : 0.0f;
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) qv[i] = 0.0f;
+    if (residual) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) qv[i] = j + i * 32 + lane == skip ? 1.0f : 0.0f;
+    }
+  };
+  auto sum_of = [&](int64_t from, int64_t end) {
+    double sum = 0.0;
+    for (int64_t j = from; j < end; j += kBatch * 32) {
+      float pv[kBatch], qv[kBatch];
+      fetch(j, end, pv, qv);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) sum += weight(pv[i], qv[i]);
+    }
+    return warp_sum(sum);
+  };
   double total = 0.0, before = 0.0;
   while (true) {
-    double sum = 0.0;
-#pragma unroll 4
-    for (int64_t j = j0 + lane; j < j1; j += 32) {
-      const float p = Val<T>::load(p_row + j);
-      float q = 0.0f;
-      if (residual) q = q_row ? Val<T>::load(q_row + j) : (j == skip ? 1.0f : 0.0f);
-      sum += weight(p, q);
-    }
-    sum = warp_sum(sum);
+    const double sum = sum_of(j0, j1);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
     double cta = 0.0;
@@ -117,47 +155,75 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
     residual = false;  // nothing is left of p above q
     __syncthreads();
   }
-  // The border, and the warp whose part it falls into: the first with a weight
-  // whose end lies behind it, or the last with one when rounding (or v >= 1) puts
-  // it at the very end.  A CTA's last such warp ends where the next CTA begins,
-  // so that the parts meet whatever the sums were rounded to.
-  const float v = __ldg(a.v + b);
-  const double edge = (v > 0.0f ? static_cast<double>(v) : 0.0) * total;
-  int64_t found = -1;
-  bool later = false, last_here = true;  // a weight in a later CTA, in a later warp of this one
-  double start = before;
-  for (int w = 0; w < warp; ++w) start += sums[w];
-  for (int w = warp + 1; w < kWarps; ++w) last_here &= sums[w] == 0.0;
-  for (int r = rank + 1; r < ranks; ++r) later |= totals[r] > 0.0;
-  const double stop = last_here ? before + totals[rank] : start + sums[warp];
-  const bool holds = sums[warp] > 0.0 && start <= edge && (edge < stop || (last_here && !later));
   if (total > 0.0) {
-    if (holds) {
-      double run = start;
-      int64_t last = -1;
-      for (int64_t jj = j0; jj < j1 && found < 0; jj += 32) {
-        const int64_t j = jj + lane;
-        double w = 0.0;
-        if (j < j1) {
-          const float p = Val<T>::load(p_row + j);
-          float q = 0.0f;
-          if (residual) q = q_row ? Val<T>::load(q_row + j) : (j == skip ? 1.0f : 0.0f);
-          w = weight(p, q);
+    // The border, and the piece it falls into: the first with a weight whose end lies
+    // behind it, or the last with one when rounding (or v >= 1) puts it at the
+    // very end.  The last such piece of what is shared out ends where that ends, so
+    // that pieces meet whatever their sums were rounded to.
+    const float v = __ldg(a.v + b);
+    const double edge = (v > 0.0f ? static_cast<double>(v) : 0.0) * total;
+    bool later = false;  // a weight behind what is shared out
+    for (int r = rank + 1; r < ranks; ++r) later |= totals[r] > 0.0;
+    double start = before, stop = before + totals[rank];
+    int64_t from = static_cast<int64_t>(rank) * kWarps * part, size = part;
+    bool here = totals[rank] > 0.0 && start <= edge && (edge < stop || !later);
+    while (here) {  // (the same in all threads of the CTA)
+      int holder = -1;
+      double run = start, begin = start, end = start;
+      bool after = later;
+      for (int w = 0; w < kWarps; ++w) {
+        if (sums[w] == 0.0) continue;
+        // the last one with a weight so far; an earlier one holds the border if it ends behind it
+        if (holder >= 0 && edge < end) {
+          after = true;
+          break;
         }
-        double inc = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double up = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += up;
-        }
-        const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && run + inc > edge);
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-        if (over) found = jj + __ffs(over) - 1;
-        if (some) last = jj + 31 - __clz(some);
-        run += __shfl_sync(0xffffffffu, inc, 31);
+        holder = w;
+        begin = run;
+        run += sums[w];
+        end = run;
       }
-      if (found < 0) found = last;
-      if (lane == 0) a.tokens[first + b] = static_cast<int32_t>(found);
+      if (holder < 0) break;  // (sums that are not 0 had such a piece)
+      bool last = true;
+      for (int w = holder + 1; w < kWarps; ++w) last &= sums[w] == 0.0;
+      if (last) end = stop;
+      later = after || !last || later;
+      start = begin;
+      stop = end;
+      const int64_t limit = min(a.V, from + (holder + 1) * size);
+      from += holder * size;
+      if (size <= 2 * kBatch * 32) {
+        if (warp != holder) break;
+        double sum = start;
+        int64_t found = -1, seen = -1;
+        for (int64_t j = from; j < limit && found < 0; j += kBatch * 32) {
+          float pv[kBatch], qv[kBatch];
+          fetch(j, limit, pv, qv);
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const double w = weight(pv[i], qv[i]);
+            double inc = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double up = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += up;
+            }
+            const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && sum + inc > edge);
+            const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+            if (over && found < 0) found = j + i * 32 + __ffs(over) - 1;
+            if (some && found < 0) seen = j + i * 32 + 31 - __clz(some);
+            sum += __shfl_sync(0xffffffffu, inc, 31);
+          }
+        }
+        if (lane == 0) a.tokens[first + b] = static_cast<int32_t>(found >= 0 ? found : seen);
+        break;
+      }
+      // Share the piece out again.
+      size = ((limit - from + kWarps - 1) / kWarps + 31) / 32 * 32;
+      const double sum = sum_of(from + warp * size, min(limit, from + (warp + 1) * size));
+      __syncthreads();  // the sums before are no longer read
+      if (lane == 0) sums[warp] = sum;
+      __syncthreads();
     }
   } else if (rank == 0 && threadIdx.x == 0) {
     a.tokens[first + b] = -1;

@@ -682,7 +682,9 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * and b [G][n][rank] contiguous, of x's type (F16 or BF16; rank a multiple of 8,
  * at most 128; k % 8 == 0), scales fp32 [G] or NULL for 1.  resid and y of type F32 or
  * x's, the same buffer with the same stride, or disjoint.  The rank values
- * between the two products are kept to more than 16 bits.
+ * between the two products are kept to more than 16 bits.  Workspace (256-byte
+ * aligned) of b2q_lora_add_workspace_bytes; 0 for few rows per adapter, which
+ * take one launch.
  *
  * b2q_draft_verify: which drafted tokens a target model keeps, from given random
  * numbers.  Request b of B has the drafts cu_drafts[b] .. cu_drafts[b+1] - 1
@@ -715,10 +717,12 @@ B2Q_API int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n,
 B2Q_API int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const float* weights,
                             const int32_t* ids, int64_t T, int64_t top, int64_t n, int otype, const void* resid,
                             int64_t resid_row_stride_bytes, void* out, int64_t out_row_stride_bytes, void* stream);
+B2Q_API size_t b2q_lora_add_workspace_bytes(int64_t T, int64_t k, int64_t adapters, int64_t rank);
 B2Q_API int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
                          const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales,
                          const int32_t* order, const int32_t* offsets, int ytype, const void* resid,
-                         int64_t resid_row_stride_bytes, void* y, int64_t y_row_stride_bytes, void* stream);
+                         int64_t resid_row_stride_bytes, void* y, int64_t y_row_stride_bytes, void* workspace,
+                         size_t workspace_bytes, void* stream);
 B2Q_API int b2q_draft_verify(int type, const void* target, int64_t target_row_stride_bytes, const void* draft_probs,
                              int64_t draft_row_stride_bytes, const int32_t* drafts, const int32_t* cu_drafts,
                              int64_t B, int64_t D, int64_t V, const float* u, const float* v, int32_t* accepted,

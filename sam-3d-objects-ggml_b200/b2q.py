@@ -127,7 +127,8 @@ def _lib_obj():
             "b2q_group_rows": (I, [P, I64, I64, P, P, P, SZ, P]),
             "b2q_mul_mat_id": (I, [I, P, I64, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, I, I, P, I64, P]),
             "b2q_moe_combine": (I, [I, P, I64, P, P, I64, I64, I64, I, P, I64, P, I64, P]),
-            "b2q_lora_add": (I, [I, P, I64, I64, I64, P, P, I64, I64, I64, P, P, P, I, P, I64, P, I64, P]),
+            "b2q_lora_add_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+            "b2q_lora_add": (I, [I, P, I64, I64, I64, P, P, I64, I64, I64, P, P, P, I, P, I64, P, I64, P, SZ, P]),
             "b2q_draft_verify": (I, [I, P, I64, P, I64, P, P, I64, I64, I64, P, P, P, P, P]),
         }
         for name, (res, args) in sig.items():
@@ -1084,6 +1085,7 @@ def moe_combine(y, weights, ids=None, resid=None, out_dtype=None, out=None, stre
 
 
 LORA_MAX_RANK = 128
+_lora_ws_bytes = functools.lru_cache(maxsize=256)(lambda T, k, G, rank: lib().b2q_lora_add_workspace_bytes(T, k, G, rank))
 
 
 def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
@@ -1108,10 +1110,14 @@ def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
     else:
         assert _are_rows(out, T, n, resid.dtype) and (out.stride(0) >= n or T <= 1)
     ytype, ys = _val_type(resid.dtype)
+    need, ws = _lora_ws_bytes(T, k, G, rank), None
+    if need:
+        ws = _empty_on(stream, need, torch.uint8, x.device)
     rc = (_lib or _lib_obj()).b2q_lora_add(
         _type16(dt), x.data_ptr(), T, k, 2 * (ldx if ldx > k else k), a.data_ptr(), b.data_ptr(), G, rank, n,
         _ptr(scales), order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * max(resid.stride(0), n),
-        out.data_ptr(), ys * max(out.stride(0), n), _raw_stream(stream, x, a, b, scales, order, offsets, resid, out))
+        out.data_ptr(), ys * max(out.stride(0), n), _ptr(ws), need,
+        _raw_stream(stream, x, a, b, scales, order, offsets, resid, out))
     if rc:
         _check("b2q_lora_add", rc)
     return out

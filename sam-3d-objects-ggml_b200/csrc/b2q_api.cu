@@ -1561,16 +1561,27 @@ int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const 
   return from_cuda(launch_combine(a, yt, ot, static_cast<cudaStream_t>(stream)));
 }
 
+static int lora_sizes(int64_t T, int64_t k, int64_t adapters, int64_t rank) {
+  if (T < 0 || k <= 0 || k % 8 != 0 || adapters <= 0 || rank <= 0 || rank % 8 != 0) return B2Q_ERR_INVALID_ARG;
+  if (T > kMaxSlots || k > (1 << 28) || adapters > kMaxGroups || rank > kLoraMaxRank) return B2Q_ERR_TOO_LARGE;
+  return B2Q_OK;
+}
+
+size_t b2q_lora_add_workspace_bytes(int64_t T, int64_t k, int64_t adapters, int64_t rank) {
+  return lora_sizes(T, k, adapters, rank) == B2Q_OK
+             ? lora_workspace(T, k, static_cast<int>(adapters), static_cast<int>(rank)) : 0;
+}
+
 int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
                  const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales, const int32_t* order,
                  const int32_t* offsets, int ytype, const void* resid, int64_t resid_row_stride_bytes, void* y,
-                 int64_t y_row_stride_bytes, void* stream) {
+                 int64_t y_row_stride_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   if (xtype != B2Q_TYPE_F16 && xtype != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
   if (ytype != B2Q_TYPE_F32 && ytype != xtype) return B2Q_ERR_UNSUPPORTED;
   const int ys = ytype == B2Q_TYPE_F32 ? 4 : 2;
-  if (T < 0 || k <= 0 || k % 8 != 0 || adapters <= 0 || rank <= 0 || rank % 8 != 0 || n < 0) return B2Q_ERR_INVALID_ARG;
-  if (T > kMaxSlots || k > (1 << 28) || n > INT_MAX || adapters > kMaxGroups || rank > kLoraMaxRank)
-    return B2Q_ERR_TOO_LARGE;
+  if (n < 0) return B2Q_ERR_INVALID_ARG;
+  if (int rc = lora_sizes(T, k, adapters, rank)) return rc;
+  if (n > INT_MAX) return B2Q_ERR_TOO_LARGE;
   const bool any = T > 0 && n > 0;
   if (any && (!x || !a || !b || !order || !offsets || !resid || !y)) return B2Q_ERR_INVALID_ARG;
   if (x_row_stride_bytes < k * 2 || y_row_stride_bytes < n * ys || resid_row_stride_bytes < n * ys ||
@@ -1578,9 +1589,11 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
     return B2Q_ERR_INVALID_ARG;
   if (!aligned(x, 16) || x_row_stride_bytes % 16 != 0 || !aligned(a, 16) || !aligned(b, 16) || !aligned(scales, 4) ||
       !aligned(order, 4) || !aligned(offsets, 4) || !aligned(resid, ys) || resid_row_stride_bytes % ys != 0 ||
-      !aligned(y, ys) || y_row_stride_bytes % ys != 0)
+      !aligned(y, ys) || y_row_stride_bytes % ys != 0 || !aligned(workspace, 256))
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
+  const size_t need = lora_workspace(T, k, static_cast<int>(adapters), static_cast<int>(rank));
+  if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
   int sms = 0;
   if (int rc = check_device(&sms)) return rc;
   LoraArgs p{};
@@ -1600,6 +1613,7 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
   p.ldr = resid_row_stride_bytes / ys;
   p.y = y;
   p.ldy = y_row_stride_bytes / ys;
+  p.part = static_cast<float*>(workspace);
   return from_cuda(launch_lora(p, val_type(xtype), val_type(ytype), sms, static_cast<cudaStream_t>(stream)));
 }
 

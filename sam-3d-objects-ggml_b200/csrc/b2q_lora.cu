@@ -2,17 +2,21 @@
 //   y[t] = resid[t] + scale_g * B_g (A_g x[t]),  g = the adapter of row t
 // (rows of no adapter: y[t] = resid[t]).
 //
-// Bound by the rows' bytes (x read, resid read, y written) or, for single tokens,
-// by latency.  One launch: a cluster of 8 CTAs has a tile of 16 or 64 sorted rows.
-//   1  each CTA multiplies its eighth of K: h = A x, m16n8k16 products
-//   2  the partial h meet in the CTAs' shared memories: each CTA adds up the eighth
-//      of the rows that is its own, scales them, and hands them to all eight
+// Bound by the rows' bytes (x and resid read, y written) or, for single tokens, by
+// latency.  h = A x enters the second product as two 16-bit numbers (the value and
+// what rounding it left) of a power of two per row, so neither fp16's range nor the
+// 8 bits of bf16 limit it.  Products are m16n8k16; K and the rank are taken in an
+// order that suits the loads: lane q of a quad has 8 consecutive values of every 32
+// (4 of 16 where the rank is at most 16).
+//
+// Few rows per adapter: one launch, a cluster of 8 CTAs per tile of 16 sorted rows.
+//   1  each CTA multiplies its eighth of K
+//   2  the partial h meet in the CTAs' shared memories: each CTA adds up its own two
+//      rows, scales them, and hands them to all eight
 //   3  each CTA makes its eighth of the columns of y
-// so x, resid and y are moved once and no partial result leaves the chip.  h enters
-// the second product as two 16-bit numbers (the value and what rounding it left)
-// of a power of two per row, so neither fp16's range nor 8 bits of bf16 limit it.
-// K and the rank are taken in an order that suits the loads: lane q of a quad has
-// 8 consecutive values of every 32 (4 of 16 where the rank is at most 16).
+// More rows: two launches over tiles of 64 sorted rows.  The first makes h (cp.async
+// stages of x's and A's rows; K shared out where the tiles are few) in fp32 in the
+// workspace; the second, launched early, adds the parts up and streams y.
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
@@ -25,22 +29,40 @@ namespace {
 
 constexpr int kRanks = 8;  // CTAs of a cluster
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kStages = 3;
+constexpr int kStages = 4;
 constexpr int kStageK = 64;
 
-template <int MT, int RP>  // 16-row groups of a tile; rank, padded to 16, 32, 64 or 128
-struct LoraShape {
-  static constexpr int M = 16 * MT;
-  static constexpr int SPLIT = kWarps / MT;  // warps that share a row group's K
-  static constexpr int PIPE = MT == 1 ? 0 : kStages * (M + RP) * 128;
-  static constexpr int PART = kWarps * 16 * RP * 4;
-  static constexpr int SUM = M * RP * 4;     // this CTA's h
-  static constexpr int PITCH = RP * 2 + (RP >= 64 ? 64 : 0);  // bytes of a row of h's 16-bit numbers: conflict-free reads
-  static constexpr int OFF_SUM = PART;
-  static constexpr int OFF_H = (PIPE > PART + SUM ? PIPE : PART + SUM);
-  static constexpr int OFF_EXP = OFF_H + 2 * M * PITCH;
+// RP: the rank, padded to 16, 32, 64 or 128.  Bytes of a row of h's 16-bit numbers: conflict-free reads.
+template <int RP>
+constexpr int kPitch = RP * 2 + (RP >= 64 ? 64 : 0);
+
+template <int RP>
+struct ClusterShape {
+  static constexpr int M = 16;
+  static constexpr int OFF_SUM = kWarps * 16 * RP * 4;  // behind the warps' parts: this CTA's h
+  static constexpr int OFF_H = OFF_SUM + M * RP * 4;
+  static constexpr int OFF_EXP = OFF_H + 2 * M * kPitch<RP>;
   static constexpr int OFF_ROW = OFF_EXP + M * 4;
   static constexpr int SMEM = OFF_ROW + M * 4;
+};
+constexpr int kTile = 64;  // rows of the two-launch form
+constexpr int kMaxSplits = 8;
+template <int RP>
+struct ShrinkShape {
+  static constexpr int STAGE = (kTile + RP) * 128;
+  static constexpr int PART = kWarps * 16 * RP * 4;
+  static constexpr int OFF_ROW = kStages * STAGE > PART ? kStages * STAGE : PART;
+  static constexpr int SMEM = OFF_ROW + kTile * 4;
+};
+template <int RP, int YS>
+struct ExpandShape {
+  static constexpr int COLS = 64, STAGES = 3;  // of one stage of y's and B's columns
+  static constexpr int YROW = COLS * YS, BROW = RP * 2;
+  static constexpr int STAGE = kTile * YROW + COLS * BROW;
+  static constexpr int OFF_H = STAGES * STAGE;
+  static constexpr int OFF_EXP = OFF_H + 2 * kTile * kPitch<RP>;
+  static constexpr int OFF_ROW = OFF_EXP + kTile * 4;
+  static constexpr int SMEM = OFF_ROW + kTile * 4;
 };
 
 template <int X>
@@ -55,8 +77,9 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// (256 bytes of a row come into the L2 at once: its next pieces are asked for soon.)
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
 // Two 16-bit numbers of type X in one word, and back.
@@ -71,48 +94,9 @@ __device__ __forceinline__ float from16(uint16_t b) {
   else return __bfloat162float(__ushort_as_bfloat16(b));
 }
 
-// Two columns of y; aligned: one access of both.
-template <int Y>
-__device__ __forceinline__ float2 load2(const typename Val<Y>::type* p, bool aligned, bool second) {
-  if (aligned && second) {
-    if constexpr (Y == 0) return *reinterpret_cast<const float2*>(p);
-    else {
-      const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-      return make_float2(from16<Y>(static_cast<uint16_t>(u)), from16<Y>(static_cast<uint16_t>(u >> 16)));
-    }
-  }
-  return make_float2(Val<Y>::load(p), second ? Val<Y>::load(p + 1) : 0.0f);
-}
-template <int Y>
-__device__ __forceinline__ void store2(typename Val<Y>::type* p, float2 v, bool aligned, bool second) {
-  if (aligned && second) {
-    if constexpr (Y == 0) *reinterpret_cast<float2*>(p) = v;
-    else *reinterpret_cast<uint32_t*>(p) = bits16<Y>(v.x) | (static_cast<uint32_t>(bits16<Y>(v.y)) << 16);
-    return;
-  }
-  *p = Val<Y>::to(v.x);
-  if (second) p[1] = Val<Y>::to(v.y);
-}
-
-template <int X, int Y, int MT, int RP>
-__global__ void __launch_bounds__(kThreads) lora_kernel(const LoraArgs p) {
-  using Sh = LoraShape<MT, RP>;
-  using YV = typename Val<Y>::type;
-  constexpr int M = Sh::M, SPLIT = Sh::SPLIT, N8 = RP / 8;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem);
-  float* sum = reinterpret_cast<float*>(smem + Sh::OFF_SUM);
-  float* power = reinterpret_cast<float*>(smem + Sh::OFF_EXP);
-  int* row_of = reinterpret_cast<int*>(smem + Sh::OFF_ROW);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, q = lane & 3;
-  const int rank = static_cast<int>(cluster_ctarank());
-  const int rg = warp % MT, split = warp / MT;
-
-  const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / kRanks, M);
-  if (t.group < 0) return;  // (all eight CTAs)
-  const bool live = t.group < p.groups;
-  if (!live && p.resid == p.y) return;
+// The rows of tile t: row_of[i], -1 where there is none.
+template <int M>
+__device__ __forceinline__ void tile_rows(const LoraArgs& p, const GroupTile& t, int* row_of) {
   for (int i = threadIdx.x; i < M; i += kThreads) {
     int r = -1;
     if (t.begin + i < t.end) {
@@ -121,95 +105,192 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const LoraArgs p) {
     }
     row_of[i] = r;
   }
+}
+
+// A row's PER rank values in a lane -> 16-bit numbers and what rounding them left, at most 1 in magnitude, and the
+// power of two that they were divided by.  (fmaxf passes over NaN; a row with an infinity keeps its values.)
+// WIDTH neighbouring lanes have the row.
+template <int X, int PER, int WIDTH>
+__device__ __forceinline__ float split_row(const float (&v)[PER], uint32_t (&hi)[PER / 2], uint32_t (&lo)[PER / 2]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+  for (int o = WIDTH / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  int e2 = 0;
+  if (top > 0.0f && top < INFINITY) frexpf(top, &e2);
+  e2 = max(-126, min(126, e2));
+  const float down = __int_as_float((127 - e2) << 23);
+#pragma unroll
+  for (int e = 0; e < PER; e += 2) {
+    uint16_t h[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float w = v[e + i] * down;
+      h[i] = bits16<X>(w);
+      const float rest = w - from16<X>(h[i]);
+      l[i] = bits16<X>(fabsf(w) < INFINITY ? rest : 0.0f);
+    }
+    hi[e / 2] = h[0] | (static_cast<uint32_t>(h[1]) << 16);
+    lo[e / 2] = l[0] | (static_cast<uint32_t>(l[1]) << 16);
+  }
+  return __int_as_float((127 + e2) << 23);
+}
+
+// Columns [n0, n1) of y for 16 rows of a tile, 32 columns at a time from n0 + split * 32 on, every `step`-th of them.
+// h: the lane's row of the 16-bit numbers (what rounding left lies `rest` bytes on); up: the powers of two of
+// rows g and g + 8.  32 columns are two groups of 16: lane q has columns 4 q .. 4 q + 3 of a group (2 q and 2 q + 1
+// of its two products), so y moves 4 values at a time.
+template <int X, int Y, int RP>
+__device__ __forceinline__ void stream_columns(const LoraArgs& p, int group, bool live, const uint8_t* h, int rest,
+                                               float up_a, float up_b, int row_a, int row_b, int64_t n0, int64_t n1,
+                                               int split, int step) {
+  using YV = typename Val<Y>::type;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const uint16_t* b = static_cast<const uint16_t*>(p.b) + static_cast<int64_t>(live ? group : 0) * p.N * p.rank;
+  const float up[2] = {up_a, up_b};
+  constexpr int YS = static_cast<int>(sizeof(YV));
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.resid) | reinterpret_cast<uintptr_t>(p.y) |
+                        static_cast<uintptr_t>(p.ldr * YS) | static_cast<uintptr_t>(p.ldy * YS)) % (4 * YS) == 0;
+  const bool have[2] = {row_a >= 0, row_b >= 0};
+  const YV* from[2] = {static_cast<const YV*>(p.resid) + (have[0] ? row_a : 0) * p.ldr + 4 * q,
+                       static_cast<const YV*>(p.resid) + (have[1] ? row_b : 0) * p.ldr + 4 * q};
+  YV* to[2] = {static_cast<YV*>(p.y) + (have[0] ? row_a : 0) * p.ldy + 4 * q,
+               static_cast<YV*>(p.y) + (have[1] ? row_b : 0) * p.ldy + 4 * q};
+  float y[2][2][4];  // [row][group of 16 columns]
+  auto read = [&](int64_t n) {
+    const bool full = aligned && n + 32 <= n1;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (full && have[r]) {
+          load_vec<Y>(from[r] + n + u * 16, y[r][u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[r][u][i] = have[r] && n + u * 16 + 4 * q + i < n1 ? Val<Y>::load(from[r] + n + u * 16 + i) : 0.0f;
+        }
+      }
+  };
+  if (n0 + split * 32 < n1) read(n0 + split * 32);
+  const int col_of = 4 * (g >> 1) + (g & 1);  // column of a group that lane row g brings; 2 more in the second product
+  for (int64_t n = n0 + split * 32; n < n1; n += step) {
+    float acc[4][4] = {};
+    if (live) {
+      const uint16_t* bn = b + (n + col_of) * p.rank;
+      const int left = static_cast<int>(min(n1 - n, int64_t{32})) - col_of;
+#pragma unroll
+      for (int kb = 0; kb < (RP == 16 ? 1 : RP / 32); ++kb) {
+        const int k = RP == 16 ? q * 4 : kb * 32 + q * 8;
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = (j >> 1) * 16 + (j & 1) * 2;
+          w[j] = make_uint4(0, 0, 0, 0);
+          if (c < left && k < p.rank) {
+            if constexpr (RP == 16) {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(bn + c * p.rank + k));
+              w[j].x = v.x, w[j].y = v.y;
+            } else {
+              w[j] = __ldg(reinterpret_cast<const uint4*>(bn + c * p.rank + k));
+            }
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {  // the numbers, then what rounding them left
+          const uint8_t* hs = h + s * rest + k * 2;
+          if constexpr (RP == 16) {
+            const uint2 u = *reinterpret_cast<const uint2*>(hs), v = *reinterpret_cast<const uint2*>(hs + 8 * kPitch<RP>);
+            const uint32_t a0[4] = {u.x, v.x, u.y, v.y};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma16<X>(acc[j], a0, w[j].x, w[j].y);
+          } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(hs), v = *reinterpret_cast<const uint4*>(hs + 8 * kPitch<RP>);
+            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              mma16<X>(acc[j], a0, w[j].x, w[j].y);
+              mma16<X>(acc[j], a1, w[j].z, w[j].w);
+            }
+          }
+        }
+      }
+    }
+    float out[2][2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (rows of no adapter stay as they are, to the bit)
+          out[r][u][i] = live ? fmaf(up[r], acc[2 * u + (i >> 1)][2 * r + (i & 1)], y[r][u][i]) : y[r][u][i];
+    // The next columns' values are asked for before these are written (y may be resid: other columns).
+    if (n + step < n1) read(n + step);
+    const bool full = aligned && n + 32 <= n1;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (!have[r]) continue;
+        if (full) {
+          store_vec<Y>(to[r] + n + u * 16, out[r][u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + u * 16 + 4 * q + i < n1) to[r][n + u * 16 + i] = Val<Y>::to(out[r][u][i]);
+        }
+      }
+  }
+}
+
+template <int X, int Y, int RP>
+__global__ void __launch_bounds__(kThreads) lora_cluster_kernel(const LoraArgs p) {
+  using Sh = ClusterShape<RP>;
+  constexpr int M = Sh::M, N8 = RP / 8;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* part = reinterpret_cast<float*>(smem);
+  float* sum = reinterpret_cast<float*>(smem + Sh::OFF_SUM);
+  float* power = reinterpret_cast<float*>(smem + Sh::OFF_EXP);
+  int* row_of = reinterpret_cast<int*>(smem + Sh::OFF_ROW);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, q = lane & 3;
+  const int rank = static_cast<int>(cluster_ctarank());
+
+  const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / kRanks, M);
+  if (t.group < 0) return;  // (all eight CTAs)
+  const bool live = t.group < p.groups;
+  if (!live && p.resid == p.y) return;
+  tile_rows<M>(p, t, row_of);
   __syncthreads();
-  const int64_t n_slice = ((p.N + kRanks - 1) / kRanks + 31) / 32 * 32;
-  const int64_t n0 = min(p.N, rank * n_slice), n1 = min(p.N, n0 + n_slice);
-  const int row_a = row_of[rg * 16 + g], row_b = row_of[rg * 16 + g + 8];
+  const int row_a = row_of[g], row_b = row_of[g + 8];
 
   if (live) {
     // ------------------------------------------------------ 1: this CTA's eighth of K
-    const int64_t k_slice = ((p.K + kRanks - 1) / kRanks + kStageK - 1) / kStageK * kStageK;
+    const int64_t k_slice = ((p.K + kRanks - 1) / kRanks + 31) / 32 * 32;
     const int64_t k0 = min(p.K, rank * k_slice), k1 = min(p.K, k0 + k_slice);
     const uint16_t* x = static_cast<const uint16_t*>(p.x);
     const uint16_t* a = static_cast<const uint16_t*>(p.a) + static_cast<int64_t>(t.group) * p.rank * p.K;
     float acc[N8][4] = {};
-    if constexpr (MT == 1) {
-      const uint16_t* xa = x + (row_a < 0 ? 0 : row_a) * p.ldx + q * 8;
-      const uint16_t* xb = x + (row_b < 0 ? 0 : row_b) * p.ldx + q * 8;
-#pragma unroll 2
-      for (int64_t k = k0 + warp * 32; k < k1; k += kWarps * 32) {
-        const bool in = k + q * 8 < k1;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        const uint4 u = in && row_a >= 0 ? __ldg(reinterpret_cast<const uint4*>(xa + k)) : zero;
-        const uint4 v = in && row_b >= 0 ? __ldg(reinterpret_cast<const uint4*>(xb + k)) : zero;
-        uint4 w[N8];
-#pragma unroll
-        for (int j = 0; j < N8; ++j)
-          w[j] = in && j * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(a + (j * 8 + g) * p.K + k + q * 8)) : zero;
-        const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-#pragma unroll
-        for (int j = 0; j < N8; ++j) {
-          mma16<X>(acc[j], a0, w[j].x, w[j].y);
-          mma16<X>(acc[j], a1, w[j].z, w[j].w);
-        }
-      }
-    } else {
-      // x rows and A's rows, 64 of K a stage; odd rows have their halves swapped.
-      constexpr int ROWS = M + RP, STAGE = ROWS * 128, PIECES = (ROWS * 8 + kThreads - 1) / kThreads;
-      const uint32_t base = smem_u32(smem);
-      const uint16_t* src[PIECES];
-      bool there[PIECES];
-      const int c = threadIdx.x & 7;
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
-        src[i] = x;
-        there[i] = false;
-        if (r < M) {
-          there[i] = row_of[r] >= 0;
-          if (there[i]) src[i] = x + row_of[r] * p.ldx;
-        } else if (r < ROWS && r - M < p.rank) {
-          there[i] = true;
-          src[i] = a + static_cast<int64_t>(r - M) * p.K;
-        }
-      }
-      int stage_in = 0;
-      int64_t k_in = k0;
-      auto ask = [&]() {
-        if (k_in < k1) {
-#pragma unroll
-          for (int i = 0; i < PIECES; ++i) {
-            const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
-            if (r < ROWS) {
-              const bool in = there[i] && k_in + c * 8 < k1;
-              cp16(base + stage_in * STAGE + r * 128 + ((c ^ ((r & 1) << 2)) << 4), src[i] + (in ? k_in + c * 8 : 0), in);
+          const uint16_t* xa = x + (row_a < 0 ? 0 : row_a) * p.ldx + q * 8;
+          const uint16_t* xb = x + (row_b < 0 ? 0 : row_b) * p.ldx + q * 8;
+    #pragma unroll 2
+          for (int64_t k = k0 + warp * 32; k < k1; k += kWarps * 32) {
+            const bool in = k + q * 8 < k1;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            const uint4 u = in && row_a >= 0 ? __ldg(reinterpret_cast<const uint4*>(xa + k)) : zero;
+            const uint4 v = in && row_b >= 0 ? __ldg(reinterpret_cast<const uint4*>(xb + k)) : zero;
+            uint4 w[N8];
+    #pragma unroll
+            for (int j = 0; j < N8; ++j)
+              w[j] = in && j * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(a + (j * 8 + g) * p.K + k + q * 8)) : zero;
+            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+    #pragma unroll
+            for (int j = 0; j < N8; ++j) {
+              mma16<X>(acc[j], a0, w[j].x, w[j].y);
+              mma16<X>(acc[j], a1, w[j].z, w[j].w);
             }
           }
-          k_in += kStageK;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
-      };
-      for (int i = 0; i < kStages - 1; ++i) ask();
-      int stage = 0;
-      for (int64_t k = k0; k < k1; k += kStageK) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncthreads();  // the stage has arrived, and the one before it has been read
-        ask();
-        const uint8_t* sp = smem + stage * STAGE + (((split * 4 + q) ^ ((g & 1) << 2)) << 4);
-        const uint4 u = *reinterpret_cast<const uint4*>(sp + (rg * 16 + g) * 128);
-        const uint4 v = *reinterpret_cast<const uint4*>(sp + (rg * 16 + g + 8) * 128);
-        const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-#pragma unroll
-        for (int j = 0; j < N8; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(sp + (M + j * 8 + g) * 128);
-          mma16<X>(acc[j], a0, w.x, w.y);
-          mma16<X>(acc[j], a1, w.z, w.w);
-        }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-      }
-      __syncthreads();  // the stages become the partial sums
-    }
 #pragma unroll
     for (int j = 0; j < N8; ++j) {
       float* d = part + (warp * 16 + g) * RP + j * 8 + 2 * q;
@@ -217,12 +298,14 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const LoraArgs p) {
       *reinterpret_cast<float2*>(d + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < M * RP; i += kThreads) {
-      const int m = i / RP, r = i % RP;
-      float v = 0.0f;
+    for (int i = threadIdx.x; i < M * RP / 4; i += kThreads) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int s = 0; s < SPLIT; ++s) v += part[((s * MT + m / 16) * 16 + (m & 15)) * RP + r];
-      sum[i] = v;
+      for (int s = 0; s < kWarps; ++s) {
+        const float4 w = *reinterpret_cast<const float4*>(part + s * 16 * RP + i * 4);
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      *reinterpret_cast<float4*>(sum + i * 4) = v;
     }
     cluster_sync();
     // --------------------------- 2: this CTA's rows, from all eight and to all eight
@@ -244,42 +327,18 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const LoraArgs p) {
           }
         }
       }
-      float top = 0.0f;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        v[e] *= scale;
-        top = fmaxf(top, fabsf(v[e]));
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // 2^e >= top: the row's numbers are at most 1.  (fmaxf passes over NaN; a row with an infinity keeps its values.)
-      int e2 = 0;
-      if (top > 0.0f && top < INFINITY) frexpf(top, &e2);
-      e2 = max(-126, min(126, e2));
-      const float down = __int_as_float((127 - e2) << 23);
+      for (int e = 0; e < PER; ++e) v[e] *= scale;
       uint32_t hi[PER / 2], lo[PER / 2];
-#pragma unroll
-      for (int e = 0; e < PER; e += 2) {
-        uint16_t h[2], l[2];
-#pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2) {
-          const float w = v[e + i2] * down;
-          h[i2] = bits16<X>(w);
-          const float rest = w - from16<X>(h[i2]);
-          l[i2] = bits16<X>(fabsf(w) < INFINITY ? rest : 0.0f);
-        }
-        hi[e / 2] = h[0] | (static_cast<uint32_t>(h[1]) << 16);
-        lo[e / 2] = l[0] | (static_cast<uint32_t>(l[1]) << 16);
-      }
-      const float up = __int_as_float((127 + e2) << 23);
+      const float up = split_row<X, PER, 32>(v, hi, lo);
 #pragma unroll
       for (int s = 0; s < kRanks; ++s) {
         if (lane < LANES) {
-          const uint32_t to = cluster_addr(smem + Sh::OFF_H + m * Sh::PITCH + lane * PER * 2, s);
+          const uint32_t to = cluster_addr(smem + Sh::OFF_H + m * kPitch<RP> + lane * PER * 2, s);
 #pragma unroll
           for (int e = 0; e < PER / 2; ++e) {
             asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + e * 4), "r"(hi[e]) : "memory");
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + M * Sh::PITCH + e * 4), "r"(lo[e]) : "memory");
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + M * kPitch<RP> + e * 4), "r"(lo[e]) : "memory");
           }
         }
         if (lane == 0)
@@ -288,128 +347,353 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const LoraArgs p) {
     }
     cluster_sync();
   }
-
   // -------------------------------------------- 3: this CTA's eighth of the columns
-  const uint16_t* b = static_cast<const uint16_t*>(p.b) + static_cast<int64_t>(live ? t.group : 0) * p.N * p.rank;
-  const uint8_t* h = smem + Sh::OFF_H + (rg * 16 + g) * Sh::PITCH;
-  const float up_a = live ? power[rg * 16 + g] : 0.0f, up_b = live ? power[rg * 16 + g + 8] : 0.0f;
-  constexpr int YS = static_cast<int>(sizeof(YV));
-  const bool aligned = (reinterpret_cast<uintptr_t>(p.resid) | reinterpret_cast<uintptr_t>(p.y) |
-                        static_cast<uintptr_t>(p.ldr * YS) | static_cast<uintptr_t>(p.ldy * YS)) % (2 * YS) == 0;
-  if (rg * 16 >= t.end - t.begin) return;  // (nothing below waits)
-  for (int64_t n = n0 + split * 32; n < n1; n += SPLIT * 32) {
-    float2 ya[4], yb[4];
-    float acc[4][4] = {};
-    const YV* ra = static_cast<const YV*>(p.resid) + (row_a < 0 ? 0 : row_a) * p.ldr;
-    const YV* rb = static_cast<const YV*>(p.resid) + (row_b < 0 ? 0 : row_b) * p.ldr;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t col = n + j * 8 + 2 * q;
-      ya[j] = yb[j] = make_float2(0.0f, 0.0f);
-      if (col < n1 && row_a >= 0) ya[j] = load2<Y>(ra + col, aligned, col + 1 < n1);
-      if (col < n1 && row_b >= 0) yb[j] = load2<Y>(rb + col, aligned, col + 1 < n1);
-    }
-    if (live) {
-      if constexpr (RP == 16) {
-        uint2 w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t col = n + j * 8 + g;
-          w[j] = col < n1 && q * 4 < p.rank ? __ldg(reinterpret_cast<const uint2*>(b + col * p.rank + q * 4)) : make_uint2(0, 0);
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {  // the numbers, then what rounding them left
-          const uint2 u = *reinterpret_cast<const uint2*>(h + s * M * Sh::PITCH + q * 8);
-          const uint2 v = *reinterpret_cast<const uint2*>(h + s * M * Sh::PITCH + 8 * Sh::PITCH + q * 8);
-          const uint32_t a0[4] = {u.x, v.x, u.y, v.y};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mma16<X>(acc[j], a0, w[j].x, w[j].y);
-        }
-      } else {
-#pragma unroll
-        for (int kb = 0; kb < RP / 32; ++kb) {
-          uint4 w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int64_t col = n + j * 8 + g;
-            w[j] = col < n1 && kb * 32 + q * 8 < p.rank
-                       ? __ldg(reinterpret_cast<const uint4*>(b + col * p.rank + kb * 32 + q * 8)) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const uint4 u = *reinterpret_cast<const uint4*>(h + s * M * Sh::PITCH + kb * 64 + q * 16);
-            const uint4 v = *reinterpret_cast<const uint4*>(h + s * M * Sh::PITCH + 8 * Sh::PITCH + kb * 64 + q * 16);
-            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              mma16<X>(acc[j], a0, w[j].x, w[j].y);
-              mma16<X>(acc[j], a1, w[j].z, w[j].w);
-            }
-          }
-        }
-      }
-    }
-    YV* oa = static_cast<YV*>(p.y) + (row_a < 0 ? 0 : row_a) * p.ldy;
-    YV* ob = static_cast<YV*>(p.y) + (row_b < 0 ? 0 : row_b) * p.ldy;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t col = n + j * 8 + 2 * q;
-      if (col >= n1) continue;
-      // (rows of no adapter stay as they are, to the bit)
-      if (live) {
-        ya[j] = make_float2(fmaf(up_a, acc[j][0], ya[j].x), fmaf(up_a, acc[j][1], ya[j].y));
-        yb[j] = make_float2(fmaf(up_b, acc[j][2], yb[j].x), fmaf(up_b, acc[j][3], yb[j].y));
-      }
-      if (row_a >= 0) store2<Y>(oa + col, ya[j], aligned, col + 1 < n1);
-      if (row_b >= 0) store2<Y>(ob + col, yb[j], aligned, col + 1 < n1);
-    }
-  }
+  const int64_t n_slice = ((p.N + kRanks - 1) / kRanks + 31) / 32 * 32;
+  const int64_t n0 = min(p.N, rank * n_slice), n1 = min(p.N, n0 + n_slice);
+  stream_columns<X, Y, RP>(p, t.group, live, smem + Sh::OFF_H + g * kPitch<RP>, M * kPitch<RP>, live ? power[g] : 0.0f,
+                           live ? power[g + 8] : 0.0f, row_a, row_b, n0, n1, warp, kWarps * 32);
 }
 
-template <int X, int Y, int MT, int RP>
-cudaError_t launch_shape(const LoraArgs& a, cudaStream_t s) {
-  using Sh = LoraShape<MT, RP>;
-  static_assert(Sh::SMEM <= 227 * 1024, "shared memory");
-  constexpr auto k = lora_kernel<X, Y, MT, RP>;
-  if (cudaError_t e = allow_smem<k>(Sh::SMEM)) return e;
-  const int64_t tiles = a.T / Sh::M + std::min<int64_t>(a.groups + 1, a.T);
-  if (tiles > INT32_MAX / kRanks) return cudaErrorInvalidValue;
+// h of one tile of 64 sorted rows over one of p.splits parts of K: p.part [splits][T][RP], rows in sorted order.
+template <int X, int RP>
+__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraArgs p) {
+  using Sh = ShrinkShape<RP>;
+  constexpr int N8 = RP / 8, ROWS = kTile + RP, PIECES = (ROWS * 8 + kThreads - 1) / kThreads;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  int* row_of = reinterpret_cast<int*>(smem + Sh::OFF_ROW);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, q = lane & 3;
+  const int rg = warp & 3, half = warp >> 2;  // 16 rows, and 32 of a stage's 64 of K
+  const int split = blockIdx.x % p.splits;
+  const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / p.splits, kTile);
+  if (t.group >= 0 && t.group < p.groups) {
+    tile_rows<kTile>(p, t, row_of);
+    __syncthreads();
+    const int64_t k_slice = ((p.K + p.splits - 1) / p.splits + kStageK - 1) / kStageK * kStageK;
+    const int64_t k0 = min(p.K, split * k_slice), k1 = min(p.K, k0 + k_slice);
+    const uint16_t* x = static_cast<const uint16_t*>(p.x);
+    const uint16_t* a = static_cast<const uint16_t*>(p.a) + static_cast<int64_t>(t.group) * p.rank * p.K;
+    // x's rows and A's rows, 64 of K a stage; odd rows have their halves swapped.
+    const uint32_t base = smem_u32(smem);
+    const uint16_t* src[PIECES];
+    bool there[PIECES];
+    const int c = threadIdx.x & 7;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
+      src[i] = x;
+      there[i] = false;
+      if (r < kTile) {
+        there[i] = row_of[r] >= 0;
+        if (there[i]) src[i] = x + row_of[r] * p.ldx;
+      } else if (r < ROWS && r - kTile < p.rank) {
+        there[i] = true;
+        src[i] = a + static_cast<int64_t>(r - kTile) * p.K;
+      }
+    }
+    int stage_in = 0;
+    int64_t k_in = k0;
+    auto ask = [&]() {
+      if (k_in < k1) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
+          if (r < ROWS) {
+            const bool in = there[i] && k_in + c * 8 < k1;
+            cp16(base + stage_in * Sh::STAGE + r * 128 + ((c ^ ((r & 1) << 2)) << 4), src[i] + (in ? k_in + c * 8 : 0), in);
+          }
+        }
+        k_in += kStageK;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+    };
+    for (int i = 0; i < kStages - 1; ++i) ask();
+    float acc[N8][4] = {};
+    int stage = 0;
+    for (int64_t k = k0; k < k1; k += kStageK) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncthreads();  // the stage has arrived, and the one before it has been read
+      ask();
+      const uint8_t* sp = smem + stage * Sh::STAGE + (((half * 4 + q) ^ ((g & 1) << 2)) << 4);
+      const uint4 u = *reinterpret_cast<const uint4*>(sp + (rg * 16 + g) * 128);
+      const uint4 v = *reinterpret_cast<const uint4*>(sp + (rg * 16 + g + 8) * 128);
+      const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+      for (int j = 0; j < N8; ++j) {
+        const uint4 w = *reinterpret_cast<const uint4*>(sp + (kTile + j * 8 + g) * 128);
+        mma16<X>(acc[j], a0, w.x, w.y);
+        mma16<X>(acc[j], a1, w.z, w.w);
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    __syncthreads();  // the stages become the halves' sums
+    float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int j = 0; j < N8; ++j) {
+      float* d = part + (warp * 16 + g) * RP + j * 8 + 2 * q;
+      *reinterpret_cast<float2*>(d) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(d + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    float* out = p.part + (split * p.T + t.begin) * RP;
+    for (int i = threadIdx.x; i < (t.end - t.begin) * RP / 4; i += kThreads) {
+      float4 v = *reinterpret_cast<const float4*>(part + i * 4);
+      const float4 w = *reinterpret_cast<const float4*>(part + kTile * RP + i * 4);
+      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      *reinterpret_cast<float4*>(out + i * 4) = v;
+    }
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// One of p.slices parts of the columns of y for a tile of 64 sorted rows.  Whole
+// groups of 64 columns come in cp.async stages (resid's values and B's rows, each
+// brought once for all warps); a warp has 16 rows and 32 of the columns.  What is
+// left, or lies on addresses that cp.async does not take, is read straight.
+template <int X, int Y, int RP>
+__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs p) {
+  using YV = typename Val<Y>::type;
+  constexpr int YS = static_cast<int>(sizeof(YV));
+  using Sh = ExpandShape<RP, YS>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* hs = smem + Sh::OFF_H;
+  float* power = reinterpret_cast<float*>(smem + Sh::OFF_EXP);
+  int* row_of = reinterpret_cast<int*>(smem + Sh::OFF_ROW);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, q = lane & 3;
+  const int rg = warp & 3, half = warp >> 2;
+  const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / p.slices, kTile);
+  if (t.group < 0) return;
+  const bool live = t.group < p.groups;
+  if (!live && p.resid == p.y) return;
+  tile_rows<kTile>(p, t, row_of);
+  __syncthreads();
+  const int count = t.end - t.begin;
+  const int64_t n_slice = ((p.N + p.slices - 1) / p.slices + Sh::COLS - 1) / Sh::COLS * Sh::COLS;
+  const int64_t n0 = min(p.N, (blockIdx.x % p.slices) * n_slice), n1 = min(p.N, n0 + n_slice);
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.resid) | reinterpret_cast<uintptr_t>(p.y) |
+                        static_cast<uintptr_t>(p.ldr * YS) | static_cast<uintptr_t>(p.ldy * YS)) % 16 == 0;
+  const int whole = live && aligned ? static_cast<int>((n1 - n0) / Sh::COLS) : 0;
+  const uint16_t* b = static_cast<const uint16_t*>(p.b) + (static_cast<int64_t>(live ? t.group : 0) * p.N + n0) * p.rank;
+
+  // What a thread fetches of a stage: 16-byte pieces of y's rows and of B's.
+  constexpr int YP = Sh::YROW / 16, BP = Sh::BROW / 16;          // pieces of a row
+  constexpr int YN = kTile * YP / kThreads, BN = (Sh::COLS * BP + kThreads - 1) / kThreads;
+  static_assert(kTile * YP % kThreads == 0, "");
+  const uint32_t base = smem_u32(smem);
+  const YV* ysrc[YN];
+  bool yhave[YN];
+#pragma unroll
+  for (int i = 0; i < YN; ++i) {
+    const int at = threadIdx.x + i * kThreads, r = row_of[at / YP];
+    yhave[i] = r >= 0;
+    ysrc[i] = static_cast<const YV*>(p.resid) + (r < 0 ? 0 : r) * p.ldr + n0 + at % YP * (16 / YS);
+  }
+  const uint16_t* bsrc[BN];
+  bool bhave[BN];
+#pragma unroll
+  for (int i = 0; i < BN; ++i) {
+    const int at = threadIdx.x + i * kThreads, r = at / BP, c = at % BP;
+    bhave[i] = c * 8 < p.rank && r < Sh::COLS;
+    bsrc[i] = b + (bhave[i] ? r * p.rank + c * 8 : 0);
+  }
+  int next = 0, put = 0;
+  auto ask = [&]() {
+    if (next < whole) {
+      const uint32_t to = base + put * Sh::STAGE;
+#pragma unroll
+      for (int i = 0; i < YN; ++i) {
+        const int at = threadIdx.x + i * kThreads, r = at / YP, c = at % YP;
+        cp16(to + r * Sh::YROW + ((c ^ ((r & 1) << 2)) << 4), ysrc[i], yhave[i]);
+        ysrc[i] += Sh::COLS;
+      }
+#pragma unroll
+      for (int i = 0; i < BN; ++i) {
+        const int at = threadIdx.x + i * kThreads, r = at / BP, c = at % BP;
+        if (Sh::COLS * BP % kThreads == 0 || r < Sh::COLS)
+          cp16(to + kTile * Sh::YROW + r * Sh::BROW + ((BP >= 8 ? c ^ ((r & 1) << 2) : c) << 4), bsrc[i], bhave[i]);
+        bsrc[i] += Sh::COLS * p.rank;
+      }
+      ++next;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put = put + 1 == Sh::STAGES ? 0 : put + 1;
+  };
+  for (int i = 0; i < Sh::STAGES - 1; ++i) ask();  // (these do not depend on the first launch)
+
+  if (live) {
+    const float scale = p.scales ? __ldg(p.scales + t.group) : 1.0f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int LANES = RP / 4;  // of a row, 4 values each
+#pragma unroll
+    for (int i = 0; i < kTile * LANES / kThreads; ++i) {
+      const int at = i * kThreads + threadIdx.x, m = at / LANES, c = at % LANES;
+      float v[4] = {};
+      if (m < count) {
+        const float4* from = reinterpret_cast<const float4*>(p.part + (t.begin + m) * static_cast<int64_t>(RP)) + c;
+        float4 w[kMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s) w[s] = s < p.splits ? from[s * p.T * (RP / 4)] : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s) v[0] += w[s].x, v[1] += w[s].y, v[2] += w[s].z, v[3] += w[s].w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= scale;
+      uint32_t hi[2], lo[2];
+      const float up = split_row<X, 4, LANES>(v, hi, lo);
+      uint2* to = reinterpret_cast<uint2*>(hs + m * kPitch<RP>) + c;
+      to[0] = make_uint2(hi[0], hi[1]);
+      to[kTile * kPitch<RP> / 8] = make_uint2(lo[0], lo[1]);
+      if (c == 0) power[m] = up;
+    }
+  }
+  __syncthreads();
+  const int m = rg * 16 + g;
+  const int row_a = row_of[m], row_b = row_of[m + 8];
+  const float up_a = live ? power[m] : 0.0f, up_b = live ? power[m + 8] : 0.0f;
+  const uint8_t* h = hs + m * kPitch<RP>;
+  constexpr int REST = kTile * kPitch<RP>;
+  constexpr int HALF = Sh::COLS / 2, UNITS = HALF / 16;  // a warp's columns, and groups of 16 of them
+  YV* ta = static_cast<YV*>(p.y) + (row_a < 0 ? 0 : row_a) * p.ldy + n0 + half * HALF + 4 * q;
+  YV* tb = static_cast<YV*>(p.y) + (row_b < 0 ? 0 : row_b) * p.ldy + n0 + half * HALF + 4 * q;
+  const int col = half * HALF + 4 * (g >> 1) + (g & 1);  // of B, and 2 more in the second product
+  const int flip = (g & 1) << 2;
+  int take = 0;
+  for (int i = 0; i < whole; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(Sh::STAGES - 2) : "memory");
+    __syncthreads();  // the stage has arrived, and the one before it has been read
+    ask();
+    const uint8_t* sp = smem + take * Sh::STAGE;
+    const uint8_t* bp = sp + kTile * Sh::YROW + col * Sh::BROW;
+    float acc[2 * UNITS][4] = {};
+#pragma unroll
+    for (int kb = 0; kb < (RP == 16 ? 1 : RP / 32); ++kb) {
+      uint4 w[2 * UNITS];
+#pragma unroll
+      for (int j = 0; j < 2 * UNITS; ++j) {
+        const uint8_t* at = bp + ((j >> 1) * 16 + (j & 1) * 2) * Sh::BROW;  // (columns of the same parity)
+        if constexpr (RP == 16) {
+          const uint2 v = *reinterpret_cast<const uint2*>(at + q * 8);
+          w[j] = make_uint4(v.x, v.y, 0, 0);
+        } else {
+          w[j] = *reinterpret_cast<const uint4*>(at + ((BP >= 8 ? (kb * 4 + q) ^ flip : kb * 4 + q) << 4));
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {  // the numbers, then what rounding them left
+        if constexpr (RP == 16) {
+          const uint2 u = *reinterpret_cast<const uint2*>(h + s * REST + q * 8);
+          const uint2 v = *reinterpret_cast<const uint2*>(h + s * REST + 8 * kPitch<RP> + q * 8);
+          const uint32_t a0[4] = {u.x, v.x, u.y, v.y};
+#pragma unroll
+          for (int j = 0; j < 2 * UNITS; ++j) mma16<X>(acc[j], a0, w[j].x, w[j].y);
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(h + s * REST + kb * 64 + q * 16);
+          const uint4 v = *reinterpret_cast<const uint4*>(h + s * REST + 8 * kPitch<RP> + kb * 64 + q * 16);
+          const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+          for (int j = 0; j < 2 * UNITS; ++j) {
+            mma16<X>(acc[j], a0, w[j].x, w[j].y);
+            mma16<X>(acc[j], a1, w[j].z, w[j].w);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      float ya[4], yb[4];
+      const int c = half * HALF + u * 16 + 4 * q, piece = c * YS / 16;
+      const int yc = ((piece ^ flip) << 4) + c * YS % 16;
+      load_vec<Y>(reinterpret_cast<const YV*>(sp + m * Sh::YROW + yc), ya);
+      load_vec<Y>(reinterpret_cast<const YV*>(sp + (m + 8) * Sh::YROW + yc), yb);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ya[e] = fmaf(up_a, acc[2 * u + (e >> 1)][e & 1], ya[e]);
+        yb[e] = fmaf(up_b, acc[2 * u + (e >> 1)][2 + (e & 1)], yb[e]);
+      }
+      if (row_a >= 0) store_vec<Y>(ta + u * 16, ya);
+      if (row_b >= 0) store_vec<Y>(tb + u * 16, yb);
+    }
+    ta += Sh::COLS;
+    tb += Sh::COLS;
+    take = take + 1 == Sh::STAGES ? 0 : take + 1;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (rg * 16 >= count) return;
+  stream_columns<X, Y, RP>(p, t.group, live, h, REST, up_a, up_b, row_a, row_b, n0 + static_cast<int64_t>(whole) * Sh::COLS,
+                           n1, half, 2 * 32);
+}
+
+int padded(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+int64_t tiles_of(const LoraArgs& a, int rows) { return a.T / rows + std::min<int64_t>(a.groups + 1, a.T); }
+bool two_launches(int64_t T, int groups) { return T > 16 * groups; }
+
+// Parts of K of the first launch, and of the columns of the second: enough CTAs for the device where tiles are few.
+int splits_of(int64_t T, int64_t K, int groups) {
+  const int64_t tiles = T / kTile + std::min<int64_t>(groups, T);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 296 / tiles, K / 256})));
+}
+
+template <int X, int Y, int RP>
+cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kRanks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * kRanks));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Sh::SMEM;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, a);
+  if (!two_launches(a.T, a.groups)) {
+    using Sh = ClusterShape<RP>;
+    constexpr auto k = lora_cluster_kernel<X, Y, RP>;
+    if (cudaError_t e = allow_smem<k>(Sh::SMEM)) return e;
+    const int64_t tiles = tiles_of(a, Sh::M);
+    if (tiles > INT32_MAX / kRanks) return cudaErrorInvalidValue;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kRanks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * kRanks));
+    cfg.dynamicSmemBytes = Sh::SMEM;
+    return cudaLaunchKernelEx(&cfg, k, a);
+  }
+  constexpr auto shrink = lora_shrink_kernel<X, RP>;
+  constexpr auto expand = lora_expand_kernel<X, Y, RP>;
+  if (cudaError_t e = allow_smem<shrink>(ShrinkShape<RP>::SMEM)) return e;
+  if (cudaError_t e = allow_smem<expand>(ExpandShape<RP, Y == 0 ? 4 : 2>::SMEM)) return e;
+  const int64_t tiles = tiles_of(a, kTile);
+  a.splits = splits_of(a.T, a.K, a.groups);
+  a.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((6 * num_sms + tiles - 1) / tiles, (a.N + 127) / 128)));
+  if (tiles > INT32_MAX / std::max(a.splits, a.slices)) return cudaErrorInvalidValue;
+  shrink<<<static_cast<unsigned>(tiles * a.splits), kThreads, ShrinkShape<RP>::SMEM, s>>>(a);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.slices));
+  cfg.dynamicSmemBytes = (ExpandShape<RP, Y == 0 ? 4 : 2>::SMEM);
+  return cudaLaunchKernelEx(&cfg, expand, a);
 }
 
 template <int X, int Y>
-cudaError_t launch_types(const LoraArgs& a, cudaStream_t s) {
-  // Tiles of 64 rows where the adapters have more than a few rows each, on average.
-  if (a.T > 16 * a.groups) {
-    if (a.rank <= 16) return launch_shape<X, Y, 4, 16>(a, s);
-    if (a.rank <= 32) return launch_shape<X, Y, 4, 32>(a, s);
-    if (a.rank <= 64) return launch_shape<X, Y, 4, 64>(a, s);
-    return launch_shape<X, Y, 4, 128>(a, s);
+cudaError_t launch_types(const LoraArgs& a, int num_sms, cudaStream_t s) {
+  switch (padded(a.rank)) {
+    case 16: return launch_shape<X, Y, 16>(a, num_sms, s);
+    case 32: return launch_shape<X, Y, 32>(a, num_sms, s);
+    case 64: return launch_shape<X, Y, 64>(a, num_sms, s);
+    default: return launch_shape<X, Y, 128>(a, num_sms, s);
   }
-  if (a.rank <= 16) return launch_shape<X, Y, 1, 16>(a, s);
-  if (a.rank <= 32) return launch_shape<X, Y, 1, 32>(a, s);
-  if (a.rank <= 64) return launch_shape<X, Y, 1, 64>(a, s);
-  return launch_shape<X, Y, 1, 128>(a, s);
 }
 
 }  // namespace
 
+size_t lora_workspace(int64_t T, int64_t K, int groups, int rank) {
+  if (T <= 0 || !two_launches(T, groups)) return 0;
+  return static_cast<size_t>(splits_of(T, K, groups)) * T * padded(rank) * 4;
+}
+
 cudaError_t launch_lora(const LoraArgs& a, int xtype, int ytype, int num_sms, cudaStream_t s) {
-  (void)num_sms;
-  if (xtype == kXF16) return ytype == kXF32 ? launch_types<1, 0>(a, s) : launch_types<1, 1>(a, s);
-  return ytype == kXF32 ? launch_types<2, 0>(a, s) : launch_types<2, 2>(a, s);
+  if (xtype == kXF16) return ytype == kXF32 ? launch_types<1, 0>(a, num_sms, s) : launch_types<1, 1>(a, num_sms, s);
+  return ytype == kXF32 ? launch_types<2, 0>(a, num_sms, s) : launch_types<2, 2>(a, num_sms, s);
 }
 
 }  // namespace b2q

@@ -17,10 +17,20 @@ compact Q4_0 weights, which rounds the activations to Q8_0 as ggml's CPU mul_mat
 does: a token's result depends, by that rounding, on which side of the number its
 step is.
 
+With `Experts` the last line is a mixture layer instead:
+
+    choice, shares, rows by expert = route(h . W_r)    b2q_mul_mat_f32, b2q_moe_route
+    z = silu(h . W_gate) * (h . W_up), per slot        b2q_mul_mat_id
+    x = x + sum of shares * (z . W_down)               b2q_mul_mat_id, b2q_moe_combine
+
+and with `Adapters` each linear that has some adds its row's low-rank product
+(b2q_lora_add), the rows sorted by adapter once per step (b2q_group_rows).
+
 `PagedCache` keeps the pools, the block tables and the free pages of a set of
 requests, and takes back the pages of those that end; the host knows the lengths
 it asked for, the device builds the rest (b2q_kv_cache_plan), so a step never
-waits for the device.
+waits for the device.  A step of drafted tokens ends with b2q_draft_verify, and
+`keep` takes back what the turned down ones had.
 
     python cached_block.py       # a prompt of 300 tokens, then 8 single tokens
 """
@@ -78,6 +88,64 @@ class PagedCache:
         self.lengths[request] = 0
 
 
+    def keep(self, request: int, length: int, stream=None) -> None:
+        """Takes a request back to its first `length` tokens (drafts that were turned down): the pages behind them
+        are free again."""
+        import torch
+        ps, old = self.page_size, self.lengths[request]
+        if not 0 <= length <= old:
+            raise ValueError("a request keeps some of its tokens")
+        first, last = -(-length // ps), -(-old // ps)
+        if last > first:
+            with torch.cuda.stream(stream):
+                self.free[self.taken - (last - first):self.taken].copy_(self.table[request, first:last])
+                self.table[request, first:last].fill_(-1)
+        self.taken -= last - first
+        self.lengths[request] = length
+
+
+class Experts:
+    """A mixture layer's weights: the router's rows fp32 [E, C]; every expert's gate and up rows (2 * hidden of C) and
+    rows of the way back (C of hidden) as GGUF Q4_0 rows, one expert under another."""
+
+    def __init__(self, dev, router, w_in, w_out, C: int, hidden: int, top: int, scoring: str = "softmax", renorm: bool = True,
+                 scale: float = 1.0, bias=None):
+        import torch
+        self.router, self.C, self.hidden, self.top, self.bias = router, C, hidden, top, bias
+        self.how = {"scoring": scoring, "renorm": renorm, "scale": scale}
+        self.w_in = b2q.weight_pack_q4_0(torch.from_numpy(w_in).to(dev), C)
+        self.w_out = b2q.weight_pack_q4_0(torch.from_numpy(w_out).to(dev), hidden)
+
+    def forward(self, h, x):
+        """x += the layer's output for the normed rows h (fp32 [tokens, C]), in place."""
+        import torch
+        logits = b2q.mul_mat_f32(self.router, h)
+        ids, shares, order, offsets = b2q.moe_route(logits, self.top, bias=self.bias, **self.how)
+        z = b2q.mul_mat_id(b2q.TYPE_Q4_0, self.w_in, self.hidden, self.C, h.half(), order, offsets, per_row=self.top, glu=True)
+        y = b2q.mul_mat_id(b2q.TYPE_Q4_0, self.w_out, self.C, self.hidden, z, order, offsets, out_dtype=torch.float32)
+        return b2q.moe_combine(y, shares, ids, resid=x, out=x)
+
+
+class Adapters:
+    """Low-rank adapters of a block's linears: {"qkv" | "out" | "fc1" | "fc2": (a [G, rank, in], b [G, out, rank])} in fp16,
+    and their scales fp32 [G] (or None)."""
+
+    def __init__(self, pairs: dict, scales=None):
+        self.pairs, self.scales = pairs, scales
+        self.count = next(iter(pairs.values()))[0].shape[0]
+
+    def plan(self, ids, stream=None):
+        """A step's rows by adapter, for every layer's pass: ids int32 [tokens], -1 for none."""
+        return b2q.group_rows(ids, self.count, stream=stream)
+
+    def add(self, name: str, y, x, rows):
+        """y (fp32) += the adapters' products of the rows x, in place."""
+        if name in self.pairs:
+            a, b = self.pairs[name]
+            b2q.lora_add(y, x.half(), a, b, self.scales, *rows, out=y)
+        return y
+
+
 class CachedBlock:
     """One block's Q4_0 weights and its forward pass on fp32 rows x [tokens, C]."""
 
@@ -86,16 +154,19 @@ class CachedBlock:
         return {"qkv": ((heads + 2 * kv_heads) * D, C), "out": (C, heads * D), "fc1": (hidden, C), "fc2": (C, hidden)}
 
     def __init__(self, dev, weights: dict, vectors: dict, C: int, heads: int, kv_heads: int, D: int, hidden: int,
-                 sections, inv_freq, window: int = 0, sinks: int = 0, unrounded_rows: int = b2q.MUL_VEC_MAX_M):
+                 sections, inv_freq, window: int = 0, sinks: int = 0, unrounded_rows: int = b2q.MUL_VEC_MAX_M,
+                 experts: Experts | None = None):
         """weights: GGUF Q4_0 rows (uint8 numpy [out, row bytes]); vectors: fp32 device tensors
         b_qkv, b_out, b1, b2 and the RMS gammas gq [heads * D], gk [kv_heads * D].  Steps of up to
-        unrounded_rows tokens keep the activations of the linears as they are, more round them to Q8_0."""
+        unrounded_rows tokens keep the activations of the linears as they are, more round them to Q8_0.
+        With experts, fc1 and fc2 (and their biases) are not used and may be absent."""
         import torch
-        self.unrounded_rows = unrounded_rows
+        self.unrounded_rows, self.experts = unrounded_rows, experts
         self.C, self.H, self.Hk, self.D, self.hidden = C, heads, kv_heads, D, hidden
         self.sections, self.inv_freq, self.window, self.sinks = tuple(sections), inv_freq, window, sinks
         self.shape = self.shapes(C, heads, kv_heads, D, hidden)
-        self.packed = {n: b2q.weight_pack_q4_0(torch.from_numpy(weights[n]).to(dev), k) for n, (_, k) in self.shape.items()}
+        self.packed = {n: b2q.weight_pack_q4_0(torch.from_numpy(weights[n]).to(dev), k) for n, (_, k) in self.shape.items()
+                       if experts is None or n in ("qkv", "out")}
         self.vec = vectors
 
     def _linear(self, name: str, x, bias, resid=None):
@@ -114,26 +185,51 @@ class CachedBlock:
         act = b2q.act_prepare(x.float())
         return b2q.mul_mat_prepared_q4_0(self.packed[name], n, k, act, m, bias=bias, resid=resid, out=resid)
 
-    def forward(self, x, cache: PagedCache, layer: int, step: dict, positions, stream=None):
+    def forward(self, x, cache: PagedCache, layer: int, step: dict, positions, stream=None, adapters: Adapters | None = None,
+                rows=None):
         """x: fp32 [tokens, C], updated in place and returned; positions int32 [axes, tokens].  With a stream the
-        whole pass belongs to it: its casts, and the pool that its temporaries come from and go back to."""
+        whole pass belongs to it: its casts, and the pool that its temporaries come from and go back to.
+        adapters: this layer's, with rows = adapters.plan(...) of the step."""
         import torch
         with torch.cuda.stream(stream):
-            return self._forward(x, cache, layer, step, positions)
+            return self._forward(x, cache, layer, step, positions, adapters, rows)
 
-    def _forward(self, x, cache: PagedCache, layer: int, step: dict, positions):
+    def _forward(self, x, cache: PagedCache, layer: int, step: dict, positions, adapters, rows):
         v = self.vec
+        add = (lambda name, y, inp: adapters.add(name, y, inp, rows)) if adapters else (lambda name, y, inp: y)
         h = b2q.norm_modulate(x)
-        qkv = self._linear("qkv", h, v["b_qkv"])
+        qkv = add("qkv", self._linear("qkv", h, v["b_qkv"]), h)
         k, vv = cache.k[layer], cache.v[layer]
         q = b2q.qkv_rope_cache(qkv, self.H, self.Hk, self.D, positions, self.sections, self.inv_freq, step["slots"], k, vv,
                                norm=True, gamma_q=v["gq"], gamma_k=v["gk"])
         o = b2q.attention_paged(q, k, vv, cache.table, step["kv_len"], step["cu"], step["max_new"], step["max_kv"], self.H,
                                 window=self.window, sinks=self.sinks)
-        self._linear("out", o, v["b_out"], resid=x)
-        h = b2q.gelu(self._linear("fc1", b2q.norm_modulate(x), v["b1"]))
-        self._linear("fc2", h, v["b2"], resid=x)
+        add("out", self._linear("out", o, v["b_out"], resid=x), o)
+        h = b2q.norm_modulate(x)
+        if self.experts is not None:
+            return self.experts.forward(h, x)
+        h = b2q.gelu(add("fc1", self._linear("fc1", h, v["b1"]), h))
+        add("fc2", self._linear("fc2", h, v["b2"], resid=x), h)
         return x
+
+
+def random_q4_0(rng, n: int, k: int):
+    """Seeded GGUF Q4_0 rows of random codes (uint8 numpy [n, row bytes])."""
+    import numpy as np
+    raw = rng.integers(0, 256, (n, k // 32, 18), dtype=np.uint8)
+    d = (rng.uniform(0.5, 1.0, (n, k // 32, 1)) * 0.3 / k ** 0.5).astype(np.float16)
+    raw[:, :, :2] = d.view(np.uint8)
+    return raw.reshape(n, -1)
+
+
+def random_experts(dev, E: int, C: int, hidden: int, top: int, seed: int = 0, **kw):
+    """A mixture layer with seeded weights, and its raw rows (router, gate and up, down)."""
+    import numpy as np
+    import torch
+    rng = np.random.default_rng(seed)
+    router = (rng.standard_normal((E, C)) / C ** 0.5).astype(np.float32)
+    w_in, w_out = random_q4_0(rng, E * 2 * hidden, C), random_q4_0(rng, E * C, hidden)
+    return Experts(dev, torch.from_numpy(router).to(dev), w_in, w_out, C, hidden, top, **kw), (router, w_in, w_out)
 
 
 def random_block(dev, C: int, heads: int, kv_heads: int, D: int, hidden: int, sections, seed: int = 0, **kw):
@@ -143,10 +239,7 @@ def random_block(dev, C: int, heads: int, kv_heads: int, D: int, hidden: int, se
     rng = np.random.default_rng(seed)
     weights = {}
     for name, (n, k) in CachedBlock.shapes(C, heads, kv_heads, D, hidden).items():
-        raw = rng.integers(0, 256, (n, k // 32, 18), dtype=np.uint8)
-        d = (rng.uniform(0.5, 1.0, (n, k // 32, 1)) * 0.3 / k ** 0.5).astype(np.float16)
-        raw[:, :, :2] = d.view(np.uint8)
-        weights[name] = raw.reshape(n, -1)
+        weights[name] = random_q4_0(rng, n, k)
     f = lambda n, mean, s: torch.from_numpy((mean + s * rng.standard_normal(n)).astype(np.float32)).to(dev)  # noqa: E731
     vec = {"b_qkv": f((heads + 2 * kv_heads) * D, 0, 0.1), "b_out": f(C, 0, 0.1), "b1": f(hidden, 0, 0.1),
            "b2": f(C, 0, 0.1), "gq": f(heads * D, 1, 0.1), "gk": f(kv_heads * D, 1, 0.1)}

@@ -994,17 +994,19 @@ def moe_route(logits, top: int, bias=None, scoring: str = "softmax", renorm: boo
     assert (ldc == 1 or E <= 1 or T == 0) and (ld >= E or T <= 1) and 0 < top <= E
     if bias is not None:
         assert _are_floats(bias, E, torch.float32)
-    dev, S = logits.device, T * top
+    dev, i32 = logits.device, torch.int32
     need = _route_ws_bytes(T, E, top)
-    ids, order, offsets, ws = _empty_on(stream, 2 * S + E + 1 + need // 4, torch.int32, dev).split((S, S, E + 1, need // 4))
-    weights = _empty_on(stream, (T, top), torch.float32, dev)
+    # (an allocation takes less host time than a view of one)
+    ids, weights = _empty_on(stream, (T, top), i32, dev), _empty_on(stream, (T, top), torch.float32, dev)
+    order, offsets = _empty_on(stream, T * top, i32, dev), _empty_on(stream, E + 1, i32, dev)
+    ws = _empty_on(stream, need, torch.uint8, dev) if need else None
     rc = (_lib or _lib_obj()).b2q_moe_route(
         dtype, logits.data_ptr(), T, E, size * (ld if ld > E else E), _ptr(bias), top, SCORING[scoring],
         1 if renorm else 0, scale, ids.data_ptr(), weights.data_ptr(), order.data_ptr(), offsets.data_ptr(),
-        ws.data_ptr() if need else None, need, _raw_stream(stream, logits, bias))
+        _ptr(ws), need, _raw_stream(stream, logits, bias))
     if rc:
         _check("b2q_moe_route", rc)
-    return ids.view(T, top), weights, order, offsets
+    return ids, weights, order, offsets
 
 
 def group_rows(ids, groups: int, stream=None):
@@ -1014,10 +1016,10 @@ def group_rows(ids, groups: int, stream=None):
     S = ids.numel()
     assert ids.dtype is torch.int32 and ids.is_contiguous()
     need = _group_ws_bytes(S, groups)
-    order, offsets, ws = _empty_on(stream, S + groups + 1 + need // 4, torch.int32, ids.device).split(
-        (S, groups + 1, need // 4))
-    rc = (_lib or _lib_obj()).b2q_group_rows(ids.data_ptr(), S, groups, order.data_ptr(), offsets.data_ptr(),
-                                             ws.data_ptr() if need else None, need, _raw_stream(stream, ids))
+    order, offsets = _empty_on(stream, S, torch.int32, ids.device), _empty_on(stream, groups + 1, torch.int32, ids.device)
+    ws = _empty_on(stream, need, torch.uint8, ids.device) if need else None
+    rc = (_lib or _lib_obj()).b2q_group_rows(ids.data_ptr(), S, groups, order.data_ptr(), offsets.data_ptr(), _ptr(ws), need,
+                                             _raw_stream(stream, ids))
     if rc:
         _check("b2q_group_rows", rc)
     return order, offsets
@@ -1140,7 +1142,7 @@ def draft_verify(target, draft_probs, drafts, cu_drafts, u, v, stream=None):
         ldq = draft_probs.stride(0)
         assert draft_probs.shape == (D, V) and _are_rows(draft_probs, D, V, target.dtype) and (ldq >= V or D <= 1)
     assert _is_list(drafts, D, i32) and _is_list(cu_drafts, B + 1, i32) and _is_list(u, D, f32) and _is_list(v, B, f32)
-    accepted, tokens = _empty_on(stream, 2 * B + D, i32, target.device).split((B, B + D))
+    accepted, tokens = _empty_on(stream, B, i32, target.device), _empty_on(stream, B + D, i32, target.device)
     rc = (_lib or _lib_obj()).b2q_draft_verify(
         dtype, target.data_ptr(), size * max(ldp, V), _ptr(draft_probs), size * max(ldq, V), drafts.data_ptr(),
         cu_drafts.data_ptr(), B, D, V, u.data_ptr(), v.data_ptr(), accepted.data_ptr(), tokens.data_ptr(),

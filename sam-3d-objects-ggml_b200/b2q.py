@@ -971,6 +971,13 @@ def _val_type(dtype):
     return _type16(dtype), 2
 
 
+def _new_on(stream, like, size, dtype):
+    """_empty_on `like`'s device, by the call that takes the least host time."""
+    if stream is None:
+        return like.new_empty(size, dtype=dtype)
+    return _empty_on(stream, size, dtype, like.device)
+
+
 def _is_list(t, n: int, dtype) -> bool:
     """t is n values of that type one after another."""
     return t.dtype is dtype and t.numel() == n and t.is_contiguous()
@@ -994,12 +1001,12 @@ def moe_route(logits, top: int, bias=None, scoring: str = "softmax", renorm: boo
     assert (ldc == 1 or E <= 1 or T == 0) and (ld >= E or T <= 1) and 0 < top <= E
     if bias is not None:
         assert _are_floats(bias, E, torch.float32)
-    dev, i32 = logits.device, torch.int32
+    i32 = torch.int32
     need = _route_ws_bytes(T, E, top)
     # (an allocation takes less host time than a view of one)
-    ids, weights = _empty_on(stream, (T, top), i32, dev), _empty_on(stream, (T, top), torch.float32, dev)
-    order, offsets = _empty_on(stream, T * top, i32, dev), _empty_on(stream, E + 1, i32, dev)
-    ws = _empty_on(stream, need, torch.uint8, dev) if need else None
+    ids, weights = _new_on(stream, logits, (T, top), i32), _new_on(stream, logits, (T, top), torch.float32)
+    order, offsets = _new_on(stream, logits, T * top, i32), _new_on(stream, logits, E + 1, i32)
+    ws = _new_on(stream, logits, need, torch.uint8) if need else None
     rc = (_lib or _lib_obj()).b2q_moe_route(
         dtype, logits.data_ptr(), T, E, size * (ld if ld > E else E), _ptr(bias), top, SCORING[scoring],
         1 if renorm else 0, scale, ids.data_ptr(), weights.data_ptr(), order.data_ptr(), offsets.data_ptr(),
@@ -1016,8 +1023,8 @@ def group_rows(ids, groups: int, stream=None):
     S = ids.numel()
     assert ids.dtype is torch.int32 and ids.is_contiguous()
     need = _group_ws_bytes(S, groups)
-    order, offsets = _empty_on(stream, S, torch.int32, ids.device), _empty_on(stream, groups + 1, torch.int32, ids.device)
-    ws = _empty_on(stream, need, torch.uint8, ids.device) if need else None
+    order, offsets = _new_on(stream, ids, S, torch.int32), _new_on(stream, ids, groups + 1, torch.int32)
+    ws = _new_on(stream, ids, need, torch.uint8) if need else None
     rc = (_lib or _lib_obj()).b2q_group_rows(ids.data_ptr(), S, groups, order.data_ptr(), offsets.data_ptr(), _ptr(ws), need,
                                              _raw_stream(stream, ids))
     if rc:
@@ -1048,7 +1055,7 @@ def mul_mat_id(wtype: int, w, n: int, k: int, x, order, offsets, per_row: int = 
     if bias is not None:
         assert _are_floats(bias, E * rows, torch.float32)
     if out is None:
-        out = _empty_on(stream, (S, n), out_dtype or dt, x.device)
+        out = _new_on(stream, x, (S, n), out_dtype or dt)
     else:
         assert _are_rows(out, S, n, out_dtype or out.dtype)
     ytype, ysize = _val_type(out.dtype)
@@ -1071,7 +1078,7 @@ def moe_combine(y, weights, ids=None, resid=None, out_dtype=None, out=None, stre
     assert S == T * top and _is_list(weights, S, torch.float32) and (ids is None or _is_list(ids, S, torch.int32))
     assert _are_rows(y, S, n, y.dtype) and (y.stride(0) >= n or S <= 1)
     if out is None:
-        out = _empty_on(stream, (T, n), out_dtype or (resid if resid is not None else y).dtype, y.device)
+        out = _new_on(stream, y, (T, n), out_dtype or (resid if resid is not None else y).dtype)
     else:
         assert _are_rows(out, T, n, out_dtype or out.dtype) and (out.stride(0) >= n or T <= 1)
     if resid is not None:
@@ -1108,13 +1115,13 @@ def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
     if scales is not None:
         assert _are_floats(scales, G, torch.float32)
     if out is None:
-        out = _empty_on(stream, (T, n), resid.dtype, x.device)
+        out = _new_on(stream, x, (T, n), resid.dtype)
     else:
         assert _are_rows(out, T, n, resid.dtype) and (out.stride(0) >= n or T <= 1)
     ytype, ys = _val_type(resid.dtype)
     need, ws = _lora_ws_bytes(T, k, G, rank), None
     if need:
-        ws = _empty_on(stream, need, torch.uint8, x.device)
+        ws = _new_on(stream, x, need, torch.uint8)
     rc = (_lib or _lib_obj()).b2q_lora_add(
         _type16(dt), x.data_ptr(), T, k, 2 * (ldx if ldx > k else k), a.data_ptr(), b.data_ptr(), G, rank, n,
         _ptr(scales), order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * max(resid.stride(0), n),
@@ -1142,7 +1149,7 @@ def draft_verify(target, draft_probs, drafts, cu_drafts, u, v, stream=None):
         ldq = draft_probs.stride(0)
         assert draft_probs.shape == (D, V) and _are_rows(draft_probs, D, V, target.dtype) and (ldq >= V or D <= 1)
     assert _is_list(drafts, D, i32) and _is_list(cu_drafts, B + 1, i32) and _is_list(u, D, f32) and _is_list(v, B, f32)
-    accepted, tokens = _empty_on(stream, B, i32, target.device), _empty_on(stream, B + D, i32, target.device)
+    accepted, tokens = _new_on(stream, target, B, i32), _new_on(stream, target, B + D, i32)
     rc = (_lib or _lib_obj()).b2q_draft_verify(
         dtype, target.data_ptr(), size * max(ldp, V), _ptr(draft_probs), size * max(ldq, V), drafts.data_ptr(),
         cu_drafts.data_ptr(), B, D, V, u.data_ptr(), v.data_ptr(), accepted.data_ptr(), tokens.data_ptr(),

@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(kThreads) lora_cluster_kernel(const LoraArgs p
   const int g = lane >> 2, q = lane & 3;
   const int rank = static_cast<int>(cluster_ctarank());
 
+  grid_wait();
   const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / kRanks, M);
   if (t.group < 0) return;  // (all eight CTAs)
   const bool live = t.group < p.groups;
@@ -365,6 +366,7 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraArgs p)
   const int g = lane >> 2, q = lane & 3;
   const int rg = warp & 3, half = warp >> 2;  // 16 rows, and 32 of a stage's 64 of K
   const int split = blockIdx.x % p.splits;
+  grid_wait();
   const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / p.splits, kTile);
   if (t.group >= 0 && t.group < p.groups) {
     tile_rows<kTile>(p, t, row_of);
@@ -464,9 +466,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
   const int g = lane >> 2, q = lane & 3;
   const int rg = warp & 3, half = warp >> 2;
   const GroupTile t = find_group_tile(p.offsets, p.groups, p.T, blockIdx.x / p.slices, kTile);
-  if (t.group < 0) return;
-  const bool live = t.group < p.groups;
-  if (!live && p.resid == p.y) return;
+  const bool live = t.group >= 0 && t.group < p.groups;
+  // The first launch had waited for all before it when it let this one begin, so only its results are waited for:
+  // by the tiles that need them, and by all others too, so that this launch does not end before it.
+  if (!live) grid_wait();
+  if (t.group < 0 || (!live && p.resid == p.y)) return;
   tile_rows<kTile>(p, t, row_of);
   __syncthreads();
   const int count = t.end - t.begin;
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
 
   if (live) {
     const float scale = p.scales ? __ldg(p.scales + t.group) : 1.0f;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
     constexpr int LANES = RP / 4;  // of a row, 4 values each
 #pragma unroll
     for (int i = 0; i < kTile * LANES / kThreads; ++i) {
@@ -637,41 +641,27 @@ int splits_of(int64_t T, int64_t K, int groups) {
 
 template <int X, int Y, int RP>
 cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   if (!two_launches(a.T, a.groups)) {
     using Sh = ClusterShape<RP>;
     constexpr auto k = lora_cluster_kernel<X, Y, RP>;
     if (cudaError_t e = allow_smem<k>(Sh::SMEM)) return e;
     const int64_t tiles = tiles_of(a, Sh::M);
     if (tiles > INT32_MAX / kRanks) return cudaErrorInvalidValue;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kRanks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * kRanks));
-    cfg.dynamicSmemBytes = Sh::SMEM;
-    return cudaLaunchKernelEx(&cfg, k, a);
+    return launch_early(k, dim3(static_cast<unsigned>(tiles * kRanks)), dim3(kThreads), Sh::SMEM, s, kRanks, a);
   }
   constexpr auto shrink = lora_shrink_kernel<X, RP>;
   constexpr auto expand = lora_expand_kernel<X, Y, RP>;
+  constexpr int expand_smem = ExpandShape<RP, Y == 0 ? 4 : 2>::SMEM;
   if (cudaError_t e = allow_smem<shrink>(ShrinkShape<RP>::SMEM)) return e;
-  if (cudaError_t e = allow_smem<expand>(ExpandShape<RP, Y == 0 ? 4 : 2>::SMEM)) return e;
+  if (cudaError_t e = allow_smem<expand>(expand_smem)) return e;
   const int64_t tiles = tiles_of(a, kTile);
   a.splits = splits_of(a.T, a.K, a.groups);
   a.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((6 * num_sms + tiles - 1) / tiles, (a.N + 127) / 128)));
   if (tiles > INT32_MAX / std::max(a.splits, a.slices)) return cudaErrorInvalidValue;
-  shrink<<<static_cast<unsigned>(tiles * a.splits), kThreads, ShrinkShape<RP>::SMEM, s>>>(a);
-  if (cudaError_t e = cudaGetLastError()) return e;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.slices));
-  cfg.dynamicSmemBytes = (ExpandShape<RP, Y == 0 ? 4 : 2>::SMEM);
-  return cudaLaunchKernelEx(&cfg, expand, a);
+  if (cudaError_t e = launch_early(shrink, dim3(static_cast<unsigned>(tiles * a.splits)), dim3(kThreads), ShrinkShape<RP>::SMEM,
+                                   s, 1, a))
+    return e;
+  return launch_early(expand, dim3(static_cast<unsigned>(tiles * a.slices)), dim3(kThreads), expand_smem, s, 1, a);
 }
 
 template <int X, int Y>

@@ -54,20 +54,21 @@ static_assert(kScaleBox % 128 == 0, "TMA destinations");
 template <int W, bool GLU>
 struct IdShape {
   static constexpr bool Q4 = W == kWQ4;
-  static constexpr int STAGES = Q4 ? 3 : 6, RAWS = Q4 ? 3 : 0;
+  // Stages of A and of B have rings of their own: B's rows take longer to come.
+  static constexpr int AS = Q4 ? 3 : 5, BS = Q4 ? 4 : 7, RAWS = Q4 ? 2 : 0;
   static constexpr int A = Q4 ? 2 * kABytes : kABytes;  // 4 bits: the weights as sums of two numbers
-  static constexpr int STAGE = A + kBBytes;
+  static constexpr int OFF_B = AS * A;
   static constexpr int EPI = Q4 ? 8 : 16;   // epilogue warps
   static constexpr int CONV = Q4 ? 8 : 0;   // widening warps
   static constexpr int GATHER = 4;          // warps that fetch rows of x
   static constexpr int WARPS = 2 + EPI + CONV + GATHER + 1, THREADS = WARPS * 32;
   static constexpr int CHUNK = GLU ? 16 : 32;  // accumulator columns that an epilogue warp has in registers
-  static constexpr int OFF_RAW = STAGES * STAGE;
+  static constexpr int OFF_RAW = OFF_B + BS * kBBytes;
   static constexpr int OFF_SWAP = OFF_RAW + RAWS * kRawStride;
   static constexpr int SWAP = GLU ? EPI * 32 * 8 * 4 : 0;
   static constexpr int OFF_PRE = OFF_SWAP + SWAP;
   static constexpr int OFF_BARS = OFF_PRE + (static_cast<int>(kMaxGroups) + 2) * 4 + 8;
-  static constexpr int NBARS = 3 * STAGES + 2 * RAWS + 2 * kAccs + 1;
+  static constexpr int NBARS = 2 * AS + 3 * BS + 2 * RAWS + 2 * kAccs + 1;
   static constexpr int SMEM = OFF_BARS + NBARS * 8 + 8 + 4 + 4 + 2 * EPI * 4 + THREADS / 32 * 4 + 1024;
 };
 static_assert(IdShape<1, true>::SMEM <= 227 * 1024 && IdShape<kWQ4, true>::SMEM <= 227 * 1024, "shared memory");
@@ -137,16 +138,18 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
   using OV = typename Val<OUT32 ? 0 : (W == 2 ? 2 : 1)>::type;
   constexpr int OT = OUT32 ? 0 : (W == 2 ? 2 : 1);
   constexpr bool Q4 = Sh::Q4;
-  constexpr int ST = Sh::STAGES, RS = Sh::RAWS;
+  constexpr int AS = Sh::AS, BS = Sh::BS, RS = Sh::RAWS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* raws = smem + Sh::OFF_RAW;
   float* swap = reinterpret_cast<float*>(smem + Sh::OFF_SWAP);
   int* pre = reinterpret_cast<int*>(smem + Sh::OFF_PRE);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::OFF_BARS);  // used in the leader
-  uint64_t* empty = full + ST;
-  uint64_t* x_full = empty + ST;  // rows of x have arrived in this CTA
-  uint64_t* raw_full = x_full + ST;
+  uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + Sh::OFF_BARS);  // used in the leader, as b_full
+  uint64_t* a_empty = a_full + AS;
+  uint64_t* b_full = a_empty + AS;
+  uint64_t* b_empty = b_full + BS;
+  uint64_t* x_full = b_empty + BS;  // rows of x have arrived in this CTA
+  uint64_t* raw_full = x_full + BS;
   uint64_t* raw_empty = raw_full + RS;
   uint64_t* acc_full = raw_empty + RS;
   uint64_t* acc_empty = acc_full + kAccs;  // used in the leader: both CTAs' epilogue warps
@@ -165,10 +168,14 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
   const int kst = static_cast<int>((p.K + kStageK - 1) / kStageK);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], (Q4 ? 0 : 1) + 2 * (Sh::CONV + 1));
+    for (int s = 0; s < AS; ++s) {
+      mbar_init(&a_full[s], Q4 ? 8 : 1);  // four widening warps of each CTA, or the producer
+      mbar_init(&a_empty[s], 1);
+    }
+    for (int s = 0; s < BS; ++s) {
+      mbar_init(&b_full[s], 2);
+      mbar_init(&b_empty[s], 1);
       mbar_init(&x_full[s], Sh::GATHER * 32);
-      mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < RS; ++s) {
       mbar_init(&raw_full[s], 1);
@@ -184,6 +191,8 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
     tma_prefetch_desc(&maps.w);
     if constexpr (Q4) tma_prefetch_desc(&maps.scales);
   }
+  // (Tensor memory too is taken only now: the kernel before may still have blocks that ask for it.)
+  grid_wait();
   if (warp == 1) {
     tmem_alloc_pair(tmem_holder, kAccs * kBN);
     tmem_relinquish_pair();
@@ -224,31 +233,31 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
     // ------------------------------------- producer: the weights, as they are stored
     if (elect_one()) {
       if constexpr (!Q4) {
-        const uint32_t full0 = cluster_addr(full, 0);
+        const uint32_t full0 = cluster_addr(a_full, 0);
         uint32_t stage = 0, phase = 0, issued_mask = 0, issued_par = 0;
         bool ok = true;
         for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
           const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
           for (int ks = 0; ks < kst; ++ks) {
-            if (!mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag)) {
+            if (!mbar_wait(&a_empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag)) {
               ok = false;
               break;
             }
-            uint8_t* sb = smem + stage * Sh::STAGE;
+            uint8_t* sb = smem + stage * Sh::A;
             const uint32_t fb = full0 + stage * 8;
-            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kABytes);  // both CTAs' bytes
+            if (leader) mbar_arrive_expect_tx(&a_full[stage], 2 * kABytes);  // both CTAs' bytes
             tma_load_4d_pair(sb, &maps.w, fb, ks * kStageK, t.r0, 0, t.e);
             issued_mask |= 1u << stage;
             issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
-            if (++stage == ST) {
+            if (++stage == AS) {
               stage = 0;
               phase ^= 1u;
             }
           }
         }
         if (leader)  // every issued copy of both CTAs lands before the pair may exit
-          for (int s = 0; s < ST; ++s)
-            if ((issued_mask >> s) & 1u) mbar_wait(&full[s], (issued_par >> s) & 1u, status, kDevWaitDrain, nullptr);
+          for (int s = 0; s < AS; ++s)
+            if ((issued_mask >> s) & 1u) mbar_wait(&a_full[s], (issued_par >> s) & 1u, status, kDevWaitDrain, nullptr);
       } else {
         uint32_t raw = 0, phase = 0, issued_mask = 0, issued_par = 0;
         bool ok = true;
@@ -281,7 +290,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------- MMA issuer (leader)
     if (leader && elect_one()) {
-      uint32_t stage = 0, phase = 0, n = 0;
+      uint32_t as = 0, aphase = 0, bs = 0, bphase = 0, n = 0;
       bool ok = true;
       for (int tile = cluster; ok && tile < num_tiles; tile += nclusters, ++n) {
         const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
@@ -291,13 +300,14 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
         tc_fence_after();
         const uint32_t d = tmem_base + a * kBN;
         for (int ks = 0; ks < kst; ++ks) {
-          if (!mbar_wait(&full[stage], phase, status, kDevWaitMma, abort_flag)) {
+          if (!mbar_wait(&b_full[bs], bphase, status, kDevWaitMma, abort_flag) ||
+              !mbar_wait(&a_full[as], aphase, status, kDevWaitMma, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_base = smem_u32(smem + stage * Sh::STAGE);
-          const uint32_t b_base = a_base + Sh::A;
+          const uint32_t a_base = smem_u32(smem + as * Sh::A);
+          const uint32_t b_base = smem_u32(smem + Sh::OFF_B + bs * kBBytes);
 #pragma unroll
           for (int j = 0; j < kStageK / 16; ++j)
             mma_f16_pair(d, smem_desc_k_sw128(a_base + j * 32), smem_desc_k_sw128(b_base + j * 32), idesc,
@@ -307,10 +317,15 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
             for (int j = 0; j < kStageK / 16; ++j)
               mma_f16_pair(d, smem_desc_k_sw128(a_base + kABytes + j * 32), smem_desc_k_sw128(b_base + j * 32), idesc, 1u);
           }
-          mma_commit_pair(&empty[stage], 0x3);
-          if (++stage == ST) {
-            stage = 0;
-            phase ^= 1u;
+          mma_commit_pair(&a_empty[as], 0x3);
+          mma_commit_pair(&b_empty[bs], 0x3);
+          if (++as == AS) {
+            as = 0;
+            aphase ^= 1u;
+          }
+          if (++bs == BS) {
+            bs = 0;
+            bphase ^= 1u;
           }
         }
         if (ok) mma_commit_pair(&acc_full[a], 0x3);
@@ -410,25 +425,33 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
   } else if (warp < 2 + Sh::EPI + Sh::CONV) {
     // -------------------------------------------- Q4_0: nibbles to the A tile
     if constexpr (Q4) {
+      // Groups of four warps take turns at the stages: while one group's stage is on its way to the tensor core the
+      // other widens the next.  A thread has a row of the CTA's 128, and its two blocks of the stage.
       const int ct = threadIdx.x - (2 + Sh::EPI) * 32;
-      const int r = ct & 127, b = ct >> 7;  // a row's block b of the stage's two
-      const uint32_t full0 = cluster_addr(full, 0);
-      uint32_t stage = 0, phase = 0, raw = 0, raw_phase = 0;
+      const int r = ct & 127, turn = ct >> 7;
+      const uint32_t full0 = cluster_addr(a_full, 0);
+      uint32_t stage = 0, phase = 0, raw = 0, raw_phase = 0, n = 0;
       bool ok = true;
       for (int tile = cluster; ok && tile < num_tiles; tile += nclusters) {
         const IdTile t = id_tile<GLU>(p, pre, tile, w_tiles, rank);
         const int64_t first = static_cast<int64_t>(t.e) * p.rows + (r < 64 ? t.r0 : t.r1);
         const int scale_at = 2 * kRawBox + (r >> 6) * kScaleBox + (static_cast<int>(first & 7) + (r & 63)) * 2;
-        for (int ks = 0; ks < kst; ++ks) {
+        for (int ks = 0; ks < kst; ++ks, ++n) {
           if (ks % 4 == 0)
             ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[raw], raw_phase, status, kDevWaitProducer, abort_flag));
           if (!ok) break;
-          const uint8_t* rb = raws + raw * kRawStride;
-          const int block = (ks % 4) * 2 + b;
-          const uint4 q = *reinterpret_cast<const uint4*>(rb + r * 128 + ((block ^ (r & 7)) << 4));
-          const uint32_t d = *reinterpret_cast<const uint16_t*>(rb + scale_at + block * (kScaleCols * 2));
-          // d as a number of 7 bits and one of 4: both times q - 8 are exact in fp16
-          const uint32_t hi2 = (d | (d << 16)) & 0xfff0fff0u, lo2 = hsub2_u(d | (d << 16), hi2);
+          const bool mine = n % (Sh::CONV / 4) == static_cast<uint32_t>(turn);
+          uint4 q[2];
+          uint32_t d[2];
+          if (mine) {
+            const uint8_t* rb = raws + raw * kRawStride;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int block = (ks % 4) * 2 + b;
+              q[b] = *reinterpret_cast<const uint4*>(rb + r * 128 + ((block ^ (r & 7)) << 4));
+              d[b] = *reinterpret_cast<const uint16_t*>(rb + scale_at + block * (kScaleCols * 2));
+            }
+          }
           if (ks % 4 == 3 || ks == kst - 1) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&raw_empty[raw]);
@@ -437,23 +460,30 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
               raw_phase ^= 1u;
             }
           }
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
-          if (!ok) break;
-          uint8_t* ab = smem + stage * Sh::STAGE + r * 128;
-          constexpr uint32_t m = 0x0f0f0f0fu;
-          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+          if (mine) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
+            if (!ok) break;
+            uint8_t* ab = smem + stage * Sh::A + r * 128;
+            constexpr uint32_t m = 0x0f0f0f0fu;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {  // values 8 j .. 8 j + 7: low nibbles of 8 bytes, then the high ones
-            const uint32_t w0 = words[(j & 1) * 2], w1 = words[(j & 1) * 2 + 1];
-            const uint2 u = codes4((j < 2 ? w0 : w0 >> 4) & m), v = codes4((j < 2 ? w1 : w1 >> 4) & m);
-            uint4* at = reinterpret_cast<uint4*>(ab + (((b * 4 + j) ^ (r & 7)) << 4));
-            at[0] = make_uint4(hmul2_u(u.x, hi2), hmul2_u(u.y, hi2), hmul2_u(v.x, hi2), hmul2_u(v.y, hi2));
-            at[kABytes / 16] = make_uint4(hmul2_u(u.x, lo2), hmul2_u(u.y, lo2), hmul2_u(v.x, lo2), hmul2_u(v.y, lo2));
+            for (int b = 0; b < 2; ++b) {
+              // d as a number of 7 bits and one of 4: both times q - 8 are exact in fp16
+              const uint32_t d2 = d[b] | (d[b] << 16), hi2 = d2 & 0xfff0fff0u, lo2 = hsub2_u(d2, hi2);
+              const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {  // values 8 j .. 8 j + 7: low nibbles of 8 bytes, then the high ones
+                const uint32_t w0 = words[(j & 1) * 2], w1 = words[(j & 1) * 2 + 1];
+                const uint2 u = codes4((j < 2 ? w0 : w0 >> 4) & m), v = codes4((j < 2 ? w1 : w1 >> 4) & m);
+                uint4* at = reinterpret_cast<uint4*>(ab + (((b * 4 + j) ^ (r & 7)) << 4));
+                at[0] = make_uint4(hmul2_u(u.x, hi2), hmul2_u(u.y, hi2), hmul2_u(v.x, hi2), hmul2_u(v.y, hi2));
+                at[kABytes / 16] = make_uint4(hmul2_u(u.x, lo2), hmul2_u(u.y, lo2), hmul2_u(v.x, lo2), hmul2_u(v.y, lo2));
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(full0 + stage * 8);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(full0 + stage * 8);
-          if (++stage == ST) {
+          if (++stage == AS) {
             stage = 0;
             phase ^= 1u;
           }
@@ -477,9 +507,9 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
         src[i] = static_cast<const uint8_t*>(p.x) + (s < 0 || s >= p.S ? 0 : s / p.per_row) * p.ldx * 2 + chunk * 16;
       }
       for (int ks = 0; ks < kst; ++ks) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(&b_empty[stage], phase ^ 1u, status, kDevWaitProducer, abort_flag));
         if (!ok) break;
-        const uint32_t dst = smem_u32(smem + stage * Sh::STAGE + Sh::A) + ((chunk ^ (row0 & 7)) << 4) + row0 * 128;
+        const uint32_t dst = smem_u32(smem + Sh::OFF_B + stage * kBBytes) + ((chunk ^ (row0 & 7)) << 4) + row0 * 128;
         const int bytes = ks * kStageK + chunk * 8 < p.K ? 16 : 0;  // zeros behind the row's end
         const int64_t at = bytes ? static_cast<int64_t>(ks) * 128 : 0;
 #pragma unroll
@@ -488,7 +518,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * 2048), "l"(src[i] + at), "r"(bytes)
                          : "memory");
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&x_full[stage])) : "memory");
-        if (++stage == ST) {
+        if (++stage == BS) {
           stage = 0;
           phase ^= 1u;
         }
@@ -499,7 +529,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
     // A thread with no copies of its own makes the arrived rows visible to the tensor core (the same fence in a
     // gather warp would wait for all that the warp has asked for) and reports them to the leader.
     if (elect_one()) {
-      const uint32_t full0 = cluster_addr(full, 0);
+      const uint32_t full0 = cluster_addr(b_full, 0);
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       for (int tile = cluster; ok && tile < num_tiles; tile += nclusters)
@@ -508,7 +538,7 @@ __global__ void __launch_bounds__(IdShape<W, GLU>::THREADS, 1)
           if (!ok) break;
           fence_proxy_async_smem();
           mbar_arrive_remote(full0 + stage * 8);
-          if (++stage == ST) {
+          if (++stage == BS) {
             stage = 0;
             phase ^= 1u;
           }
@@ -529,17 +559,6 @@ template <int W, bool GLU, bool OUT32>
 cudaError_t launch_shape(const MulMatIdArgs& a, const IdMaps& maps, int64_t tiles, cudaStream_t s) {
   using Sh = IdShape<W, GLU>;
   auto kernel = mul_mat_id_kernel<W, GLU, OUT32>;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(Sh::THREADS);
-  cfg.dynamicSmemBytes = Sh::SMEM;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   // Once per device: the shared memory, and how many pairs can be resident at once.
   static std::atomic<uint64_t> ready{0};
   static std::atomic<int> max_clusters[64];
@@ -548,15 +567,25 @@ cudaError_t launch_shape(const MulMatIdArgs& a, const IdMaps& maps, int64_t tile
   const uint64_t bit = uint64_t{1} << dev;
   if (!(ready.load(std::memory_order_acquire) & bit)) {
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM)) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(Sh::THREADS);
+    cfg.dynamicSmemBytes = Sh::SMEM;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     int n = 0;
     if (cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) return e;
     if (n < 1) return cudaErrorInvalidConfiguration;
     max_clusters[dev].store(n);
     ready.fetch_or(bit, std::memory_order_acq_rel);
   }
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(tiles, max_clusters[dev].load())));
-  return cudaLaunchKernelEx(&cfg, kernel, maps, a);
+  const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(tiles, max_clusters[dev].load()));
+  return launch_early(kernel, dim3(2 * pairs), dim3(Sh::THREADS), Sh::SMEM, s, 2, maps, a);
 }
 
 }  // namespace

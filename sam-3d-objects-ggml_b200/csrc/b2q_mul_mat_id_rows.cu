@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1) id_rows_kernel(const MulMatIdArgs
   const int r_tiles = static_cast<int>((p.n + ROWS - 1) / ROWS);
   const int pitch = static_cast<int>(x_pitch(p.K));
 
+  grid_wait();
   // pre[e]: tiles of the experts before e.
   int carry = 0;
   for (int e0 = 0; e0 <= p.E; e0 += kThreads) {
@@ -354,8 +355,7 @@ cudaError_t launch_shape(const MulMatIdArgs& a, int num_sms, cudaStream_t s) {
   if (nt < 1) return cudaErrorInvalidValue;
   constexpr auto k = id_rows_kernel<GLU, OUT32>;
   if (cudaError_t e = allow_smem<k>(kSmemMax)) return e;
-  k<<<num_sms, kThreads, kFixed + nt * 8 * pitch, s>>>(a, nt * 8);
-  return cudaGetLastError();
+  return launch_early(k, dim3(static_cast<unsigned>(num_sms)), dim3(kThreads), kFixed + nt * 8 * pitch, s, 1, a, nt * 8);
 }
 
 }  // namespace

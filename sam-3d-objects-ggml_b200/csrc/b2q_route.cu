@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int E = a.E;
   const bool one = a.run_counts == nullptr;
+  grid_wait();
   if (!one) {
     for (int i = threadIdx.x; i <= E; i += kThreads) smem[i] = 0;
     __syncthreads();
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
 __global__ void __launch_bounds__(kThreads) count_kernel(const int32_t* ids, int S, int groups, int run_slots,
                                                          int32_t* run_counts) {
   extern __shared__ int smem[];
+  grid_wait();
   for (int i = threadIdx.x; i <= groups; i += kThreads) smem[i] = 0;
   __syncthreads();
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * run_slots;
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const int32_t* ids, int
 __global__ void __launch_bounds__(kThreads) place_kernel(const int32_t* ids, int S, int groups, int run_slots,
                                                          const int32_t* run_counts, int32_t* order, int32_t* offsets) {
   extern __shared__ int smem[];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
   place_run(ids, S, groups, blockIdx.x, gridDim.x, run_slots, run_counts, order, offsets, smem);
 }
 
@@ -285,17 +287,8 @@ cudaError_t launch_place(const int32_t* ids, int64_t S, int groups, int runs, in
                          int32_t* order, int32_t* offsets, cudaStream_t s) {
   const size_t smem = place_smem(groups);
   if (cudaError_t e = set_smem(reinterpret_cast<const void*>(place_kernel), smem)) return e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(runs));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = run_counts ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, place_kernel, ids, static_cast<int>(S), groups, run_slots, run_counts, order, offsets);
+  return launch_early(place_kernel, dim3(static_cast<unsigned>(runs)), dim3(kThreads), smem, s, 1, ids, static_cast<int>(S),
+                      groups, run_slots, run_counts, order, offsets);
 }
 
 // y [T * top] rows -> out [T] rows: out = resid + sum_j w_j y_j, choices in
@@ -307,6 +300,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   using OV = typename Val<O>::type;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t n = (static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x) * N;
+  grid_wait();
   if (t >= a.T || n >= a.n) return;
   float sum[N] = {}, more[N];
   if (a.resid) load_vec<O>(static_cast<const OV*>(a.resid) + t * a.ldr + n, more);
@@ -357,8 +351,7 @@ cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
     const int nv = (a.E + 31) / 32;
     auto go = [&](auto k) {
       if (cudaError_t e = set_smem(reinterpret_cast<const void*>(k), smem)) return e;
-      k<<<p.runs, kThreads, smem, s>>>(a);
-      return cudaSuccess;
+      return launch_early(k, dim3(static_cast<unsigned>(p.runs)), dim3(kThreads), smem, s, 1, a);
     };
     if (nv <= 1) return go(route_kernel<T, 1>);
     if (nv <= 2) return go(route_kernel<T, 2>);
@@ -372,9 +365,7 @@ cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
   };
   const cudaError_t err = type == kXF32 ? run(std::integral_constant<int, 0>())
                           : type == kXF16 ? run(std::integral_constant<int, 1>()) : run(std::integral_constant<int, 2>());
-  if (err != cudaSuccess) return err;
-  if (cudaError_t e = cudaGetLastError()) return e;
-  if (one) return cudaSuccess;
+  if (err != cudaSuccess || one) return err;
   return launch_place(a.ids, a.T * a.top, a.E, p.runs, p.run_units * a.top, a.run_counts, a.order, a.offsets, s);
 }
 
@@ -383,8 +374,9 @@ cudaError_t launch_group_rows(const int32_t* ids, int64_t S, int groups, int32_t
   const RunPlan p = run_plan(S, 1);
   if (p.runs == 1)
     return launch_place(ids, S, groups, 1, static_cast<int>(std::max<int64_t>(S, 1)), nullptr, order, offsets, s);
-  count_kernel<<<p.runs, kThreads, (groups + 1) * 4, s>>>(ids, static_cast<int>(S), groups, p.run_units, run_counts);
-  if (cudaError_t e = cudaGetLastError()) return e;
+  if (cudaError_t e = launch_early(count_kernel, dim3(static_cast<unsigned>(p.runs)), dim3(kThreads), (groups + 1) * 4, s, 1, ids,
+                                   static_cast<int>(S), groups, p.run_units, run_counts))
+    return e;
   return launch_place(ids, S, groups, p.runs, p.run_units, run_counts, order, offsets, s);
 }
 
@@ -404,18 +396,16 @@ cudaError_t launch_combine(const CombineArgs& a, int ytype, int otype, cudaStrea
   const dim3 grid(static_cast<unsigned>((a.T + block.y - 1) / block.y), static_cast<unsigned>((cols + tx - 1) / tx));
   auto pick = [&](auto y, auto o) {
     constexpr int Y = decltype(y)::value, O = decltype(o)::value, N = Y == 0 || O == 0 ? 4 : 8;
-    auto k = vec ? combine_kernel<Y, O, N> : combine_kernel<Y, O, 1>;
-    k<<<grid, block, 0, s>>>(a);
+    return launch_early(vec ? combine_kernel<Y, O, N> : combine_kernel<Y, O, 1>, grid, block, 0, s, 1, a);
   };
   auto pick_o = [&](auto y) {
-    if (otype == kXF32) pick(y, std::integral_constant<int, 0>());
-    else if (otype == kXF16) pick(y, std::integral_constant<int, 1>());
-    else pick(y, std::integral_constant<int, 2>());
+    return otype == kXF32   ? pick(y, std::integral_constant<int, 0>())
+           : otype == kXF16 ? pick(y, std::integral_constant<int, 1>())
+                            : pick(y, std::integral_constant<int, 2>());
   };
-  if (ytype == kXF32) pick_o(std::integral_constant<int, 0>());
-  else if (ytype == kXF16) pick_o(std::integral_constant<int, 1>());
-  else pick_o(std::integral_constant<int, 2>());
-  return cudaGetLastError();
+  return ytype == kXF32   ? pick_o(std::integral_constant<int, 0>())
+         : ytype == kXF16 ? pick_o(std::integral_constant<int, 1>())
+                          : pick_o(std::integral_constant<int, 2>());
 }
 
 }  // namespace b2q

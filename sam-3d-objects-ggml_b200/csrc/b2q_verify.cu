@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ranks = a.ranks, rank = ranks > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int64_t b = blockIdx.x / ranks;
+  grid_wait();
   const int64_t lo = min(max(static_cast<int64_t>(__ldg(a.cu + b)), int64_t{0}), a.D);
   const int64_t hi = min(max(static_cast<int64_t>(__ldg(a.cu + b + 1)), lo), a.D);
   const V* target = static_cast<const V*>(a.target);
@@ -235,18 +236,7 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
 cudaError_t launch_verify(VerifyArgs a, int type, cudaStream_t s) {
   a.ranks = kVerifyRanks;
   void (*kernels[3])(const VerifyArgs) = {verify_kernel<0>, verify_kernel<1>, verify_kernel<2>};
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(a.ranks);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(a.B * a.ranks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernels[type], a);
+  return launch_early(kernels[type], dim3(static_cast<unsigned>(a.B * a.ranks)), dim3(kThreads), 0, s, a.ranks, a);
 }
 
 }  // namespace b2q

@@ -7,10 +7,10 @@
 //   offsets = where each expert's slots begin
 //
 // A row's experts are spread over the lanes of one warp and stay in registers,
-// as unsigned numbers that order as the keys do (-0 as 0, NaN as -infinity).  Each
-// choice is one warp maximum (redux) of the lanes' largest and, among the lanes
-// that hold it, one minimum of the expert's number; its lane then looks for its
-// next largest.
+// as unsigned numbers that order as the keys do (-0 as 0, NaN as -infinity); up to 8
+// of a lane are sorted first.  Each choice is one warp maximum (redux) of the lanes'
+// largest and, among the lanes that hold it, one minimum of the expert's number;
+// its lane then moves on to its next largest.
 //
 // The sort is a counting sort without float work or global atomics: every CTA
 // counts the experts of its run of slots; then every CTA adds up the counts of
@@ -99,23 +99,32 @@ __device__ void place_run(const int32_t* ids, int S, int groups, int run, int ru
   }
   __syncthreads();
   if (run_counts) {
-    for (int g = lane; g < G; g += 32) {
-      int all = 0, before = 0;
+    // (six groups of a lane and five runs asked for at a time)
+    for (int g0 = lane; g0 < G; g0 += 6 * 32) {
+      int all[6] = {}, before[6] = {};
       for (int r0 = warp; r0 < runs; r0 += 5 * kWarps) {
-        int c[5];
+        int c[5][6];
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-          const int r = r0 + i * kWarps;
-          c[i] = r < runs ? __ldg(run_counts + static_cast<int64_t>(r) * G + g) : 0;
-        }
+        for (int i = 0; i < 5; ++i)
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-          all += c[i];
-          if (r0 + i * kWarps < run) before += c[i];
-        }
+          for (int j = 0; j < 6; ++j) {
+            const int r = r0 + i * kWarps, g = g0 + 32 * j;
+            c[i][j] = r < runs && g < G ? __ldg(run_counts + static_cast<int64_t>(r) * G + g) : 0;
+          }
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+#pragma unroll
+          for (int j = 0; j < 6; ++j) {
+            all[j] += c[i][j];
+            if (r0 + i * kWarps < run) before[j] += c[i][j];
+          }
       }
-      atomicAdd(&total[g], all);
-      atomicAdd(&base[g], before);
+#pragma unroll
+      for (int j = 0; j < 6; ++j)
+        if (g0 + 32 * j < G) {
+          atomicAdd(&total[g0 + 32 * j], all[j]);
+          atomicAdd(&base[g0 + 32 * j], before[j]);
+        }
     }
     __syncthreads();
   }
@@ -188,20 +197,49 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
     if (t + kWarps < t1) fetch(t + kWarps);
     float picked = 0.0f;  // lane j: the logit of choice j
     int chosen = -1;
-    for (int j = 0; j < a.top; ++j) {
-      uint32_t best = key[0];
+    if constexpr (NV <= 8) {
+      // The lane's keys in falling order, equal ones in the experts' order (neighbours change places only where the
+      // later is larger), with their places as digits of `places`: a choice takes the first and moves the others up.
+      uint32_t places = 0x76543210u;
 #pragma unroll
-      for (int i = 1; i < NV; ++i) best = max(best, key[i]);
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      if (top <= kKeyNone) break;  // only -infinity is left
-      unsigned mine = 0x7fffffffu;  // the lane's lowest expert with that key
+      for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = NV - 1; i >= 0; --i)
-        if (key[i] == top) mine = lane + 32 * i;
-      const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine));
+        for (int i = n & 1; i + 1 < NV; i += 2) {
+          const bool change = key[i + 1] > key[i];
+          const uint32_t high = max(key[i], key[i + 1]), low = min(key[i], key[i + 1]);
+          key[i] = high;
+          key[i + 1] = low;
+          const uint32_t differ = ((places >> 4) ^ places) & (0xfu << (4 * i));  // of the two digits
+          places ^= change ? differ | (differ << 4) : 0u;
+        }
+      for (int j = 0; j < a.top; ++j) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
+        if (top <= kKeyNone) break;  // only -infinity is left
+        const unsigned mine = lane + 32 * (places & 15u);
+        const unsigned e = __reduce_min_sync(0xffffffffu, key[0] == top ? mine : 0x7fffffffu);
+        const bool taken = mine == e;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) key[i] = e == lane + 32 * i ? 0u : key[i];
-      chosen = lane == j ? e : chosen;
+        for (int i = 0; i + 1 < NV; ++i) key[i] = taken ? key[i + 1] : key[i];
+        key[NV - 1] = taken ? 0u : key[NV - 1];
+        places = taken ? places >> 4 : places;
+        chosen = lane == j ? static_cast<int>(e) : chosen;
+      }
+    } else {
+      for (int j = 0; j < a.top; ++j) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) best = max(best, key[i]);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        if (top <= kKeyNone) break;
+        unsigned mine = 0x7fffffffu;  // the lane's lowest expert with that key
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i)
+          if (key[i] == top) mine = lane + 32 * i;
+        const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = e == lane + 32 * i ? 0u : key[i];
+        chosen = lane == j ? e : chosen;
+      }
     }
     const bool there = chosen >= 0;
     // lane j: the logit of choice j, from the lane that has it

@@ -70,37 +70,58 @@ struct Val<2> {
   static __device__ __forceinline__ __nv_bfloat16 to(float v) { return __float2bfloat16_rn(v); }
 };
 
-// N values (1, or as many as 4 or 8) in one load or store of their size.
+// N values (1, or as many as 4 or 8) in one load or store of their size; Raw: as
+// they are loaded, which takes half the registers for 16-bit values.
 template <int T, int N>
-__device__ __forceinline__ void load_vec(const typename Val<T>::type* p, float (&v)[N]) {
+struct Raw {
+  uint32_t w[T == 0 ? N : N / 2];
+};
+template <int T>
+struct Raw<T, 1> {
+  typename Val<T>::type v;
+};
+template <int T, int N>
+__device__ __forceinline__ Raw<T, N> load_raw(const typename Val<T>::type* p) {
+  Raw<T, N> r;
   if constexpr (N == 1) {
-    v[0] = Val<T>::load(p);
-  } else if constexpr (T == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 f = *reinterpret_cast<const float4*>(p + i);
-      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
-    }
+    r.v = *p;
   } else {
-    uint32_t w[N / 2];
-    if constexpr (N == 8) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-    } else {
-      static_assert(N == 4, "");
+    constexpr int WORDS = T == 0 ? N : N / 2;
+    if constexpr (WORDS == 2) {
       const uint2 u = *reinterpret_cast<const uint2*>(p);
-      w[0] = u.x, w[1] = u.y;
-    }
+      r.w[0] = u.x, r.w[1] = u.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      if constexpr (T == 1) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+        r.w[i] = u.x, r.w[i + 1] = u.y, r.w[i + 2] = u.z, r.w[i + 3] = u.w;
       }
     }
   }
+  return r;
+}
+template <int T, int N>
+__device__ __forceinline__ void from_raw(const Raw<T, N>& r, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = Val<T>::load(&r.v);
+  } else if constexpr (T == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (T == 1) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(r.w[i] << 16), v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+template <int T, int N>
+__device__ __forceinline__ void load_vec(const typename Val<T>::type* p, float (&v)[N]) {
+  from_raw<T, N>(load_raw<T, N>(p), v);
 }
 template <int T, int N>
 __device__ __forceinline__ void store_vec(typename Val<T>::type* p, const float (&v)[N]) {

@@ -340,29 +340,39 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   const int64_t n = (static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x) * N;
   grid_wait();
   if (t >= a.T || n >= a.n) return;
-  float sum[N] = {}, more[N];
-  if (a.resid) load_vec<O>(static_cast<const OV*>(a.resid) + t * a.ldr + n, more);
+  float sum[N] = {};
+  Raw<O, N> more;
+  if (a.resid) more = load_raw<O, N>(static_cast<const OV*>(a.resid) + t * a.ldr + n);
   const YV* y = static_cast<const YV*>(a.y) + t * a.top * a.ldy + n;
   const float* w = a.weights + t * a.top;
   const int32_t* ids = a.ids ? a.ids + t * a.top : nullptr;
   for (int j0 = 0; j0 < a.top; j0 += 4) {
-    float v[4][N], share[4];
+    Raw<Y, N> raw[4];
+    float share[4];
+    bool there[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool there = j0 + j < a.top && !(ids && __ldg(ids + j0 + j) < 0);
-      share[j] = there ? __ldg(w + j0 + j) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[j][i] = 0.0f;
-      if (there) load_vec<Y>(y + (j0 + j) * a.ldy, v[j]);
+      there[j] = j0 + j < a.top && !(ids && __ldg(ids + j0 + j) < 0);
+      if (there[j]) {
+        share[j] = __ldg(w + j0 + j);
+        raw[j] = load_raw<Y, N>(y + (j0 + j) * a.ldy);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
+      if (there[j]) {
+        float v[N];
+        from_raw<Y, N>(raw[j], v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum[i] = fmaf(share[j], v[j][i], sum[i]);
+        for (int i = 0; i < N; ++i) sum[i] = fmaf(share[j], v[i], sum[i]);
+      }
   }
-  if (a.resid)
+  if (a.resid) {
+    float v[N];
+    from_raw<O, N>(more, v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] += more[i];
+    for (int i = 0; i < N; ++i) sum[i] += v[i];
+  }
   store_vec<O>(static_cast<OV*>(a.out) + t * a.ldo + n, sum);
 }
 

@@ -245,7 +245,7 @@ __device__ __forceinline__ void stream_columns(const LoraArgs& p, int group, boo
 }
 
 template <int X, int Y, int RP>
-__global__ void __launch_bounds__(kThreads) lora_cluster_kernel(const LoraArgs p) {
+__global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kernel(const LoraArgs p) {
   using Sh = ClusterShape<RP>;
   constexpr int M = Sh::M, N8 = RP / 8;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -631,7 +631,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
 
 int padded(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 int64_t tiles_of(const LoraArgs& a, int rows) { return a.T / rows + std::min<int64_t>(a.groups + 1, a.T); }
-bool two_launches(int64_t T, int groups) { return T > 16 * groups; }
+// One launch while its tiles of 16 rows (about half a tile more per adapter than the rows fill) are not many times
+// what is resident at once.  Measured, one launch against two: 2048 x 6144, rank 64, 32 adapters of 16 rows 13.7 us
+// against 27.0, of 32 rows 28.6 against 31.8, of 64 rows 53 against 36; 2048 x 2048, rank 128, 32 adapters of 16 rows
+// 18.7 against 34.5, of 32 rows 38.6 against 39.0, 4 adapters of 128 rows 25 against 17.
+bool two_launches(int64_t T, int groups, int rank) {
+  return T / 16 + std::min<int64_t>(groups, T) / 2 > (rank <= 64 ? 96 : 48);
+}
 
 // Parts of K of the first launch, and of the columns of the second: enough CTAs for the device where tiles are few.
 int splits_of(int64_t T, int64_t K, int groups) {
@@ -641,7 +647,7 @@ int splits_of(int64_t T, int64_t K, int groups) {
 
 template <int X, int Y, int RP>
 cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
-  if (!two_launches(a.T, a.groups)) {
+  if (!two_launches(a.T, a.groups, a.rank)) {
     using Sh = ClusterShape<RP>;
     constexpr auto k = lora_cluster_kernel<X, Y, RP>;
     if (cudaError_t e = allow_smem<k>(Sh::SMEM)) return e;
@@ -677,7 +683,7 @@ cudaError_t launch_types(const LoraArgs& a, int num_sms, cudaStream_t s) {
 }  // namespace
 
 size_t lora_workspace(int64_t T, int64_t K, int groups, int rank) {
-  if (T <= 0 || !two_launches(T, groups)) return 0;
+  if (T <= 0 || !two_launches(T, groups, rank)) return 0;
   return static_cast<size_t>(splits_of(T, K, groups)) * T * padded(rank) * 4;
 }
 

@@ -383,7 +383,8 @@ def call_lora(c, **kw):
 @pytest.mark.parametrize("dt,out", [("f16", "f32"), ("bf16", "f32"), ("f16", "f16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("T,G,rank,k,n", [(1, 1, 8, 8, 1), (1, 3, 16, 64, 64), (5, 40, 8, 1000, 33), (32, 24, 16, 4096, 520),
                                           (64, 2, 128, 256, 130), (300, 3, 64, 520, 1030), (1000, 5, 24, 136, 77),
-                                          (2500, 2, 40, 72, 264), (70, 70, 104, 2048, 16)])
+                                          (2500, 2, 40, 72, 264), (70, 70, 104, 2048, 16), (1700, 3, 16, 256, 129),
+                                          (1800, 9, 64, 1032, 200), (1600, 2, 128, 136, 321), (3000, 40, 32, 64, 96)])
 def test_lora(dev, dt, out, T, G, rank, k, n):
     c = make_lora(dev, T, G, rank, k, n, dt, out, seed=T + n)
     ref, tol = lora_reference(c)
@@ -396,21 +397,22 @@ def test_lora(dev, dt, out, T, G, rank, k, n):
     assert call_lora(c2, out=mine) is mine and torch.equal(mine, y)
 
 
-def test_lora_without_scales_and_with_strides(dev):
-    c = make_lora(dev, 90, 4, 16, 128, 100, "f16", "f32", seed=2)
+@pytest.mark.parametrize("T", [90, 1900])
+def test_lora_without_scales_and_with_strides(dev, T):
+    c = make_lora(dev, T, 4, 16, 128, 100, "f16", "f32", seed=2)
     c["scales"] = None
     ref, tol = lora_reference(c, scales=False)
-    wide = torch.zeros(90, 160, dtype=torch.float16, device=dev)
+    wide = torch.zeros(T, 160, dtype=torch.float16, device=dev)
     wide[:, :128] = c["x"]
-    res = torch.zeros(90, 111, device=dev)
+    res = torch.zeros(T, 111, device=dev)
     res[:, 3:103] = c["resid"]
-    out = torch.full((90, 107), 7.0, device=dev)
+    out = torch.full((T, 107), 7.0, device=dev)
     y = call_lora(dict(c, x=wide[:, :128], resid=res[:, 3:103]), out=out[:, 1:101])
     check_rows(y, ref, tol)
     assert bool((out[:, 0] == 7.0).all()) and bool((out[:, 101:] == 7.0).all())
 
 
-@pytest.mark.parametrize("T", [20, 400])
+@pytest.mark.parametrize("T", [20, 400, 2000])
 @pytest.mark.parametrize("big", [3e4, 1e-6])
 def test_lora_rank_values_beyond_16_bits(dev, T, big):
     """A x that overflows fp16, or lies among its smallest numbers, still counts."""
@@ -424,8 +426,9 @@ def test_lora_rank_values_beyond_16_bits(dev, T, big):
     check_rows(call_lora(c), ref, tol)
 
 
-def test_lora_non_finite_rows_stay_alone(dev):
-    c = make_lora(dev, 200, 2, 16, 128, 64, "bf16", "f32", seed=4)
+@pytest.mark.parametrize("T", [200, 2200])
+def test_lora_non_finite_rows_stay_alone(dev, T):
+    c = make_lora(dev, T, 2, 16, 128, 64, "bf16", "f32", seed=4)
     clean = call_lora(c)
     c["x"][31] = math.nan
     c["ids"][31] = 0
@@ -433,7 +436,7 @@ def test_lora_non_finite_rows_stay_alone(dev):
     c["ids"][100] = 1
     order, offsets = b2q.group_rows(c["ids"], 2)
     y = call_lora(c)
-    keep = torch.ones(200, dtype=torch.bool, device=dev)
+    keep = torch.ones(T, dtype=torch.bool, device=dev)
     keep[[31, 100]] = False
     ref, tol = lora_reference(c)
     check_rows(y[keep], ref[keep], tol[keep])
@@ -441,8 +444,9 @@ def test_lora_non_finite_rows_stay_alone(dev):
     assert clean.shape == y.shape
 
 
-def test_lora_with_a_broken_plan_stays_inside(dev):
-    c = make_lora(dev, 64, 4, 8, 64, 40, "f16", "f32", seed=6)
+@pytest.mark.parametrize("T", [64, 2000])
+def test_lora_with_a_broken_plan_stays_inside(dev, T):
+    c = make_lora(dev, T, 4, 8, 64, 40, "f16", "f32", seed=6)
     order, offsets = b2q.group_rows(c["ids"], 4)
     bad = order.clone()
     bad[[1, 30]] = torch.tensor([-5, 1 << 29], dtype=torch.int32, device=dev)
@@ -504,3 +508,39 @@ def test_on_a_given_stream(dev):
     z = b2q.lora_add(lo["resid"], lo["x"], lo["a"], lo["b"], lo["scales"], o2, f2, stream=s)
     s.synchronize()
     assert torch.equal(y, want) and torch.equal(z, want_lo)
+
+
+@pytest.mark.parametrize("T", [30, 2000])
+def test_calls_that_follow_one_another_wait_for_one_another(dev, T):
+    """Buffers written and read by neighbouring calls (a launch may begin while the one before it ends): 60 rounds of
+    products, adapters and joins over the same rows give, bit for bit, what they give one by one."""
+    E, top, C, F, G = 6, 2, 128, 96, 3
+    g = torch.Generator(device=dev).manual_seed(T)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    w1, w2 = (r(E, 2 * F, C) / 11).bfloat16(), (r(E, C, F) / 10).bfloat16()
+    a, b, ids = (r(G, 16, C) / 11).bfloat16(), (0.3 * r(G, C, 16) / 4).bfloat16(), torch.randint(-1, G, (T,), generator=g, device=dev).int()
+    rows = b2q.group_rows(ids, G)
+    x = r(T, C)
+    z, y = torch.empty(T * top, F, dtype=torch.bfloat16, device=dev), torch.empty(T * top, C, device=dev)
+
+    def round_(x, wait):
+        h = (x * torch.rsqrt(x.square().mean(1, keepdim=True))).bfloat16()
+        wait()
+        choice, share, order, offsets = b2q.moe_route(h[:, :E], top)
+        wait()
+        b2q.mul_mat_id(b2q.TYPE_BF16, w1, F, C, h, order, offsets, per_row=top, glu=True, out=z)
+        wait()
+        b2q.mul_mat_id(b2q.TYPE_BF16, w2, C, F, z, order, offsets, out=y)
+        wait()
+        b2q.moe_combine(y, share, choice, resid=x, out=x)
+        wait()
+        b2q.lora_add(x, h, a, b, None, *rows, out=x)
+        wait()
+
+    slow = x.clone()
+    for _ in range(60):
+        round_(slow, torch.cuda.synchronize)
+    fast = x.clone()
+    for _ in range(60):
+        round_(fast, lambda: None)
+    assert torch.equal(fast, slow) and bool(torch.isfinite(fast).all())

@@ -103,7 +103,7 @@ def lora(**kw):
     (dict(T=(1 << 30) + 1), TOO), (dict(n=1 << 31, ldr=1 << 33, ldy=1 << 33), TOO), (dict(x=FAKE + 8), ALIGN), (dict(ldx=136), ALIGN),
     (dict(a=FAKE + 8), ALIGN), (dict(b=FAKE + 8), ALIGN), (dict(sc=FAKE + 2), ALIGN), (dict(order=FAKE + 2), ALIGN),
     (dict(off=FAKE + 2), ALIGN), (dict(res=FAKE + 2), ALIGN), (dict(ldr=130, y=2 * FAKE), ALIGN), (dict(y=FAKE + 2), ALIGN),
-    (dict(ws=FAKE + 16), ALIGN), (dict(T=1000, ws=None), WS), (dict(T=1000, wsb=100), WS), (dict(T=0), OK), (dict(n=0), OK),
+    (dict(ws=FAKE + 16), ALIGN), (dict(T=5000, ws=None), WS), (dict(T=5000, wsb=100), WS), (dict(T=0), OK), (dict(n=0), OK),
 ])
 def test_lora_checks(b2q_mod, kw, expect):
     assert lora(**kw) == expect
@@ -135,5 +135,5 @@ def test_workspace_sizes(b2q_mod):
     assert L.b2q_moe_route_workspace_bytes(10000, 64, 65) == 0        # invalid sizes
     assert L.b2q_group_rows_workspace_bytes(100, 64) == 0 < L.b2q_group_rows_workspace_bytes(100000, 64)
     assert L.b2q_group_rows_workspace_bytes(100000, 0) == 0
-    assert L.b2q_lora_add_workspace_bytes(8, 64, 8, 16) == 0 < L.b2q_lora_add_workspace_bytes(1000, 64, 8, 16)
-    assert L.b2q_lora_add_workspace_bytes(1000, 64, 8, 12) == 0
+    assert L.b2q_lora_add_workspace_bytes(8, 64, 8, 16) == 0 < L.b2q_lora_add_workspace_bytes(5000, 64, 8, 16)
+    assert L.b2q_lora_add_workspace_bytes(5000, 64, 8, 12) == 0

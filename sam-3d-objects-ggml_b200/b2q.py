@@ -1051,7 +1051,7 @@ def mul_mat_id(wtype: int, w, n: int, k: int, x, order, offsets, per_row: int = 
     else:
         assert _type16(dt) == wtype and w.dtype is dt and w.shape == (E, rows, k)
         lde, ldw, ldwc = w.stride()
-        assert ldwc == 1 and ldw >= k
+        assert ldwc == 1 and ldw >= k and (lde > 0 or E <= 1)
     if bias is not None:
         assert _are_floats(bias, E * rows, torch.float32)
     if out is None:

@@ -1487,7 +1487,7 @@ int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t
   if (x_rows < (slots + per_row - 1) / per_row) return B2Q_ERR_INVALID_ARG;
   const bool any = slots > 0 && n > 0;
   if (any && (!w || !x || !order || !offsets || !y)) return B2Q_ERR_INVALID_ARG;
-  if ((!q4 && (w_row_stride_bytes < k * 2 || (experts > 1 && w_expert_stride_bytes < 0))) || x_row_stride_bytes < k * 2 ||
+  if ((!q4 && (w_row_stride_bytes < k * 2 || (experts > 1 && w_expert_stride_bytes <= 0))) || x_row_stride_bytes < k * 2 ||
       y_row_stride_bytes < n * ysize)
     return B2Q_ERR_INVALID_ARG;
   if (!aligned(w, q4 ? 256 : 16) || (!q4 && (w_row_stride_bytes % 16 != 0 || w_expert_stride_bytes % 16 != 0)) ||

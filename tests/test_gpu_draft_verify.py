@@ -180,3 +180,13 @@ def test_in_a_graph(dev):
         graph.replay()
         ra, rt = reference(*args)
         assert accepted.tolist() == ra and tokens.tolist() == rt
+
+
+def test_rows_behind_the_last_request_are_empty(dev):
+    """A batch with room for more drafts than it has: the tokens behind its last request are -1, its others as ever."""
+    args = make(dev, [3, 1, 2, 4], 200, "f32", seed=5)
+    args[3] = torch.tensor([0, 3, 4, 6], dtype=torch.int32, device=dev)  # three requests of 6 drafts; 10 are there
+    args[0], args[5] = args[0][:13], args[5][:3]
+    accepted, tokens = b2q.draft_verify(*args)
+    ra, rt = reference(args[0], args[1], args[2], args[3], args[4], args[5])
+    assert accepted.tolist() == ra and tokens.tolist() == rt + [-1] * 4

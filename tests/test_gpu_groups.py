@@ -281,6 +281,32 @@ def test_mul_mat_id_strides(dev):
     assert bool((out[:, 72:] == 7.0).all())
 
 
+@pytest.mark.parametrize("layout", ["padded", "rows first", "one expert"])
+def test_mul_mat_id_glu_strides(dev, layout):
+    """Gate and up rows of experts that lie an odd number of rows apart, of row-major stacks, and of one expert."""
+    E = 1 if layout == "one expert" else 5
+    c = make_experts(dev, 90, E, 1, 36, 64, "bf16", glu=True, seed=4)
+    ref, tol = experts_reference(c)
+    if layout == "rows first":
+        wide = torch.full((72, E, 64), math.nan, dtype=torch.bfloat16, device=dev)
+        wide.copy_(c["w"].transpose(0, 1))
+        c["w"] = wide.transpose(0, 1)
+    else:
+        wide = torch.full((E, 75, 72), math.nan, dtype=torch.bfloat16, device=dev)
+        wide[:, :72, :64] = c["w"]
+        c["w"] = wide[:, :72, :64]
+    check_rows(call_experts(c), ref, tol)
+
+
+@pytest.mark.parametrize("k,T", [(4096, 3), (4096, 150), (6144, 5), (4480, 40)])
+def test_mul_mat_id_q4_long_rows(dev, k, T):
+    """Rows that fill the few-row kernel's shared memory (8 slots at a time), and rows that do not fit it."""
+    for glu in (False, True):
+        c = make_experts(dev, T, 4, 2, 40, k, "q4_0", glu, seed=k)
+        ref, tol = experts_reference(c)
+        check_rows(call_experts(c), ref, tol)
+
+
 def test_mul_mat_id_inputs_of_other_rows_do_not_reach_a_row(dev):
     """A row of NaN and one of infinities among the rows of one expert, and an expert of NaN."""
     c = make_experts(dev, 200, 3, 1, 64, 128, "bf16", seed=5, ids=torch.zeros(200, 1, dtype=torch.int32, device=dev))

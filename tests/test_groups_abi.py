@@ -55,7 +55,7 @@ def mmid(**kw):
 
 @pytest.mark.parametrize("kw,expect", [
     (dict(E=0), ARG), (dict(n=-1), ARG), (dict(k=0), ARG), (dict(k=60), ARG), (dict(wt=2, k=48, ldx=128), ARG), (dict(xr=-1), ARG),
-    (dict(S=-1), ARG), (dict(pr=0), ARG), (dict(glu=2), ARG), (dict(xr=9), ARG), (dict(ldw=112), ARG), (dict(lde=-16), ARG),
+    (dict(S=-1), ARG), (dict(pr=0), ARG), (dict(glu=2), ARG), (dict(xr=9), ARG), (dict(ldw=112), ARG), (dict(lde=-16), ARG), (dict(lde=0), ARG),
     (dict(ldx=112), ARG), (dict(ldy=30), ARG), (dict(w=None), ARG), (dict(x=None), ARG), (dict(order=None), ARG),
     (dict(off=None), ARG), (dict(y=None), ARG), (dict(wt=8), UNSUP), (dict(wt=12), UNSUP), (dict(wt=0), UNSUP),
     (dict(yt=30), UNSUP), (dict(wt=30, yt=1), UNSUP), (dict(wt=2, yt=30), UNSUP), (dict(E=1025), TOO),

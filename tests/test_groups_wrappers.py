@@ -88,7 +88,7 @@ def test_group_rows_refuses(lib_calls, ids):
 @pytest.mark.parametrize("kw", [
     dict(x=z(6, 32, dt=F16)), dict(x=z(6, 64, dt=BF16)), dict(x=z(6, 64)), dict(x=z(64, 6, dt=F16).t()),
     dict(x=z(64, dt=F16).expand(6, 64)), dict(w=z(4, 16, 32, dt=F16)), dict(w=z(4, 32, 64, dt=F16)), dict(w=z(4, 16, 64)),
-    dict(w=z(3, 16, 64, dt=F16)), dict(w=z(4, 64, 16, dt=F16).transpose(1, 2)), dict(order=z(12, dt=I64)),
+    dict(w=z(3, 16, 64, dt=F16)), dict(w=z(16, 64, dt=F16).expand(4, 16, 64)), dict(w=z(4, 64, 16, dt=F16).transpose(1, 2)), dict(order=z(12, dt=I64)),
     dict(order=z(24, dt=I32)[::2]), dict(offsets=z(5, dt=I64)), dict(bias=z(63)), dict(bias=z(64, dt=F16)),
     dict(out=z(12, 8, dt=F16)), dict(out=z(11, 16, dt=F16)), dict(out=z(16, 12, dt=F16).t()), dict(out=z(12, 16), out_dtype=F16),
     dict(out_dtype=I32), dict(wtype=b2q.TYPE_BF16), dict(glu=True, w=z(4, 16, 64, dt=F16)),

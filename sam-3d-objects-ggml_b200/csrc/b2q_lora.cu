@@ -3,9 +3,9 @@
 // (rows of no adapter: y[t] = resid[t]).
 //
 // Bound by the rows' bytes (x and resid read, y written) or, for single tokens, by
-// latency.  h = A x enters the second product as two 16-bit numbers (the value and
-// what rounding it left) of a power of two per row, so neither fp16's range nor the
-// 8 bits of bf16 limit it.  Products are m16n8k16; K and the rank are taken in an
+// latency.  h = A x enters the second product as a sum of 16-bit numbers (two, or
+// three of bf16: the value, and what rounding it left) of a power of two per row, so
+// neither fp16's range nor the 8 bits of bf16 limit it.  Products are m16n8k16; K and the rank are taken in an
 // order that suits the loads: lane q of a quad has 8 consecutive values of every 32
 // (4 of 16 where the rank is at most 16).
 //
@@ -36,12 +36,17 @@ constexpr int kStageK = 64;
 template <int RP>
 constexpr int kPitch = RP * 2 + (RP >= 64 ? 64 : 0);
 
-template <int RP>
+// Numbers that make up one of h: 22 bits of fp16, 24 of bf16; 16 of bf16 where y has 8.  (4096 x 6144, rank 64, bf16,
+// fp32 y: 112 us and an error of 4e-7 with three, 101 us and 1e-6 with two.)
+template <int X, int Y>
+constexpr int kTerms = X == 2 && Y == 0 ? 3 : 2;
+
+template <int X, int Y, int RP>
 struct ClusterShape {
   static constexpr int M = 16;
   static constexpr int OFF_SUM = kWarps * 16 * RP * 4;  // behind the warps' parts: this CTA's h
   static constexpr int OFF_H = OFF_SUM + M * RP * 4;
-  static constexpr int OFF_EXP = OFF_H + 2 * M * kPitch<RP>;
+  static constexpr int OFF_EXP = OFF_H + kTerms<X, Y> * M * kPitch<RP>;
   static constexpr int OFF_ROW = OFF_EXP + M * 4;
   static constexpr int SMEM = OFF_ROW + M * 4;
 };
@@ -54,13 +59,14 @@ struct ShrinkShape {
   static constexpr int OFF_ROW = kStages * STAGE > PART ? kStages * STAGE : PART;
   static constexpr int SMEM = OFF_ROW + kTile * 4;
 };
-template <int RP, int YS>
+template <int X, int Y, int RP>
 struct ExpandShape {
+  static constexpr int YS = Y == 0 ? 4 : 2;
   static constexpr int COLS = 64, STAGES = 3;  // of one stage of y's and B's columns
   static constexpr int YROW = COLS * YS, BROW = RP * 2;
   static constexpr int STAGE = kTile * YROW + COLS * BROW;
   static constexpr int OFF_H = STAGES * STAGE;
-  static constexpr int OFF_EXP = OFF_H + 2 * kTile * kPitch<RP>;
+  static constexpr int OFF_EXP = OFF_H + kTerms<X, Y> * kTile * kPitch<RP>;
   static constexpr int OFF_ROW = OFF_EXP + kTile * 4;
   static constexpr int SMEM = OFF_ROW + kTile * 4;
 };
@@ -107,11 +113,11 @@ __device__ __forceinline__ void tile_rows(const LoraArgs& p, const GroupTile& t,
   }
 }
 
-// A row's PER rank values in a lane -> 16-bit numbers and what rounding them left, at most 1 in magnitude, and the
-// power of two that they were divided by.  (fmaxf passes over NaN; a row with an infinity keeps its values.)
-// WIDTH neighbouring lanes have the row.
-template <int X, int PER, int WIDTH>
-__device__ __forceinline__ float split_row(const float (&v)[PER], uint32_t (&hi)[PER / 2], uint32_t (&lo)[PER / 2]) {
+// A row's PER rank values in a lane -> the 16-bit numbers that they are sums of, at most 1 in magnitude, pairs in a
+// word; returns the power of two that they were divided by.  (fmaxf passes over NaN; a row with an infinity keeps its
+// values.)  WIDTH neighbouring lanes have the row.
+template <int X, int Y, int PER, int WIDTH>
+__device__ __forceinline__ float split_row(const float (&v)[PER], uint32_t (&terms)[kTerms<X, Y>][PER / 2]) {
   float top = 0.0f;
 #pragma unroll
   for (int e = 0; e < PER; ++e) top = fmaxf(top, fabsf(v[e]));
@@ -123,22 +129,24 @@ __device__ __forceinline__ float split_row(const float (&v)[PER], uint32_t (&hi)
   const float down = __int_as_float((127 - e2) << 23);
 #pragma unroll
   for (int e = 0; e < PER; e += 2) {
-    uint16_t h[2], l[2];
+    float w[2] = {v[e] * down, v[e + 1] * down};
+    const bool finite[2] = {fabsf(w[0]) < INFINITY, fabsf(w[1]) < INFINITY};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float w = v[e + i] * down;
-      h[i] = bits16<X>(w);
-      const float rest = w - from16<X>(h[i]);
-      l[i] = bits16<X>(fabsf(w) < INFINITY ? rest : 0.0f);
+    for (int s = 0; s < kTerms<X, Y>; ++s) {
+      uint16_t h[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        h[i] = bits16<X>(w[i]);
+        w[i] = finite[i] ? w[i] - from16<X>(h[i]) : 0.0f;  // exact
+      }
+      terms[s][e / 2] = h[0] | (static_cast<uint32_t>(h[1]) << 16);
     }
-    hi[e / 2] = h[0] | (static_cast<uint32_t>(h[1]) << 16);
-    lo[e / 2] = l[0] | (static_cast<uint32_t>(l[1]) << 16);
   }
   return __int_as_float((127 + e2) << 23);
 }
 
 // Columns [n0, n1) of y for 16 rows of a tile, 32 columns at a time from n0 + split * 32 on, every `step`-th of them.
-// h: the lane's row of the 16-bit numbers (what rounding left lies `rest` bytes on); up: the powers of two of
+// h: the lane's row of the 16-bit numbers (what rounding left lies `rest` bytes on, and so on); up: the powers of two of
 // rows g and g + 8.  32 columns are two groups of 16: lane q has columns 4 q .. 4 q + 3 of a group (2 q and 2 q + 1
 // of its two products), so y moves 4 values at a time.
 template <int X, int Y, int RP>
@@ -198,7 +206,7 @@ __device__ __forceinline__ void stream_columns(const LoraArgs& p, int group, boo
           }
         }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {  // the numbers, then what rounding them left
+        for (int s = 0; s < kTerms<X, Y>; ++s) {  // the numbers, then what rounding them left
           const uint8_t* hs = h + s * rest + k * 2;
           if constexpr (RP == 16) {
             const uint2 u = *reinterpret_cast<const uint2*>(hs), v = *reinterpret_cast<const uint2*>(hs + 8 * kPitch<RP>);
@@ -246,7 +254,7 @@ __device__ __forceinline__ void stream_columns(const LoraArgs& p, int group, boo
 
 template <int X, int Y, int RP>
 __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kernel(const LoraArgs p) {
-  using Sh = ClusterShape<RP>;
+  using Sh = ClusterShape<X, Y, RP>;
   constexpr int M = Sh::M, N8 = RP / 8;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* part = reinterpret_cast<float*>(smem);
@@ -330,17 +338,17 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
       }
 #pragma unroll
       for (int e = 0; e < PER; ++e) v[e] *= scale;
-      uint32_t hi[PER / 2], lo[PER / 2];
-      const float up = split_row<X, PER, 32>(v, hi, lo);
+      uint32_t terms[kTerms<X, Y>][PER / 2];
+      const float up = split_row<X, Y, PER, 32>(v, terms);
 #pragma unroll
       for (int s = 0; s < kRanks; ++s) {
         if (lane < LANES) {
           const uint32_t to = cluster_addr(smem + Sh::OFF_H + m * kPitch<RP> + lane * PER * 2, s);
 #pragma unroll
-          for (int e = 0; e < PER / 2; ++e) {
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + e * 4), "r"(hi[e]) : "memory");
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + M * kPitch<RP> + e * 4), "r"(lo[e]) : "memory");
-          }
+          for (int k = 0; k < kTerms<X, Y>; ++k)
+#pragma unroll
+            for (int e = 0; e < PER / 2; ++e)
+              asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + k * M * kPitch<RP> + e * 4), "r"(terms[k][e]) : "memory");
         }
         if (lane == 0)
           asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr(power + m, s)), "f"(up) : "memory");
@@ -457,7 +465,7 @@ template <int X, int Y, int RP>
 __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs p) {
   using YV = typename Val<Y>::type;
   constexpr int YS = static_cast<int>(sizeof(YV));
-  using Sh = ExpandShape<RP, YS>;
+  using Sh = ExpandShape<X, Y, RP>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* hs = smem + Sh::OFF_H;
   float* power = reinterpret_cast<float*>(smem + Sh::OFF_EXP);
@@ -544,11 +552,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= scale;
-      uint32_t hi[2], lo[2];
-      const float up = split_row<X, 4, LANES>(v, hi, lo);
+      uint32_t terms[kTerms<X, Y>][2];
+      const float up = split_row<X, Y, 4, LANES>(v, terms);
       uint2* to = reinterpret_cast<uint2*>(hs + m * kPitch<RP>) + c;
-      to[0] = make_uint2(hi[0], hi[1]);
-      to[kTile * kPitch<RP> / 8] = make_uint2(lo[0], lo[1]);
+#pragma unroll
+      for (int k = 0; k < kTerms<X, Y>; ++k) to[k * (kTile * kPitch<RP> / 8)] = make_uint2(terms[k][0], terms[k][1]);
       if (c == 0) power[m] = up;
     }
   }
@@ -585,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
         }
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {  // the numbers, then what rounding them left
+      for (int s = 0; s < kTerms<X, Y>; ++s) {  // the numbers, then what rounding them left
         if constexpr (RP == 16) {
           const uint2 u = *reinterpret_cast<const uint2*>(h + s * REST + q * 8);
           const uint2 v = *reinterpret_cast<const uint2*>(h + s * REST + 8 * kPitch<RP> + q * 8);
@@ -648,7 +656,7 @@ int splits_of(int64_t T, int64_t K, int groups) {
 template <int X, int Y, int RP>
 cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
   if (!two_launches(a.T, a.groups, a.rank)) {
-    using Sh = ClusterShape<RP>;
+    using Sh = ClusterShape<X, Y, RP>;
     constexpr auto k = lora_cluster_kernel<X, Y, RP>;
     if (cudaError_t e = allow_smem<k>(Sh::SMEM)) return e;
     const int64_t tiles = tiles_of(a, Sh::M);
@@ -657,7 +665,7 @@ cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
   }
   constexpr auto shrink = lora_shrink_kernel<X, RP>;
   constexpr auto expand = lora_expand_kernel<X, Y, RP>;
-  constexpr int expand_smem = ExpandShape<RP, Y == 0 ? 4 : 2>::SMEM;
+  constexpr int expand_smem = ExpandShape<X, Y, RP>::SMEM;
   if (cudaError_t e = allow_smem<shrink>(ShrinkShape<RP>::SMEM)) return e;
   if (cudaError_t e = allow_smem<expand>(expand_smem)) return e;
   const int64_t tiles = tiles_of(a, kTile);

@@ -17,6 +17,11 @@
 // More rows: two launches over tiles of 64 sorted rows.  The first makes h (cp.async
 // stages of x's and A's rows; K shared out where the tiles are few) in fp32 in the
 // workspace; the second, launched early, adds the parts up and streams y.
+//
+// Measured: 32 rows of 24 adapters, rank 16, 4096 -> 4096: 6.5 us, one chain of
+// latencies; 8.7k rows of 7 adapters, rank 64, 4096 -> 6144, bf16: 112 us, 4280 GB/s, of
+// which the second launch runs at 5300 (y's stages 32 columns wide instead of 64: 17 us
+// more; read into registers instead: 30 more).
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"

@@ -19,6 +19,10 @@
 // come from the lanes that hold the same expert.  The second launch is made
 // early (programmatic dependent launch).  Where one CTA can do it all, it does:
 // one launch.
+//
+// Measured: 12 tokens, 6 of 64 experts: 4.7 us, one CTA's chain; 20471 tokens, 8 of 160:
+// 23.4 us, 600 instructions a row in two thirds of the issue slots (a thread a row
+// with its choices in registers: 49 us for the first launch instead of 22).
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"
 

@@ -481,6 +481,43 @@ def test_lora_with_a_broken_plan_stays_inside(dev, T):
     torch.cuda.synchronize()
 
 
+# ----------------------------------------------------------------------------------------------------- far apart rows
+def test_rows_further_apart_than_32_bits_count(dev):
+    """Rows of x, y, resid and probabilities whose offsets pass 2^32 values: the results of the same rows close together."""
+    far = 1 << 27  # 40 rows: 5.4e9 values of 2 bytes, in two buffers
+    one, two = (torch.empty(39 * far + 256, dtype=torch.float16, device=dev) for _ in range(2))
+
+    def spread(buf, t):
+        v = buf.as_strided((t.shape[0], t.shape[1]), (far, 1))
+        v.copy_(t)
+        return v
+
+    c = make_experts(dev, 40, 4, 1, 96, 64, "f16", seed=1, ids=torch.arange(40, dtype=torch.int32, device=dev).view(40, 1) % 4)
+    want = call_experts(c)
+    y = two.as_strided((40, 96), (far, 1))
+    got = call_experts(dict(c, x=spread(one, c["x"])), out=y)
+    assert torch.equal(got, want)
+    q = make_experts(dev, 40, 4, 1, 96, 64, "q4_0", seed=1, ids=c["ids"])
+    want = call_experts(q)
+    assert torch.equal(call_experts(dict(q, x=spread(one, q["x"])), out=y), want)
+    share = torch.rand(20, 2, device=dev)
+    want = b2q.moe_combine(want, share)
+    assert torch.equal(b2q.moe_combine(y, share), want)
+    for G in (4, 1):
+        lo = make_lora(dev, 40, G, 16, 64, 80, "f16", "f16", seed=2)
+        want = call_lora(lo)
+        assert torch.equal(call_lora(dict(lo, x=spread(one, lo["x"]), resid=spread(two, lo["resid"])), out=two.as_strided((40, 80), (far, 1))), want)
+    p = torch.softmax(2 * torch.randn(30, 200, device=dev), -1).half()
+    cu = torch.arange(0, 21, 2, dtype=torch.int32, device=dev)
+    drafts = p[:20].argmax(1).int()
+    u, v = torch.rand(20, device=dev), torch.rand(10, device=dev)
+    a, b = b2q.draft_verify(p, p[:20].contiguous(), drafts, cu, u, v)
+    a2, b2 = b2q.draft_verify(spread(one, p), spread(two, p[:20]), drafts, cu, u, v)
+    assert torch.equal(a, a2) and torch.equal(b, b2)
+    logits = torch.randn(40, 50, device=dev).half()
+    assert torch.equal(b2q.moe_route(logits, 4)[0], b2q.moe_route(spread(one, logits), 4)[0])
+
+
 # ------------------------------------------------------------------------------------------- together, and in a graph
 def test_an_expert_layer_in_a_graph_on_its_own_stream(dev):
     """Router, both products and the join, captured once and replayed on new inputs; two graphs side by side."""

@@ -696,8 +696,9 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * the first that does not is replaced by a draw from max(target - draft_probs, 0)
  * of its row (from target where that is 0 everywhere), and when all stay, a draw
  * from the last row follows.  A draw takes the first token at which the running
- * sum passes v[b] times the sum (64-bit sums; rows need not add up to 1; NaN,
- * infinities and negative values count as 0; -1 when nothing is left).
+ * sum passes v[b] times the sum (64-bit sums; rows need not add up to 1; target
+ * values that are NaN, infinite or negative, or whose draft value is NaN, and
+ * negative draft values count as 0; -1 when nothing is left).
  * accepted int32 [B]: drafts that stay; tokens int32 [D + B], laid out as
  * target's rows: those drafts, the drawn token, -1 after it (and behind the last
  * request, where cu_drafts[B] < D).  Tokens outside 0 .. V - 1 are turned down. */

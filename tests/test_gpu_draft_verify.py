@@ -29,7 +29,7 @@ def reference(target, guess, drafts, cu, u, v):
                 if 0 <= d < V and float(u[i]) * q[d] < p[d]:
                     new.append(int(d))
                     continue
-                weight = np.where((p > q) & np.isfinite(p) & (p > 0), p - q, 0.0)
+                weight = np.where((p > q) & np.isfinite(p) & (p > 0), p - np.maximum(q, 0.0), 0.0)
             if weight.sum() == 0:
                 weight = clean(p)
             break
@@ -133,6 +133,7 @@ def test_rows_with_nothing_and_with_no_numbers(dev):
     args[0][6, ::2] = math.nan
     args[0][6, 1] = math.inf
     args[1][5, ::3] = math.nan
+    args[1][5, 1::3] = -0.5
     args[0][9] = -1.0
     check(args)
 

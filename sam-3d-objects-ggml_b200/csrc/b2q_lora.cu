@@ -286,25 +286,25 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
     const uint16_t* x = static_cast<const uint16_t*>(p.x);
     const uint16_t* a = static_cast<const uint16_t*>(p.a) + static_cast<int64_t>(t.group) * p.rank * p.K;
     float acc[N8][4] = {};
-          const uint16_t* xa = x + (row_a < 0 ? 0 : row_a) * p.ldx + q * 8;
-          const uint16_t* xb = x + (row_b < 0 ? 0 : row_b) * p.ldx + q * 8;
-    #pragma unroll 2
-          for (int64_t k = k0 + warp * 32; k < k1; k += kWarps * 32) {
-            const bool in = k + q * 8 < k1;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            const uint4 u = in && row_a >= 0 ? __ldg(reinterpret_cast<const uint4*>(xa + k)) : zero;
-            const uint4 v = in && row_b >= 0 ? __ldg(reinterpret_cast<const uint4*>(xb + k)) : zero;
-            uint4 w[N8];
-    #pragma unroll
-            for (int j = 0; j < N8; ++j)
-              w[j] = in && j * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(a + (j * 8 + g) * p.K + k + q * 8)) : zero;
-            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-    #pragma unroll
-            for (int j = 0; j < N8; ++j) {
-              mma16<X>(acc[j], a0, w[j].x, w[j].y);
-              mma16<X>(acc[j], a1, w[j].z, w[j].w);
-            }
-          }
+    const uint16_t* xa = x + (row_a < 0 ? 0 : row_a) * p.ldx + q * 8;
+    const uint16_t* xb = x + (row_b < 0 ? 0 : row_b) * p.ldx + q * 8;
+#pragma unroll 2
+    for (int64_t k = k0 + warp * 32; k < k1; k += kWarps * 32) {
+      const bool in = k + q * 8 < k1;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      const uint4 u = in && row_a >= 0 ? __ldg(reinterpret_cast<const uint4*>(xa + k)) : zero;
+      const uint4 v = in && row_b >= 0 ? __ldg(reinterpret_cast<const uint4*>(xb + k)) : zero;
+      uint4 w[N8];
+#pragma unroll
+      for (int j = 0; j < N8; ++j)
+        w[j] = in && j * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(a + (j * 8 + g) * p.K + k + q * 8)) : zero;
+      const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+      for (int j = 0; j < N8; ++j) {
+        mma16<X>(acc[j], a0, w[j].x, w[j].y);
+        mma16<X>(acc[j], a1, w[j].z, w[j].w);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < N8; ++j) {
       float* d = part + (warp * 16 + g) * RP + j * 8 + 2 * q;

@@ -1057,7 +1057,7 @@ def mul_mat_id(wtype: int, w, n: int, k: int, x, order, offsets, per_row: int = 
     if out is None:
         out = _new_on(stream, x, (S, n), out_dtype or dt)
     else:
-        assert _are_rows(out, S, n, out_dtype or out.dtype)
+        assert _are_rows(out, S, n, out_dtype or out.dtype) and (out.stride(0) >= n or S <= 1)
     ytype, ysize = _val_type(out.dtype)
     rc = (_lib or _lib_obj()).b2q_mul_mat_id(
         wtype, w.data_ptr(), E, n, k, ldw * 2, lde * 2, x.data_ptr(), x_rows, 2 * (ldx if ldx > k else k),
@@ -1082,7 +1082,8 @@ def moe_combine(y, weights, ids=None, resid=None, out_dtype=None, out=None, stre
     else:
         assert _are_rows(out, T, n, out_dtype or out.dtype) and (out.stride(0) >= n or T <= 1)
     if resid is not None:
-        assert resid is out or (_are_rows(resid, T, n, out.dtype) and resid.shape == (T, n))
+        assert resid is out or (_are_rows(resid, T, n, out.dtype) and resid.shape == (T, n) and
+                                (resid.stride(0) >= n or T <= 1))
     (yt, ys), (ot, os_) = _val_type(y.dtype), _val_type(out.dtype)
     rc = (_lib or _lib_obj()).b2q_moe_combine(
         yt, y.data_ptr(), ys * max(y.stride(0), n), weights.data_ptr(), _ptr(ids), T, top, n, ot, _ptr(resid),

@@ -91,7 +91,7 @@ def test_group_rows_refuses(lib_calls, ids):
     dict(w=z(3, 16, 64, dt=F16)), dict(w=z(16, 64, dt=F16).expand(4, 16, 64)), dict(w=z(4, 64, 16, dt=F16).transpose(1, 2)), dict(order=z(12, dt=I64)),
     dict(order=z(24, dt=I32)[::2]), dict(offsets=z(5, dt=I64)), dict(bias=z(63)), dict(bias=z(64, dt=F16)),
     dict(out=z(12, 8, dt=F16)), dict(out=z(11, 16, dt=F16)), dict(out=z(16, 12, dt=F16).t()), dict(out=z(12, 16), out_dtype=F16),
-    dict(out_dtype=I32), dict(wtype=b2q.TYPE_BF16), dict(glu=True, w=z(4, 16, 64, dt=F16)),
+    dict(out=z(16, dt=F16).expand(12, 16)), dict(out_dtype=I32), dict(wtype=b2q.TYPE_BF16), dict(glu=True, w=z(4, 16, 64, dt=F16)),
     dict(wtype=b2q.TYPE_Q4_0, w=z(100, dt=torch.uint8)),
     dict(wtype=b2q.TYPE_Q4_0, w=z(4 * 16 * 64, dt=torch.uint8), x=z(6, 64, dt=BF16)),
 ])
@@ -112,6 +112,7 @@ def test_mul_mat_id_passes_strides(lib_calls):
     dict(weights=z(2, 4).t()), dict(ids=z(4, 3, dt=I32)), dict(ids=z(4, 2, dt=I64)), dict(resid=z(4, 15)), dict(resid=z(3, 16)),
     dict(resid=z(4, 16), out_dtype=F16), dict(out=z(4, 15, dt=F16)), dict(out=z(16, 4).t()),
     dict(resid=z(4, 16, dt=F16), out=z(4, 16)), dict(y=z(16, dt=F16).expand(8, 16)), dict(out=z(16).expand(4, 16)),
+    dict(resid=z(16).expand(4, 16)), dict(resid=z(16).expand(4, 16), out=z(4, 16)),
 ])
 def test_combine_refuses(lib_calls, kw):
     refused(lib_calls, join, **kw)

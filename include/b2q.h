@@ -648,7 +648,8 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  *   offsets int32 [G + 1]  group g owns the sorted slots offsets[g] .. offsets[g + 1] - 1
  *   order   int32 [S]      the slots by group, in slot order inside one; those of no group last
  * Plans that the calls below did not make are clamped to their buffers, never
- * trusted.  All results are the same from call to call: no atomics on floats.
+ * trusted.  Rows of a result may lie beside the rows of an operand in one table,
+ * but not on them (refused), except for a resid that is the result.  All results are the same from call to call: no atomics on floats.
  *
  * b2q_moe_route: logits [T][E] of type F32, F16 or BF16.  Each token's choices
  * are its `top` largest of logit + bias (bias fp32 [E] or NULL; the sum in

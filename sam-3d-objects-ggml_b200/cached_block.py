@@ -87,7 +87,6 @@ class PagedCache:
         self.taken -= pages
         self.lengths[request] = 0
 
-
     def keep(self, request: int, length: int, stream=None) -> None:
         """Takes a request back to its first `length` tokens (drafts that were turned down): the pages behind them
         are free again."""

@@ -1397,6 +1397,20 @@ static int val_size(int vt) { return vt == kXF32 ? 4 : 2; }
 // The slots of a plan are numbered with 32 bits.
 constexpr int64_t kMaxSlots = 1 << 30;
 
+// Whether rows of two buffers touch.  Buffers that share a stretch of memory may
+// still be columns of one table, which rows at the same stride show.
+static bool rows_touch(const void* p, int64_t p_rows, int64_t p_stride, int64_t p_width, const void* q, int64_t q_rows,
+                       int64_t q_stride, int64_t q_width) {
+  if (p_rows == 0 || q_rows == 0) return false;
+  const __int128 p0 = reinterpret_cast<uintptr_t>(p), q0 = reinterpret_cast<uintptr_t>(q);
+  if (p0 + static_cast<__int128>(p_rows - 1) * p_stride + p_width <= q0 ||
+      q0 + static_cast<__int128>(q_rows - 1) * q_stride + q_width <= p0)
+    return false;
+  if (p_stride != q_stride) return true;
+  const int64_t shift = static_cast<int64_t>(((q0 - p0) % p_stride + p_stride) % p_stride);
+  return shift < p_width || shift + q_width > p_stride;
+}
+
 static int route_sizes(int64_t T, int64_t E, int64_t top) {
   if (T < 0 || E <= 0 || top <= 0 || top > E) return B2Q_ERR_INVALID_ARG;
   if (E > kMaxGroups || top > kRouteMaxTop || T > kMaxSlots / top) return B2Q_ERR_TOO_LARGE;
@@ -1495,6 +1509,7 @@ int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t
       !aligned(bias, 4) || !aligned(y, ysize) || y_row_stride_bytes % ysize != 0)
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
+  if (rows_touch(x, x_rows, x_row_stride_bytes, k * 2, y, slots, y_row_stride_bytes, n * ysize)) return B2Q_ERR_INVALID_ARG;
   int sms = 0;
   if (int rc = check_device(&sms)) return rc;
   MulMatIdArgs a{};
@@ -1545,6 +1560,9 @@ int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const 
       (resid && (!aligned(resid, os) || resid_row_stride_bytes % os != 0)))
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
+  if (rows_touch(y, T * top, y_row_stride_bytes, n * ys, out, T, out_row_stride_bytes, n * os) ||
+      (resid && resid != out && rows_touch(resid, T, resid_row_stride_bytes, n * os, out, T, out_row_stride_bytes, n * os)))
+    return B2Q_ERR_INVALID_ARG;
   if (int rc = check_device(nullptr)) return rc;
   CombineArgs a{};
   a.y = y;
@@ -1594,6 +1612,9 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
   if (!any) return B2Q_OK;
   const size_t need = lora_workspace(T, k, static_cast<int>(adapters), static_cast<int>(rank));
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
+  if (rows_touch(x, T, x_row_stride_bytes, k * 2, y, T, y_row_stride_bytes, n * ys) ||
+      (resid != y && rows_touch(resid, T, resid_row_stride_bytes, n * ys, y, T, y_row_stride_bytes, n * ys)))
+    return B2Q_ERR_INVALID_ARG;
   int sms = 0;
   if (int rc = check_device(&sms)) return rc;
   LoraArgs p{};

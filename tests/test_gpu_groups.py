@@ -281,6 +281,30 @@ def test_mul_mat_id_strides(dev):
     assert bool((out[:, 72:] == 7.0).all())
 
 
+@pytest.mark.parametrize("wname", ["f16", "q4_0"])
+@pytest.mark.parametrize("T", [3, 700])
+def test_results_beside_their_operands(dev, wname, T):
+    """Columns of one table are disjoint although their memory is not."""
+    c = make_experts(dev, T, 4, 1, 64, 64, wname, seed=5)
+    ref, tol = experts_reference(c)
+    table = torch.full((T, 144), 7.0, dtype=torch.float16, device=dev)
+    table[:, :64] = c["x"]
+    call_experts(dict(c, x=table[:, :64]), out=table[:, 72:136])
+    check_rows(table[:, 72:136], ref, tol)
+    assert torch.equal(table[:, :64], c["x"]) and bool((table[:, 64:72] == 7.0).all()) and bool((table[:, 136:] == 7.0).all())
+    with pytest.raises(RuntimeError):
+        call_experts(dict(c, x=table[:, :64]), out=table[:, 56:120])
+    c = make_lora(dev, T, 4, 16, 64, 64, "f16", "f16", seed=5)
+    ref, tol = lora_reference(c)
+    table[:, :64], table[:, 72:136] = c["x"], c["resid"]
+    y = table[:, 72:136]
+    call_lora(dict(c, x=table[:, :64], resid=y), out=y)
+    check_rows(y, ref, tol)
+    assert torch.equal(table[:, :64], c["x"]) and bool((table[:, 64:72] == 7.0).all()) and bool((table[:, 136:] == 7.0).all())
+    with pytest.raises(RuntimeError):
+        call_lora(dict(c, x=table[:, :64]), out=table[:, 56:120])
+
+
 @pytest.mark.parametrize("layout", ["padded", "rows first", "one expert"])
 def test_mul_mat_id_glu_strides(dev, layout):
     """Gate and up rows of experts that lie an odd number of rows apart, of row-major stacks, and of one expert."""

@@ -109,6 +109,23 @@ def test_lora_checks(b2q_mod, kw, expect):
     assert lora(**kw) == expect
 
 
+@pytest.mark.parametrize("call", [
+    lambda: mmid(),                                                       # x itself
+    lambda: mmid(y=FAKE - 32 * 19),                                       # its last row on x's first
+    lambda: mmid(y=FAKE + 128 * 9 + 126),                                 # its first row on x's last value
+    lambda: mmid(y=FAKE + 100, ldy=128),                                  # columns of one table that share some
+    lambda: join(o=FAKE + 32, ldo=64),
+    lambda: join(o=FAKE, ldo=64),
+    lambda: join(r=2 * FAKE + 64),                                        # a row further
+    lambda: join(r=2 * FAKE + 32, ldr=96, ldo=96),
+    lambda: lora(xt=1, yt=1, ldy=64, ldr=64),                             # x is y
+    lambda: lora(y=2 * FAKE, res=2 * FAKE + 128),
+    lambda: lora(y=2 * FAKE, res=2 * FAKE - 64, ldy=160, ldr=160),
+])
+def test_results_on_operands_are_refused(b2q_mod, call):
+    assert call() == ARG
+
+
 def verify(**kw):
     a = dict(ty=0, t=FAKE, ldt=400, g=FAKE, ldg=400, d=FAKE, cu=FAKE, B=3, D=6, V=100, u=FAKE, v=FAKE, acc=FAKE, tok=FAKE)
     a.update(kw)

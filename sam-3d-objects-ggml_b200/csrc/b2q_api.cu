@@ -1587,7 +1587,7 @@ static int lora_sizes(int64_t T, int64_t k, int64_t adapters, int64_t rank) {
 
 size_t b2q_lora_add_workspace_bytes(int64_t T, int64_t k, int64_t adapters, int64_t rank) {
   return lora_sizes(T, k, adapters, rank) == B2Q_OK
-             ? lora_workspace(T, k, static_cast<int>(adapters), static_cast<int>(rank)) : 0;
+             ? lora_workspace(T, static_cast<int>(adapters), static_cast<int>(rank)) : 0;
 }
 
 int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
@@ -1610,7 +1610,7 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
       !aligned(y, ys) || y_row_stride_bytes % ys != 0 || !aligned(workspace, 256))
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
-  const size_t need = lora_workspace(T, k, static_cast<int>(adapters), static_cast<int>(rank));
+  const size_t need = lora_workspace(T, static_cast<int>(adapters), static_cast<int>(rank));
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
   if (rows_touch(x, T, x_row_stride_bytes, k * 2, y, T, y_row_stride_bytes, n * ys) ||
       (resid != y && rows_touch(resid, T, resid_row_stride_bytes, n * ys, y, T, y_row_stride_bytes, n * ys)))

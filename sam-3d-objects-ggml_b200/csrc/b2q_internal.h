@@ -457,10 +457,10 @@ struct LoraArgs {
   int64_t ldr;
   void* y;
   int64_t ldy;
-  float* part;         // workspace of the two-launch form: [splits][T][padded rank]
+  float* part;         // workspace of the two-launch form: [T][padded rank]
   int splits, slices;  // parts of K and of the columns
 };
-size_t lora_workspace(int64_t T, int64_t K, int groups, int rank);
+size_t lora_workspace(int64_t T, int groups, int rank);
 cudaError_t launch_lora(const LoraArgs& a, int xtype, int ytype, int num_sms, cudaStream_t s);
 
 constexpr int kVerifyRanks = 8;  // CTAs of one request

@@ -15,13 +15,14 @@
 //      rows, scales them, and hands them to all eight
 //   3  each CTA makes its eighth of the columns of y
 // More rows: two launches over tiles of 64 sorted rows.  The first makes h (cp.async
-// stages of x's and A's rows; K shared out where the tiles are few) in fp32 in the
-// workspace; the second, launched early, adds the parts up and streams y.
+// stages of x's and A's rows; where the tiles are few, a cluster shares out K and adds
+// the parts up) in fp32 in the workspace; the second, launched early, streams y.
 //
 // Measured: 32 rows of 24 adapters, rank 16, 4096 -> 4096: 6.5 us, one chain of
-// latencies; 8.7k rows of 7 adapters, rank 64, 4096 -> 6144, bf16: 112 us, 4280 GB/s, of
-// which the second launch runs at 5300 (y's stages 32 columns wide instead of 64: 17 us
-// more; read into registers instead: 30 more).
+// latencies; 8.7k rows of 7 adapters, rank 64, 4096 -> 6144, bf16: 105 us, 4550 GB/s
+// (y's stages 32 columns wide instead of 64: 17 us more; read into registers instead: 30
+// more; the parts of K added up by every CTA of the second launch instead: 3 to 5 more,
+// 27 of 186 at rank 128; tiles of 128 rows in the first: 10 more).
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"
 #include "b2q_ptx.cuh"
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
                            live ? power[g + 8] : 0.0f, row_a, row_b, n0, n1, warp, kWarps * 32);
 }
 
-// h of one tile of 64 sorted rows over one of p.splits parts of K: p.part [splits][T][RP], rows in sorted order.
+// h of one tile of 64 sorted rows, K shared out over a cluster of p.splits CTAs: p.part [T][RP], rows in sorted order.
 template <int X, int RP>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraArgs p) {
   using Sh = ShrinkShape<RP>;
@@ -450,14 +451,31 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraArgs p)
       *reinterpret_cast<float2*>(d) = make_float2(acc[j][0], acc[j][1]);
       *reinterpret_cast<float2*>(d + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
     }
-    __syncthreads();
-    float* out = p.part + (split * p.T + t.begin) * RP;
-    for (int i = threadIdx.x; i < (t.end - t.begin) * RP / 4; i += kThreads) {
-      float4 v = *reinterpret_cast<const float4*>(part + i * 4);
-      const float4 w = *reinterpret_cast<const float4*>(part + kTile * RP + i * 4);
-      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    // A cluster's CTAs have the parts of K of one tile: each adds up a share of it, parts in order.
+    if (p.splits > 1) cluster_sync();
+    else __syncthreads();
+    float* out = p.part + t.begin * static_cast<int64_t>(RP);
+    for (int i = split * kThreads + threadIdx.x; i < (t.end - t.begin) * RP / 4; i += p.splits * kThreads) {
+      float4 w[kMaxSplits][2];
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[s][h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (s < p.splits)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(w[s][h].x), "=f"(w[s][h].y), "=f"(w[s][h].z), "=f"(w[s][h].w)
+                         : "r"(cluster_addr(part + h * kTile * RP + i * 4, s))
+                         : "memory");
+        }
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v.x += w[s][h].x, v.y += w[s][h].y, v.z += w[s][h].z, v.w += w[s][h].w;
       *reinterpret_cast<float4*>(out + i * 4) = v;
     }
+    if (p.splits > 1) cluster_sync();  // (nobody leaves before all have read)
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
@@ -549,11 +567,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
       float v[4] = {};
       if (m < count) {
         const float4* from = reinterpret_cast<const float4*>(p.part + (t.begin + m) * static_cast<int64_t>(RP)) + c;
-        float4 w[kMaxSplits];
-#pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s) w[s] = s < p.splits ? from[s * p.T * (RP / 4)] : make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s) v[0] += w[s].x, v[1] += w[s].y, v[2] += w[s].z, v[3] += w[s].w;
+        const float4 w = *from;
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= scale;
@@ -644,18 +659,23 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
 
 int padded(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 int64_t tiles_of(const LoraArgs& a, int rows) { return a.T / rows + std::min<int64_t>(a.groups + 1, a.T); }
-// One launch while its tiles of 16 rows (about half a tile more per adapter than the rows fill) are not many times
-// what is resident at once.  Measured, one launch against two: 2048 x 6144, rank 64, 32 adapters of 16 rows 13.7 us
-// against 27.0, of 32 rows 28.6 against 31.8, of 64 rows 53 against 36; 2048 x 2048, rank 128, 32 adapters of 16 rows
-// 18.7 against 34.5, of 32 rows 38.6 against 39.0, 4 adapters of 128 rows 25 against 17.
+// One launch while its tiles of 16 rows are few; many adapters cost it half a tile each and the two launches most of
+// a tile of 64.  Measured, one launch against two, 2048 x 2048 and 4096 x 6144 (us): rank 64, 512 rows of 16 adapters
+// 14/16 and 30/28, 768 of 16 17/16 and 32/30, 768 of 64 26/30 and 48/59, 1536 of 64 37/31 and 65/57; rank 16, 768 rows of
+// 16 10/11 and 20/19, 1024 of 16 15/13 and 29/25, 1024 of 64 17/17 and 32/37; rank 128, 256 rows of 16 20/20 and 40/44,
+// 512 of 16 30/22 and 59/46, 512 of 64 58/53 and 101/104.
 bool two_launches(int64_t T, int groups, int rank) {
-  return T / 16 + std::min<int64_t>(groups, T) / 2 > (rank <= 64 ? 96 : 48);
+  return T / 16 > (rank > 64 ? 20 : (rank > 16 ? 36 : 44) + std::min<int64_t>(groups, T) / 2);
 }
 
-// Parts of K of the first launch, and of the columns of the second: enough CTAs for the device where tiles are few.
-int splits_of(int64_t T, int64_t K, int groups) {
+// Parts of K of the first launch, the CTAs of a cluster: up to three CTAs an SM, or two of the 96 KB ones of rank 128,
+// where tiles are few.  Measured at rank 64, 4096 -> 4096, 8.7k rows of 32 adapters: with three 110 us, with two 119;
+// 4096 x 6144 of 7 adapters: with two or three 123, with four 130.  Rank 128, 2048 rows of 8 adapters, 2048 x 2048: with
+// two 36, with three 41.
+int splits_of(int64_t T, int64_t K, int groups, int rank) {
   const int64_t tiles = T / kTile + std::min<int64_t>(groups, T);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 296 / tiles, K / 256})));
+  const int64_t most = std::min<int64_t>({kMaxSplits, (rank <= 64 ? 444 : 296) / tiles, K / 256});
+  return most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
 }
 
 template <int X, int Y, int RP>
@@ -674,11 +694,13 @@ cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
   if (cudaError_t e = allow_smem<shrink>(ShrinkShape<RP>::SMEM)) return e;
   if (cudaError_t e = allow_smem<expand>(expand_smem)) return e;
   const int64_t tiles = tiles_of(a, kTile);
-  a.splits = splits_of(a.T, a.K, a.groups);
-  a.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((6 * num_sms + tiles - 1) / tiles, (a.N + 127) / 128)));
+  a.splits = splits_of(a.T, a.K, a.groups, a.rank);
+  // (and the parts of the columns of the second, of at least 256: 128 cost 31 -> 34 us at 4096 rows of 16 adapters, rank
+  // 64, 2048 x 2048.  5 CTAs an SM against 6: 105 us against 109 for the 8.7k rows above, 77 against 73 for rank 16.)
+  a.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((5 * num_sms + tiles - 1) / tiles, (a.N + 255) / 256)));
   if (tiles > INT32_MAX / std::max(a.splits, a.slices)) return cudaErrorInvalidValue;
   if (cudaError_t e = launch_early(shrink, dim3(static_cast<unsigned>(tiles * a.splits)), dim3(kThreads), ShrinkShape<RP>::SMEM,
-                                   s, 1, a))
+                                   s, a.splits, a))
     return e;
   return launch_early(expand, dim3(static_cast<unsigned>(tiles * a.slices)), dim3(kThreads), expand_smem, s, 1, a);
 }
@@ -695,9 +717,9 @@ cudaError_t launch_types(const LoraArgs& a, int num_sms, cudaStream_t s) {
 
 }  // namespace
 
-size_t lora_workspace(int64_t T, int64_t K, int groups, int rank) {
+size_t lora_workspace(int64_t T, int groups, int rank) {
   if (T <= 0 || !two_launches(T, groups, rank)) return 0;
-  return static_cast<size_t>(splits_of(T, K, groups)) * T * padded(rank) * 4;
+  return static_cast<size_t>(T) * padded(rank) * 4;
 }
 
 cudaError_t launch_lora(const LoraArgs& a, int xtype, int ytype, int num_sms, cudaStream_t s) {

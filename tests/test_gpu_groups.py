@@ -447,6 +447,17 @@ def test_lora(dev, dt, out, T, G, rank, k, n):
     assert call_lora(c2, out=mine) is mine and torch.equal(mine, y)
 
 
+@pytest.mark.parametrize("k", [264, 520, 1032, 2056])
+@pytest.mark.parametrize("T,G,rank,n", [(830, 2, 64, 130), (830, 5, 8, 64), (400, 3, 72, 256), (7000, 2, 40, 72)])
+def test_lora_parts_of_k(dev, k, T, G, rank, n):
+    """Two launches, K shared out over one to eight blocks, some of which may have nothing."""
+    c = make_lora(dev, T, G, rank, k, n, "f16", "f32", seed=6)
+    ref, tol = lora_reference(c)
+    y = call_lora(c)
+    check_rows(y, ref, tol)
+    assert torch.equal(y, call_lora(c))
+
+
 @pytest.mark.parametrize("T", [90, 1900])
 def test_lora_without_scales_and_with_strides(dev, T):
     c = make_lora(dev, T, 4, 16, 128, 100, "f16", "f32", seed=2)

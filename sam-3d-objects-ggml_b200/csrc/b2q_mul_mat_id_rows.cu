@@ -44,7 +44,24 @@ static_assert(kSlot % 128 == 0, "a chunk's places are found by changing bits of 
 
 // Bytes of a slot's row of x in shared memory: whole chunks, and 64 more, so that
 // the rows of a quad's neighbours lie in other banks.
-__host__ __device__ __forceinline__ int64_t x_pitch(int64_t K) { return (K + kChunkK - 1) / kChunkK * kChunkK * 2 + 64; }
+__host__ __device__ constexpr int64_t x_pitch(int64_t K) { return (K + kChunkK - 1) / kChunkK * kChunkK * 2 + 64; }
+
+// 8-slot tiles of x's rows that a launch has shared memory for; 0: rows of K do not fit.
+constexpr int launch_tiles(int64_t K) {
+  const int64_t fit = (kSmemMax - kFixed) / (8 * x_pitch(K));
+  return static_cast<int>(fit < kMaxNT ? fit : kMaxNT);
+}
+// 8-slot tiles that a run with slots for nt of them multiplies, and so reads: no more than there are rows for.
+constexpr int product_tiles(int nt) { return nt; }
+constexpr bool products_stay_inside() {
+  for (int64_t K = 32; launch_tiles(K) > 0; K += 32)
+    for (int nt = 1; nt <= launch_tiles(K); ++nt) {
+      const int64_t last_row = product_tiles(nt) * 8 - 1, values = (K + kChunkK - 1) / kChunkK * kChunkK;
+      if (last_row * x_pitch(K) + values * 2 > launch_tiles(K) * 8 * x_pitch(K)) return false;
+    }
+  return true;
+}
+static_assert(products_stay_inside(), "a product reads rows of x behind those that there is shared memory for");
 
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1,
                                       float c2, float c3) {
@@ -336,9 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1) id_rows_kernel(const MulMatIdArgs
     }
     __syncthreads();
     const int from = start + warp;
-    if (nt <= 1) tiles_of(std::integral_constant<int, 1>(), r, first, from, last);
-    else if (nt == 2) tiles_of(std::integral_constant<int, 2>(), r, first, from, last);
-    else tiles_of(std::integral_constant<int, 4>(), r, first, from, last);
+    if (nt <= 1) tiles_of(std::integral_constant<int, product_tiles(1)>(), r, first, from, last);
+    else if (nt == 2) tiles_of(std::integral_constant<int, product_tiles(2)>(), r, first, from, last);
+    else if (nt == 3) tiles_of(std::integral_constant<int, product_tiles(3)>(), r, first, from, last);
+    else tiles_of(std::integral_constant<int, product_tiles(kMaxNT)>(), r, first, from, last);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   // Slots of no group: rows of zeros.
@@ -355,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) id_rows_kernel(const MulMatIdArgs
 template <bool GLU, bool OUT32>
 cudaError_t launch_shape(const MulMatIdArgs& a, int num_sms, cudaStream_t s) {
   const int64_t pitch = x_pitch(a.K);
-  const int nt = static_cast<int>(std::min<int64_t>(kMaxNT, (kSmemMax - kFixed) / (8 * pitch)));
+  const int nt = launch_tiles(a.K);
   if (nt < 1) return cudaErrorInvalidValue;
   constexpr auto k = id_rows_kernel<GLU, OUT32>;
   if (cudaError_t e = allow_smem<k>(kSmemMax)) return e;
@@ -364,7 +382,7 @@ cudaError_t launch_shape(const MulMatIdArgs& a, int num_sms, cudaStream_t s) {
 
 }  // namespace
 
-bool id_rows_fits(int64_t K) { return 8 * x_pitch(K) <= kSmemMax - kFixed; }
+bool id_rows_fits(int64_t K) { return launch_tiles(K) > 0; }
 
 cudaError_t launch_id_rows(const MulMatIdArgs& a, int ytype, int num_sms, cudaStream_t s) {
   const bool out32 = ytype == kXF32;

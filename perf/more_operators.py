@@ -241,11 +241,12 @@ def _own_route(s):
 def _own_experts(s):
     b2q = _b2q()
     wtype = {"f16": b2q.TYPE_F16, "bf16": b2q.TYPE_BF16, "q4_0": b2q.TYPE_Q4_0}[s["weights"]]
+    # (rows that are joined stay fp32 until then: the joined ones are rounded, once)
     y = b2q.mul_mat_id(wtype, s["w"], s["n"], s["k"], s["x"], s["order"], s["offsets"], per_row=s["per_row"],
-                       glu=s["glu"], out_dtype=torch.float32 if s["out"] == "f32" else None)
+                       glu=s["glu"], out_dtype=None if s["out"] == "rows" else torch.float32)
     if s["out"] == "rows":
         return y
-    return b2q.moe_combine(y, s["share"], s["ids"], resid=s["resid"])
+    return b2q.moe_combine(y, s["share"], s["ids"], resid=s["resid"], out_dtype=torch.float32 if s["out"] == "f32" else s["dt"])
 
 
 def _own_adapters(s):

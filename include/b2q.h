@@ -654,7 +654,10 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * b2q_moe_route: logits [T][E] of type F32, F16 or BF16.  Each token's choices
  * are its `top` largest of logit + bias (bias fp32 [E] or NULL; the sum in
  * fp32), largest first, ties to the lower expert; -infinity and NaN are never
- * chosen.  ids int32 [T][top] (-1 where nothing was left to choose), weights
+ * chosen.  With B2Q_SCORE_BIAS added to the scoring and a bias, the choice is by
+ * score + bias instead (the fp32 sum of the fp32 softmax or sigmoid score and
+ * the bias): routers whose experts were balanced by a correction bias choose so,
+ * and the two choices differ.  The bias never enters the weights.  ids int32 [T][top] (-1 where nothing was left to choose), weights
  * fp32 [T][top]: softmax over the E logits (NaN left out) or sigmoid of the
  * chosen ones, divided by their sum if renorm (0 where that is 0), times scale;
  * 0 for id -1.  order [T * top] and offsets [E + 1] are the plan of the slots
@@ -703,7 +706,7 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * accepted int32 [B]: drafts that stay; tokens int32 [D + B], laid out as
  * target's rows: those drafts, the drawn token, -1 after it (and behind the last
  * request, where cu_drafts[B] < D).  Tokens outside 0 .. V - 1 are turned down. */
-enum b2q_scoring { B2Q_SCORE_SOFTMAX = 0, B2Q_SCORE_SIGMOID = 1 };
+enum b2q_scoring { B2Q_SCORE_SOFTMAX = 0, B2Q_SCORE_SIGMOID = 1, B2Q_SCORE_BIAS = 4 /* added to either */ };
 B2Q_API size_t b2q_moe_route_workspace_bytes(int64_t T, int64_t E, int64_t top);
 B2Q_API int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t row_stride_bytes,
                           const float* bias, int64_t top, int scoring, int renorm, float scale, int32_t* ids,

@@ -986,14 +986,17 @@ def _is_list(t, n: int, dtype) -> bool:
 _route_ws_bytes = functools.lru_cache(maxsize=256)(lambda T, E, top: lib().b2q_moe_route_workspace_bytes(T, E, top))
 _group_ws_bytes = functools.lru_cache(maxsize=256)(lambda S, groups: lib().b2q_group_rows_workspace_bytes(S, groups))
 SCORING = {"softmax": 0, "sigmoid": 1}
+BIAS_ON = {"logit": 0, "score": 4}
 
 
 def moe_route(logits, top: int, bias=None, scoring: str = "softmax", renorm: bool = True, scale: float = 1.0,
-              stream=None):
+              stream=None, bias_on: str = "logit"):
     """The router of an expert layer, logits [T, E] (fp32, fp16 or bf16) -> (ids int32 [T, top], weights fp32
     [T, top], order int32 [T * top], offsets int32 [E + 1]): every token's `top` largest of logit + bias (ties
     to the lower expert, -infinity and NaN never; -1 where none is left), their softmax or sigmoid weights,
-    and the plan of the slots token * top + choice by expert."""
+    and the plan of the slots token * top + choice by expert.  bias_on="score" chooses by score + bias, the
+    scores being the softmax or sigmoid: what a trained router's correction bias is for.  The weights never
+    have the bias in them."""
     torch = _torch()
     T, E = logits.shape
     ld, ldc = logits.stride()
@@ -1008,7 +1011,7 @@ def moe_route(logits, top: int, bias=None, scoring: str = "softmax", renorm: boo
     order, offsets = _new_on(stream, logits, T * top, i32), _new_on(stream, logits, E + 1, i32)
     ws = _new_on(stream, logits, need, torch.uint8) if need else None
     rc = (_lib or _lib_obj()).b2q_moe_route(
-        dtype, logits.data_ptr(), T, E, size * (ld if ld > E else E), _ptr(bias), top, SCORING[scoring],
+        dtype, logits.data_ptr(), T, E, size * (ld if ld > E else E), _ptr(bias), top, SCORING[scoring] + BIAS_ON[bias_on],
         1 if renorm else 0, scale, ids.data_ptr(), weights.data_ptr(), order.data_ptr(), offsets.data_ptr(),
         _ptr(ws), need, _raw_stream(stream, logits, bias))
     if rc:

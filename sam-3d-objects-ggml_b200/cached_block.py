@@ -105,13 +105,15 @@ class PagedCache:
 
 class Experts:
     """A mixture layer's weights: the router's rows fp32 [E, C]; every expert's gate and up rows (2 * hidden of C) and
-    rows of the way back (C of hidden) as GGUF Q4_0 rows, one expert under another."""
+    rows of the way back (C of hidden) as GGUF Q4_0 rows, one expert under another.  bias (fp32 [E]) is the router's
+    correction bias: it is added to the scores for the choice, and never enters the shares; bias_on="logit" adds it
+    to the logits instead."""
 
     def __init__(self, dev, router, w_in, w_out, C: int, hidden: int, top: int, scoring: str = "softmax", renorm: bool = True,
-                 scale: float = 1.0, bias=None):
+                 scale: float = 1.0, bias=None, bias_on: str = "score"):
         import torch
         self.router, self.C, self.hidden, self.top, self.bias = router, C, hidden, top, bias
-        self.how = {"scoring": scoring, "renorm": renorm, "scale": scale}
+        self.how = {"scoring": scoring, "renorm": renorm, "scale": scale, "bias_on": bias_on}
         self.w_in = b2q.weight_pack_q4_0(torch.from_numpy(w_in).to(dev), C)
         self.w_out = b2q.weight_pack_q4_0(torch.from_numpy(w_out).to(dev), hidden)
 

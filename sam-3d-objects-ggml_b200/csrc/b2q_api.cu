@@ -1431,7 +1431,8 @@ int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t ro
   if (vt < 0) return B2Q_ERR_UNSUPPORTED;
   if (int rc = route_sizes(T, E, top)) return rc;
   const int size = val_size(vt);
-  if ((scoring != B2Q_SCORE_SOFTMAX && scoring != B2Q_SCORE_SIGMOID) || (renorm != 0 && renorm != 1) ||
+  const int score = scoring & ~B2Q_SCORE_BIAS;
+  if ((score != B2Q_SCORE_SOFTMAX && score != B2Q_SCORE_SIGMOID) || (renorm != 0 && renorm != 1) ||
       !std::isfinite(scale) || !offsets || (T > 0 && (!logits || !ids || !weights || !order)) ||
       row_stride_bytes < E * size)
     return B2Q_ERR_INVALID_ARG;
@@ -1448,7 +1449,8 @@ int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t ro
   a.E = static_cast<int>(E);
   a.top = static_cast<int>(top);
   a.bias = bias;
-  a.scoring = scoring;
+  a.scoring = score;
+  a.on_score = bias && score != scoring;  // (without a bias both ways choose alike)
   a.renorm = renorm;
   a.scale = scale;
   a.ids = ids;

@@ -396,6 +396,7 @@ struct RouteArgs {
   int E, top;
   const float* bias;   // [E] or nullptr
   int scoring;         // 0 softmax, 1 sigmoid
+  int on_score;        // the bias is added to the scores, not to the logits
   int renorm;
   float scale;
   int32_t* ids;        // [T][top]

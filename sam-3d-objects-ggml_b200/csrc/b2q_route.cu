@@ -1,7 +1,8 @@
 // b2q_route.cu -- the router of an expert layer and the plan of rows that go by
 // group.
 //
-//   key_e = logit_e + bias_e; the `top` largest keys, ties to the lower expert
+//   key_e = logit_e + bias_e, or score_e + bias_e with the softmax or sigmoid scores; the `top` largest keys, ties to
+//   the lower expert
 //   w_j   = softmax or sigmoid of the chosen logits, times scale
 //   order   = the slots (token * top + choice) sorted by expert, stable
 //   offsets = where each expert's slots begin
@@ -168,8 +169,9 @@ __device__ void place_run(const int32_t* ids, int S, int groups, int run, int ru
 
 size_t place_smem(int groups) { return (static_cast<size_t>(kWarps + 2) * (groups + 1) + kWarps) * 4; }
 
-// NV: experts of a lane.
-template <int T, int NV>
+// NV: experts of a lane.  ON_SCORE: the bias is added to the scores.  (A kernel of its own: the scores of all experts
+// before the choice are work that the others do not have.)
+template <int T, int NV, bool ON_SCORE>
 __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
   extern __shared__ int smem[];
   using V = typename Val<T>::type;
@@ -192,11 +194,36 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
   if (t0 + warp < t1) fetch(t0 + warp);
   for (int64_t t = t0 + warp; t < t1; t += kWarps) {
     uint32_t key[NV];
+    if constexpr (ON_SCORE) {
+      float m = -INFINITY, z = 0.0f;  // of the softmax, as for the weights below
+      if (a.scoring == 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      x[i] = next[i];
-      const int e = lane + 32 * i;
-      key[i] = e < E ? key_bits(a.bias ? x[i] + __ldg(a.bias + e) : x[i]) : 0u;
+        for (int i = 0; i < NV; ++i) m = fmaxf(m, next[i]);  // (fmaxf passes over NaN)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (next[i] > -INFINITY) z += next[i] == m ? 1.0f : expf(next[i] - m);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        x[i] = next[i];
+        const int e = lane + 32 * i;
+        key[i] = 0u;
+        if (x[i] > -INFINITY) {  // (neither NaN nor an expert behind the last)
+          const float score = a.scoring == 1 ? 1.0f / (1.0f + expf(-x[i])) : (x[i] == m ? 1.0f : expf(x[i] - m)) / z;
+          key[i] = key_bits(score + __ldg(a.bias + e));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        x[i] = next[i];
+        const int e = lane + 32 * i;
+        key[i] = e < E ? key_bits(a.bias ? x[i] + __ldg(a.bias + e) : x[i]) : 0u;
+      }
     }
     if (t + kWarps < t1) fetch(t + kWarps);
     float picked = 0.0f;  // lane j: the logit of choice j
@@ -405,15 +432,19 @@ cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
       if (cudaError_t e = set_smem(reinterpret_cast<const void*>(k), smem)) return e;
       return launch_early(k, dim3(static_cast<unsigned>(p.runs)), dim3(kThreads), smem, s, 1, a);
     };
-    if (nv <= 1) return go(route_kernel<T, 1>);
-    if (nv <= 2) return go(route_kernel<T, 2>);
-    if (nv <= 3) return go(route_kernel<T, 3>);
-    if (nv <= 4) return go(route_kernel<T, 4>);
-    if (nv <= 5) return go(route_kernel<T, 5>);
-    if (nv <= 6) return go(route_kernel<T, 6>);
-    if (nv <= 8) return go(route_kernel<T, 8>);
-    if (nv <= 16) return go(route_kernel<T, 16>);
-    return go(route_kernel<T, 32>);
+    auto shape = [&](auto on) {
+      constexpr bool ON = decltype(on)::value;
+      if (nv <= 1) return go(route_kernel<T, 1, ON>);
+      if (nv <= 2) return go(route_kernel<T, 2, ON>);
+      if (nv <= 3) return go(route_kernel<T, 3, ON>);
+      if (nv <= 4) return go(route_kernel<T, 4, ON>);
+      if (nv <= 5) return go(route_kernel<T, 5, ON>);
+      if (nv <= 6) return go(route_kernel<T, 6, ON>);
+      if (nv <= 8) return go(route_kernel<T, 8, ON>);
+      if (nv <= 16) return go(route_kernel<T, 16, ON>);
+      return go(route_kernel<T, 32, ON>);
+    };
+    return a.on_score ? shape(std::true_type()) : shape(std::false_type());
   };
   const cudaError_t err = type == kXF32 ? run(std::integral_constant<int, 0>())
                           : type == kXF16 ? run(std::integral_constant<int, 1>()) : run(std::integral_constant<int, 2>());

@@ -1,11 +1,14 @@
 """Calls for rows that go by group at the borders between their kernels' forms, against plain 64-bit arithmetic
 (tolerances as in test_gpu_groups.py, and equality where every value is exact)."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 import b2q
-from test_gpu_groups import call_experts, check_rows, experts_reference, make_experts
+import cached_block as cb
+from test_gpu_groups import DT, call_experts, check_rows, experts_reference, make_experts, plan_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +34,106 @@ def test_mul_mat_id_q4_groups_of_every_number_of_tiles(dev, k, counts):
         ref, tol = experts_reference(c)
         for out in (None, torch.float32):
             check_rows(call_experts(c, out_dtype=out), ref, tol)
+
+
+# --------------------------------------------------------------------------------- a bias on the router's scores
+def scores_of(x, scoring):
+    """fp64 scores of numpy logits; NaN and -infinity have none (-infinity)."""
+    z = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    if scoring == "sigmoid":
+        s = 1 / (1 + np.exp(-z))
+    else:
+        m = np.maximum(z.max(1, keepdims=True), -1e300)
+        s = np.exp(z - m)
+        s /= np.maximum(s.sum(1, keepdims=True), 1e-300)
+    return np.where(z == -np.inf, -np.inf, s), s
+
+
+def check_scored(got, x, bias, top, scoring, renorm, scale):
+    """Each choice's score + bias against the 64-bit ones: no better one left out or behind a worse one, but for the
+    rounding of a score (exp of a number of at most 100, a division, a sum of E terms) and of the sum with the bias."""
+    ids, weights, order, offsets = (t.cpu().numpy() for t in got)
+    T, E = x.shape
+    open_, score = scores_of(x, scoring)
+    with np.errstate(invalid="ignore"):
+        key = open_ + bias.astype(np.float64)
+    key = np.where(np.isnan(key) | (open_ == -np.inf), -np.inf, key)
+    tol = (E + 120) * 2.0 ** -24
+    want = np.minimum((key > -np.inf).sum(1), top)
+    assert np.array_equal((ids >= 0).sum(1), want) and np.all(ids[np.arange(top) >= want[:, None]] == -1)
+    there = ids >= 0
+    mine = np.take_along_axis(key, np.maximum(ids, 0), 1)
+    best = -np.sort(-key, axis=1)[:, :top]
+    slack = 2 * tol * (1 + np.abs(np.where(there, best, 0)))  # of two keys, whose scores are at most 1
+    assert np.all(np.abs(np.where(there, mine, 0) - np.where(there, best, 0)) <= slack)
+    assert all(len(set(r[r >= 0])) == (r >= 0).sum() for r in ids)
+    w = np.where(there, np.take_along_axis(score, np.maximum(ids, 0), 1), 0.0)
+    if renorm:
+        w = w / np.where(w.sum(1, keepdims=True) > 0, w.sum(1, keepdims=True), 1)
+    assert np.all(np.abs(weights - w * scale) <= 2 * tol * np.abs(w * scale) + 1e-37)
+    ro, rf = plan_reference(ids, E)
+    assert np.array_equal(order, ro) and np.array_equal(offsets, rf)
+
+
+@pytest.mark.parametrize("T,E,top", [(1, 1, 1), (12, 64, 6), (33, 33, 4), (700, 160, 8), (4097, 31, 3), (513, 1024, 32), (90, 200, 8),
+                                     (9, 300, 32)])
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+def test_route_bias_on_scores(dev, T, E, top, ty):
+    g = torch.Generator(device=dev).manual_seed(T + E)
+    x = (2 * torch.randn(T, E, generator=g, device=dev)).to(DT[ty])
+    bias = 0.3 * torch.randn(E, generator=g, device=dev)
+    n = x.float().cpu().numpy()
+    for scoring in ("softmax", "sigmoid"):
+        for renorm in (True, False):
+            got = b2q.moe_route(x, top, bias=bias, scoring=scoring, renorm=renorm, scale=2.5, bias_on="score")
+            check_scored(got, n, bias.cpu().numpy(), top, scoring, renorm, 2.5)
+            plain = b2q.moe_route(x, top, scoring=scoring, renorm=renorm, scale=2.5)
+            none = b2q.moe_route(x, top, scoring=scoring, renorm=renorm, scale=2.5, bias_on="score")
+            assert all(torch.equal(p, q) for p, q in zip(plain, none))
+
+
+def test_route_bias_on_scores_is_another_choice(dev):
+    """A bias of 0.1 puts a sigmoid score of 0.95 in front of one of 0.99, whose logit it could not reach."""
+    x = torch.tensor([[math.log(99), math.log(19), 0.0]], device=dev)  # scores 0.99, 0.95, 0.5
+    bias = torch.tensor([0.0, 0.1, 0.0], device=dev)
+    assert b2q.moe_route(x, 1, bias=bias, scoring="sigmoid", bias_on="score")[0].tolist() == [[1]]
+    assert b2q.moe_route(x, 1, bias=bias, scoring="sigmoid")[0].tolist() == [[0]]
+
+
+@pytest.mark.parametrize("T", [5, 1500])
+def test_route_bias_on_scores_of_masked_experts(dev, T):
+    """-infinity and NaN are not chosen however large their bias; a bias of -infinity or NaN takes an expert out."""
+    E, top = 40, 6
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((T, E)).astype(np.float32)
+    x[0, ::3] = np.nan
+    x[1] = -np.inf
+    x[2] = np.nan
+    x[3] = -np.inf
+    x[3, [7, 30]] = [1.0, 2.0]
+    x[4, 5:] = -np.inf
+    bias = (0.2 * rng.standard_normal(E)).astype(np.float32)
+    bias[[0, 3, 6, 11]] = 5.0
+    bias[9], bias[14] = -np.inf, np.nan
+    for scoring in ("softmax", "sigmoid"):
+        for renorm in (True, False):
+            got = b2q.moe_route(torch.from_numpy(x).to(dev), top, bias=torch.from_numpy(bias).to(dev), scoring=scoring,
+                                renorm=renorm, bias_on="score")
+            check_scored(got, x, bias, top, scoring, renorm, 1.0)
+
+
+def test_experts_take_a_correction_bias_on_the_scores(dev):
+    experts, (router, _, _) = cb.random_experts(dev, 8, 64, 32, 2, scoring="sigmoid", bias=None)
+    g = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(50, 64, generator=g, device=dev)
+    h = b2q.norm_modulate(x)
+    logits = b2q.mul_mat_f32(experts.router, h)
+    bias = 0.4 * torch.randn(8, generator=g, device=dev)
+    ids, shares, _, _ = b2q.moe_route(logits, 2, bias=bias, scoring="sigmoid", bias_on="score")
+    assert not torch.equal(ids, b2q.moe_route(logits, 2, bias=bias, scoring="sigmoid")[0])
+    experts.bias = bias
+    got = experts.forward(h, x.clone())
+    order, offsets = b2q.group_rows(ids, 8)
+    z = b2q.mul_mat_id(b2q.TYPE_Q4_0, experts.w_in, 32, 64, h.half(), order, offsets, per_row=2, glu=True)
+    y = b2q.mul_mat_id(b2q.TYPE_Q4_0, experts.w_out, 64, 32, z, order, offsets, out_dtype=torch.float32)
+    assert torch.equal(got, b2q.moe_combine(y, shares, ids, resid=x))

@@ -24,7 +24,8 @@ With `Experts` the last line is a mixture layer instead:
     x = x + sum of shares * (z . W_down)               b2q_mul_mat_id, b2q_moe_combine
 
 and with `Adapters` each linear that has some adds its row's low-rank product
-(b2q_lora_add), the rows sorted by adapter once per step (b2q_group_rows).
+(b2q_lora_add), the rows sorted by adapter once per step (b2q_group_rows); beside
+experts those are qkv and out.
 
 `PagedCache` keeps the pools, the block tables and the free pages of a set of
 requests, and takes back the pages of those that end; the host knows the lengths
@@ -129,9 +130,11 @@ class Experts:
 
 class Adapters:
     """Low-rank adapters of a block's linears: {"qkv" | "out" | "fc1" | "fc2": (a [G, rank, in], b [G, out, rank])} in fp16,
-    and their scales fp32 [G] (or None)."""
+    and their scales fp32 [G] (or None).  A block with experts has no fc1 and fc2 and refuses adapters for them."""
 
     def __init__(self, pairs: dict, scales=None):
+        if not pairs or not set(pairs) <= {"qkv", "out", "fc1", "fc2"}:
+            raise ValueError("adapters belong to qkv, out, fc1 or fc2")
         self.pairs, self.scales = pairs, scales
         self.count = next(iter(pairs.values()))[0].shape[0]
 
@@ -192,12 +195,14 @@ class CachedBlock:
         whole pass belongs to it: its casts, and the pool that its temporaries come from and go back to.
         adapters: this layer's, with rows = adapters.plan(...) of the step."""
         import torch
+        if self.experts is not None and adapters is not None and ("fc1" in adapters.pairs or "fc2" in adapters.pairs):
+            raise ValueError("adapters for fc1 or fc2, whose place the experts have taken")
         with torch.cuda.stream(stream):
             return self._forward(x, cache, layer, step, positions, adapters, rows)
 
     def _forward(self, x, cache: PagedCache, layer: int, step: dict, positions, adapters, rows):
         v = self.vec
-        add = (lambda name, y, inp: adapters.add(name, y, inp, rows)) if adapters else (lambda name, y, inp: y)
+        add = (lambda name, y, inp: adapters.add(name, y, inp, rows)) if adapters is not None else (lambda name, y, inp: y)
         h = b2q.norm_modulate(x)
         qkv = add("qkv", self._linear("qkv", h, v["b_qkv"]), h)
         k, vv = cache.k[layer], cache.v[layer]

@@ -104,6 +104,17 @@ class PagedCache:
         self.lengths[request] = length
 
 
+def fp16_rows(x):
+    """(fp16 rows, powers of two fp32 [rows]) whose products are the rows of x, up to the rounding of fp16: a row whose
+    values pass fp16's range is divided by its power of two, for all others that is 1."""
+    import torch
+    top = x.abs().amax(1).float()
+    exponent = torch.frexp(top).exponent
+    above = torch.where(torch.isfinite(top), exponent - 15, 0).clamp(min=0).int()
+    power = ((above + 127) << 23).view(torch.float32)
+    return (x / power[:, None]).half(), power
+
+
 class Experts:
     """A mixture layer's weights: the router's rows fp32 [E, C]; every expert's gate and up rows (2 * hidden of C) and
     rows of the way back (C of hidden) as GGUF Q4_0 rows, one expert under another.  bias (fp32 [E]) is the router's
@@ -115,15 +126,36 @@ class Experts:
         import torch
         self.router, self.C, self.hidden, self.top, self.bias = router, C, hidden, top, bias
         self.how = {"scoring": scoring, "renorm": renorm, "scale": scale, "bias_on": bias_on}
-        self.w_in = b2q.weight_pack_q4_0(torch.from_numpy(w_in).to(dev), C)
+        raw = torch.from_numpy(w_in).to(dev)
+        self.hidden_fits_fp16 = self.hidden_bound(raw, C, hidden) <= 65504 * (1 - 2.0 ** -8)
+        self.w_in = b2q.weight_pack_q4_0(raw, C)
         self.w_out = b2q.weight_pack_q4_0(torch.from_numpy(w_out).to(dev), hidden)
 
+    @staticmethod
+    def hidden_bound(raw, C: int, hidden: int) -> float:
+        """What |silu(gate) * up| cannot pass for normed rows (no longer than sqrt(C)): C |gate row| |up row|, the largest."""
+        import torch
+        worst = 0.0
+        for rows in raw.view(-1, 2 * hidden, C // 32, 18):  # an expert at a time
+            d = rows[:, :, :2].contiguous().view(torch.float16)[:, :, 0].double()
+            codes = torch.cat([rows[:, :, 2:] & 15, rows[:, :, 2:] >> 4], -1).int() - 8
+            length = (d.square() * codes.square().sum(-1)).sum(-1).sqrt()
+            bound = float((C * length[:hidden] * length[hidden:]).max())
+            worst = max(worst, bound) if bound == bound else float("inf")
+        return worst
+
     def forward(self, h, x):
-        """x += the layer's output for the normed rows h (fp32 [tokens, C]), in place."""
+        """x += the layer's output for the normed rows h (fp32 [tokens, C], no longer than sqrt(C)), in place.  The rows of
+        both products are fp16; hidden values that the weights let pass its range (hidden_bound) are taken by a
+        power of two per row, which their shares give back."""
         import torch
         logits = b2q.mul_mat_f32(self.router, h)
         ids, shares, order, offsets = b2q.moe_route(logits, self.top, bias=self.bias, **self.how)
-        z = b2q.mul_mat_id(b2q.TYPE_Q4_0, self.w_in, self.hidden, self.C, h.half(), order, offsets, per_row=self.top, glu=True)
+        z = b2q.mul_mat_id(b2q.TYPE_Q4_0, self.w_in, self.hidden, self.C, h.half(), order, offsets, per_row=self.top, glu=True,
+                           out_dtype=None if self.hidden_fits_fp16 else torch.float32)
+        if not self.hidden_fits_fp16:
+            z, power = fp16_rows(z)
+            shares = shares * power.view_as(shares)
         y = b2q.mul_mat_id(b2q.TYPE_Q4_0, self.w_out, self.C, self.hidden, z, order, offsets, out_dtype=torch.float32)
         return b2q.moe_combine(y, shares, ids, resid=x, out=x)
 

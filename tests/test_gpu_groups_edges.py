@@ -8,6 +8,8 @@ import torch
 
 import b2q
 import cached_block as cb
+from test_gpu_expert_block import experts_reference as layer_reference
+from test_gpu_cached_block import layer_norm
 from test_gpu_groups import DT, call_experts, check_rows, experts_reference, make_experts, plan_reference
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +139,70 @@ def test_experts_take_a_correction_bias_on_the_scores(dev):
     z = b2q.mul_mat_id(b2q.TYPE_Q4_0, experts.w_in, 32, 64, h.half(), order, offsets, per_row=2, glu=True)
     y = b2q.mul_mat_id(b2q.TYPE_Q4_0, experts.w_out, 64, 32, z, order, offsets, out_dtype=torch.float32)
     assert torch.equal(got, b2q.moe_combine(y, shares, ids, resid=x))
+
+
+# ----------------------------------------------------------------------------- values beyond fp16's range in a block
+def scaled_q4_0(raw, by):
+    """GGUF Q4_0 rows times a power of two."""
+    rows, width = raw.shape
+    raw = raw.reshape(rows, width // 18, 18).copy()
+    raw[:, :, :2] = (raw[:, :, :2].copy().view(np.float16) * np.float16(by)).view(np.uint8)
+    return raw.reshape(rows, width)
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 90])
+@pytest.mark.parametrize("big", [False, True])
+def test_experts_hidden_values_beyond_fp16(dev, tokens, big):
+    """Rows in fp16 of a power of two (2^-11 for h and for the hidden values), everything else fp32 or exact."""
+    C, E, F, top = 256, 8, 160, 3
+    experts, (router, w_in, w_out) = cb.random_experts(dev, E, C, F, top, seed=tokens)
+    assert experts.hidden_fits_fp16
+    if big:
+        w_in = scaled_q4_0(w_in, 128.0)
+        experts = cb.Experts(dev, torch.from_numpy(router).to(dev), w_in, w_out, C, F, top)
+        assert not experts.hidden_fits_fp16
+    g = torch.Generator(device=dev).manual_seed(tokens)
+    x = torch.randn(tokens, C, generator=g, device=dev)
+    h = layer_norm(x.double())
+    ref, gap = layer_reference(h, (router, w_in, w_out), E, F, top)
+    assert float(gap) > 1e-5
+    if big:
+        gates = h @ dequantized(w_in, C, dev).view(E * 2 * F, C).t()
+        assert float((gates.view(tokens, E, 2, F)[:, :, 0].clamp(min=0) * gates.view(tokens, E, 2, F)[:, :, 1]).abs().max()) > 65504
+    y = experts.forward(b2q.norm_modulate(x), torch.zeros_like(x))
+    assert float((y.double() - ref).norm() / ref.norm()) <= 2.0 ** -9
+
+
+def dequantized(raw, k, dev):
+    blk = torch.from_numpy(raw).to(dev).view(raw.shape[0], k // 32, 18)
+    d = blk[:, :, :2].contiguous().view(torch.float16).double()
+    return (d * (torch.cat([blk[:, :, 2:] & 15, blk[:, :, 2:] >> 4], -1).double() - 8)).view(raw.shape[0], k)
+
+
+def test_experts_bound_of_the_hidden_values_holds(dev):
+    """A row along an expert's gate row, as long as a normed row can be."""
+    C, E, F = 128, 3, 64
+    _, (_, w_in, _) = cb.random_experts(dev, E, C, F, 1, seed=3)
+    w = dequantized(w_in, C, dev).view(E, 2, F, C)
+    bound = cb.Experts.hidden_bound(torch.from_numpy(w_in).to(dev), C, F)
+    lengths = w.square().sum(-1).sqrt()
+    assert abs(bound - C * float((lengths[:, 0] * lengths[:, 1]).max())) <= 1e-9 * bound
+    h = w / lengths[..., None] * C ** 0.5
+    gate, up = w[:, 0].flatten(0, 1), w[:, 1].flatten(0, 1)
+    for rows in (h[:, 0].flatten(0, 1), h[:, 1].flatten(0, 1)):
+        z = rows @ gate.t()
+        assert float((z * torch.sigmoid(z) * (rows @ up.t())).abs().max()) <= bound
+
+
+def test_fp16_rows(dev):
+    x = torch.tensor([[1.0, -3.0, 65504.0], [1e-3, 2.0, -3.0], [0.0, 0.0, 0.0], [3e38, 1.0, -1e30], [math.inf, 1.0, 2.0],
+                      [math.nan, 4.0, 5.0], [-70000.0, 3.0, 8.0]], device=dev)
+    h, power = cb.fp16_rows(x)
+    assert power.tolist() == [2.0, 1.0, 1.0, 2.0 ** 113, 1.0, 1.0, 4.0]
+    back = h.double() * power.double()[:, None]
+    fine = torch.isfinite(x)
+    smallest = 2.0 ** -25 * power.double()[:, None].expand_as(x)
+    assert bool(((back - x.double()).abs() <= 2.0 ** -11 * x.double().abs() + smallest)[fine].all())
+    assert back[4, 0] == math.inf and bool(torch.isnan(back[5, 0]))
+    assert cb.fp16_rows(x[:0])[0].shape == (0, 3)
+    assert torch.equal(cb.fp16_rows(x[1:2].bfloat16())[0], x[1:2].bfloat16().half())

@@ -689,6 +689,9 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * between the two products are kept to more than 16 bits.  Workspace (256-byte
  * aligned) of b2q_lora_add_workspace_bytes; 0 for few rows per adapter, which
  * take one launch.
+ * b2q_lora_add_rows: the same with a scale per row beside the adapter's
+ * (row_scales fp32 [T], or NULL for 1): x whose rows were divided by a power of
+ * two to fit 16 bits gets its products back whole.
  *
  * b2q_draft_verify: which drafted tokens a target model keeps, from given random
  * numbers.  Request b of B has the drafts cu_drafts[b] .. cu_drafts[b+1] - 1
@@ -728,6 +731,11 @@ B2Q_API int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t
                          const int32_t* order, const int32_t* offsets, int ytype, const void* resid,
                          int64_t resid_row_stride_bytes, void* y, int64_t y_row_stride_bytes, void* workspace,
                          size_t workspace_bytes, void* stream);
+B2Q_API int b2q_lora_add_rows(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
+                              const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales,
+                              const float* row_scales, const int32_t* order, const int32_t* offsets, int ytype,
+                              const void* resid, int64_t resid_row_stride_bytes, void* y, int64_t y_row_stride_bytes,
+                              void* workspace, size_t workspace_bytes, void* stream);
 B2Q_API int b2q_draft_verify(int type, const void* target, int64_t target_row_stride_bytes, const void* draft_probs,
                              int64_t draft_row_stride_bytes, const int32_t* drafts, const int32_t* cu_drafts,
                              int64_t B, int64_t D, int64_t V, const float* u, const float* v, int32_t* accepted,

@@ -129,6 +129,7 @@ def _lib_obj():
             "b2q_moe_combine": (I, [I, P, I64, P, P, I64, I64, I64, I, P, I64, P, I64, P]),
             "b2q_lora_add_workspace_bytes": (SZ, [I64, I64, I64, I64]),
             "b2q_lora_add": (I, [I, P, I64, I64, I64, P, P, I64, I64, I64, P, P, P, I, P, I64, P, I64, P, SZ, P]),
+            "b2q_lora_add_rows": (I, [I, P, I64, I64, I64, P, P, I64, I64, I64, P, P, P, P, I, P, I64, P, I64, P, SZ, P]),
             "b2q_draft_verify": (I, [I, P, I64, P, I64, P, P, I64, I64, I64, P, P, P, P, P]),
         }
         for name, (res, args) in sig.items():
@@ -1101,11 +1102,11 @@ LORA_MAX_RANK = 128
 _lora_ws_bytes = functools.lru_cache(maxsize=256)(lambda T, k, G, rank: lib().b2q_lora_add_workspace_bytes(T, k, G, rank))
 
 
-def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
+def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None, row_scales=None):
     """resid + scales[g] * (x . a[g]^T) . b[g]^T row by row, g the adapter that the plan (group_rows of the rows'
     adapters) gives the row; rows without one stay as they are.  resid [T, n] fp32 or of x's type, x [T, k]
     fp16 or bf16, a [G, rank, k] and b [G, n, rank] of x's type, scales fp32 [G] or None
-    (out=resid updates in place)."""
+    (out=resid updates in place).  row_scales fp32 [T]: a row's own scale beside its adapter's."""
     torch = _torch()
     T, k = x.shape
     G, rank, ka = a.shape
@@ -1118,6 +1119,7 @@ def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
     assert _is_list(order, T, torch.int32) and _is_list(offsets, G + 1, torch.int32)
     if scales is not None:
         assert _are_floats(scales, G, torch.float32)
+    assert _are_floats(row_scales, T, torch.float32)
     if out is None:
         out = _new_on(stream, x, (T, n), resid.dtype)
     else:
@@ -1126,11 +1128,11 @@ def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None):
     need, ws = _lora_ws_bytes(T, k, G, rank), None
     if need:
         ws = _new_on(stream, x, need, torch.uint8)
-    rc = (_lib or _lib_obj()).b2q_lora_add(
-        _type16(dt), x.data_ptr(), T, k, 2 * (ldx if ldx > k else k), a.data_ptr(), b.data_ptr(), G, rank, n,
-        _ptr(scales), order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * max(resid.stride(0), n),
-        out.data_ptr(), ys * max(out.stride(0), n), _ptr(ws), need,
-        _raw_stream(stream, x, a, b, scales, order, offsets, resid, out))
+    L = _lib or _lib_obj()
+    head = (_type16(dt), x.data_ptr(), T, k, 2 * (ldx if ldx > k else k), a.data_ptr(), b.data_ptr(), G, rank, n, _ptr(scales))
+    tail = (order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * max(resid.stride(0), n), out.data_ptr(),
+            ys * max(out.stride(0), n), _ptr(ws), need, _raw_stream(stream, x, a, b, scales, row_scales, order, offsets, resid, out))
+    rc = L.b2q_lora_add(*head, *tail) if row_scales is None else L.b2q_lora_add_rows(*head, row_scales.data_ptr(), *tail)
     if rc:
         _check("b2q_lora_add", rc)
     return out

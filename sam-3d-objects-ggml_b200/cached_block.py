@@ -175,10 +175,17 @@ class Adapters:
         return b2q.group_rows(ids, self.count, stream=stream)
 
     def add(self, name: str, y, x, rows):
-        """y (fp32) += the adapters' products of the rows x, in place."""
+        """y (fp32) += the adapters' products of the rows x, in place.  The rows are taken as fp16: normed ones (qkv, fc1)
+        and those of an fp16 cache (out) lie in its range, others are divided by a power of two that comes back."""
+        import torch
         if name in self.pairs:
             a, b = self.pairs[name]
-            b2q.lora_add(y, x.half(), a, b, self.scales, *rows, out=y)
+            power = None
+            if name in ("qkv", "fc1") or x.dtype is torch.float16:
+                x = x.half()
+            else:
+                x, power = fp16_rows(x)
+            b2q.lora_add(y, x, a, b, self.scales, *rows, out=y, row_scales=power)
         return y
 
 

@@ -1596,6 +1596,15 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
                  const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales, const int32_t* order,
                  const int32_t* offsets, int ytype, const void* resid, int64_t resid_row_stride_bytes, void* y,
                  int64_t y_row_stride_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  return b2q_lora_add_rows(xtype, x, T, k, x_row_stride_bytes, a, b, adapters, rank, n, scales, nullptr, order, offsets, ytype,
+                           resid, resid_row_stride_bytes, y, y_row_stride_bytes, workspace, workspace_bytes, stream);
+}
+
+int b2q_lora_add_rows(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_stride_bytes, const void* a,
+                      const void* b, int64_t adapters, int64_t rank, int64_t n, const float* scales,
+                      const float* row_scales, const int32_t* order, const int32_t* offsets, int ytype,
+                      const void* resid, int64_t resid_row_stride_bytes, void* y, int64_t y_row_stride_bytes,
+                      void* workspace, size_t workspace_bytes, void* stream) {
   if (xtype != B2Q_TYPE_F16 && xtype != B2Q_TYPE_BF16) return B2Q_ERR_UNSUPPORTED;
   if (ytype != B2Q_TYPE_F32 && ytype != xtype) return B2Q_ERR_UNSUPPORTED;
   const int ys = ytype == B2Q_TYPE_F32 ? 4 : 2;
@@ -1607,7 +1616,7 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
   if (x_row_stride_bytes < k * 2 || y_row_stride_bytes < n * ys || resid_row_stride_bytes < n * ys ||
       (resid == y && resid_row_stride_bytes != y_row_stride_bytes))
     return B2Q_ERR_INVALID_ARG;
-  if (!aligned(x, 16) || x_row_stride_bytes % 16 != 0 || !aligned(a, 16) || !aligned(b, 16) || !aligned(scales, 4) ||
+  if (!aligned(x, 16) || x_row_stride_bytes % 16 != 0 || !aligned(a, 16) || !aligned(b, 16) || !aligned(scales, 4) || !aligned(row_scales, 4) ||
       !aligned(order, 4) || !aligned(offsets, 4) || !aligned(resid, ys) || resid_row_stride_bytes % ys != 0 ||
       !aligned(y, ys) || y_row_stride_bytes % ys != 0 || !aligned(workspace, 256))
     return B2Q_ERR_MISALIGNED;
@@ -1630,6 +1639,7 @@ int b2q_lora_add(int xtype, const void* x, int64_t T, int64_t k, int64_t x_row_s
   p.groups = static_cast<int>(adapters);
   p.rank = static_cast<int>(rank);
   p.scales = scales;
+  p.row_scales = row_scales;
   p.order = order;
   p.offsets = offsets;
   p.resid = resid;

@@ -452,7 +452,8 @@ struct LoraArgs {
   int64_t T, K, N, ldx;
   const void *a, *b;  // [groups][rank][K], [groups][N][rank]
   int groups, rank;
-  const float* scales;  // [groups] or nullptr
+  const float* scales;      // [groups] or nullptr
+  const float* row_scales;  // [T] or nullptr
   const int32_t *order, *offsets;
   const void* resid;
   int64_t ldr;

@@ -1,6 +1,6 @@
 // b2q_lora.cu -- low-rank adapters of many requests beside a shared projection:
 //   y[t] = resid[t] + scale_g * B_g (A_g x[t]),  g = the adapter of row t
-// (rows of no adapter: y[t] = resid[t]).
+// (rows of no adapter: y[t] = resid[t]; a scale per row may come in beside the adapter's).
 //
 // Bound by the rows' bytes (x and resid read, y written) or, for single tokens, by
 // latency.  h = A x enters the second product as a sum of 16-bit numbers (two, or
@@ -117,6 +117,10 @@ __device__ __forceinline__ void tile_rows(const LoraArgs& p, const GroupTile& t,
     }
     row_of[i] = r;
   }
+}
+
+__device__ __forceinline__ float row_scale(const LoraArgs& p, int row) {
+  return p.row_scales && row >= 0 ? __ldg(p.row_scales + row) : 1.0f;
 }
 
 // A row's PER rank values in a lane -> the 16-bit numbers that they are sums of, at most 1 in magnitude, pairs in a
@@ -342,8 +346,9 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
           }
         }
       }
+      const float own = scale * row_scale(p, row_of[m]);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] *= scale;
+      for (int e = 0; e < PER; ++e) v[e] *= own;
       uint32_t terms[kTerms<X, Y>][PER / 2];
       const float up = split_row<X, Y, PER, 32>(v, terms);
 #pragma unroll
@@ -570,8 +575,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
         const float4 w = *from;
         v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
       }
+      const float own = scale * row_scale(p, row_of[m]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] *= scale;
+      for (int e = 0; e < 4; ++e) v[e] *= own;
       uint32_t terms[kTerms<X, Y>][2];
       const float up = split_row<X, Y, 4, LANES>(v, terms);
       uint2* to = reinterpret_cast<uint2*>(hs + m * kPitch<RP>) + c;

@@ -10,7 +10,8 @@ import b2q
 import cached_block as cb
 from test_gpu_expert_block import experts_reference as layer_reference
 from test_gpu_cached_block import layer_norm
-from test_gpu_groups import DT, call_experts, check_rows, experts_reference, make_experts, plan_reference
+from test_gpu_groups import (DT, call_experts, call_lora, check_rows, experts_reference, lora_reference, make_experts, make_lora,
+                             plan_reference)
 
 pytestmark = pytest.mark.gpu
 
@@ -206,3 +207,41 @@ def test_fp16_rows(dev):
     assert back[4, 0] == math.inf and bool(torch.isnan(back[5, 0]))
     assert cb.fp16_rows(x[:0])[0].shape == (0, 3)
     assert torch.equal(cb.fp16_rows(x[1:2].bfloat16())[0], x[1:2].bfloat16().half())
+
+
+@pytest.mark.parametrize("dt,out", [("f16", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("T,G,rank", [(5, 3, 8), (90, 4, 16), (700, 2, 64), (2500, 3, 24), (1500, 2, 128)])
+def test_lora_scales_of_rows(dev, dt, out, T, G, rank):
+    """Powers of two per row: what the rows give that were multiplied by them in 64 bits."""
+    c = make_lora(dev, T, G, rank, 136, 77, dt, out, seed=T)
+    g = torch.Generator(device=dev).manual_seed(1)
+    power = 2.0 ** torch.randint(-6, 7, (T,), generator=g, device=dev).float()
+    ref, tol = lora_reference(dict(c, x=c["x"].double() * power.double()[:, None]))
+    y = call_lora(c, row_scales=power)
+    check_rows(y, ref, tol)
+    none = c["ids"] < 0
+    assert torch.equal(y[none], c["resid"][none])
+    assert torch.equal(call_lora(c, row_scales=torch.ones(T, device=dev)), call_lora(c))
+
+
+@pytest.mark.parametrize("T", [3, 200])
+@pytest.mark.parametrize("name,dtype", [("fc2", torch.float32), ("out", torch.bfloat16)])
+def test_adapters_rows_beyond_fp16(dev, T, name, dtype):
+    """Rows in fp16 of a power of two: 2^-11 of each value, and what the smallest numbers of fp16 lose of the row's largest."""
+    G, rank, k, n = 3, 16, 256, 96
+    c = make_lora(dev, T, G, rank, k, n, "f16", "f32", seed=T)
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = (torch.randn(T, k, generator=g, device=dev) * 10.0 ** (6 - torch.arange(T, device=dev)[:, None] * 3 % 10)).to(dtype)
+    assert float(x.abs().max()) > 65504
+    adapters = cb.Adapters({name: (c["a"], c["b"])}, c["scales"])
+    y = adapters.add(name, torch.zeros(T, n, device=dev), x, adapters.plan(c["ids"]))
+    exact = dict(c, x=x.double(), resid=torch.zeros(T, n, device=dev))
+    ref, tol = lora_reference(exact)
+    rounded = 2.0 ** -11 * x.double().abs() + 2.0 ** -25 * (x.double().abs().amax(1, keepdim=True) / 2 ** 14).clamp(min=1)
+    for i in range(G):
+        t = torch.nonzero(c["ids"] == i).flatten()
+        tol[t] += float(c["scales"][i]) * rounded[t] @ c["a"][i].double().abs().t() @ c["b"][i].double().abs().t() * (1 + 2.0 ** -10)
+    check_rows(y, ref, tol)
+    small = x.abs().amax(1) < 2 ** 15  # rows that fit are taken as they were
+    want = adapters.add(name, torch.zeros(T, n, device=dev), x.half(), adapters.plan(c["ids"]))
+    assert torch.equal(y[small], want[small])

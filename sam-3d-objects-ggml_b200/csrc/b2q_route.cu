@@ -167,7 +167,7 @@ __device__ void place_run(const int32_t* ids, int S, int groups, int run, int ru
   }
 }
 
-size_t place_smem(int groups) { return (static_cast<size_t>(kWarps + 2) * (groups + 1) + kWarps) * 4; }
+constexpr size_t place_smem(int groups) { return (static_cast<size_t>(kWarps + 2) * (groups + 1) + kWarps) * 4; }
 
 // NV: experts of a lane.  ON_SCORE: the bias is added to the scores.  (A kernel of its own: the scores of all experts
 // before the choice are work that the others do not have.)
@@ -347,15 +347,11 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const int32_t* ids, int
   place_run(ids, S, groups, blockIdx.x, gridDim.x, run_slots, run_counts, order, offsets, smem);
 }
 
-cudaError_t set_smem(const void* f, size_t bytes) {
-  return bytes > 48 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes))
-                           : cudaSuccess;
-}
-
 cudaError_t launch_place(const int32_t* ids, int64_t S, int groups, int runs, int run_slots, const int32_t* run_counts,
                          int32_t* order, int32_t* offsets, cudaStream_t s) {
   const size_t smem = place_smem(groups);
-  if (cudaError_t e = set_smem(reinterpret_cast<const void*>(place_kernel), smem)) return e;
+  // (always the most that any call needs: calls of other sizes from other threads share the setting)
+  if (cudaError_t e = allow_smem<place_kernel>(place_smem(kMaxGroups))) return e;
   return launch_early(place_kernel, dim3(static_cast<unsigned>(runs)), dim3(kThreads), smem, s, 1, ids, static_cast<int>(S),
                       groups, run_slots, run_counts, order, offsets);
 }
@@ -428,21 +424,21 @@ cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
   auto run = [&](auto ty) {
     constexpr int T = decltype(ty)::value;
     const int nv = (a.E + 31) / 32;
-    auto go = [&](auto k) {
-      if (cudaError_t e = set_smem(reinterpret_cast<const void*>(k), smem)) return e;
+    auto go = [&](auto nv_c, auto on) {
+      constexpr auto k = route_kernel<T, decltype(nv_c)::value, decltype(on)::value>;
+      if (cudaError_t e = allow_smem<k>(place_smem(kMaxGroups))) return e;
       return launch_early(k, dim3(static_cast<unsigned>(p.runs)), dim3(kThreads), smem, s, 1, a);
     };
     auto shape = [&](auto on) {
-      constexpr bool ON = decltype(on)::value;
-      if (nv <= 1) return go(route_kernel<T, 1, ON>);
-      if (nv <= 2) return go(route_kernel<T, 2, ON>);
-      if (nv <= 3) return go(route_kernel<T, 3, ON>);
-      if (nv <= 4) return go(route_kernel<T, 4, ON>);
-      if (nv <= 5) return go(route_kernel<T, 5, ON>);
-      if (nv <= 6) return go(route_kernel<T, 6, ON>);
-      if (nv <= 8) return go(route_kernel<T, 8, ON>);
-      if (nv <= 16) return go(route_kernel<T, 16, ON>);
-      return go(route_kernel<T, 32, ON>);
+      if (nv <= 1) return go(std::integral_constant<int, 1>(), on);
+      if (nv <= 2) return go(std::integral_constant<int, 2>(), on);
+      if (nv <= 3) return go(std::integral_constant<int, 3>(), on);
+      if (nv <= 4) return go(std::integral_constant<int, 4>(), on);
+      if (nv <= 5) return go(std::integral_constant<int, 5>(), on);
+      if (nv <= 6) return go(std::integral_constant<int, 6>(), on);
+      if (nv <= 8) return go(std::integral_constant<int, 8>(), on);
+      if (nv <= 16) return go(std::integral_constant<int, 16>(), on);
+      return go(std::integral_constant<int, 32>(), on);
     };
     return a.on_score ? shape(std::true_type()) : shape(std::false_type());
   };

@@ -1,6 +1,7 @@
 """Calls for rows that go by group at the borders between their kernels' forms, against plain 64-bit arithmetic
 (tolerances as in test_gpu_groups.py, and equality where every value is exact)."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -245,3 +246,40 @@ def test_adapters_rows_beyond_fp16(dev, T, name, dtype):
     small = x.abs().amax(1) < 2 ** 15  # rows that fit are taken as they were
     want = adapters.add(name, torch.zeros(T, n, device=dev), x.half(), adapters.plan(c["ids"]))
     assert torch.equal(y[small], want[small])
+
+
+# ------------------------------------------------------------------------------------------- calls from two threads
+@pytest.mark.parametrize("S", [400, 3000])
+def test_plans_of_many_and_of_few_groups_from_two_threads(dev, S):
+    """Two threads on streams of their own, one with 1024 groups, one with 400 (which need 137 KB and 53 KB of shared
+    memory), in turn and at once."""
+    failures = []
+
+    def work(groups, top):
+        try:
+            rng = np.random.default_rng(groups)
+            ids = rng.integers(-2, groups + 2, S).astype(np.int32)
+            ro, rf = plan_reference(ids, groups)
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                on = torch.from_numpy(ids).to(dev)
+                x = torch.from_numpy(rng.standard_normal((S // top, groups)).astype(np.float32)).to(dev)
+                first = None
+                for _ in range(300):
+                    order, offsets = b2q.group_rows(on, groups)
+                    route = b2q.moe_route(x, top)
+                    first = route if first is None else first
+                s.synchronize()
+                assert np.array_equal(order.cpu().numpy(), ro) and np.array_equal(offsets.cpu().numpy(), rf)
+                assert all(torch.equal(a, b) for a, b in zip(route, first))
+        except Exception as e:  # noqa: BLE001
+            failures.append((groups, repr(e)))
+
+    for groups in (1024, 400, 1024):
+        work(groups, 2)
+    threads = [threading.Thread(target=work, args=(g, 2)) for g in (1024, 400, 1024, 390)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures

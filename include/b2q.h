@@ -649,7 +649,9 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  *   order   int32 [S]      the slots by group, in slot order inside one; those of no group last
  * Plans that the calls below did not make are clamped to their buffers, never
  * trusted.  Rows of a result may lie beside the rows of an operand in one table,
- * but not on them (refused), except for a resid that is the result.  All results are the same from call to call: no atomics on floats.
+ * but not on them: results and workspaces that lie on an operand or on one
+ * another are refused, except for a resid that is the result.  All results are
+ * the same from call to call: no atomics on floats.
  *
  * b2q_moe_route: logits [T][E] of type F32, F16 or BF16.  Each token's choices
  * are its `top` largest of logit + bias (bias fp32 [E] or NULL; the sum in

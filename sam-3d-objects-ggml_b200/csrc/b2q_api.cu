@@ -9,6 +9,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 namespace {
 
@@ -1411,6 +1412,29 @@ static bool rows_touch(const void* p, int64_t p_rows, int64_t p_stride, int64_t 
   return shift < p_width || shift + q_width > p_stride;
 }
 
+// A buffer of a call: rows, or one stretch of bytes.  Absent or empty ones touch nothing.
+struct Span {
+  const void* p;
+  int64_t rows, stride, width;
+};
+static Span list_of(const void* p, int64_t bytes) { return {p, p && bytes > 0 ? 1 : 0, bytes, bytes}; }
+static Span rows_of(const void* p, int64_t rows, int64_t stride, int64_t width) {
+  return {p, p && width > 0 ? rows : 0, stride, width};
+}
+// Whether a buffer that is written lies on one that is read, or on another that is written.
+static bool spans_touch(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  auto touch = [](const Span& a, const Span& b) {
+    return rows_touch(a.p, a.rows, a.stride, a.width, b.p, b.rows, b.stride, b.width);
+  };
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span* v = w + 1; v != written.end(); ++v)
+      if (touch(*w, *v)) return true;
+    for (const Span& r : read)
+      if (touch(*w, r)) return true;
+  }
+  return false;
+}
+
 static int route_sizes(int64_t T, int64_t E, int64_t top) {
   if (T < 0 || E <= 0 || top <= 0 || top > E) return B2Q_ERR_INVALID_ARG;
   if (E > kMaxGroups || top > kRouteMaxTop || T > kMaxSlots / top) return B2Q_ERR_TOO_LARGE;
@@ -1441,6 +1465,11 @@ int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t ro
     return B2Q_ERR_MISALIGNED;
   const size_t need = run_bytes(run_plan(T, static_cast<int>(top)), E);
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
+  const int64_t slots = T * top * 4;
+  if (spans_touch({list_of(ids, slots), list_of(weights, slots), list_of(order, slots), list_of(offsets, (E + 1) * 4),
+                   list_of(workspace, need)},
+                  {rows_of(logits, T, row_stride_bytes, E * size), list_of(bias, E * 4)}))
+    return B2Q_ERR_INVALID_ARG;
   if (int rc = check_device(nullptr)) return rc;
   RouteArgs a{};
   a.logits = logits;
@@ -1479,6 +1508,8 @@ int b2q_group_rows(const int32_t* ids, int64_t S, int64_t groups, int32_t* order
     return B2Q_ERR_MISALIGNED;
   const size_t need = run_bytes(run_plan(S, 1), groups);
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
+  if (spans_touch({list_of(order, S * 4), list_of(offsets, (groups + 1) * 4), list_of(workspace, need)}, {list_of(ids, S * 4)}))
+    return B2Q_ERR_INVALID_ARG;
   if (int rc = check_device(nullptr)) return rc;
   return from_cuda(launch_group_rows(ids, S, static_cast<int>(groups), order, offsets,
                                      static_cast<int32_t*>(workspace), static_cast<cudaStream_t>(stream)));
@@ -1511,7 +1542,12 @@ int b2q_mul_mat_id(int wtype, const void* w, int64_t experts, int64_t n, int64_t
       !aligned(bias, 4) || !aligned(y, ysize) || y_row_stride_bytes % ysize != 0)
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
-  if (rows_touch(x, x_rows, x_row_stride_bytes, k * 2, y, slots, y_row_stride_bytes, n * ysize)) return B2Q_ERR_INVALID_ARG;
+  const int64_t w_bytes = q4 ? static_cast<int64_t>(b2q_weight_packed_q4_0_bytes(experts * rows, k))
+                             : (experts - 1) * w_expert_stride_bytes + (rows - 1) * w_row_stride_bytes + k * 2;
+  if (spans_touch({rows_of(y, slots, y_row_stride_bytes, n * ysize)},
+                  {rows_of(x, x_rows, x_row_stride_bytes, k * 2), list_of(w, w_bytes), list_of(bias, experts * rows * 4),
+                   list_of(order, slots * 4), list_of(offsets, (experts + 1) * 4)}))
+    return B2Q_ERR_INVALID_ARG;
   int sms = 0;
   if (int rc = check_device(&sms)) return rc;
   MulMatIdArgs a{};
@@ -1562,8 +1598,9 @@ int b2q_moe_combine(int ytype, const void* y, int64_t y_row_stride_bytes, const 
       (resid && (!aligned(resid, os) || resid_row_stride_bytes % os != 0)))
     return B2Q_ERR_MISALIGNED;
   if (!any) return B2Q_OK;
-  if (rows_touch(y, T * top, y_row_stride_bytes, n * ys, out, T, out_row_stride_bytes, n * os) ||
-      (resid && resid != out && rows_touch(resid, T, resid_row_stride_bytes, n * os, out, T, out_row_stride_bytes, n * os)))
+  if (spans_touch({rows_of(out, T, out_row_stride_bytes, n * os)},
+                  {rows_of(y, T * top, y_row_stride_bytes, n * ys), list_of(weights, T * top * 4), list_of(ids, T * top * 4),
+                   rows_of(resid != out ? resid : nullptr, T, resid_row_stride_bytes, n * os)}))
     return B2Q_ERR_INVALID_ARG;
   if (int rc = check_device(nullptr)) return rc;
   CombineArgs a{};
@@ -1623,8 +1660,11 @@ int b2q_lora_add_rows(int xtype, const void* x, int64_t T, int64_t k, int64_t x_
   if (!any) return B2Q_OK;
   const size_t need = lora_workspace(T, static_cast<int>(adapters), static_cast<int>(rank));
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
-  if (rows_touch(x, T, x_row_stride_bytes, k * 2, y, T, y_row_stride_bytes, n * ys) ||
-      (resid != y && rows_touch(resid, T, resid_row_stride_bytes, n * ys, y, T, y_row_stride_bytes, n * ys)))
+  if (spans_touch({rows_of(y, T, y_row_stride_bytes, n * ys), list_of(workspace, need)},
+                  {rows_of(x, T, x_row_stride_bytes, k * 2), list_of(a, adapters * rank * k * 2), list_of(b, adapters * n * rank * 2),
+                   list_of(scales, adapters * 4), list_of(row_scales, T * 4), list_of(order, T * 4),
+                   list_of(offsets, (adapters + 1) * 4),
+                   rows_of(resid != y ? resid : nullptr, T, resid_row_stride_bytes, n * ys)}))
     return B2Q_ERR_INVALID_ARG;
   int sms = 0;
   if (int rc = check_device(&sms)) return rc;
@@ -1667,6 +1707,10 @@ int b2q_draft_verify(int type, const void* target, int64_t target_row_stride_byt
       !aligned(cu_drafts, 4) || !aligned(u, 4) || !aligned(v, 4) || !aligned(accepted, 4) || !aligned(tokens, 4))
     return B2Q_ERR_MISALIGNED;
   if (B == 0) return B2Q_OK;
+  if (spans_touch({list_of(accepted, B * 4), list_of(tokens, (D + B) * 4)},
+                  {rows_of(target, D + B, target_row_stride_bytes, V * size), rows_of(draft_probs, D, draft_row_stride_bytes, V * size),
+                   list_of(drafts, D * 4), list_of(cu_drafts, (B + 1) * 4), list_of(u, D * 4), list_of(v, B * 4)}))
+    return B2Q_ERR_INVALID_ARG;
   if (int rc = check_device(nullptr)) return rc;
   VerifyArgs a{};
   a.target = target;

@@ -62,3 +62,66 @@ def lora_rows(rs, **kw):
                                           (abi.FAKE, dict(T=0), abi.OK), (abi.FAKE, dict(T=5000, ws=None), abi.WS)])
 def test_lora_rows_checks(b2q_mod, rs, kw, expect):
     assert lora_rows(rs, **kw) == expect
+
+
+# ------------------------------------------------------------------ results on operands, and on one another
+# Buffers a megabyte apart, so that only what a case moves lies on something.
+MB = 1 << 20
+
+
+def at(i):
+    return 64 * MB + i * MB
+
+
+def apart_route(**kw):
+    a = dict(x=at(0), bias=at(1), ids=at(2), w=at(3), order=at(4), off=at(5), ws=at(6), T=400, top=2)
+    a.update(kw)
+    return abi.route(**a)
+
+
+def apart_rows(**kw):
+    a = dict(ids=at(0), order=at(1), off=at(2), ws=at(3), S=3000)
+    a.update(kw)
+    return abi.rows(**a)
+
+
+def apart_mmid(**kw):
+    a = dict(w=at(0), x=at(1), order=at(2), off=at(3), bias=at(4), y=at(5))
+    a.update(kw)
+    return abi.mmid(**a)
+
+
+def apart_join(**kw):
+    a = dict(y=at(0), w=at(1), ids=at(2), r=at(3), o=at(4))
+    a.update(kw)
+    return abi.join(**a)
+
+
+def apart_lora(**kw):
+    a = dict(x=at(0), a=at(2), b=at(3), sc=at(4), order=at(5), off=at(6), res=at(8), y=at(10), ws=at(12), T=2000)
+    a.update(kw)
+    return lora_rows(at(7), **a)
+
+
+def apart_verify(**kw):
+    a = dict(t=at(0), g=at(1), d=at(2), cu=at(3), u=at(4), v=at(5), acc=at(6), tok=at(7))
+    a.update(kw)
+    return abi.verify(**a)
+
+
+CALLS = [
+    (apart_route, [("ids", [at(0), at(0) + 32 * 400 - 4, at(1) + 28, at(1) - 3196, at(3), at(4), at(5), at(6)]), ("w", [at(0), at(1), at(4)]),
+                   ("order", [at(0) + 32, at(1), at(5) - 3196]), ("off", [at(0), at(1) - 32]), ("ws", [at(0), at(1), at(2) + 3196])]),
+    (apart_rows, [("order", [at(0), at(0) + 11996, at(2), at(3)]), ("off", [at(0) + 4, at(3)]), ("ws", [at(0)])]),
+    (apart_mmid, [("y", [at(0), at(0) + 3 * 2048 + 15 * 128 + 96, at(1), at(2) + 76, at(3) + 16, at(4) + 252, at(4) - 32 * 19 - 30])]),
+    (apart_join, [("o", [at(0), at(1) + 28, at(2) - 64 * 3 - 60, at(2), at(3) + 64])]),
+    (apart_lora, [("y", [at(0), at(2) + 3 * 16 * 64 * 2 - 4, at(3), at(4) + 8, at(5), at(6) + 12, at(7) + 7996, at(8) + 128, at(12)]),
+                  ("ws", [at(0), at(2), at(3), at(4), at(5), at(6), at(7), at(8), at(10)])]),
+    (apart_verify, [("acc", [at(0), at(1), at(2), at(3) + 12, at(4), at(5), at(7) + 32]),
+                    ("tok", [at(0) + 400 * 8 + 396, at(1), at(2) + 20, at(3), at(4) - 32, at(5)])]),
+]
+
+
+@pytest.mark.parametrize("call,name,where", [(c, n, p) for c, moves in CALLS for n, ps in moves for p in ps])
+def test_results_on_any_operand_are_refused(b2q_mod, call, name, where):
+    assert call(**{name: where}) == abi.ARG

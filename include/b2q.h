@@ -677,7 +677,10 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * type; wtype Q4_0: b2q_weight_pack_q4_0 of the E * (n or 2 n) rows one under
  * another (strides ignored, k % 32 == 0), x F16 -- not rounded to 8 bits.  x has
  * x_rows rows (at least ceil(slots / per_row)), 16-byte aligned.  ytype F32 or
- * x's type.  fp32 sums.
+ * x's type.  fp32 sums.  Q4_0 weights enter exactly as long as they lie
+ * in fp16's range (|8 d| < 65504 for a block's scale d); of blocks with larger
+ * scales, weights beyond it may count as infinite.  A row of x that is not finite
+ * gives a row that is not (infinities or NaN).
  *
  * b2q_moe_combine: out[t] = resid[t] + sum_j weights[t][j] y[t * top + j], in
  * fp32, choices in order; rows whose ids[t][j] is negative are not read (ids may

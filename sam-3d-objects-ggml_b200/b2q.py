@@ -1040,7 +1040,8 @@ def mul_mat_id(wtype: int, w, n: int, k: int, x, order, offsets, per_row: int = 
                out_dtype=None, out=None, stream=None):
     """Row x[s // per_row] times the weight of slot s's expert, for every slot of the plan -> [slots, n] of x's
     type (or fp32); with glu the weight has 2 n rows and the result is silu(first n) * last n.  w: [E, n or
-    2 n, k] of x's type (TYPE_F16, TYPE_BF16), or weight_pack_q4_0 of all experts' rows (TYPE_Q4_0, x fp16).
+    2 n, k] of x's type (TYPE_F16, TYPE_BF16), or weight_pack_q4_0 of all experts' rows (TYPE_Q4_0, x fp16; weights
+    beyond fp16's range, from scales of 8188 on, may count as infinite).
     Slots without an expert give rows of 0."""
     torch = _torch()
     E, S = offsets.numel() - 1, order.numel()

@@ -283,3 +283,83 @@ def test_plans_of_many_and_of_few_groups_from_two_threads(dev, S):
     for t in threads:
         t.join()
     assert not failures, failures
+
+
+# -------------------------------------------------------------------------------------- what is exact, to the bit
+def q4_case(dev, counts, n, k, d, seed):
+    """4-bit experts whose blocks have the scales d (fp16 [rows, k / 32]), x the unit rows: slot s has column 37 s."""
+    E, S = len(counts), sum(counts)
+    c = make_experts(dev, S, E, 1, n, k, "q4_0", seed=seed, ids=slots_of(counts, dev))
+    g = torch.Generator(device=dev).manual_seed(seed)
+    raw = torch.randint(0, 256, (E * n, k // 32, 18), dtype=torch.uint8, generator=g, device=dev)
+    raw[:, :, :2] = d.view(torch.uint8).view(E * n, k // 32, 2)
+    codes = torch.cat([raw[:, :, 2:] & 15, raw[:, :, 2:] >> 4], -1).double() - 8
+    c["w64"] = (codes * d.double()[:, :, None]).view(E, n, k)
+    c["w"] = b2q.weight_pack_q4_0(raw.view(E * n, -1), k)
+    column = 37 * torch.arange(S, device=dev) % k
+    c["x"] = torch.zeros(S, k, dtype=torch.float16, device=dev)
+    c["x"][torch.arange(S, device=dev), column] = 1.0
+    return c, c["w64"][c["ids"].view(-1).long(), :, column]
+
+
+@pytest.mark.parametrize("counts", [[5, 9, 0, 20], [300, 41]])  # the rows kernel, and the tile kernel
+@pytest.mark.parametrize("k", [64, 1408])
+def test_mul_mat_id_q4_weights_are_exact(dev, counts, k):
+    """Every 4-bit weight as it is: scales of 11 bits, the smallest numbers of fp16, and the largest with |8 d| < 65504."""
+    n = 96
+    rng = np.random.default_rng(k)
+    size = (len(counts) * n, k // 32)
+    ordinary = rng.uniform(0.5, 2.0, size) * 2.0 ** rng.integers(-12, 3, size) * rng.choice([-1, 1], size)
+    smallest = rng.integers(0, 2048, size) * 2.0 ** -24
+    largest = rng.choice([8184.0, -8184.0, 4093.0, 8180.0], size)
+    for d in (ordinary, smallest, largest):
+        c, want = q4_case(dev, counts, n, k, torch.from_numpy(d.astype(np.float16)).to(dev), seed=k)
+        y = call_experts(c, out_dtype=torch.float32)
+        assert torch.equal(y.double(), want)
+
+
+@pytest.mark.parametrize("counts", [[5, 9, 0, 20], [17, 2, 24, 16], [300, 41], [257, 600, 3]])
+@pytest.mark.parametrize("n,k", [(40, 96), (130, 416), (200, 1408), (64, 4096)])
+def test_mul_mat_id_q4_sums_are_those_of_fp32(dev, counts, n, k):
+    """An fp32 sum of two products a weight (the weight as two numbers) and nothing else."""
+    for glu in (False, True):
+        c = make_experts(dev, sum(counts), len(counts), 1, n, k, "q4_0", glu, seed=k, ids=slots_of(counts, dev))
+        ref, _ = experts_reference(c)
+        mag = torch.zeros(sum(counts), n * (1 + glu), dtype=torch.float64, device=dev)
+        z = torch.zeros_like(mag)
+        for e in range(len(counts)):
+            s = torch.nonzero(c["ids"].view(-1) == e).flatten()
+            mag[s] = c["x"][s].double().abs() @ c["w64"][e].abs().t()
+            z[s] = c["x"][s].double() @ c["w64"][e].t()
+        dz = (2 * k + 8) * 2.0 ** -24 * mag
+        if glu:  # as of the 16-bit weights: |silu'| < 1.1, exp, a sum, a division and two products
+            gate, up = z[:, :n], z[:, n:]
+            silu = gate * torch.sigmoid(gate)
+            tol = 1.1 * dz[:, :n] * up.abs() + silu.abs() * dz[:, n:] + 1.1 * dz[:, :n] * dz[:, n:] + 2.0 ** -20 * (silu * up).abs()
+        else:
+            tol = dz
+        check_rows(call_experts(c, out_dtype=torch.float32), ref, tol)
+
+
+@pytest.mark.parametrize("T", [5, 40, 1500])
+@pytest.mark.parametrize("rank", [8, 16, 32, 64, 128])
+@pytest.mark.parametrize("dt,bits", [("bf16", 24), ("f16", 22)])
+def test_lora_rank_values_are_exact(dev, T, rank, dt, bits):
+    """Rank values of 24 bits (bf16: three numbers of 8) or 22 (fp16: two of 11) come through B = 1 as they are."""
+    rng = np.random.default_rng(rank)
+    piece = bits // (3 if dt == "bf16" else 2)
+    h = rng.integers(2 ** (bits - 1), 2 ** bits, rank)  # of one row, all of one size
+    parts = [(h >> (bits - piece * (i + 1))) & (2 ** piece - 1) for i in range(bits // piece)]
+    assert np.array_equal(sum(p << (bits - piece * (i + 1)) for i, p in enumerate(parts)), h)
+    a = torch.zeros(1, rank, 64, dtype=torch.float64, device=dev)
+    x = torch.zeros(T, 64, dtype=torch.float64, device=dev)
+    for i, p in enumerate(parts):  # x a: the pieces' sum
+        a[0, :, 5 + 20 * i] = torch.from_numpy(p * 2.0 ** -piece).to(dev)
+        x[:, 5 + 20 * i] = 2.0 ** (-piece * i)
+    want = torch.from_numpy(h * 2.0 ** -bits).to(dev)
+    assert torch.equal(x.to(DT[dt]).double(), x) and torch.equal(a.to(DT[dt]).double(), a)
+    assert torch.equal((x @ a[0].t()), want.expand(T, rank))
+    ids = torch.zeros(T, dtype=torch.int32, device=dev)
+    c = {"x": x.to(DT[dt]), "a": a.to(DT[dt]), "b": torch.eye(rank, device=dev).to(DT[dt])[None].contiguous(), "scales": None,
+         "resid": torch.zeros(T, rank, device=dev), "ids": ids}
+    assert torch.equal(call_lora(c).double(), want.expand(T, rank))

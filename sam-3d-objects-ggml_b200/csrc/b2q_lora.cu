@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
     for (int i = warp; i < MINE; i += kWarps) {
       const int m = rank * MINE + i;
       float v[PER] = {};
-      if (lane < LANES) {
+      if (lane * PER < p.rank) {  // (what an infinite x makes of A's missing rows is no number)
 #pragma unroll
         for (int s = 0; s < kRanks; ++s) {
           const uint32_t from = cluster_addr(sum + m * RP + lane * PER, s);
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const LoraArgs
     for (int i = 0; i < kTile * LANES / kThreads; ++i) {
       const int at = i * kThreads + threadIdx.x, m = at / LANES, c = at % LANES;
       float v[4] = {};
-      if (m < count) {
+      if (m < count && c * 4 < p.rank) {  // (what an infinite x makes of A's missing rows is no number)
         const float4* from = reinterpret_cast<const float4*>(p.part + (t.begin + m) * static_cast<int64_t>(RP)) + c;
         const float4 w = *from;
         v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;

@@ -363,3 +363,20 @@ def test_lora_rank_values_are_exact(dev, T, rank, dt, bits):
     c = {"x": x.to(DT[dt]), "a": a.to(DT[dt]), "b": torch.eye(rank, device=dev).to(DT[dt])[None].contiguous(), "scales": None,
          "resid": torch.zeros(T, rank, device=dev), "ids": ids}
     assert torch.equal(call_lora(c).double(), want.expand(T, rank))
+
+
+@pytest.mark.parametrize("T", [5, 1500])
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 64, 72])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_lora_infinite_values_of_one_sign_stay_infinite(dev, T, rank, dt):
+    """Ranks between the kernel's widths: no NaN out of an infinity where the formula has none."""
+    c = make_lora(dev, T, 2, rank, 64, 40, dt, "f32", seed=rank)
+    c["a"], c["b"] = c["a"].abs() + 2.0 ** -6, c["b"].abs() + 2.0 ** -6
+    c["ids"][:] = torch.arange(T, device=dev) % 2
+    c["x"][1, 3], c["x"][2, 60] = math.inf, -math.inf
+    y = call_lora(c)
+    assert bool((y[1] == math.inf).all()) and bool((y[2] == -math.inf).all())
+    keep = torch.ones(T, dtype=torch.bool, device=dev)
+    keep[[1, 2]] = False
+    ref, tol = lora_reference(c)
+    check_rows(y[keep], ref[keep], tol[keep])

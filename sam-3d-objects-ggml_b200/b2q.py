@@ -979,6 +979,11 @@ def _new_on(stream, like, size, dtype):
     return _empty_on(stream, size, dtype, like.device)
 
 
+def _row_step(t, rows: int, width: int) -> int:
+    """Values from a row to the next; one row alone has none, whatever its tensor's stride says."""
+    return t.stride(0) if rows > 1 else width
+
+
 def _is_list(t, n: int, dtype) -> bool:
     """t is n values of that type one after another."""
     return t.dtype is dtype and t.numel() == n and t.is_contiguous()
@@ -1012,7 +1017,7 @@ def moe_route(logits, top: int, bias=None, scoring: str = "softmax", renorm: boo
     order, offsets = _new_on(stream, logits, T * top, i32), _new_on(stream, logits, E + 1, i32)
     ws = _new_on(stream, logits, need, torch.uint8) if need else None
     rc = (_lib or _lib_obj()).b2q_moe_route(
-        dtype, logits.data_ptr(), T, E, size * (ld if ld > E else E), _ptr(bias), top, SCORING[scoring] + BIAS_ON[bias_on],
+        dtype, logits.data_ptr(), T, E, size * (ld if T > 1 else E), _ptr(bias), top, SCORING[scoring] + BIAS_ON[bias_on],
         1 if renorm else 0, scale, ids.data_ptr(), weights.data_ptr(), order.data_ptr(), offsets.data_ptr(),
         _ptr(ws), need, _raw_stream(stream, logits, bias))
     if rc:
@@ -1065,9 +1070,9 @@ def mul_mat_id(wtype: int, w, n: int, k: int, x, order, offsets, per_row: int = 
         assert _are_rows(out, S, n, out_dtype or out.dtype) and (out.stride(0) >= n or S <= 1)
     ytype, ysize = _val_type(out.dtype)
     rc = (_lib or _lib_obj()).b2q_mul_mat_id(
-        wtype, w.data_ptr(), E, n, k, ldw * 2, lde * 2, x.data_ptr(), x_rows, 2 * (ldx if ldx > k else k),
+        wtype, w.data_ptr(), E, n, k, ldw * 2, lde * 2, x.data_ptr(), x_rows, 2 * (ldx if x_rows > 1 else k),
         order.data_ptr(), offsets.data_ptr(), S, per_row, _ptr(bias), 1 if glu else 0, ytype, out.data_ptr(),
-        ysize * max(out.stride(0), n), _raw_stream(stream, x, w, order, offsets, bias, out))
+        ysize * _row_step(out, S, n), _raw_stream(stream, x, w, order, offsets, bias, out))
     if rc:
         _check("b2q_mul_mat_id", rc)
     return out
@@ -1091,8 +1096,8 @@ def moe_combine(y, weights, ids=None, resid=None, out_dtype=None, out=None, stre
                                 (resid.stride(0) >= n or T <= 1))
     (yt, ys), (ot, os_) = _val_type(y.dtype), _val_type(out.dtype)
     rc = (_lib or _lib_obj()).b2q_moe_combine(
-        yt, y.data_ptr(), ys * max(y.stride(0), n), weights.data_ptr(), _ptr(ids), T, top, n, ot, _ptr(resid),
-        0 if resid is None else os_ * max(resid.stride(0), n), out.data_ptr(), os_ * max(out.stride(0), n),
+        yt, y.data_ptr(), ys * _row_step(y, S, n), weights.data_ptr(), _ptr(ids), T, top, n, ot, _ptr(resid),
+        0 if resid is None else os_ * _row_step(resid, T, n), out.data_ptr(), os_ * _row_step(out, T, n),
         _raw_stream(stream, y, weights, ids, resid, out))
     if rc:
         _check("b2q_moe_combine", rc)
@@ -1130,9 +1135,9 @@ def lora_add(resid, x, a, b, scales, order, offsets, out=None, stream=None, row_
     if need:
         ws = _new_on(stream, x, need, torch.uint8)
     L = _lib or _lib_obj()
-    head = (_type16(dt), x.data_ptr(), T, k, 2 * (ldx if ldx > k else k), a.data_ptr(), b.data_ptr(), G, rank, n, _ptr(scales))
-    tail = (order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * max(resid.stride(0), n), out.data_ptr(),
-            ys * max(out.stride(0), n), _ptr(ws), need, _raw_stream(stream, x, a, b, scales, row_scales, order, offsets, resid, out))
+    head = (_type16(dt), x.data_ptr(), T, k, 2 * (ldx if T > 1 else k), a.data_ptr(), b.data_ptr(), G, rank, n, _ptr(scales))
+    tail = (order.data_ptr(), offsets.data_ptr(), ytype, resid.data_ptr(), ys * _row_step(resid, T, n), out.data_ptr(),
+            ys * _row_step(out, T, n), _ptr(ws), need, _raw_stream(stream, x, a, b, scales, row_scales, order, offsets, resid, out))
     rc = L.b2q_lora_add(*head, *tail) if row_scales is None else L.b2q_lora_add_rows(*head, row_scales.data_ptr(), *tail)
     if rc:
         _check("b2q_lora_add", rc)
@@ -1158,7 +1163,7 @@ def draft_verify(target, draft_probs, drafts, cu_drafts, u, v, stream=None):
     assert _is_list(drafts, D, i32) and _is_list(cu_drafts, B + 1, i32) and _is_list(u, D, f32) and _is_list(v, B, f32)
     accepted, tokens = _new_on(stream, target, B, i32), _new_on(stream, target, B + D, i32)
     rc = (_lib or _lib_obj()).b2q_draft_verify(
-        dtype, target.data_ptr(), size * max(ldp, V), _ptr(draft_probs), size * max(ldq, V), drafts.data_ptr(),
+        dtype, target.data_ptr(), size * (ldp if rows > 1 else V), _ptr(draft_probs), size * (ldq if D > 1 else V), drafts.data_ptr(),
         cu_drafts.data_ptr(), B, D, V, u.data_ptr(), v.data_ptr(), accepted.data_ptr(), tokens.data_ptr(),
         _raw_stream(stream, target, draft_probs, drafts, cu_drafts, u, v))
     if rc:

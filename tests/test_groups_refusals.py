@@ -6,7 +6,7 @@ import torch
 import b2q
 import cached_block as cb
 import test_groups_abi as abi
-from test_groups_wrappers import F16, lib_calls, lora, refused, route, z  # noqa: F401
+from test_groups_wrappers import F16, F32, I32, join, lib_calls, lora, mmid, refused, route, verify, z  # noqa: F401
 
 
 @pytest.mark.parametrize("sc", [2, 3, 6, 8, -1, -4])
@@ -125,3 +125,34 @@ CALLS = [
 @pytest.mark.parametrize("call,name,where", [(c, n, p) for c, moves in CALLS for n, ps in moves for p in ps])
 def test_results_on_any_operand_are_refused(b2q_mod, call, name, where):
     assert call(**{name: where}) == abi.ARG
+
+
+def one_row(width, step, dt):
+    """A row of a table whose rows are `step` values apart."""
+    return z(3, step, dt=dt)[1:2, :width]
+
+
+def test_the_stride_of_a_single_row_does_not_matter(lib_calls):
+    """Rows cut out of tables of any width, and results that are the residual by another view of it."""
+    mmid(rows=1, per_row=1, x=one_row(64, 99, F16), order=z(1, dt=I32), out=one_row(16, 33, F16))
+    resid = one_row(16, 50, F32)
+    join(T=1, y=one_row(16, 77, F16), weights=z(1, 1), ids=z(1, 1, dt=I32), resid=resid, out=resid.view(16).unsqueeze(0))
+    join(T=1, y=one_row(16, 77, F16), weights=z(1, 1), ids=z(1, 1, dt=I32), out=one_row(16, 5000, F32))
+    lora(T=1, x=one_row(64, 67, F16), resid=one_row(32, 41, F32), order=z(1, dt=I32))
+    route(T=1, logits=one_row(8, 13, F32))
+    verify(B=1, D=0, target=one_row(20, 23, F32), draft_probs=z(0, 20), drafts=z(0, dt=I32), u=z(0), v=z(1))
+    a = [c[1] for c in lib_calls]
+    assert a[0][9] == 128 and a[0][18] == 32
+    assert a[1][2] == 32 and a[1][10] == a[1][12] == 64 and a[1][9] == a[1][11]
+    assert a[2][2] == 32 and a[2][12] == 64
+    assert a[3][4] == 128 and a[3][15] == a[3][17] == 128
+    assert a[4][4] == 32 and a[5][2] == 80
+
+
+def test_strides_of_more_rows_are_passed(lib_calls):
+    join(y=z(8, 20, dt=F16)[:, :16], out=z(4, 40)[:, :16])
+    lora(x=z(6, 72, dt=F16)[:, :64], resid=z(6, 40)[:, :32])
+    route(logits=z(5, 11)[:, :8])
+    verify(target=z(8, 24)[:, :20], draft_probs=z(5, 28)[:, :20])
+    a = [c[1] for c in lib_calls]
+    assert a[0][2] == 40 and a[0][12] == 160 and a[1][4] == 144 and a[1][15] == 160 and a[2][4] == 44 and a[3][2] == 96 and a[3][4] == 112

@@ -678,9 +678,9 @@ bool two_launches(int64_t T, int groups, int rank) {
 // where tiles are few.  Measured at rank 64, 4096 -> 4096, 8.7k rows of 32 adapters: with three 110 us, with two 119;
 // 4096 x 6144 of 7 adapters: with two or three 123, with four 130.  Rank 128, 2048 rows of 8 adapters, 2048 x 2048: with
 // two 36, with three 41.
-int splits_of(int64_t T, int64_t K, int groups, int rank) {
+int splits_of(int64_t T, int64_t K, int groups, int rank, int num_sms) {
   const int64_t tiles = T / kTile + std::min<int64_t>(groups, T);
-  const int64_t most = std::min<int64_t>({kMaxSplits, (rank <= 64 ? 444 : 296) / tiles, K / 256});
+  const int64_t most = std::min<int64_t>({kMaxSplits, (rank <= 64 ? 3 : 2) * num_sms / tiles, K / 256});
   return most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
 }
 
@@ -700,7 +700,7 @@ cudaError_t launch_shape(LoraArgs a, int num_sms, cudaStream_t s) {
   if (cudaError_t e = allow_smem<shrink>(ShrinkShape<RP>::SMEM)) return e;
   if (cudaError_t e = allow_smem<expand>(expand_smem)) return e;
   const int64_t tiles = tiles_of(a, kTile);
-  a.splits = splits_of(a.T, a.K, a.groups, a.rank);
+  a.splits = splits_of(a.T, a.K, a.groups, a.rank, num_sms);
   // (and the parts of the columns of the second, of at least 256: 128 cost 31 -> 34 us at 4096 rows of 16 adapters, rank
   // 64, 2048 x 2048.  5 CTAs an SM against 6: 105 us against 109 for the 8.7k rows above, 77 against 73 for rank 16.)
   a.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((5 * num_sms + tiles - 1) / tiles, (a.N + 255) / 256)));

@@ -1104,7 +1104,6 @@ def moe_combine(y, weights, ids=None, resid=None, out_dtype=None, out=None, stre
     return out
 
 
-LORA_MAX_RANK = 128
 _lora_ws_bytes = functools.lru_cache(maxsize=256)(lambda T, k, G, rank: lib().b2q_lora_add_workspace_bytes(T, k, G, rank))
 
 

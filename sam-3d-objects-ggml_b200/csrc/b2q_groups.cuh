@@ -48,6 +48,12 @@ cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
 
+// 16 bytes into shared memory, zeros where there is nothing.  (256 bytes of a row come into the L2 at once: its next
+// pieces are asked for soon.)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 // Values of type kXF32 / kXF16 / kXBF16 as fp32, and back with one rounding.
 template <int T>
 struct Val;

@@ -465,7 +465,6 @@ struct LoraArgs {
 size_t lora_workspace(int64_t T, int groups, int rank);
 cudaError_t launch_lora(const LoraArgs& a, int xtype, int ytype, int num_sms, cudaStream_t s);
 
-constexpr int kVerifyRanks = 8;  // CTAs of one request
 struct VerifyArgs {
   const void* target;  // [D + B] rows of V, ldp elements apart
   const void* guess;   // [D] rows of V, ldq apart, or nullptr
@@ -473,8 +472,7 @@ struct VerifyArgs {
   int64_t ldp, ldq, B, D, V;
   const float *u, *v;
   int32_t *accepted, *tokens;
-  int ranks;
 };
-cudaError_t launch_verify(VerifyArgs a, int type, cudaStream_t s);
+cudaError_t launch_verify(const VerifyArgs& a, int type, cudaStream_t s);
 
 }  // namespace b2q

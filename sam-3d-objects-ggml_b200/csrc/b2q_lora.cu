@@ -89,11 +89,6 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// (256 bytes of a row come into the L2 at once: its next pieces are asked for soon.)
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
 // Two 16-bit numbers of type X in one word, and back.
 template <int X>
 __device__ __forceinline__ uint16_t bits16(float v) {

@@ -27,6 +27,7 @@ namespace b2q {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kRanks = 8;  // CTAs of one request
 constexpr int kBatch = 8;  // values of a row that a thread asks for at a time
 
 // One weight of the draw: target probability p above draft probability q (a
@@ -46,10 +47,10 @@ __device__ __forceinline__ double warp_sum(double v) {
 template <int T>
 __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a) {
   using V = typename Val<T>::type;
-  __shared__ double sums[kWarps], totals[kVerifyRanks], mine;
+  __shared__ double sums[kWarps], totals[kRanks], mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ranks = a.ranks, rank = ranks > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int64_t b = blockIdx.x / ranks;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int64_t b = blockIdx.x / kRanks;
   grid_wait();
   const int64_t lo = min(max(static_cast<int64_t>(__ldg(a.cu + b)), int64_t{0}), a.D);
   const int64_t hi = min(max(static_cast<int64_t>(__ldg(a.cu + b + 1)), lo), a.D);
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
     if (threadIdx.x == 0) a.accepted[b] = static_cast<int32_t>(first - lo);
   }
   // This warp's part of the vocabulary.
-  const int64_t part = ((a.V + static_cast<int64_t>(ranks) * kWarps - 1) / (ranks * kWarps) + 31) / 32 * 32;
+  const int64_t part = ((a.V + kRanks * kWarps - 1) / (kRanks * kWarps) + 31) / 32 * 32;
   const int64_t j0 = min(a.V, (static_cast<int64_t>(rank) * kWarps + warp) * part);
   const int64_t j1 = min(a.V, j0 + part);
   bool residual = down;
@@ -147,21 +148,16 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
     __syncthreads();
     double cta = 0.0;
     for (int w = 0; w < kWarps; ++w) cta += sums[w];
-    if (ranks > 1) {
-      if (threadIdx.x == 0) mine = cta;
-      cluster_sync();
-      if (threadIdx.x < ranks) {
-        double v;
-        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_addr(&mine, threadIdx.x)) : "memory");
-        totals[threadIdx.x] = v;
-      }
-      cluster_sync();  // (and nobody overwrites or leaves before all have read)
-    } else {
-      if (threadIdx.x == 0) totals[0] = cta;
-      __syncthreads();
+    if (threadIdx.x == 0) mine = cta;
+    cluster_sync();
+    if (threadIdx.x < kRanks) {
+      double v;
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_addr(&mine, threadIdx.x)) : "memory");
+      totals[threadIdx.x] = v;
     }
+    cluster_sync();  // (and nobody overwrites or leaves before all have read)
     total = 0.0, before = 0.0;
-    for (int r = 0; r < ranks; ++r) {
+    for (int r = 0; r < kRanks; ++r) {
       if (r == rank) before = total;
       total += totals[r];
     }
@@ -177,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
     const float v = __ldg(a.v + b);
     const double edge = (v > 0.0f ? static_cast<double>(v) : 0.0) * total;
     bool later = false;  // a weight behind what is shared out
-    for (int r = rank + 1; r < ranks; ++r) later |= totals[r] > 0.0;
+    for (int r = rank + 1; r < kRanks; ++r) later |= totals[r] > 0.0;
     double start = before, stop = before + totals[rank];
     int64_t from = static_cast<int64_t>(rank) * kWarps * part, size = part;
     bool here = totals[rank] > 0.0 && start <= edge && (edge < stop || !later);
@@ -246,10 +242,9 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
 
 }  // namespace
 
-cudaError_t launch_verify(VerifyArgs a, int type, cudaStream_t s) {
-  a.ranks = kVerifyRanks;
+cudaError_t launch_verify(const VerifyArgs& a, int type, cudaStream_t s) {
   void (*kernels[3])(const VerifyArgs) = {verify_kernel<0>, verify_kernel<1>, verify_kernel<2>};
-  return launch_early(kernels[type], dim3(static_cast<unsigned>(a.B * a.ranks)), dim3(kThreads), 0, s, a.ranks, a);
+  return launch_early(kernels[type], dim3(static_cast<unsigned>(a.B * kRanks)), dim3(kThreads), 0, s, kRanks, a);
 }
 
 }  // namespace b2q

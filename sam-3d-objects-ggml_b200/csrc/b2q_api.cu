@@ -1445,7 +1445,7 @@ static size_t run_bytes(const RunPlan& p, int64_t groups) {
 }
 
 size_t b2q_moe_route_workspace_bytes(int64_t T, int64_t E, int64_t top) {
-  return route_sizes(T, E, top) == B2Q_OK ? run_bytes(run_plan(T, static_cast<int>(top)), E) : 0;
+  return route_sizes(T, E, top) == B2Q_OK ? run_bytes(route_plan(T, E, top), E) : 0;
 }
 
 int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t row_stride_bytes, const float* bias,
@@ -1463,7 +1463,7 @@ int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t ro
   if (!aligned(logits, size) || row_stride_bytes % size != 0 || !aligned(bias, 4) || !aligned(ids, 4) ||
       !aligned(weights, 4) || !aligned(order, 4) || !aligned(offsets, 4) || !aligned(workspace, 4))
     return B2Q_ERR_MISALIGNED;
-  const size_t need = run_bytes(run_plan(T, static_cast<int>(top)), E);
+  const size_t need = run_bytes(route_plan(T, E, top), E);
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
   const int64_t slots = T * top * 4;
   if (spans_touch({list_of(ids, slots), list_of(weights, slots), list_of(order, slots), list_of(offsets, (E + 1) * 4),
@@ -1497,7 +1497,7 @@ static int group_sizes(int64_t S, int64_t groups) {
 }
 
 size_t b2q_group_rows_workspace_bytes(int64_t S, int64_t groups) {
-  return group_sizes(S, groups) == B2Q_OK ? run_bytes(run_plan(S, 1), groups) : 0;
+  return group_sizes(S, groups) == B2Q_OK ? run_bytes(rows_plan(S), groups) : 0;
 }
 
 int b2q_group_rows(const int32_t* ids, int64_t S, int64_t groups, int32_t* order, int32_t* offsets, void* workspace,
@@ -1506,7 +1506,7 @@ int b2q_group_rows(const int32_t* ids, int64_t S, int64_t groups, int32_t* order
   if (!offsets || (S > 0 && (!ids || !order))) return B2Q_ERR_INVALID_ARG;
   if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || !aligned(workspace, 4))
     return B2Q_ERR_MISALIGNED;
-  const size_t need = run_bytes(run_plan(S, 1), groups);
+  const size_t need = run_bytes(rows_plan(S), groups);
   if (need > 0 && (!workspace || workspace_bytes < need)) return B2Q_ERR_WORKSPACE;
   if (spans_touch({list_of(order, S * 4), list_of(offsets, (groups + 1) * 4), list_of(workspace, need)}, {list_of(ids, S * 4)}))
     return B2Q_ERR_INVALID_ARG;

@@ -389,7 +389,8 @@ constexpr int64_t kRouteMaxTop = 32;  // choices of one token (one a lane)
 struct RunPlan {
   int runs = 1, run_units = 0;
 };
-RunPlan run_plan(int64_t units, int per_unit);
+RunPlan route_plan(int64_t T, int64_t E, int64_t top);  // of the router, in tokens
+RunPlan rows_plan(int64_t S);                           // of given groups, in slots
 struct RouteArgs {
   const void* logits;  // [T] rows of E, ld elements apart
   int64_t T, ld;

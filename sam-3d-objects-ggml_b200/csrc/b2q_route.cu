@@ -34,9 +34,17 @@ namespace b2q {
 namespace {
 
 constexpr int kWarps = 32, kThreads = kWarps * 32;
-constexpr int kRunSlots = 512;       // of one CTA, at least
 constexpr int kMaxRuns = 148;
-constexpr int kOneSlots = 512;       // up to these many slots one CTA does everything
+// Rows of logits that a CTA has, at least (a row a warp), and up to which one CTA does everything: twice as many where a
+// row is little work.  Measured, one launch against two (us): 64 rows of 64 experts, one, two and eight choices 6.0/6.7,
+// 6.4/6.9, 8.1/7.7; 48 of 256, eight 12.1/10.5; 64 of 1024, one 47/27.  At least 32 rows a CTA against 64 and 128: 512 rows
+// of 64 experts, eight choices 8.2, 10.2, 15.1; 4736 of 256 14.1, 18.9, 29.4; 2048 of 1024 61, 108, 195.
+constexpr int kRouteRun = 32;
+int route_one(int E, int top) { return E <= 64 && top <= 4 ? 64 : 32; }
+// Slots of given groups, the same.  One launch against two: 2000 slots of 8, 64, 256 and 1024 groups 4.3/5.3, 5.9/5.8,
+// 6.4/6.7, 9.2/12.3; 3000 4.9/5.4, 7.2/5.9, 7.9/6.9, 10.7/12.5.  At least 512 slots a CTA against 256 and 1024: 8192 of 64
+// groups 6.1, 6.5, 6.8; of 1024 13.6, 16.6, 13.7.
+constexpr int kRowsRun = 512, kRowsOne = 2048;
 
 __device__ __forceinline__ uint32_t key_bits(float v) {
   if (v != v) v = -INFINITY;
@@ -405,18 +413,24 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
 
 }  // namespace
 
-RunPlan run_plan(int64_t units, int per_unit) {
+namespace {
+RunPlan plan_of(int64_t units, int one, int least) {
   RunPlan p;
-  const int64_t slots = units * per_unit;
-  if (slots <= kOneSlots) return p;
-  int64_t runs = std::min<int64_t>(kMaxRuns, (slots + kRunSlots - 1) / kRunSlots);
+  if (units <= one) return p;
+  const int64_t runs = std::min<int64_t>(kMaxRuns, (units + least - 1) / least);
   p.run_units = static_cast<int>((units + runs - 1) / runs);
   p.runs = static_cast<int>((units + p.run_units - 1) / p.run_units);
   return p;
 }
+}  // namespace
+
+RunPlan route_plan(int64_t T, int64_t E, int64_t top) {
+  return plan_of(T, route_one(static_cast<int>(E), static_cast<int>(top)), kRouteRun);
+}
+RunPlan rows_plan(int64_t S) { return plan_of(S, kRowsOne, kRowsRun); }
 
 cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
-  const RunPlan p = run_plan(a.T, a.top);
+  const RunPlan p = route_plan(a.T, a.E, a.top);
   const bool one = p.runs == 1;
   a.run_rows = one ? a.T : p.run_units;
   const size_t smem = one ? place_smem(a.E) : (a.E + 1) * 4;
@@ -450,7 +464,7 @@ cudaError_t launch_route(RouteArgs a, int type, cudaStream_t s) {
 
 cudaError_t launch_group_rows(const int32_t* ids, int64_t S, int groups, int32_t* order, int32_t* offsets,
                               int32_t* run_counts, cudaStream_t s) {
-  const RunPlan p = run_plan(S, 1);
+  const RunPlan p = rows_plan(S);
   if (p.runs == 1)
     return launch_place(ids, S, groups, 1, static_cast<int>(std::max<int64_t>(S, 1)), nullptr, order, offsets, s);
   if (cudaError_t e = launch_early(count_kernel, dim3(static_cast<unsigned>(p.runs)), dim3(kThreads), (groups + 1) * 4, s, 1, ids,

@@ -11,8 +11,8 @@ import b2q
 import cached_block as cb
 from test_gpu_expert_block import experts_reference as layer_reference
 from test_gpu_cached_block import layer_norm
-from test_gpu_groups import (DT, call_experts, call_lora, check_rows, experts_reference, lora_reference, make_experts, make_lora,
-                             plan_reference)
+from test_gpu_groups import (DT, call_experts, call_lora, check_route, check_rows, experts_reference, lora_reference, make_experts,
+                             make_lora, plan_reference)
 
 pytestmark = pytest.mark.gpu
 
@@ -380,3 +380,21 @@ def test_lora_infinite_values_of_one_sign_stay_infinite(dev, T, rank, dt):
     keep[[1, 2]] = False
     ref, tol = lora_reference(c)
     check_rows(y[keep], ref[keep], tol[keep])
+
+
+# ------------------------------------------------------------------------------ where the plans go from one launch to two
+@pytest.mark.parametrize("T", [31, 32, 33, 63, 64, 65, 96, 97, 4735, 4736, 4737])
+@pytest.mark.parametrize("E,top", [(5, 2), (64, 4), (64, 5), (65, 4), (300, 8), (1024, 1)])
+def test_route_of_one_launch_and_of_two(dev, T, E, top):
+    g = torch.Generator(device=dev).manual_seed(T + E)
+    x = 2 * torch.randn(T, E, generator=g, device=dev)
+    check_route(b2q.moe_route(x, top), x, None, top, "softmax", True)
+
+
+@pytest.mark.parametrize("S", [511, 513, 2047, 2048, 2049, 2560, 2561, 75775, 75777])
+@pytest.mark.parametrize("groups", [1, 64, 1024])
+def test_group_rows_of_one_launch_and_of_two(dev, S, groups):
+    ids = np.random.default_rng(S).integers(-1, groups + 1, S).astype(np.int32)
+    order, offsets = b2q.group_rows(torch.from_numpy(ids).to(dev), groups)
+    ro, rf = plan_reference(ids, groups)
+    assert np.array_equal(order.cpu().numpy(), ro) and np.array_equal(offsets.cpu().numpy(), rf)

@@ -156,3 +156,13 @@ def test_strides_of_more_rows_are_passed(lib_calls):
     verify(target=z(8, 24)[:, :20], draft_probs=z(5, 28)[:, :20])
     a = [c[1] for c in lib_calls]
     assert a[0][2] == 40 and a[0][12] == 160 and a[1][4] == 144 and a[1][15] == 160 and a[2][4] == 44 and a[3][2] == 96 and a[3][4] == 112
+
+
+def test_workspaces_of_plans(b2q_mod):
+    """None for one launch; the counts of every run for two."""
+    L = b2q.lib()
+    for T, E, top, need in [(0, 64, 4, 0), (64, 64, 4, 0), (65, 64, 4, 3 * 65 * 4), (32, 65, 4, 0), (33, 65, 4, 2 * 66 * 4),
+                            (33, 64, 5, 2 * 65 * 4), (4736, 64, 1, 148 * 65 * 4), (100000, 1024, 1, 148 * 1025 * 4)]:
+        assert L.b2q_moe_route_workspace_bytes(T, E, top) == need
+    for S, G, need in [(0, 8, 0), (2048, 8, 0), (2049, 8, 5 * 9 * 4), (1000000, 1024, 148 * 1025 * 4)]:
+        assert L.b2q_group_rows_workspace_bytes(S, G) == need

@@ -47,9 +47,13 @@ constexpr int kStageK = 64;           // values of K per stage: 128 bytes
 constexpr int kABytes = kBM * kStageK * 2;
 constexpr int kBBytes = kBN / 2 * kStageK * 2;
 constexpr int kAccs = 2;
-// Rows per expert, on average, up to which the rows kernel does 4-bit weights.  Measured, 32 experts, gate and up,
-// rows kernel against this one: 2048 -> 1408 with 4, 16, 32 rows an expert 44 us against 83, 66 against 84, 92 against
-// 88; 1024 -> 512 19 against 23, 28 against 24, 34 against 26.
+// Rows per expert, on average, up to which the rows kernel does 4-bit weights.  Measured over 21 shapes (8, 32 and 128
+// experts, K 256 to 4096, 512 to 2816 weight rows, cold weights), rows kernel over this one: 0.72 of the time with 8 rows an
+// expert (0.48 to 0.96), 0.82 with 12 (0.57 to 1.09), 0.89 with 16 (0.65 to 1.19), 1.00 with 24 (0.79 to 1.31).  With 16
+// it loses where this kernel's tiles just fill their waves or leave most pairs idle anyway: 32 and 8 experts of gate and
+// up 1024 -> 512 28.6 us against 25.0 and 18.2 against 15.3, 512 -> 512 18.8 against 18.1, 8 experts of 1408 -> 2048 20.4
+// against 18.9; and gains 66.5 against 84.8 (32 experts, 2048 -> 1408), 41.8 against 52.5 (1408 -> 2048), 62 against 82 (128
+// of 512 -> 2048).
 constexpr int kFewRows = 16;
 // Q4_0: a raw slot is 256 values of the CTA's 128 rows: nibbles in two boxes of
 // 64 rows, and each box's fp16 scales from the multiple of 8 rows below its first

@@ -321,12 +321,16 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
       }
       *reinterpret_cast<float4*>(sum + i * 4) = v;
     }
+    // (asked for before the others are waited for)
+    constexpr int MINE = M / kRanks;
+    float scale = p.scales ? __ldg(p.scales + t.group) : 1.0f;
+    if (p.row_scales && warp < MINE) scale *= row_scale(p, row_of[rank * MINE + warp]);
     cluster_sync();
     // --------------------------- 2: this CTA's rows, from all eight and to all eight
-    const float scale = p.scales ? __ldg(p.scales + t.group) : 1.0f;
-    constexpr int MINE = M / kRanks, PER = RP >= 64 ? RP / 32 : 2, LANES = RP / PER;  // rows; values of a lane
-    for (int i = warp; i < MINE; i += kWarps) {
-      const int m = rank * MINE + i;
+    constexpr int PER = RP >= 64 ? RP / 32 : 2, LANES = RP / PER;  // rows; values of a lane
+    static_assert(MINE <= kWarps, "a row a warp");
+    if (warp < MINE) {
+      const int m = rank * MINE + warp;
       float v[PER] = {};
       if (lane * PER < p.rank) {  // (what an infinite x makes of A's missing rows is no number)
 #pragma unroll
@@ -344,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, RP <= 64 ? 2 : 1) lora_cluster_kerne
 #pragma unroll
       for (int e = 0; e < PER; ++e) v[e] *= scale;
       uint32_t terms[kTerms<X, Y>][PER / 2];
-      const float up = split_row<X, Y, PER, 32>(v, terms) * row_scale(p, row_of[m]);
+      const float up = split_row<X, Y, PER, 32>(v, terms);
 #pragma unroll
       for (int s = 0; s < kRanks; ++s) {
         if (lane < LANES) {

@@ -712,8 +712,8 @@ B2Q_API int b2q_mul_vec(int wtype, const void* packed, int64_t n, int64_t k, int
  * values that are NaN, infinite or negative, or whose draft value is NaN, and
  * negative draft values count as 0; -1 when nothing is left).
  * accepted int32 [B]: drafts that stay; tokens int32 [D + B], laid out as
- * target's rows: those drafts, the drawn token, -1 after it (and behind the last
- * request, where cu_drafts[B] < D).  Tokens outside 0 .. V - 1 are turned down. */
+ * target's rows: those drafts, the drawn token, -1 after it (and before the first
+ * request and behind the last, where cu_drafts[0] > 0 or cu_drafts[B] < D).  Tokens outside 0 .. V - 1 are turned down. */
 enum b2q_scoring { B2Q_SCORE_SOFTMAX = 0, B2Q_SCORE_SIGMOID = 1, B2Q_SCORE_BIAS = 4 /* added to either */ };
 B2Q_API size_t b2q_moe_route_workspace_bytes(int64_t T, int64_t E, int64_t top);
 B2Q_API int b2q_moe_route(int type, const void* logits, int64_t T, int64_t E, int64_t row_stride_bytes,

@@ -83,7 +83,9 @@ __global__ void __launch_bounds__(kThreads, 6) verify_kernel(const VerifyArgs a)
   if (rank == 0) {
     for (int64_t i = lo + threadIdx.x; i <= hi; i += kThreads)
       if (i != first) a.tokens[i + b] = i < first ? __ldg(a.drafts + i) : -1;
-    if (b == a.B - 1)  // rows behind the last request
+    if (b == 0)  // rows before the first request, and behind the last
+      for (int64_t i = threadIdx.x; i < lo; i += kThreads) a.tokens[i] = -1;
+    if (b == a.B - 1)
       for (int64_t i = hi + 1 + threadIdx.x; i <= a.D; i += kThreads) a.tokens[i + b] = -1;
     if (threadIdx.x == 0) a.accepted[b] = static_cast<int32_t>(first - lo);
   }

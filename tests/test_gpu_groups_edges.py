@@ -398,3 +398,23 @@ def test_group_rows_of_one_launch_and_of_two(dev, S, groups):
     order, offsets = b2q.group_rows(torch.from_numpy(ids).to(dev), groups)
     ro, rf = plan_reference(ids, groups)
     assert np.array_equal(order.cpu().numpy(), ro) and np.array_equal(offsets.cpu().numpy(), rf)
+
+
+# --------------------------------------------------------------------------------------- requests of a larger buffer
+@pytest.mark.parametrize("before,behind", [(0, 0), (3, 0), (0, 4), (700, 600)])
+def test_verify_rows_before_the_first_request_and_behind_the_last(dev, before, behind):
+    """A stretch of a buffer's requests: its own rows as if it were alone, -1 in all others."""
+    g = torch.Generator(device=dev).manual_seed(before)
+    B, D, V = 3, 7, 90
+    p = torch.softmax(2 * torch.randn(before + D + B + behind, V, generator=g, device=dev), -1)
+    q = torch.softmax(2 * torch.randn(before + D + behind, V, generator=g, device=dev), -1)
+    drafts = torch.randint(0, V, (before + D + behind,), generator=g, device=dev).int()
+    u, v = torch.rand(before + D + behind, generator=g, device=dev), torch.rand(B, generator=g, device=dev)
+    cu = torch.tensor([0, 2, 2, 7], dtype=torch.int32, device=dev)
+    alone = b2q.draft_verify(p[before:before + D + B].contiguous(), q[before:before + D].contiguous(), drafts[before:before + D].contiguous(),
+                             cu, u[before:before + D].contiguous(), v)
+    # memory that is not -1 by chance: the allocator hands out what was just freed
+    torch.full((before + D + B + behind,), 77, dtype=torch.int32, device=dev)
+    accepted, tokens = b2q.draft_verify(p, q, drafts, cu + before, u, v)
+    assert torch.equal(accepted, alone[0]) and torch.equal(tokens[before:before + D + B], alone[1])
+    assert bool((tokens[:before] == -1).all()) and bool((tokens[before + D + B:] == -1).all())

@@ -138,7 +138,7 @@ class Experts:
         worst = 0.0
         for rows in raw.view(-1, 2 * hidden, C // 32, 18):  # an expert at a time
             d = rows[:, :, :2].contiguous().view(torch.float16)[:, :, 0].double()
-            codes = torch.cat([rows[:, :, 2:] & 15, rows[:, :, 2:] >> 4], -1).int() - 8
+            codes = torch.cat([rows[:, :, 2:] & 15, rows[:, :, 2:] >> 4], -1).to(torch.int16) - 8
             length = (d.square() * codes.square().sum(-1)).sum(-1).sqrt()
             bound = float((C * length[:hidden] * length[hidden:]).max())
             worst = max(worst, bound) if bound == bound else float("inf")

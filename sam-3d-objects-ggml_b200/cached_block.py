@@ -31,7 +31,9 @@ experts those are qkv and out.
 requests, and takes back the pages of those that end; the host knows the lengths
 it asked for, the device builds the rest (b2q_kv_cache_plan), so a step never
 waits for the device.  A step of drafted tokens ends with b2q_draft_verify, and
-`keep` takes back what the turned down ones had.
+`keep` takes back what the turned down ones had; the lengths to keep are host
+numbers, so whoever drafts reads the accepted counts back first, and waits for
+that step.
 
     python cached_block.py       # a prompt of 300 tokens, then 8 single tokens
 """

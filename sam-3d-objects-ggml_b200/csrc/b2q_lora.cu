@@ -18,8 +18,8 @@
 // stages of x's and A's rows; where the tiles are few, a cluster shares out K and adds
 // the parts up) in fp32 in the workspace; the second, launched early, streams y.
 //
-// Measured: 32 rows of 24 adapters, rank 16, 4096 -> 4096: 6.5 us, one chain of
-// latencies; 8.7k rows of 7 adapters, rank 64, 4096 -> 6144, bf16: 105 us, 4550 GB/s
+// Measured: 32 rows of 24 adapters, rank 16, 4096 -> 4096: 6.6 us, one chain of
+// latencies; 8.7k rows of 7 adapters, rank 64, 4096 -> 6144, bf16: 106 us, 4530 GB/s
 // (y's stages 32 columns wide instead of 64: 17 us more; read into registers instead: 30
 // more; the parts of K added up by every CTA of the second launch instead: 3 to 5 more,
 // 27 of 186 at rank 128; tiles of 128 rows in the first: 10 more).
@@ -42,8 +42,8 @@ constexpr int kStageK = 64;
 template <int RP>
 constexpr int kPitch = RP * 2 + (RP >= 64 ? 64 : 0);
 
-// Numbers that make up one of h: 22 bits of fp16, 24 of bf16; 16 of bf16 where y has 8.  (4096 x 6144, rank 64, bf16,
-// fp32 y: 112 us and an error of 4e-7 with three, 101 us and 1e-6 with two.)
+// Numbers that make up one of h: 22 bits of fp16, 24 of bf16; 16 of bf16 where y has 8.  (8700 rows, 4096 x 6144, bf16, fp32
+// y: rank 64 108 us and an error of 2.6e-7 with three, 99 us and 5.8e-7 with two; rank 128 196 and 4.7e-7, 169 and 9.3e-7.)
 template <int X, int Y>
 constexpr int kTerms = X == 2 && Y == 0 ? 3 : 2;
 
@@ -676,9 +676,9 @@ bool two_launches(int64_t T, int groups, int rank) {
 }
 
 // Parts of K of the first launch, the CTAs of a cluster: up to three CTAs an SM, or two of the 96 KB ones of rank 128,
-// where tiles are few.  Measured at rank 64, 4096 -> 4096, 8.7k rows of 32 adapters: with three 110 us, with two 119;
-// 4096 x 6144 of 7 adapters: with two or three 123, with four 130.  Rank 128, 2048 rows of 8 adapters, 2048 x 2048: with
-// two 36, with three 41.
+// where tiles are few.  Measured (8700 rows, bf16), rank 64, 4096 -> 4096 of 32 adapters: with three or four 95 us, with
+// two 102; 4096 x 6144 of 7: with two or three 108, with four 112; 2000 rows of 8, 2048 x 2048, fp16: with two 19.6, with three
+// 21.0.  Rank 128, 2000 rows of 8, 2048 x 2048: with two 37.4, with three 39.3.
 int splits_of(int64_t T, int64_t K, int groups, int rank, int num_sms) {
   const int64_t tiles = T / kTile + std::min<int64_t>(groups, T);
   const int64_t most = std::min<int64_t>({kMaxSplits, (rank <= 64 ? 3 : 2) * num_sms / tiles, K / 256});

@@ -23,8 +23,9 @@
 // exact in fp16, and two MMAs add up to the weight as it is (|8 d| < 65504).
 // Few rows with such weights go to b2q_mul_mat_id_rows.cu.
 //
-// Measured: gate and up of 8192 tokens x 4 of 32 experts, 2048 -> 1408, bf16: 326 us,
-// 1160 TFLOP/s, tensor pipe 63% active (TMA gathers of 4 rows instead of cp.async 946,
+// Measured: gate and up of 8192 tokens x 4 of 32 experts, 2048 -> 1408, bf16: 326 us alone,
+// 1160 TFLOP/s, tensor pipe 63% active; 388, 975 TFLOP/s, in calls that follow one
+// another for seconds, where the power cap holds the clocks down (TMA gathers of 4 rows instead of cp.async 946,
 // a sorted copy of x and TMA boxes 353); of 40 tokens x 4 of 64 experts, 2048 -> 1024:
 // 77 us, 5790 GB/s; one token x 6 experts, 2048 -> 1408: 20 us, 3400 GB/s, a third of it
 // set-up.

@@ -16,7 +16,7 @@
 // Codes become q - 8 in fp16, which is exact; a block's sums are scaled by d and
 // added in fp32, so a weight's value is never rounded.
 //
-// Measured: 24 tokens x 6 of 64 experts, 1408 -> 2048: 32 us for 87 MB; 8 of them until
+// Measured: 24 tokens x 6 of 64 experts, 1408 -> 2048: 34 us for 87 MB; 8 of them until
 // the first products (plan, first rows of x), 16 if nothing were computed, and the
 // rest issue slots (8 warps an SM 35, 14 and 16 with shorter rings 33 to 36).
 #include "b2q_groups.cuh"

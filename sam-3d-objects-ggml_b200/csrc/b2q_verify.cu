@@ -16,7 +16,7 @@
 // Bound by that read; a thread asks for 8 values of each row at a time, and an SM
 // has 6 CTAs, so that enough are on their way (rows of any alignment: values are
 // read one by one, 32 neighbours a warp).  Measured: 96 requests of up to 7 drafts,
-// 151001 tokens, fp32: 27.5 us for 90 MB; 4 requests of 32000 tokens, bf16: 7.9 us (512
+// 151001 tokens, fp32: 27.4 us for 90 MB; 4 requests of 32000 tokens, bf16: 7.8 us (512
 // threads a CTA, four values at a time and one warp after the border: 105 and 11).
 #include "b2q_groups.cuh"
 #include "b2q_internal.h"

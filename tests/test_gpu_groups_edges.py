@@ -418,3 +418,40 @@ def test_verify_rows_before_the_first_request_and_behind_the_last(dev, before, b
     accepted, tokens = b2q.draft_verify(p, q, drafts, cu + before, u, v)
     assert torch.equal(accepted, alone[0]) and torch.equal(tokens[before:before + D + B], alone[1])
     assert bool((tokens[:before] == -1).all()) and bool((tokens[before + D + B:] == -1).all())
+
+
+# ------------------------------------------------------------------------- experts and adapters in one block
+@pytest.mark.parametrize("counts", [[3, 2], [70, 41]])
+def test_block_with_experts_and_adapters_of_the_attention(dev, counts):
+    """What the block gives with both: its attention with adapters (of a block whose last linears add nothing), then the
+    experts on that."""
+    C, heads, D, hidden, sections, G, rank = 256, 4, 64, 512, (12, 10, 10), 3, 16
+    _, weights = cb.random_block(dev, C, heads, heads, D, hidden, sections, seed=5)
+    weights["fc2"] = np.zeros_like(weights["fc2"])
+    g = torch.Generator(device=dev).manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    vec = {"b_qkv": 0.1 * r(3 * heads * D), "b_out": 0.1 * r(C), "b1": 0.1 * r(hidden), "b2": torch.zeros(C, device=dev),
+           "gq": 1 + 0.1 * r(heads * D), "gk": 1 + 0.1 * r(heads * D)}
+    freq = 1e4 ** (-torch.cat([torch.arange(n, device=dev) / n for n in sections]))
+    make = lambda **kw: cb.CachedBlock(dev, weights, vec, C, heads, heads, D, hidden, sections, freq, unrounded_rows=128, **kw)  # noqa: E731
+    experts, _ = cb.random_experts(dev, 6, C, 96, 2, seed=2)
+    both, attention = make(experts=experts), make()
+    shapes = cb.CachedBlock.shapes(C, heads, heads, D, hidden)
+    pairs = {n: ((r(G, rank, shapes[n][1]) / shapes[n][1] ** 0.5).half(), (0.3 * r(G, shapes[n][0], rank) / rank ** 0.5).half())
+             for n in ("qkv", "out")}
+    adapters = cb.Adapters(pairs)
+    ids = torch.repeat_interleave(torch.tensor([2, -1]), torch.tensor(counts)).int().to(dev)
+    x = r(sum(counts), C)
+
+    def run(block, adapters):
+        cache = cb.PagedCache(dev, 1, 2, heads, D, pages=20, page_size=16, max_len=128)
+        step = cache.plan(counts)
+        pos = step["pos"]
+        grid = torch.stack([pos, pos // 7, pos % 7]).int().contiguous()
+        rows = adapters.plan(ids) if adapters else None
+        return block.forward(x.clone(), cache, 0, step, grid, adapters=adapters, rows=rows)
+
+    mid = run(attention, adapters)
+    assert torch.equal(run(both, adapters), experts.forward(b2q.norm_modulate(mid), mid.clone()))
+    plain = run(both, None)
+    assert torch.equal(run(both, adapters)[counts[0]:], plain[counts[0]:]) and not torch.equal(run(both, adapters), plain)
